@@ -42,7 +42,7 @@ extern "C" {
 /* Tokens (batch*grid*grid) or workspace rows per call: fewer than 2^31 - 2^16, so a chunk's
  * end (chunks x tokens-per-chunk < tokens + chunks) and a thread's next token stay in int32. */
 #define SIHC_MAX_TOKENS (((int64_t)1 << 31) - ((int64_t)1 << 16))
-#define SIHC_ABI_VERSION 6
+#define SIHC_ABI_VERSION 7
 /* Bytes of the per-GPU scratch array of sihc_event_backward_noalloc (64 MiB). */
 #define SIHC_SCRATCH_BYTES (64u << 20)
 
@@ -309,6 +309,81 @@ int sihc_fma_rate(void *out, int chains, int form, int blocks, int iters, void *
 /* Plain device copy of `bytes` bytes (16-byte vectors). No reference counterpart: it is
  * the calibration kernel for HBM counters and the practical bandwidth ceiling. */
 int sihc_copy(const void *src, void *dst, size_t bytes, void *stream);
+
+/* ---- Operators that condition a denoiser on an encoder's states (since ABI 7). No reference
+ * counterpart: the reference's class table, norms and attention are plain PyTorch. ---- */
+
+/* out[n,:] = scale * table[ids[n],:] (fp32 product, rounded once). table is [rows, channels],
+ * out [tokens, channels], both packed, in dtype; ids are int32 or int64 (id_bits 32 or 64).
+ * Ids outside [0, rows) select the last row (the host wrappers reject them). */
+int sihc_embedding(const void *table, const void *ids, void *out, int64_t tokens, int64_t rows,
+                   int channels, float scale, int id_bits, int dtype, void *stream);
+
+size_t sihc_embedding_backward_workspace_size(int64_t tokens, int64_t rows, int channels);
+/* Adjoint of sihc_embedding: grad_table[r,:] = scale * sum of grad[n,:] over the tokens n with
+ * ids[n] == r, in fp32 and in a fixed order (no atomics on values: identical inputs give
+ * identical bits), rounded once; zero where no token selects a row, and for the row `padding`
+ * (-1: none). Every row is written. grad_table must be 16-byte aligned. */
+int sihc_embedding_backward(const void *grad, const void *ids, void *grad_table, int64_t tokens,
+                            int64_t rows, int channels, float scale, int64_t padding, int id_bits,
+                            int dtype, void *workspace, size_t workspace_bytes, void *stream);
+
+enum { SIHC_ACT_NONE = 0, SIHC_ACT_SILU = 1 };
+
+size_t sihc_group_norm_workspace_size(int64_t batch, int64_t pixels, int channels, int groups,
+                                      int dtype);
+/* Group norm with an activation over a packed [batch, pixels, channels] tensor: per image and
+ * group of channels/groups adjacent channels, m and r = 1/sqrt(variance + eps) over its pixels
+ * and channels, y = act(weight * (x - m) * r + bias). weight and bias are [channels] in w_dtype
+ * (fp32 or dtype). stats, if given, receives [batch, groups] pairs (m, r) for the backward.
+ * The workspace may be NULL where its size is 0. */
+int sihc_group_norm(const void *x, const void *weight, const void *bias, void *y, float *stats,
+                    int64_t batch, int64_t pixels, int channels, int groups, float eps, int act,
+                    int dtype, int w_dtype, void *workspace, size_t workspace_bytes, void *stream);
+
+size_t sihc_group_norm_backward_workspace_size(int64_t batch, int64_t pixels, int channels,
+                                               int groups, int dtype);
+/* Adjoint of sihc_group_norm from its input and stats: grad_x in dtype, grad_weight and
+ * grad_bias [channels] in w_dtype, summed in fp32 in a fixed order. No output may overlap an
+ * input or another output. */
+int sihc_group_norm_backward(const void *grad, const void *x, const void *weight, const void *bias,
+                             const float *stats, void *grad_x, void *grad_weight, void *grad_bias,
+                             int64_t batch, int64_t pixels, int channels, int groups, int act,
+                             int dtype, int w_dtype, void *workspace, size_t workspace_bytes,
+                             void *stream);
+
+/* Sizes of a cross attention: heads is a multiple of kv_heads (query head h attends with key
+ * and value head h / (heads / kv_heads)); dim is 1..SIHC_MAX_HEAD_DIM. Strides are in elements
+ * between batch rows, tokens and heads; the channels of a head are adjacent. */
+#define SIHC_MAX_HEAD_DIM 128
+typedef struct {
+  int64_t batch;
+  int queries, keys, heads, kv_heads, dim;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  float scale;
+  int dtype;
+} sihc_attention;
+
+size_t sihc_cross_attention_workspace_size(const sihc_attention *a);
+/* out[b,i,h,:] = sum over j < lengths[b] of softmax_j(scale * q[b,i,h,:] . k[b,j,g,:]) v[b,j,g,:],
+ * with g the key and value head of h. q is [batch, queries, heads, dim], k and v are [batch, keys,
+ * kv_heads, dim], strided; out is packed. lengths (int32 [batch], NULL: all keys) are clamped to
+ * [0, keys]; a row of length 0 gives zeros, and what k and v hold past a length is not used.
+ * stats, if given, receives [batch, heads, queries] pairs (the largest scaled score in units of
+ * log 2, the reciprocal of the sum of 2^(score - largest)) for the backward. */
+int sihc_cross_attention(const sihc_attention *a, const void *q, const void *k, const void *v,
+                         const int32_t *lengths, void *out, float *stats, void *workspace,
+                         size_t workspace_bytes, void *stream);
+
+size_t sihc_cross_attention_backward_workspace_size(const sihc_attention *a);
+/* Adjoint of sihc_cross_attention from its inputs, output and stats. grad, out and grad_q are
+ * packed [batch, queries, heads, dim], grad_k and grad_v packed [batch, keys, kv_heads, dim];
+ * keys past a length get zero gradients. Sums in fp32 in a fixed order, without atomics. */
+int sihc_cross_attention_backward(const sihc_attention *a, const void *grad, const void *q,
+                                  const void *k, const void *v, const int32_t *lengths,
+                                  const void *out, const float *stats, void *grad_q, void *grad_k,
+                                  void *grad_v, void *workspace, size_t workspace_bytes,
+                                  void *stream);
 
 #ifdef __cplusplus
 }

@@ -13,11 +13,14 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_ROOT = Path(__file__).resolve().parent
 REPO_ROOT = PKG_ROOT.parent
-SOURCES = [PKG_ROOT / "csrc" / "sihc_kernels.hip"]
+SOURCES = [PKG_ROOT / "csrc" / name
+           for name in ("sihc_kernels.hip", "embedding.hip", "group_norm.hip", "cross_attention.hip")]
 OUTPUT = PKG_ROOT / "sihc_hip" / "libsihc_hip.so"
 SELFTEST_SOURCE = PKG_ROOT / "csrc" / "abi_selftest.c"
 SELFTEST = PKG_ROOT / "sihc_hip" / "sihc_abi_selftest"
@@ -34,20 +37,23 @@ def hipcc_path() -> str:
     raise RuntimeError("hipcc not found: the SiHC HIP library cannot be built")
 
 
-def command(output: Path = OUTPUT) -> list[str]:
+def compile_command(source: Path, output: Path) -> list[str]:
     return [
         hipcc_path(),
         f"--offload-arch={ARCH}",
         "-O3",
         "-std=c++17",
         "-fPIC",
-        "-shared",
         "-Wall",
         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         "-I", str(REPO_ROOT / "include"),
-        *[str(s) for s in SOURCES],
+        "-c", str(source),
         "-o", str(output),
     ]
+
+
+def link_command(objects: list[Path], output: Path = OUTPUT) -> list[str]:
+    return [hipcc_path(), f"--offload-arch={ARCH}", "-fPIC", "-shared", *map(str, objects), "-o", str(output)]
 
 
 def selftest_command(output: Path = SELFTEST) -> list[str]:
@@ -105,7 +111,11 @@ def build(verbose: bool = False) -> Path:
     """Compile the library, the C-ABI self-test and the native dispatch (always; atomically
     replaces an existing build)."""
     tmp = OUTPUT.with_suffix(".so.tmp")
-    _run(command(tmp), verbose)
+    with tempfile.TemporaryDirectory(prefix="sihc_build_") as folder:
+        objects = [Path(folder) / (source.stem + ".o") for source in SOURCES]
+        with ThreadPoolExecutor(len(SOURCES)) as pool:  # one compiler process per source
+            list(pool.map(lambda job: _run(compile_command(*job), verbose), zip(SOURCES, objects)))
+        _run(link_command(objects, tmp), verbose)
     os.replace(tmp, OUTPUT)
     tmp = SELFTEST.with_name(SELFTEST.name + ".tmp")
     _run(selftest_command(tmp), verbose)

@@ -1,0 +1,534 @@
+// Cross attention to states of another length, and its gradients.
+//
+//   S = scale q k^T over the first lengths[b] keys, P = softmax(S), O = P v
+//   dV = P^T dO;  dP = dO V^T;  dS = P (dP - rowsum(dO O));  dQ = scale dS K;  dK = scale dS^T Q
+//
+// Every product runs on the matrix cores in 32 x 32 tiles (bf16 32x32x16, fp32 32x32x2, fp32 sums).
+// A wave owns 32 rows of one side, one a lane pair, as the columns of its tiles: queries in the
+// forward and the query gradient, keys in the key and value gradients. The other side passes
+// through LDS in pieces that the block's waves share. The tile of scores then has its own row's
+// 32 values in the registers of two lanes, 16 each, so that the softmax needs one exchange per
+// tile, and the probabilities are already laid out as an operand of the next product, whose
+// contraction runs over them in the order the registers have (the other operand is read in the
+// same order). Transposed operands are read from LDS by the transposing load.
+//
+// The query rows of all heads that share a key head are one list of rows (head by head), so shared
+// heads fill tiles together, and their key gradients are one sum.
+//
+// Rounding: probabilities and score gradients enter their products in the inputs' type; scores,
+// statistics, sums and the row sums of dO O stay in fp32.
+#include "cond_common.h"
+
+namespace {
+using namespace sihc_cond;
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int PIECE = 64;  // rows of the other side in LDS at a time
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Args {
+  const void *q, *k, *v, *grad, *out;
+  void *o, *dq, *dk, *dv;
+  const int32_t* lengths;
+  float2* stats;
+  float* delta;  // [batch, heads, queries] rowsum(dO O)
+  int64_t qs[3], ks[3], vs[3];
+  int64_t batch;
+  int queries, keys, heads, shared, each, dim;
+  int64_t rows;   // query rows of a key head: each * queries
+  int64_t tiles;  // blocks of a key head
+  float scale;
+};
+
+// ------------------------------------------------------------------------------ fragments
+template <typename T, int DP>
+struct Lds {  // a piece in LDS: rows of DP channels (zeros past dim), padded against bank conflicts
+  static constexpr int STRIDE = DP + 16 / int(sizeof(T));
+  static constexpr int SIZE = PIECE * STRIDE + 32;  // (the last row's reads may run past its end)
+};
+template <int DP>
+constexpr int d_tiles() { return (DP + 31) / 32; }
+
+// A wave's own 32 rows as the right operand of a product over channels.
+template <typename T, int DP>
+struct Own;
+template <int DP>
+struct Own<bf16, DP> { bf16x8 v[DP / 16]; };
+template <int DP>
+struct Own<float, DP> { f32x4 v[DP / 8]; };
+
+// n elements of a row from p, as far as the row's `left` go, zeros past them.
+template <typename T, int N>
+__device__ __forceinline__ Vec<T, N> load_some(const T* p, int left) {
+  if (left >= N) return load<T, N>(p);
+  T e[N] = {};
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < left) e[i] = p[i];
+  Vec<T, N> v;
+  __builtin_memcpy(&v.raw, e, sizeof(e));
+  return v;
+}
+template <typename T, int DP>
+__device__ __forceinline__ void load_own(Own<T, DP>& own, const T* row, bool valid, int dim, int half) {
+  constexpr int N = 16 / int(sizeof(T));  // 8 or 4: the lane's channels of one step
+  constexpr int STEPS = DP / (2 * N);
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k) {
+    const int c = k * 2 * N + half * N;
+    const Vec<T, N> v = valid ? load_some<T, N>(row + c, dim - c) : Vec<T, N>::zero();
+    __builtin_memcpy(&own.v[k], &v.raw, 16);
+  }
+}
+
+// acc[r, own] = sum over channels of piece[r, c] own[c], r one of 32 rows from `piece`.
+template <int DP>
+__device__ __forceinline__ f32x16 rows_product(const bf16* piece, const Own<bf16, DP>& own, int lane, int half) {
+  f32x16 acc = {};
+  const bf16* p = piece + lane * Lds<bf16, DP>::STRIDE + half * 8;
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k)
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(p + k * 16), own.v[k], acc, 0, 0, 0);
+  return acc;
+}
+template <int DP>
+__device__ __forceinline__ f32x16 rows_product(const float* piece, const Own<float, DP>& own, int lane, int half) {
+  f32x16 acc = {};
+  const float* p = piece + lane * Lds<float, DP>::STRIDE + half * 4;
+#pragma unroll
+  for (int k = 0; k < DP / 8; ++k) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p + k * 8);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], own.v[k][j], acc, 0, 0, 0);
+  }
+  return acc;
+}
+// Row of a tile that register i of a lane's half holds.
+__device__ __forceinline__ constexpr int row_of(int i, int half) { return (i / 4) * 8 + half * 4 + i % 4; }
+
+// acc[t][c, own] += sum over the 32 rows r from `piece` of piece[r, 32 t + c] p[r, own].
+template <int DP>
+__device__ __forceinline__ void columns_product(f32x16* acc, const bf16* piece, const f32x16& p, int lane, int half) {
+  constexpr int S = Lds<bf16, DP>::STRIDE;
+  typedef __attribute__((address_space(3))) s16x4* LdsPtr;
+  const int j = lane & 15;
+  const bf16* at = piece + (half * 4 + j / 4) * S + (lane & 16) + (j % 4) * 4;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    bf16x8 b;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b[i] = static_cast<__bf16>(p[k * 8 + i]);
+#pragma unroll
+    for (int t = 0; t < d_tiles<DP>(); ++t) {
+      const bf16* low = at + k * 16 * S + t * 32;
+      const s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)low);
+      const s16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(low + 8 * S));
+      const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+      acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc[t], 0, 0, 0);
+    }
+  }
+}
+template <int DP>
+__device__ __forceinline__ void columns_product(f32x16* acc, const float* piece, const f32x16& p, int lane, int half) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+#pragma unroll
+    for (int t = 0; t < d_tiles<DP>(); ++t)
+      acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(piece[row_of(i, half) * Lds<float, DP>::STRIDE + t * 32 + lane], p[i],
+                                                    acc[t], 0, 0, 0);
+}
+
+// PIECE rows into LDS: row(r) is the address of row r < valid; zeros past them.
+template <typename T, int DP, int THREADS, typename Row>
+__device__ __forceinline__ void stage(T* lds, Row row, int valid, int dim) {
+  constexpr int N = 16 / int(sizeof(T)), VECS = DP / N;
+  for (int i = int(threadIdx.x); i < PIECE * VECS; i += THREADS) {
+    const int r = i / VECS, c = (i - r * VECS) * N;
+    const Vec<T, N> v = r < valid ? load_some<T, N>(row(r) + c, dim - c) : Vec<T, N>::zero();
+    *reinterpret_cast<u32x4*>(lds + r * Lds<T, DP>::STRIDE + c) = v.raw;
+  }
+}
+
+// A lane's row of sums (its registers hold 4 adjacent channels each), times f.
+template <typename T, int DP>
+__device__ __forceinline__ void store_row(T* row, const f32x16* acc, float f, int dim, int half) {
+#pragma unroll
+  for (int t = 0; t < d_tiles<DP>(); ++t)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int c = t * 32 + row_of(i, half);
+      float e[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) e[j] = acc[t][i + j] * f;
+      if (c + 4 <= dim) {
+        store<T, 4>(row + c, Vec<T, 4>::of(e));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (c + j < dim) row[c + j] = from_f32<T>(e[j]);
+      }
+    }
+}
+
+// ------------------------------------------------------------------------------ addresses
+struct Unit {  // what a block works on
+  int64_t b, tile;
+  int g;    // key head
+  int len;  // keys of the batch row
+};
+__device__ __forceinline__ Unit unit_of(const Args& a) {
+  const int64_t block = xcd_block(int(blockIdx.x), int(gridDim.x));
+  Unit u;
+  const int64_t bg = block / a.tiles;
+  u.tile = block - bg * a.tiles;
+  u.b = bg / a.shared;
+  u.g = int(bg - u.b * a.shared);
+  u.len = a.lengths ? min(max(a.lengths[u.b], 0), a.keys) : a.keys;
+  return u;
+}
+struct QueryRow {
+  int head, query;
+};
+__device__ __forceinline__ QueryRow query_row(const Args& a, const Unit& u, int64_t r) {
+  const uint32_t h = uint32_t(r) / uint32_t(a.queries);
+  return {u.g * a.each + int(h), int(uint32_t(r) - h * uint32_t(a.queries))};
+}
+template <typename T>
+__device__ __forceinline__ const T* q_at(const Args& a, const Unit& u, QueryRow r) {
+  return static_cast<const T*>(a.q) + u.b * a.qs[0] + r.query * a.qs[1] + r.head * a.qs[2];
+}
+__device__ __forceinline__ int64_t packed_q(const Args& a, const Unit& u, QueryRow r) {
+  return ((u.b * a.queries + r.query) * a.heads + r.head) * a.dim;
+}
+__device__ __forceinline__ int64_t stat_at(const Args& a, const Unit& u, QueryRow r) {
+  return (u.b * a.heads + r.head) * a.queries + r.query;
+}
+template <typename T>
+__device__ __forceinline__ const T* k_at(const Args& a, const Unit& u, int64_t key) {
+  return static_cast<const T*>(a.k) + u.b * a.ks[0] + key * a.ks[1] + u.g * a.ks[2];
+}
+template <typename T>
+__device__ __forceinline__ const T* v_at(const Args& a, const Unit& u, int64_t key) {
+  return static_cast<const T*>(a.v) + u.b * a.vs[0] + key * a.vs[1] + u.g * a.vs[2];
+}
+
+// -------------------------------------------------------------------------------- forward
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void k_attend(Args a) {
+  __shared__ __attribute__((aligned(16))) T lds_k[Lds<T, DP>::SIZE], lds_v[Lds<T, DP>::SIZE];
+  const Unit u = unit_of(a);
+  const int lane = int(threadIdx.x & 31), half = int(threadIdx.x >> 5 & 1), wave = int(threadIdx.x >> 6);
+  const int64_t r = u.tile * (NW * 32) + wave * 32 + lane;
+  const bool valid = r < a.rows;
+  const QueryRow qr = query_row(a, u, valid ? r : 0);
+  Own<T, DP> q;
+  load_own<T, DP>(q, q_at<T>(a, u, qr), valid, a.dim, half);
+  f32x16 o[d_tiles<DP>()] = {};
+  float top = -INFINITY, sum = 0.f;  // sum: of the keys of this lane's half
+  const float c = a.scale * LOG2E;
+  for (int k0 = 0; k0 < u.len; k0 += PIECE) {
+    const int here = min(PIECE, u.len - k0);
+    __syncthreads();
+    stage<T, DP, NW * 64>(lds_k, [&](int i) { return k_at<T>(a, u, k0 + i); }, here, a.dim);
+    stage<T, DP, NW * 64>(lds_v, [&](int i) { return v_at<T>(a, u, k0 + i); }, here, a.dim);
+    __syncthreads();
+    f32x16 s[2];
+    float most = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      s[t] = rows_product<DP>(lds_k + t * 32 * Lds<T, DP>::STRIDE, q, lane, half);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[t][i] = t * 32 + row_of(i, half) < here ? s[t][i] * c : -INFINITY;
+        most = fmaxf(most, s[t][i]);
+      }
+    }
+    most = fmaxf(most, __shfl_xor(most, 32));
+    const float now = fmaxf(top, most);
+    const float base = now == -INFINITY ? 0.f : now;  // (every score so far is -inf)
+    const float keep = __builtin_amdgcn_exp2f(top - base);
+    top = now;
+    sum *= keep;
+#pragma unroll
+    for (int t = 0; t < d_tiles<DP>(); ++t) o[t] *= keep;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - base);
+        sum += s[t][i];
+      }
+      columns_product<DP>(o, lds_v + t * 32 * Lds<T, DP>::STRIDE, s[t], lane, half);
+    }
+  }
+  sum += __shfl_xor(sum, 32);
+  if (!valid) return;
+  const float inverse = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // (NaN stays NaN)
+  store_row<T, DP>(static_cast<T*>(a.o) + packed_q(a, u, qr), o, inverse, a.dim, half);
+  if (a.stats && half == 0) a.stats[stat_at(a, u, qr)] = {top == -INFINITY ? 0.f : top, inverse};
+}
+
+// ------------------------------------------------------------------ gradient of the queries
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void k_attend_dq(Args a) {
+  __shared__ __attribute__((aligned(16))) T lds_k[Lds<T, DP>::SIZE], lds_v[Lds<T, DP>::SIZE];
+  const Unit u = unit_of(a);
+  const int lane = int(threadIdx.x & 31), half = int(threadIdx.x >> 5 & 1), wave = int(threadIdx.x >> 6);
+  const int64_t r = u.tile * (NW * 32) + wave * 32 + lane;
+  const bool valid = r < a.rows;
+  const QueryRow qr = query_row(a, u, valid ? r : 0);
+  Own<T, DP> q, g;
+  load_own<T, DP>(q, q_at<T>(a, u, qr), valid, a.dim, half);
+  load_own<T, DP>(g, static_cast<const T*>(a.grad) + packed_q(a, u, qr), valid, a.dim, half);
+  float delta = 0.f;
+  {
+    Own<T, DP> o;
+    load_own<T, DP>(o, static_cast<const T*>(a.out) + packed_q(a, u, qr), valid, a.dim, half);
+    constexpr int N = 16 / int(sizeof(T));
+#pragma unroll
+    for (int k = 0; k < DP / (2 * N); ++k)
+#pragma unroll
+      for (int i = 0; i < N; ++i) delta = fmaf(float(g.v[k][i]), float(o.v[k][i]), delta);
+    delta += __shfl_xor(delta, 32);
+  }
+  const float2 st = valid ? a.stats[stat_at(a, u, qr)] : float2{0.f, 0.f};
+  if (valid && half == 0) a.delta[stat_at(a, u, qr)] = delta;
+  f32x16 dq[d_tiles<DP>()] = {};
+  const float c = a.scale * LOG2E;
+  for (int k0 = 0; k0 < u.len; k0 += PIECE) {
+    const int here = min(PIECE, u.len - k0);
+    __syncthreads();
+    stage<T, DP, NW * 64>(lds_k, [&](int i) { return k_at<T>(a, u, k0 + i); }, here, a.dim);
+    stage<T, DP, NW * 64>(lds_v, [&](int i) { return v_at<T>(a, u, k0 + i); }, here, a.dim);
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const T* kp = lds_k + t * 32 * Lds<T, DP>::STRIDE;
+      f32x16 s = rows_product<DP>(kp, q, lane, half);
+      const f32x16 dp = rows_product<DP>(lds_v + t * 32 * Lds<T, DP>::STRIDE, g, lane, half);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float p = __builtin_amdgcn_exp2f(s[i] * c - st.x) * st.y;
+        s[i] = t * 32 + row_of(i, half) < here ? p * (dp[i] - delta) : 0.f;
+      }
+      columns_product<DP>(dq, kp, s, lane, half);
+    }
+  }
+  if (valid) store_row<T, DP>(static_cast<T*>(a.dq) + packed_q(a, u, qr), dq, a.scale, a.dim, half);
+}
+
+// --------------------------------------------------------- gradients of the keys and values
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void k_attend_dkv(Args a) {
+  __shared__ __attribute__((aligned(16))) T lds_q[Lds<T, DP>::SIZE], lds_g[Lds<T, DP>::SIZE];
+  __shared__ __attribute__((aligned(16))) float lds_top[PIECE], lds_inverse[PIECE], lds_delta[PIECE];
+  const Unit u = unit_of(a);
+  const int lane = int(threadIdx.x & 31), half = int(threadIdx.x >> 5 & 1), wave = int(threadIdx.x >> 6);
+  const int64_t key = u.tile * (NW * 32) + wave * 32 + lane;
+  const bool valid = key < u.len;
+  Own<T, DP> k, v;
+  load_own<T, DP>(k, k_at<T>(a, u, valid ? key : 0), valid, a.dim, half);
+  load_own<T, DP>(v, v_at<T>(a, u, valid ? key : 0), valid, a.dim, half);
+  f32x16 dk[d_tiles<DP>()] = {}, dv[d_tiles<DP>()] = {};
+  const float c = a.scale * LOG2E;
+  if (u.tile * (NW * 32) < u.len) {
+    for (int64_t r0 = 0; r0 < a.rows; r0 += PIECE) {
+      const int here = int(min(int64_t(PIECE), a.rows - r0));
+      __syncthreads();
+      stage<T, DP, NW * 64>(lds_q, [&](int i) { return q_at<T>(a, u, query_row(a, u, r0 + i)); }, here, a.dim);
+      stage<T, DP, NW * 64>(
+          lds_g, [&](int i) { return static_cast<const T*>(a.grad) + packed_q(a, u, query_row(a, u, r0 + i)); }, here,
+          a.dim);
+      for (int i = int(threadIdx.x); i < PIECE; i += NW * 64) {
+        float2 st = {0.f, 0.f};
+        float delta = 0.f;
+        if (i < here) {
+          const int64_t at = stat_at(a, u, query_row(a, u, r0 + i));
+          st = a.stats[at];
+          delta = a.delta[at];
+        }
+        lds_top[i] = st.x;
+        lds_inverse[i] = st.y;
+        lds_delta[i] = delta;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const T *qp = lds_q + t * 32 * Lds<T, DP>::STRIDE, *gp = lds_g + t * 32 * Lds<T, DP>::STRIDE;
+        f32x16 s = rows_product<DP>(qp, k, lane, half);
+        f32x16 dp = rows_product<DP>(gp, v, lane, half);
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const int row = t * 32 + row_of(i, half);
+          const f32x4 top = *reinterpret_cast<const f32x4*>(lds_top + row);
+          const f32x4 inverse = *reinterpret_cast<const f32x4*>(lds_inverse + row);
+          const f32x4 delta = *reinterpret_cast<const f32x4*>(lds_delta + row);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            s[i + j] = __builtin_amdgcn_exp2f(s[i + j] * c - top[j]) * inverse[j];
+            dp[i + j] = s[i + j] * (dp[i + j] - delta[j]);
+          }
+        }
+        columns_product<DP>(dv, gp, s, lane, half);
+        columns_product<DP>(dk, qp, dp, lane, half);
+      }
+    }
+  }
+  if (key >= a.keys) return;
+  if (!valid) {  // past the length: the sums of this lane's column mean nothing
+#pragma unroll
+    for (int t = 0; t < d_tiles<DP>(); ++t) dk[t] = dv[t] = f32x16{};
+  }
+  const int64_t at = ((u.b * a.keys + key) * a.shared + u.g) * a.dim;
+  store_row<T, DP>(static_cast<T*>(a.dk) + at, dk, a.scale, a.dim, half);
+  store_row<T, DP>(static_cast<T*>(a.dv) + at, dv, 1.f, a.dim, half);
+}
+
+// ---------------------------------------------------------------------------------- host
+int check_args(const char* what, const sihc_attention* a) {
+  if (!a) return fail(SIHC_ERR_INVALID, "%s: null sizes", what);
+  if (!valid_dtype(a->dtype)) return fail(SIHC_ERR_INVALID, "%s: bad dtype %d", what, a->dtype);
+  if (a->batch < 0 || a->queries < 0 || a->keys < 0 || a->heads <= 0 || a->kv_heads <= 0 || a->dim <= 0)
+    return fail(SIHC_ERR_INVALID, "%s: bad sizes", what);
+  if (a->heads % a->kv_heads)
+    return fail(SIHC_ERR_INVALID, "%s: %d query heads do not share %d key heads", what, a->heads, a->kv_heads);
+  if (a->dim > SIHC_MAX_HEAD_DIM)
+    return fail(SIHC_ERR_INVALID, "%s: heads of %d channels (at most %d)", what, a->dim, SIHC_MAX_HEAD_DIM);
+  // row lists and tiles are counted in int32; stats and packed offsets in int64
+  const int64_t rows = int64_t(a->queries) * (a->heads / a->kv_heads);
+  if (rows >= SIHC_MAX_TOKENS || a->keys >= SIHC_MAX_TOKENS ||
+      (a->batch && (rows / 32 + a->keys / 32 + 2) > 0x7fffffff / (a->batch * a->kv_heads)))
+    return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
+  return SIHC_OK;
+}
+Args args_of(const sihc_attention* s) {
+  Args a{};
+  for (int i = 0; i < 3; ++i) {
+    a.qs[i] = s->q_stride[i];
+    a.ks[i] = s->k_stride[i];
+    a.vs[i] = s->v_stride[i];
+  }
+  a.batch = s->batch;
+  a.queries = s->queries;
+  a.keys = s->keys;
+  a.heads = s->heads;
+  a.shared = s->kv_heads;
+  a.each = s->heads / s->kv_heads;
+  a.dim = s->dim;
+  a.rows = int64_t(a.each) * a.queries;
+  a.scale = s->scale;
+  return a;
+}
+// Calls f(T, DP): the smallest compiled width of a head.
+template <typename F>
+int by_width(const sihc_attention* s, F&& f) {
+  return by_dtype(s->dtype, [&](auto t) {
+    if (s->dim <= 32) return f(t, IC<32>{});
+    if (s->dim <= 64) return f(t, IC<64>{});
+    if (s->dim <= 80) return f(t, IC<80>{});
+    if (s->dim <= 96) return f(t, IC<96>{});
+    return f(t, IC<128>{});
+  });
+}
+// Calls f(NW) with the waves of a block over `rows` rows of its own side.
+template <typename F>
+int by_waves(int64_t rows, F&& f) {
+  return rows <= 32 ? f(IC<1>{}) : f(IC<4>{});
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t sihc_cross_attention_workspace_size(const sihc_attention*) { return 0; }
+
+int sihc_cross_attention(const sihc_attention* s, const void* q, const void* k, const void* v, const int32_t* lengths,
+                         void* out, float* stats, void*, size_t, void* stream) {
+  const char* what = "sihc_cross_attention";
+  if (int rc = check_args(what, s)) return rc;
+  if (s->batch == 0 || s->queries == 0) return SIHC_OK;
+  if (!q || !out || (s->keys && (!k || !v))) return fail(SIHC_ERR_INVALID, "%s: null pointer", what);
+  if (!aligned(stats, 8)) return fail(SIHC_ERR_INVALID, "%s: misaligned stats", what);
+  Args a = args_of(s);
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.lengths = lengths;
+  a.o = out;
+  a.stats = reinterpret_cast<float2*>(stats);
+  return by_width(s, [&](auto t, auto dp) {
+    return by_waves(a.rows, [&](auto nw) {
+      constexpr int NW = decltype(nw)::value;
+      a.tiles = ceil_div(a.rows, NW * 32);
+      hipLaunchKernelGGL((k_attend<decltype(t), decltype(dp)::value, NW>),
+                         dim3(unsigned(a.tiles * a.batch * a.shared)), dim3(NW * 64), 0,
+                         static_cast<hipStream_t>(stream), a);
+      return check_launch(what);
+    });
+  });
+}
+
+size_t sihc_cross_attention_backward_workspace_size(const sihc_attention* s) {
+  if (!s || s->batch <= 0 || s->queries <= 0 || s->heads <= 0) return 0;
+  return size_t(s->batch) * size_t(s->queries) * size_t(s->heads) * 4;
+}
+
+int sihc_cross_attention_backward(const sihc_attention* s, const void* grad, const void* q, const void* k,
+                                  const void* v, const int32_t* lengths, const void* out, const float* stats,
+                                  void* grad_q, void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+  const char* what = "sihc_cross_attention_backward";
+  if (int rc = check_args(what, s)) return rc;
+  if (s->batch == 0) return SIHC_OK;
+  if (s->queries && (!grad || !q || !out || !stats || !grad_q)) return fail(SIHC_ERR_INVALID, "%s: null pointer", what);
+  if (s->keys && (!k || !v || !grad_k || !grad_v)) return fail(SIHC_ERR_INVALID, "%s: null pointer", what);
+  for (const void* in : {grad, q, k, v, out})
+    for (const void* to : {grad_q, grad_k, grad_v})
+      if (in && in == to) return fail(SIHC_ERR_INVALID, "%s: an output is one of the inputs", what);
+  const size_t need = sihc_cross_attention_backward_workspace_size(s);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(SIHC_ERR_INVALID, "%s: workspace of %zu bytes required, got %zu", what, need, workspace_bytes);
+  if (!aligned(workspace, 16) || !aligned(stats, 8))
+    return fail(SIHC_ERR_INVALID, "%s: misaligned workspace or stats", what);
+  Args a = args_of(s);
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.grad = grad;
+  a.out = out;
+  a.dq = grad_q;
+  a.dk = grad_k;
+  a.dv = grad_v;
+  a.lengths = lengths;
+  a.stats = reinterpret_cast<float2*>(const_cast<float*>(stats));
+  a.delta = static_cast<float*>(workspace);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return by_width(s, [&](auto t, auto dp) {
+    using T = decltype(t);
+    constexpr int DP = decltype(dp)::value;
+    int rc = SIHC_OK;
+    if (a.queries)
+      rc = by_waves(a.rows, [&](auto nw) {
+        constexpr int NW = decltype(nw)::value;
+        a.tiles = ceil_div(a.rows, NW * 32);
+        hipLaunchKernelGGL((k_attend_dq<T, DP, NW>), dim3(unsigned(a.tiles * a.batch * a.shared)), dim3(NW * 64), 0, st,
+                           a);
+        return check_launch(what);
+      });
+    if (rc || !a.keys) return rc;
+    return by_waves(a.keys, [&](auto nw) {
+      constexpr int NW = decltype(nw)::value;
+      a.tiles = ceil_div(a.keys, NW * 32);
+      hipLaunchKernelGGL((k_attend_dkv<T, DP, NW>), dim3(unsigned(a.tiles * a.batch * a.shared)), dim3(NW * 64), 0, st,
+                         a);
+      return check_launch(what);
+    });
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,466 @@
+// Embedding lookup with scaling, and its table gradient by sorted tokens.
+//
+//   out[n, :]  = scale * table[id_n, :]
+//   grad[r, :] = scale * sum over n ascending with id_n = r of dout[n, :]
+//
+// Both are bound by memory: the lookup reads a row and writes a row per token, the gradient
+// reads the tokens' rows and writes the whole table's. Ids outside the table select its last
+// row in both (the host wrappers reject them), so no access can leave it.
+//
+// The gradient takes no atomics on values. Few tokens: every block owns a few table rows, lists
+// the tokens that select them in ascending order and sums their rows. Many tokens: the ids are
+// sorted, stably, by a radix sort of at most 10 bits a pass, and the sorted tokens are cut into
+// chunks of equal length, so that a frequent row costs no block more than a rare one: a wave
+// sums the runs of its chunk, stores the runs that end inside it, and leaves a partial row for
+// one that goes on, which a second kernel sums in ascending order.
+#include "cond_common.h"
+
+namespace {
+using namespace sihc_cond;
+
+constexpr int TILE = 2048;        // keys a block sorts in one pass, 8 a thread
+constexpr int CHUNK = 32;         // sorted tokens a wave sums
+constexpr int FEW_TOKENS = 1024;  // up to here the rows' tokens are listed by scanning all ids
+constexpr int FEW_ROWS = 8;       // table rows of a block there
+
+template <typename I>
+__device__ __forceinline__ uint32_t id_at(const I* ids, int64_t n, uint32_t rows) {
+  const uint64_t id = uint64_t(int64_t(ids[n]));  // a negative id is larger than any row
+  return id < rows ? uint32_t(id) : rows - 1u;
+}
+
+// ------------------------------------------------------------------------------- lookup
+// One vector a thread; the last vector of a row that V does not divide moves back to end with it.
+template <typename T, typename I, int V>
+__global__ __launch_bounds__(256) void k_embed(const T* __restrict__ table, const I* __restrict__ ids,
+                                               T* __restrict__ out, int64_t items, uint32_t rows, int C, int vecs,
+                                               float scale) {
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= items) return;
+  const int64_t n = items <= 0x7fffffff ? int64_t(uint32_t(i) / uint32_t(vecs)) : i / vecs;
+  const int c = min(int(i - n * vecs) * V, C - V);
+  float v[V];
+  load<T, V>(table + int64_t(id_at(ids, n, rows)) * C + c).to(v);
+#pragma unroll
+  for (int k = 0; k < V; ++k) v[k] *= scale;
+  store<T, V>(out + n * C + c, Vec<T, V>::of(v));
+}
+
+// ------------------------------------------------------------------- gradient, few tokens
+// Each thread owns an ascending run of the ids, so a prefix sum of the threads' matches lists the
+// block's tokens in ascending order.
+template <typename T, typename I, int V>
+__global__ __launch_bounds__(256) void k_embed_grad_few(const T* __restrict__ grad, const I* __restrict__ ids,
+                                                        T* __restrict__ out, int tokens, uint32_t rows, int C, int vecs,
+                                                        float scale, int64_t padding) {
+  __shared__ uint32_t list[FEW_TOKENS];  // token << 3 | row of the block
+  __shared__ int wave_total[4];
+  const int tid = int(threadIdx.x);
+  const uint32_t r0 = blockIdx.x * FEW_ROWS;
+  const int per = (tokens + 255) / 256, begin = min(tokens, tid * per), end = min(tokens, begin + per);
+  uint32_t found[FEW_TOKENS / 256];
+  int count = 0;
+#pragma unroll
+  for (int k = 0; k < FEW_TOKENS / 256; ++k) {
+    found[k] = ~0u;
+    if (begin + k < end) {
+      const uint32_t id = id_at(ids, begin + k, rows);
+      if (id - r0 < uint32_t(FEW_ROWS) && int64_t(id) != padding) {
+        found[k] = uint32_t(begin + k) << 3 | (id - r0);
+        ++count;
+      }
+    }
+  }
+  int before = count;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(before, d);
+    if ((tid & 63) >= d) before += o;
+  }
+  if ((tid & 63) == 63) wave_total[tid >> 6] = before;
+  __syncthreads();
+  int total = 0;
+  before -= count;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < (tid >> 6)) before += wave_total[w];
+    total += wave_total[w];
+  }
+#pragma unroll
+  for (int k = 0; k < FEW_TOKENS / 256; ++k)
+    if (found[k] != ~0u) list[before++] = found[k];
+  __syncthreads();
+  const int here = min(FEW_ROWS, int(rows - r0));
+  for (int item = tid; item < here * vecs; item += 256) {
+    const int row = item / vecs, c = min((item - row * vecs) * V, C - V);
+    float sum[V] = {};
+    for (int k = 0; k < total; ++k) {
+      if (int(list[k] & 7u) != row) continue;
+      float v[V];
+      load<T, V>(grad + int64_t(list[k] >> 3) * C + c).to(v);
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum[e] += v[e];
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) sum[e] *= scale;
+    store<T, V>(out + (int64_t(r0) + row) * C + c, Vec<T, V>::of(sum));
+  }
+}
+
+// ------------------------------------------------------------------------------ the sort
+// Keys of the first pass come from the ids: padding tokens get the key `rows`, which sorts last.
+template <typename I>
+struct IdKeys {
+  const I* ids;
+  uint32_t rows;
+  int64_t padding;
+  __device__ __forceinline__ u32x2 operator()(int64_t n) const {
+    const uint32_t id = id_at(ids, n, rows);
+    return u32x2{int64_t(id) == padding ? rows : id, uint32_t(n)};
+  }
+};
+struct PairKeys {
+  const u32x2* pairs;
+  __device__ __forceinline__ u32x2 operator()(int64_t n) const { return pairs[n]; }
+};
+
+// hist[tile][digit]: keys of the tile with that digit.
+template <typename K>
+__global__ __launch_bounds__(256) void k_sort_count(K keys, uint32_t* __restrict__ hist, int64_t n, int shift, int bins) {
+  __shared__ uint32_t h[1024];
+  for (int b = int(threadIdx.x); b < bins; b += 256) h[b] = 0;
+  __syncthreads();
+  const int64_t base = int64_t(blockIdx.x) * TILE;
+#pragma unroll
+  for (int k = 0; k < TILE / 256; ++k) {
+    const int64_t i = base + k * 256 + threadIdx.x;
+    if (i < n) atomicAdd(&h[(keys(i).x >> shift) & uint32_t(bins - 1)], 1u);
+  }
+  __syncthreads();
+  for (int b = int(threadIdx.x); b < bins; b += 256) hist[int64_t(blockIdx.x) * bins + b] = h[b];
+}
+
+// Where each tile's keys of each digit go: start[tile][digit] = keys of smaller digits + keys of
+// this digit in earlier tiles. One block; a thread owns one digit.
+__global__ __launch_bounds__(1024) void k_sort_scan(uint32_t* __restrict__ hist, int tiles, int bins) {
+  __shared__ uint32_t wave_total[16];
+  const int b = int(threadIdx.x), wave = b >> 6;
+  uint32_t total = 0;
+  if (b < bins)
+    for (int t = 0; t < tiles; ++t) {
+      const uint32_t c = hist[int64_t(t) * bins + b];
+      hist[int64_t(t) * bins + b] = total;
+      total += c;
+    }
+  uint32_t before = total;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t o = __shfl_up(before, d);
+    if ((b & 63) >= d) before += o;
+  }
+  if ((b & 63) == 63) wave_total[wave] = before;
+  __syncthreads();
+  before -= total;
+  for (int w = 0; w < wave; ++w) before += wave_total[w];
+  if (b < bins)
+    for (int t = 0; t < tiles; ++t) hist[int64_t(t) * bins + b] += before;
+}
+
+// Stable scatter of a tile: a wave takes 64 keys at a time in ascending order; a key's place among
+// its equals is the waves before, the wave's steps before, and the lanes before (a ballot a bit).
+template <typename K>
+__global__ __launch_bounds__(256) void k_sort_scatter(K keys, const uint32_t* __restrict__ start,
+                                                      u32x2* __restrict__ out, int64_t n, int shift, int bits) {
+  __shared__ uint32_t count[4][1024];
+  const int tid = int(threadIdx.x), wave = tid >> 6, lane = tid & 63, bins = 1 << bits;
+  for (int b = tid; b < 4 * 1024; b += 256) (&count[0][0])[b] = 0;
+  __syncthreads();
+  constexpr int STEPS = TILE / 256;
+  const int64_t base = int64_t(blockIdx.x) * TILE + wave * (TILE / 4);
+  u32x2 key[STEPS];
+  uint32_t rank[STEPS];
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k) {
+    const int64_t i = base + k * 64 + lane;
+    key[k] = i < n ? keys(i) : u32x2{0, 0};
+  }
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k) {
+    const bool valid = base + k * 64 + lane < n;
+    const uint32_t d = (key[k].x >> shift) & uint32_t(bins - 1);
+    uint64_t same = __ballot(valid);
+    for (int bit = 0; bit < bits; ++bit) {
+      const uint64_t set = __ballot((d >> bit) & 1u);
+      same &= (d >> bit) & 1u ? set : ~set;
+    }
+    const int below = __popcll(same & ((uint64_t(1) << lane) - 1));
+    uint32_t had = 0;
+    if (valid) had = count[wave][d];
+    rank[k] = had + uint32_t(below);
+    __builtin_amdgcn_wave_barrier();  // (the counters are this wave's own: LDS keeps its order)
+    if (valid && below == 0) count[wave][d] = had + uint32_t(__popcll(same));
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+  for (int b = tid; b < bins; b += 256) {
+    uint32_t at = start[int64_t(blockIdx.x) * bins + b];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t c = count[w][b];
+      count[w][b] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k)
+    if (base + k * 64 + lane < n) out[count[wave][(key[k].x >> shift) & uint32_t(bins - 1)] + rank[k]] = key[k];
+}
+
+// ----------------------------------------------------------------- gradient, sorted tokens
+__global__ __launch_bounds__(256) void k_zero(u32x4* __restrict__ p, int64_t n16, int64_t bytes) {
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n16; i += int64_t(gridDim.x) * 256) p[i] = u32x4{};
+  if (blockIdx.x == 0 && threadIdx.x < (bytes & 15)) reinterpret_cast<uint8_t*>(p + n16)[threadIdx.x] = 0;
+}
+
+// One wave: CHUNK sorted tokens x 64 vectors of the row. partial[chunk][0]: the run that the chunk
+// before began; [1]: the run that begins here and goes on in the next chunk. A run through the whole
+// chunk is [0].
+template <typename T, int V>
+__global__ __launch_bounds__(256) void k_embed_grad(const T* __restrict__ grad, const u32x2* __restrict__ sorted,
+                                                    T* __restrict__ out, float* __restrict__ partial, int64_t n,
+                                                    int64_t chunks, uint32_t rows, int C, int slices, float scale) {
+  const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t chunk = item / slices;
+  if (chunk >= chunks) return;
+  const int lane = int(threadIdx.x & 63), cb = (int(item - chunk * slices) * 64 + lane) * V;
+  const bool on = cb < C;
+  const int c = min(cb, C - V);
+  const int64_t first = chunk * CHUNK;
+  const int here = int(min(int64_t(CHUNK), n - first));
+  const u32x2 mine = sorted[first + min(lane, here - 1)];  // (lanes past CHUNK repeat the last)
+  const uint32_t prev = first ? sorted[first - 1].x : ~0u;
+  const uint32_t next = first + here < n ? sorted[first + here].x : ~0u;
+  float sum[V] = {};
+  bool head = __shfl(mine.x, 0) == prev;  // the run began before this chunk
+  for (int k0 = 0; k0 < here; k0 += 8) {
+    Vec<T, V> v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int k = min(k0 + j, here - 1);
+      v[j] = load<T, V>(grad + int64_t(__shfl(mine.y, k)) * C + c);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int k = k0 + j;
+      if (k >= here) break;
+      const uint32_t row = __shfl(mine.x, k);
+      float f[V];
+      v[j].to(f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum[e] += f[e];
+      const bool last = k + 1 == here;
+      const uint32_t after = last ? next : __shfl(mine.x, min(k + 1, 63));
+      if (after == row && !last) continue;
+      const bool goes_on = last && after == row;
+      if (on && row < rows) {
+        if (head || goes_on) {
+          float* p = partial + (chunk * 2 + (head ? 0 : 1)) * C + c;
+#pragma unroll
+          for (int e = 0; e < V; ++e) p[e] = sum[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) sum[e] *= scale;
+          store<T, V>(out + int64_t(row) * C + c, Vec<T, V>::of(sum));
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum[e] = 0.f;
+      head = false;
+    }
+  }
+}
+
+// The runs that cross chunks. A block looks at one chunk: where a run begins in it and goes on, its
+// partial rows of this chunk and the following ones are summed, by 4 thread rows over ascending
+// quarters of the run's chunks, then the quarters in order.
+template <typename T>
+__global__ __launch_bounds__(256) void k_embed_grad_runs(const u32x2* __restrict__ sorted,
+                                                         const float* __restrict__ partial, T* __restrict__ out,
+                                                         int64_t n, uint32_t rows, int C, float scale) {
+  __shared__ float quarter[4][64];
+  const int64_t chunk = blockIdx.x, edge = (chunk + 1) * CHUNK;
+  if (edge >= n) return;
+  const uint32_t row = sorted[edge - 1].x;
+  if (row >= rows || sorted[edge].x != row) return;                            // no run goes on
+  if (sorted[chunk * CHUNK].x == row && chunk && sorted[chunk * CHUNK - 1].x == row) return;  // it began before
+  int64_t low = edge + 1, high = n;  // first position past the run
+  while (low < high) {
+    const int64_t mid = (low + high) / 2;
+    if (sorted[mid].x == row) low = mid + 1;
+    else high = mid;
+  }
+  const int64_t last = (low - 1) / CHUNK, parts = last - chunk, each = (parts + 3) / 4;
+  const int lane = int(threadIdx.x & 63), q = int(threadIdx.x >> 6);
+  for (int c0 = 0; c0 < C; c0 += 64) {
+    const int c = min(c0 + lane, C - 1);
+    float sum = q == 0 ? partial[(chunk * 2 + 1) * C + c] : 0.f;
+    const int64_t begin = chunk + 1 + q * each, end = min(last + 1, begin + each);
+#pragma unroll 8
+    for (int64_t k = begin; k < end; ++k) sum += partial[k * 2 * C + c];
+    quarter[q][lane] = sum;
+    __syncthreads();
+    if (q == 0 && c0 + lane < C)
+      out[int64_t(row) * C + c] =
+          from_f32<T>(scale * (((quarter[0][lane] + quarter[1][lane]) + quarter[2][lane]) + quarter[3][lane]));
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------------- host
+// The widest vector of a row, at most 16 bytes and the row.
+int row_vec(int C, int elem) {
+  for (int v : {8, 4, 2})
+    if (v * elem <= 16 && v <= C) return v;
+  return 1;
+}
+template <typename F>
+int by_vec(int v, F&& f) {
+  switch (v) {
+    case 8: return f(IC<8>{});
+    case 4: return f(IC<4>{});
+    case 2: return f(IC<2>{});
+    default: return f(IC<1>{});
+  }
+}
+template <typename F>
+int by_id(int id_bits, F&& f) {
+  return id_bits == 32 ? f(int32_t{}) : f(int64_t{});
+}
+
+struct SortPlan {
+  int passes, bits;  // of at most 10 bits each
+  int64_t tiles, chunks;
+  size_t pairs_bytes, hist_bytes, partial_bytes;  // two pair arrays, one histogram, the partial rows
+  size_t total() const { return 2 * pairs_bytes + hist_bytes + partial_bytes; }
+};
+SortPlan sort_plan(int64_t tokens, int64_t rows, int C) {
+  SortPlan p{};
+  int bits = 1;
+  while ((int64_t(1) << bits) < rows + 1) ++bits;
+  p.passes = (bits + 9) / 10;
+  p.bits = (bits + p.passes - 1) / p.passes;
+  p.tiles = ceil_div(tokens, TILE);
+  p.chunks = ceil_div(tokens, CHUNK);
+  p.pairs_bytes = size_t(ceil_div(tokens * 8, 256)) * 256;
+  p.hist_bytes = size_t(ceil_div(p.tiles * (int64_t(4) << p.bits), 256)) * 256;
+  p.partial_bytes = size_t(p.chunks) * 2 * size_t(C) * 4;
+  return p;
+}
+
+int check_sizes(const char* what, int64_t tokens, int64_t rows, int C, int id_bits, int dtype) {
+  if (tokens < 0 || tokens >= SIHC_MAX_TOKENS || rows <= 0 || rows >= SIHC_MAX_TOKENS || C <= 0 || C > (1 << 24))
+    return fail(SIHC_ERR_INVALID, "%s: bad sizes", what);
+  if (id_bits != 32 && id_bits != 64) return fail(SIHC_ERR_INVALID, "%s: ids of %d bits (32 or 64)", what, id_bits);
+  if (!valid_dtype(dtype)) return fail(SIHC_ERR_INVALID, "%s: bad dtype %d", what, dtype);
+  return SIHC_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int sihc_embedding(const void* table, const void* ids, void* out, int64_t tokens, int64_t rows, int channels,
+                   float scale, int id_bits, int dtype, void* stream) {
+  const char* what = "sihc_embedding";
+  if (int rc = check_sizes(what, tokens, rows, channels, id_bits, dtype)) return rc;
+  if (tokens == 0) return SIHC_OK;
+  if (!table || !ids || !out) return fail(SIHC_ERR_INVALID, "%s: null pointer", what);
+  return by_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    return by_id(id_bits, [&](auto i) {
+      using I = decltype(i);
+      return by_vec(row_vec(channels, int(sizeof(T))), [&](auto v) {
+        constexpr int V = decltype(v)::value;
+        if constexpr (V * sizeof(T) <= 16) {
+          const int vecs = int(ceil_div(channels, V));
+          const int64_t items = tokens * vecs, blocks = ceil_div(items, 256);
+          if (blocks > 0x7fffffff) return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
+          hipLaunchKernelGGL((k_embed<T, I, V>), dim3(unsigned(blocks)), dim3(256), 0, static_cast<hipStream_t>(stream),
+                             static_cast<const T*>(table), static_cast<const I*>(ids), static_cast<T*>(out), items,
+                             uint32_t(rows), channels, vecs, scale);
+        }
+        return check_launch(what);
+      });
+    });
+  });
+}
+
+size_t sihc_embedding_backward_workspace_size(int64_t tokens, int64_t rows, int channels) {
+  if (tokens <= FEW_TOKENS || rows <= 0 || channels <= 0) return 0;
+  return sort_plan(tokens, rows, channels).total();
+}
+
+int sihc_embedding_backward(const void* grad, const void* ids, void* grad_table, int64_t tokens, int64_t rows,
+                            int channels, float scale, int64_t padding, int id_bits, int dtype, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  const char* what = "sihc_embedding_backward";
+  if (int rc = check_sizes(what, tokens, rows, channels, id_bits, dtype)) return rc;
+  if (!grad_table || (tokens && (!grad || !ids))) return fail(SIHC_ERR_INVALID, "%s: null pointer", what);
+  if (grad_table == grad || grad_table == ids) return fail(SIHC_ERR_INVALID, "%s: an output is one of the inputs", what);
+  const size_t need = sihc_embedding_backward_workspace_size(tokens, rows, channels);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(SIHC_ERR_INVALID, "%s: workspace of %zu bytes required, got %zu", what, need, workspace_bytes);
+  if (need && !aligned(workspace, 16)) return fail(SIHC_ERR_INVALID, "%s: workspace must be 16-byte aligned", what);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return by_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    return by_id(id_bits, [&](auto i) {
+      using I = decltype(i);
+      return by_vec(row_vec(channels, int(sizeof(T))), [&](auto v) {
+        constexpr int V = decltype(v)::value;
+        if constexpr (V * sizeof(T) <= 16) {
+          const int vecs = int(ceil_div(channels, V));
+          const T* g = static_cast<const T*>(grad);
+          const I* id = static_cast<const I*>(ids);
+          T* out = static_cast<T*>(grad_table);
+          if (tokens <= FEW_TOKENS) {
+            hipLaunchKernelGGL((k_embed_grad_few<T, I, V>), dim3(unsigned(ceil_div(rows, FEW_ROWS))), dim3(256), 0, st, g,
+                               id, out, int(tokens), uint32_t(rows), channels, vecs, scale, padding);
+            return check_launch(what);
+          }
+          const SortPlan p = sort_plan(tokens, rows, channels);
+          char* w = static_cast<char*>(workspace);
+          u32x2* pairs[2] = {reinterpret_cast<u32x2*>(w), reinterpret_cast<u32x2*>(w + p.pairs_bytes)};
+          uint32_t* hist = reinterpret_cast<uint32_t*>(w + 2 * p.pairs_bytes);
+          float* partial = reinterpret_cast<float*>(w + 2 * p.pairs_bytes + p.hist_bytes);
+          const int64_t bytes = rows * channels * int64_t(sizeof(T));
+          // (an output that is not 16-byte aligned is cleared by its leading bytes first)
+          if (!aligned(out, 16)) return fail(SIHC_ERR_INVALID, "%s: grad_table must be 16-byte aligned", what);
+          hipLaunchKernelGGL(k_zero, dim3(unsigned(std::min<int64_t>(ceil_div(bytes, 4096) + 1, 256 * 16))), dim3(256), 0,
+                             st, reinterpret_cast<u32x4*>(out), bytes / 16, bytes);
+          const dim3 grid(static_cast<unsigned>(p.tiles));
+          auto pass = [&](auto keys, u32x2* to, int shift) {
+            using K = decltype(keys);
+            hipLaunchKernelGGL(k_sort_count<K>, grid, dim3(256), 0, st, keys, hist, tokens, shift, 1 << p.bits);
+            hipLaunchKernelGGL(k_sort_scan, dim3(1), dim3(1024), 0, st, hist, int(p.tiles), 1 << p.bits);
+            hipLaunchKernelGGL(k_sort_scatter<K>, grid, dim3(256), 0, st, keys, hist, to, tokens, shift, p.bits);
+          };
+          pass(IdKeys<I>{id, uint32_t(rows), padding}, pairs[0], 0);
+          for (int k = 1; k < p.passes; ++k) pass(PairKeys{pairs[(k + 1) & 1]}, pairs[k & 1], k * p.bits);
+          const u32x2* sorted = pairs[(p.passes - 1) & 1];
+          const int slices = int(ceil_div(vecs, 64));
+          const int64_t blocks = ceil_div(p.chunks * slices, 4);
+          if (blocks > 0x7fffffff) return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
+          hipLaunchKernelGGL((k_embed_grad<T, V>), dim3(unsigned(blocks)), dim3(256), 0, st, g, sorted, out, partial,
+                             tokens, p.chunks, uint32_t(rows), channels, slices, scale);
+          hipLaunchKernelGGL(k_embed_grad_runs<T>, dim3(unsigned(p.chunks)), dim3(256), 0, st, sorted, partial, out,
+                             tokens, uint32_t(rows), channels, scale);
+        }
+        return check_launch(what);
+      });
+    });
+  });
+}
+
+}  // extern "C"

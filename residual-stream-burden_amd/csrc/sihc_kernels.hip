@@ -4322,6 +4322,12 @@ int scratch_address(const char* what, void** out) {
 
 }  // namespace
 
+// The error record of the library's other files (cond_common.h).
+__attribute__((visibility("hidden"))) int sihc_record_error(int code, const char* message) {
+  g_last_error = message;
+  return code;
+}
+
 // ==================================================================================
 // C ABI
 // ==================================================================================

@@ -6,11 +6,14 @@ Modules
   blockwise_kernels  drop-in for the reference's block-wise adapters
   event_ops          per-event fused write+read (literal schedule) with autograd
   indexed            spatially indexed (int32 state index) gather/scatter and read/write
+  conditioning       embedding lookup, cross attention and group norm with an activation: what
+                     conditions a denoiser on an encoder's states
   launch             tensor-level launchers over the C ABI (include/sihc_hip.h)
 """
 from ._lib import LIB_PATH, lib  # noqa: F401
 from .sublayer_kernels import sublayer_read, sublayer_triangular, sublayer_write  # noqa: F401
 from .event_ops import event_write_read, literal_stage  # noqa: F401
+from .conditioning import cross_attention, embedding_lookup, group_norm_act  # noqa: F401
 
 __all__ = ["LIB_PATH", "lib", "sublayer_read", "sublayer_write", "sublayer_triangular",
-           "event_write_read", "literal_stage"]
+           "event_write_read", "literal_stage", "embedding_lookup", "cross_attention", "group_norm_act"]

@@ -10,16 +10,31 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().with_name("libsihc_hip.so")
-ABI_VERSION = 6
+ABI_VERSION = 7
 MAX_EVENTS = 32
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+ACT_NONE = 0
+ACT_SILU = 1
+MAX_HEAD_DIM = 128
 
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int
 _i64 = ctypes.c_int64
 _sz = ctypes.c_size_t
 _vpp = ctypes.POINTER(ctypes.c_void_p)
+
+
+class Attention(ctypes.Structure):
+    """sihc_attention of include/sihc_hip.h."""
+    _fields_ = [("batch", ctypes.c_int64), ("queries", ctypes.c_int), ("keys", ctypes.c_int),
+                ("heads", ctypes.c_int), ("kv_heads", ctypes.c_int), ("dim", ctypes.c_int),
+                ("q_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3),
+                ("v_stride", ctypes.c_int64 * 3), ("scale", ctypes.c_float), ("dtype", ctypes.c_int)]
+
+
+_f32 = ctypes.c_float
+_attp = ctypes.POINTER(Attention)
 
 # name -> (restype, argtypes); mirrors include/sihc_hip.h one for one.
 PROTOTYPES: dict[str, tuple] = {
@@ -59,6 +74,20 @@ PROTOTYPES: dict[str, tuple] = {
     "sihc_stream": (_i32, [_vpp, _i32, _vpp, _i32, _sz, _i32, _vp]),
     "sihc_stream_mix": (_i32, [_vpp, _i32, _i32, _vpp, _i32, _i32, _i32, _sz, _vp, _vp]),
     "sihc_copy": (_i32, [_vp, _vp, _sz, _vp]),
+    "sihc_embedding": (_i32, [_vp, _vp, _vp, _i64, _i64, _i32, _f32, _i32, _i32, _vp]),
+    "sihc_embedding_backward_workspace_size": (_sz, [_i64, _i64, _i32]),
+    "sihc_embedding_backward": (_i32, [_vp, _vp, _vp, _i64, _i64, _i32, _f32, _i64, _i32, _i32, _vp, _sz, _vp]),
+    "sihc_group_norm_workspace_size": (_sz, [_i64, _i64, _i32, _i32, _i32]),
+    "sihc_group_norm": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _f32, _i32, _i32, _i32, _vp, _sz,
+                               _vp]),
+    "sihc_group_norm_backward_workspace_size": (_sz, [_i64, _i64, _i32, _i32, _i32]),
+    "sihc_group_norm_backward": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _i32,
+                                        _i32, _vp, _sz, _vp]),
+    "sihc_cross_attention_workspace_size": (_sz, [_attp]),
+    "sihc_cross_attention": (_i32, [_attp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "sihc_cross_attention_backward_workspace_size": (_sz, [_attp]),
+    "sihc_cross_attention_backward": (_i32, [_attp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
+                                             _vp]),
     "sihc_fma_rate": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp]),
 }
 

@@ -16,9 +16,10 @@ from typing import Optional, Sequence
 import torch
 from torch import Tensor
 
-from ._lib import DTYPE_BF16, DTYPE_F32, MAX_EVENTS, check, lib, ptr_array
+from ._lib import ACT_NONE, ACT_SILU, DTYPE_BF16, DTYPE_F32, MAX_EVENTS, Attention, check, lib, ptr_array
 
 _DTYPES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
+ACTIVATIONS = {"none": ACT_NONE, "silu": ACT_SILU}
 
 
 def dtype_code(dtype: torch.dtype) -> int:
@@ -293,8 +294,104 @@ def copy_(dst: Tensor, src: Tensor) -> Tensor:
     return dst
 
 
+def _id_bits(ids: Tensor) -> int:
+    return 32 if ids.dtype == torch.int32 else 64
+
+
+@_on_tensor_device
+def embedding(table: Tensor, ids: Tensor, scale: float) -> Tensor:
+    """scale * table[ids] as [*ids.shape, C]."""
+    out = torch.empty((*ids.shape, table.shape[1]), device=table.device, dtype=table.dtype)
+    check(lib().sihc_embedding(table.data_ptr(), ids.data_ptr(), out.data_ptr(), ids.numel(), *table.shape, scale,
+                               _id_bits(ids), dtype_code(table.dtype), _stream(table.device)))
+    return out
+
+
+@_on_tensor_device
+def embedding_backward(grad: Tensor, ids: Tensor, rows: int, scale: float, padding: int) -> Tensor:
+    """The whole table's gradient [rows, C]: zero where no id selects a row, and for row `padding`."""
+    channels = grad.shape[-1]
+    out = torch.empty((rows, channels), device=grad.device, dtype=grad.dtype)
+    L = lib()
+    ws = _workspace(L.sihc_embedding_backward_workspace_size(ids.numel(), rows, channels), grad.device)
+    check(L.sihc_embedding_backward(grad.data_ptr(), ids.data_ptr(), out.data_ptr(), ids.numel(), rows, channels,
+                                    scale, padding, _id_bits(ids), dtype_code(grad.dtype), ws.data_ptr(),
+                                    ws.numel() * 4, _stream(grad.device)))
+    return out
+
+
+def _pixels(x: Tensor) -> int:
+    return x[0, ..., 0].numel() if x.shape[0] else 0
+
+
+@_on_tensor_device
+def group_norm(x: Tensor, weight: Tensor, bias: Tensor, groups: int, eps: float,
+               act: str) -> tuple[Tensor, Tensor]:
+    """(act(group norm of x [B,...,C]), [B,groups,2] means and reciprocal deviations)."""
+    batch, pixels, channels = x.shape[0], _pixels(x), x.shape[-1]
+    out = torch.empty_like(x)
+    stats = torch.empty((batch, groups, 2), device=x.device, dtype=torch.float32)
+    L, code = lib(), dtype_code(x.dtype)
+    nbytes = L.sihc_group_norm_workspace_size(batch, pixels, channels, groups, code)
+    ws = _workspace(nbytes, x.device) if nbytes else None
+    check(L.sihc_group_norm(x.data_ptr(), weight.data_ptr(), bias.data_ptr(), out.data_ptr(), stats.data_ptr(), batch,
+                            pixels, channels, groups, eps, ACTIVATIONS[act], code, dtype_code(weight.dtype), _ptr(ws),
+                            nbytes, _stream(x.device)))
+    return out, stats
+
+
+@_on_tensor_device
+def group_norm_backward(grad: Tensor, x: Tensor, weight: Tensor, bias: Tensor, stats: Tensor, groups: int,
+                        act: str) -> tuple[Tensor, Tensor, Tensor]:
+    """(input gradient, weight gradient, bias gradient) of group_norm."""
+    batch, pixels, channels = x.shape[0], _pixels(x), x.shape[-1]
+    dx, dw, db = torch.empty_like(x), torch.empty_like(weight), torch.empty_like(bias)
+    L, code = lib(), dtype_code(x.dtype)
+    ws = _workspace(L.sihc_group_norm_backward_workspace_size(batch, pixels, channels, groups, code), x.device)
+    check(L.sihc_group_norm_backward(grad.data_ptr(), x.data_ptr(), weight.data_ptr(), bias.data_ptr(),
+                                     stats.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(), batch, pixels,
+                                     channels, groups, ACTIVATIONS[act], code, dtype_code(weight.dtype),
+                                     ws.data_ptr(), ws.numel() * 4, _stream(x.device)))
+    return dx, dw, db
+
+
+def _attention(q: Tensor, k: Tensor, v: Tensor, scale: float) -> Attention:
+    strides = [(ctypes.c_int64 * 3)(*t.stride()[:3]) for t in (q, k, v)]
+    return Attention(q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3], *strides, scale,
+                     dtype_code(q.dtype))
+
+
+@_on_tensor_device
+def cross_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor],
+                    scale: float) -> tuple[Tensor, Tensor]:
+    """(attention of q [B,Lq,H,D] over k, v [B,Lk,KH,D], [B,H,Lq,2] softmax statistics)."""
+    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    stats = torch.empty((q.shape[0], q.shape[2], q.shape[1], 2), device=q.device, dtype=torch.float32)
+    L, a = lib(), _attention(q, k, v, scale)
+    nbytes = L.sihc_cross_attention_workspace_size(ctypes.byref(a))
+    ws = _workspace(nbytes, q.device) if nbytes else None
+    check(L.sihc_cross_attention(ctypes.byref(a), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(lengths),
+                                 out.data_ptr(), stats.data_ptr(), _ptr(ws), nbytes, _stream(q.device)))
+    return out, stats
+
+
+@_on_tensor_device
+def cross_attention_backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor], out: Tensor,
+                             stats: Tensor, scale: float) -> tuple[Tensor, Tensor, Tensor]:
+    """(query, key, value gradients) of cross_attention, packed."""
+    dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
+    L, a = lib(), _attention(q, k, v, scale)
+    ws = _workspace(L.sihc_cross_attention_backward_workspace_size(ctypes.byref(a)), q.device)
+    check(L.sihc_cross_attention_backward(ctypes.byref(a), grad.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                          _ptr(lengths), out.data_ptr(), stats.data_ptr(), dq.data_ptr(),
+                                          dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws.numel() * 4,
+                                          _stream(q.device)))
+    return dq, dk, dv
+
+
 __all__ = [
-    "MAX_EVENTS", "dtype_code", "carrier_geometry", "read", "write", "weight_grad", "read_backward",
+    "MAX_EVENTS", "ACTIVATIONS", "embedding", "embedding_backward", "group_norm", "group_norm_backward",
+    "cross_attention", "cross_attention_backward", "dtype_code", "carrier_geometry", "read", "write", "weight_grad", "read_backward",
     "write_backward", "triangular",
     "triangular_gamma_grad", "triangular_backward", "event_forward", "event_backward", "gather_cells",
     "scatter_cells", "scatter_add_cells", "copy_",
