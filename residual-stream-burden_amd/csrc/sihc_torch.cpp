@@ -1,14 +1,14 @@
 // Native dispatch of the eager `sihc::` ops.
 //
-// The Python custom ops (sihc_hip/sublayer_kernels.py, event_ops.py, indexed.py, kernels.py)
-// cost 50-120 us of interpreter and dispatcher time per forward and backward pair, more than
-// the kernels of a small or ordinary call take. Each function here takes the arguments of one
+// The Python custom ops (sihc_hip/sublayer_kernels.py, event_ops.py, indexed.py, kernels.py,
+// conditioning.py) cost 50-150 us of interpreter and dispatcher time per forward and backward pair,
+// more than the kernels of a small or ordinary call take. Each function here takes the arguments of one
 // of those ops and, where the call is plain, allocates the outputs, enqueues the C-ABI call on
 // the current stream and records one C++ autograd node whose backward does the same.
 //
-// Plain means: exactly the tensors and shapes that the op accepts, all packed, dense, on one
-// GPU and not empty, of type torch.Tensor or torch.nn.Parameter, and nothing in force that has
-// to see the op: no dispatch or function mode (tracing, fake tensors, selective checkpointing),
+// Plain means: exactly the tensors and shapes that the op accepts, all packed (attention: with
+// adjacent channels), dense, on one GPU and not empty, of type torch.Tensor or
+// torch.nn.Parameter, and nothing in force that has to see the op: no dispatch or function mode (tracing, fake tensors, selective checkpointing),
 // no functorch transform, no forward-mode tangent, and no kernel or autocast rule that the
 // program registered for the op itself. Anything else returns NotImplemented and
 // the caller runs the Python op, which validates, raises and composes as it always did. The
@@ -59,15 +59,16 @@ bool plain_mode() {
   if (!(tls.included_ - c10::default_included_set).empty()) return false;
   return !at::impl::torch_function_mode_enabled();
 }
-bool plain(const Tensor& t) {
+bool plain_strided(const Tensor& t) {
   static const c10::DispatchKeySet special({c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot,
                                             c10::DispatchKey::FuncTorchBatched,
                                             c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize,
                                             c10::DispatchKey::Conjugate, c10::DispatchKey::Negative,
                                             c10::DispatchKey::ZeroTensor});
   return t.defined() && t.is_cuda() && t.layout() == c10::kStrided && !t.is_quantized() && !t.is_nested() &&
-         !t.key_set().has_any(special) && t.is_contiguous() && !t._fw_grad(0).defined();
+         !t.key_set().has_any(special) && !t._fw_grad(0).defined();
 }
+bool plain(const Tensor& t) { return plain_strided(t) && t.is_contiguous(); }
 bool below_autograd() {
   const auto tls = c10::impl::tls_local_dispatch_key_set();
   return tls.excluded_.has(c10::DispatchKey::AutogradCUDA);
@@ -167,6 +168,41 @@ bool scatter_fits(const Tensor& cells, const Tensor& index) {
   return s.grid * s.grid == cells.size(1) && index_shape(index, cells, s);
 }
 
+bool embed_fits(const Tensor& table, const Tensor& ids) {
+  return plain(table) && plain(ids) && table.dim() == 2 && table.numel() != 0 && ids.numel() != 0 &&
+         dtype_code(table) >= 0 && (ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong) &&
+         ids.device() == table.device() && table.size(1) < (int64_t(1) << 31);
+}
+bool norm_fits(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t groups) {
+  if (!plain(x) || !plain(weight) || !plain(bias) || x.dim() < 2 || x.numel() == 0 || dtype_code(x) < 0) return false;
+  const int64_t c = x.size(-1);
+  if (groups < 1 || c % groups || c >= (int64_t(1) << 31)) return false;
+  for (const Tensor* w : {&weight, &bias})
+    if (w->dim() != 1 || w->size(0) != c || w->device() != x.device() || w->scalar_type() != weight.scalar_type())
+      return false;
+  return weight.scalar_type() == x.scalar_type() || weight.scalar_type() == at::kFloat;
+}
+bool attention_fits(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths) {
+  for (const Tensor* t : {&q, &k, &v})
+    if (!plain_strided(*t) || t->dim() != 4 || t->numel() == 0 || t->scalar_type() != q.scalar_type() ||
+        t->device() != q.device() || (t->size(3) > 1 && t->stride(3) != 1) || t->size(1) >= (int64_t(1) << 31) ||
+        t->size(2) >= (int64_t(1) << 31))
+      return false;
+  if (dtype_code(q) < 0 || !k.sizes().equals(v.sizes()) || k.size(0) != q.size(0) || k.size(3) != q.size(3) ||
+      q.size(3) > SIHC_MAX_HEAD_DIM || q.size(2) % k.size(2))
+    return false;
+  return !lengths.defined() || (plain(lengths) && lengths.scalar_type() == at::kInt && lengths.dim() == 1 &&
+                                lengths.size(0) == q.size(0) && lengths.device() == q.device());
+}
+// `t` is a packed tensor like `like` (an output gradient, a saved output).
+bool same(const Tensor& t, const Tensor& like) {
+  return plain(t) && t.sizes().equals(like.sizes()) && t.scalar_type() == like.scalar_type() &&
+         t.device() == like.device();
+}
+bool stats_fits(const Tensor& t, at::IntArrayRef sizes, const Tensor& like) {
+  return plain(t) && t.sizes().equals(sizes) && t.scalar_type() == at::kFloat && t.device() == like.device();
+}
+
 // ----------------------------------------------------------------------- the C-ABI calls
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream(); }
 void check(int rc, bool forward) {
@@ -256,6 +292,8 @@ auto registered(const char* name) {
 }
 // A backward may launch directly: nothing recorded or in force (its operands are asked apart).
 bool direct() { return !at::GradMode::is_enabled() && plain_mode(); }
+
+std::optional<Tensor> maybe(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 
 // What a profiler sees of a call: the op's name and its arguments (made only if one looks).
 using Args = std::vector<c10::IValue>;
@@ -559,6 +597,184 @@ struct ScatterFn : torch::autograd::Function<ScatterFn> {
   }
 };
 
+// ------------------------------------------------------------------ conditioning operators
+int id_bits(const Tensor& ids) { return ids.scalar_type() == at::kInt ? 32 : 64; }
+Tensor run_embed(const Tensor& table, const Tensor& ids, double scale) {
+  const c10::DeviceGuard guard(table.device());
+  std::vector<int64_t> sizes(ids.sizes().begin(), ids.sizes().end());
+  sizes.push_back(table.size(1));
+  Tensor out = at::empty(sizes, table.options());
+  check(sihc_embedding(table.const_data_ptr(), ids.const_data_ptr(), out.data_ptr(), ids.numel(), table.size(0),
+                       int(table.size(1)), float(scale), id_bits(ids), dtype_code(table), stream_of(table)),
+        true);
+  return out;
+}
+struct EmbedFn : torch::autograd::Function<EmbedFn> {
+  static constexpr bool is_traceable = true;
+  static Tensor forward(AutogradContext* ctx, const Tensor& table, const Tensor& ids, double scale, int64_t padding) {
+    ctx->save_for_backward({ids});
+    ctx->saved_data["rows"] = table.size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    return run_embed(table, ids, scale);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor ids = ctx->get_saved_variables()[0], grad = grads[0].contiguous();
+    const int64_t rows = ctx->saved_data["rows"].toInt(), padding = ctx->saved_data["padding"].toInt();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    Tensor out;
+    if (direct() && plain(ids) && plain(grad) && grad.dim() == ids.dim() + 1 && grad.numel() != 0 &&
+        grad.sizes().slice(0, size_t(ids.dim())).equals(ids.sizes()) && dtype_code(grad) >= 0 &&
+        (ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong) && ids.device() == grad.device()) {
+      RECORD_FUNCTION("sihc::embedding_lookup_backward", (Args{grad, ids, rows, scale, padding}));
+      const c10::DeviceGuard device(grad.device());
+      const int c = int(grad.size(-1));
+      out = at::empty({rows, c}, grad.options());
+      const Tensor ws = workspace(sihc_embedding_backward_workspace_size(ids.numel(), rows, c), grad);
+      check(sihc_embedding_backward(grad.const_data_ptr(), ids.const_data_ptr(), out.data_ptr(), ids.numel(), rows, c,
+                                    float(scale), padding, id_bits(ids), dtype_code(grad), ws.data_ptr(),
+                                    size_t(ws.numel()) * 4, stream_of(grad)),
+            false);
+    } else {
+      static auto op = registered<Tensor(const Tensor&, const Tensor&, int64_t, double, int64_t)>(
+          "sihc::embedding_lookup_backward");
+      out = op.call(grad, ids, rows, scale, padding);
+    }
+    return {out, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+int64_t pixels_of(const Tensor& x) { return x.numel() / (x.size(0) * x.size(-1)); }
+int act_code(const std::string& act) { return act == "silu" ? SIHC_ACT_SILU : SIHC_ACT_NONE; }
+variable_list run_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t groups, double eps,
+                       const std::string& act) {
+  const c10::DeviceGuard guard(x.device());
+  const int64_t b = x.size(0), n = pixels_of(x);
+  const int c = int(x.size(-1)), g = int(groups);
+  Tensor y = at::empty_like(x), stats = at::empty({b, groups, 2}, x.options().dtype(at::kFloat)), ws;
+  const size_t bytes = sihc_group_norm_workspace_size(b, n, c, g, dtype_code(x));
+  if (bytes) ws = workspace(bytes, x);
+  check(sihc_group_norm(x.const_data_ptr(), weight.const_data_ptr(), bias.const_data_ptr(), y.data_ptr(),
+                        stats.data_ptr<float>(), b, n, c, g, float(eps), act_code(act), dtype_code(x),
+                        dtype_code(weight), bytes ? ws.data_ptr() : nullptr, bytes, stream_of(x)),
+        true);
+  return {y, stats};
+}
+struct NormFn : torch::autograd::Function<NormFn> {
+  static constexpr bool is_traceable = true;
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& bias,
+                               int64_t groups, double eps, const std::string& act) {
+    variable_list out = run_norm(x, weight, bias, groups, eps, act);
+    ctx->mark_non_differentiable({out[1]});
+    ctx->save_for_backward({x, weight, bias, out[1]});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["act"] = act;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &stats = saved[3];
+    const Tensor grad = grads[0].contiguous();
+    const int64_t groups = ctx->saved_data["groups"].toInt();
+    const std::string act = ctx->saved_data["act"].toStringRef();
+    Tensor dx, dw, db;
+    if (direct() && norm_fits(x, weight, bias, groups) && same(grad, x) &&
+        stats_fits(stats, {x.size(0), groups, 2}, x)) {
+      RECORD_FUNCTION("sihc::group_norm_act_backward", (Args{grad, x, weight, bias, stats, groups, act}));
+      const c10::DeviceGuard device(x.device());
+      const int64_t b = x.size(0), n = pixels_of(x);
+      const int c = int(x.size(-1)), g = int(groups);
+      dx = at::empty_like(x);
+      dw = at::empty_like(weight);
+      db = at::empty_like(bias);
+      const Tensor ws = workspace(sihc_group_norm_backward_workspace_size(b, n, c, g, dtype_code(x)), x);
+      check(sihc_group_norm_backward(grad.const_data_ptr(), x.const_data_ptr(), weight.const_data_ptr(),
+                                     bias.const_data_ptr(), stats.const_data_ptr<float>(), dx.data_ptr(),
+                                     dw.data_ptr(), db.data_ptr(), b, n, c, g, act_code(act), dtype_code(x),
+                                     dtype_code(weight), ws.data_ptr(), size_t(ws.numel()) * 4, stream_of(x)),
+            false);
+    } else {
+      static auto op = registered<std::tuple<Tensor, Tensor, Tensor>(
+          const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, int64_t, c10::string_view)>(
+          "sihc::group_norm_act_backward");
+      std::tie(dx, dw, db) = op.call(grad, x, weight, bias, stats, groups, act);
+    }
+    return {dx, dw, db, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+sihc_attention attention_of(const Tensor& q, const Tensor& k, const Tensor& v, double scale) {
+  sihc_attention a{};
+  a.batch = q.size(0);
+  a.queries = int(q.size(1));
+  a.keys = int(k.size(1));
+  a.heads = int(q.size(2));
+  a.kv_heads = int(k.size(2));
+  a.dim = int(q.size(3));
+  for (int i = 0; i < 3; ++i) {
+    a.q_stride[i] = q.stride(i);
+    a.k_stride[i] = k.stride(i);
+    a.v_stride[i] = v.stride(i);
+  }
+  a.scale = float(scale);
+  a.dtype = dtype_code(q);
+  return a;
+}
+variable_list run_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths, double scale) {
+  const c10::DeviceGuard guard(q.device());
+  const sihc_attention a = attention_of(q, k, v, scale);
+  Tensor out = at::empty(q.sizes(), q.options()), ws;
+  Tensor stats = at::empty({q.size(0), q.size(2), q.size(1), 2}, q.options().dtype(at::kFloat));
+  const size_t bytes = sihc_cross_attention_workspace_size(&a);
+  if (bytes) ws = workspace(bytes, q);
+  check(sihc_cross_attention(&a, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), index_ptr(lengths),
+                             out.data_ptr(), stats.data_ptr<float>(), bytes ? ws.data_ptr() : nullptr, bytes,
+                             stream_of(q)),
+        true);
+  return {out, stats};
+}
+struct AttentionFn : torch::autograd::Function<AttentionFn> {
+  static constexpr bool is_traceable = true;
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                               const std::optional<Tensor>& lengths, double scale) {
+    const Tensor n = lengths.value_or(Tensor());
+    variable_list out = run_attention(q, k, v, n, scale);
+    ctx->mark_non_differentiable({out[1]});
+    ctx->save_for_backward({q, k, v, n, out[0], out[1]});
+    ctx->saved_data["scale"] = scale;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &n = saved[3], &out = saved[4], &stats = saved[5];
+    const Tensor grad = grads[0].contiguous();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    Tensor dq, dk, dv;
+    if (direct() && attention_fits(q, k, v, n) && same(grad, out) && grad.sizes().equals(q.sizes()) &&
+        grad.scalar_type() == q.scalar_type() && grad.device() == q.device() &&
+        stats_fits(stats, {q.size(0), q.size(2), q.size(1), 2}, q)) {
+      RECORD_FUNCTION("sihc::cross_attention_backward", (Args{grad, q, k, v, maybe(n), out, stats, scale}));
+      const c10::DeviceGuard device(q.device());
+      const sihc_attention a = attention_of(q, k, v, scale);
+      dq = at::empty(q.sizes(), q.options());
+      dk = at::empty(k.sizes(), k.options());
+      dv = at::empty(v.sizes(), v.options());
+      const Tensor ws = workspace(sihc_cross_attention_backward_workspace_size(&a), q);
+      check(sihc_cross_attention_backward(&a, grad.const_data_ptr(), q.const_data_ptr(), k.const_data_ptr(),
+                                          v.const_data_ptr(), index_ptr(n), out.const_data_ptr(),
+                                          stats.const_data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                          ws.data_ptr(), size_t(ws.numel()) * 4, stream_of(q)),
+            false);
+    } else {
+      static auto op = registered<std::tuple<Tensor, Tensor, Tensor>(
+          const Tensor&, const Tensor&, const Tensor&, const Tensor&, const std::optional<Tensor>&, const Tensor&,
+          const Tensor&, double)>("sihc::cross_attention_backward");
+      std::tie(dq, dk, dv) = op.call(grad, q, k, v, maybe(n), out, stats, scale);
+    }
+    return {dq, dk, dv, Tensor(), Tensor()};
+  }
+};
+
 // ------------------------------------------------------------------------ Python entries
 PyObject* to_list(const variable_list& ts) {
   PyObject* out = PyList_New(Py_ssize_t(ts.size()));
@@ -615,7 +831,6 @@ auto call(PyObject* self, A&& args, F&& f) {
 }
 // Below autograd (a custom op's own body, inference mode) and under no_grad nothing is recorded.
 bool unrecorded() { return !at::GradMode::is_enabled() || below_autograd(); }
-std::optional<Tensor> maybe(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 
 PyObject* read_impl(PyObject* self, PyObject* const* args, bool indexed) {
   return guarded(self, [&]() -> PyObject* {
@@ -734,6 +949,73 @@ PyObject* py_scatter(PyObject* self, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
+bool unwrap_number(PyObject* o, double& v) {
+  if (!PyFloat_CheckExact(o) && !PyLong_CheckExact(o)) return false;
+  v = PyFloat_AsDouble(o);
+  if (!PyErr_Occurred()) return true;
+  PyErr_Clear();
+  return false;
+}
+bool unwrap_integer(PyObject* o, int64_t& v) {
+  if (!PyLong_CheckExact(o)) return false;
+  v = PyLong_AsLongLong(o);
+  if (!PyErr_Occurred()) return true;
+  PyErr_Clear();
+  return false;
+}
+PyObject* pair_of(const variable_list& ts) {
+  PyObject* pair = PyTuple_New(2);
+  for (int i = 0; pair && i < 2; ++i) PyTuple_SET_ITEM(pair, i, THPVariable_Wrap(ts[size_t(i)]));
+  return pair;
+}
+PyObject* py_embed(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  if (n != 4) return not_implemented();
+  return guarded(self, [&]() -> PyObject* {
+    Tensor table, ids;
+    double scale;
+    int64_t padding;
+    if (!unwrap(args[0], table) || !unwrap(args[1], ids) || !unwrap_number(args[2], scale) ||
+        !unwrap_integer(args[3], padding) || !embed_fits(table, ids))
+      return not_implemented();
+    return THPVariable_Wrap(call(self, [&] { return Args{table, ids, scale, padding}; }, [&] {
+      return unrecorded() ? run_embed(table, ids, scale) : EmbedFn::apply(table, ids, scale, padding);
+    }));
+  });
+}
+PyObject* py_norm(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  if (n != 6 || !PyUnicode_CheckExact(args[5])) return not_implemented();
+  const bool silu = PyUnicode_CompareWithASCIIString(args[5], "silu") == 0;
+  if (!silu && PyUnicode_CompareWithASCIIString(args[5], "none") != 0) return not_implemented();
+  const std::string act = silu ? "silu" : "none";
+  return guarded(self, [&]() -> PyObject* {
+    Tensor x, weight, bias;
+    int64_t groups;
+    double eps;
+    if (!unwrap(args[0], x) || !unwrap(args[1], weight) || !unwrap(args[2], bias) ||
+        !unwrap_integer(args[3], groups) || !unwrap_number(args[4], eps) || !norm_fits(x, weight, bias, groups))
+      return not_implemented();
+    return pair_of(call(self, [&] { return Args{x, weight, bias, groups, eps, act}; }, [&] {
+      return unrecorded() ? run_norm(x, weight, bias, groups, eps, act)
+                          : NormFn::apply(x, weight, bias, groups, eps, act);
+    }));
+  });
+}
+PyObject* py_attention(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  if (n != 5) return not_implemented();
+  return guarded(self, [&]() -> PyObject* {
+    Tensor q, k, v, lengths;
+    double scale;
+    if (!unwrap(args[0], q) || !unwrap(args[1], k) || !unwrap(args[2], v) ||
+        (args[3] != Py_None && !unwrap(args[3], lengths)) || !unwrap_number(args[4], scale) ||
+        !attention_fits(q, k, v, lengths))
+      return not_implemented();
+    return pair_of(call(self, [&] { return Args{q, k, v, maybe(lengths), scale}; }, [&] {
+      return unrecorded() ? run_attention(q, k, v, lengths, scale)
+                          : AttentionFn::apply(q, k, v, maybe(lengths), scale);
+    }));
+  });
+}
+
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyMethodDef define(const char* name) {
   return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F)), METH_FASTCALL, nullptr};
@@ -743,7 +1025,8 @@ PyMethodDef entries[] = {
     define<py_triangular>("sublayer_triangular"), define<py_event>("event_write_read"),
     define<py_indexed_read>("indexed_read"), define<py_indexed_write>("indexed_write"),
     define<py_block_write>("block_write"),   define<py_gather>("gather_cells"),
-    define<py_scatter>("scatter_cells"),
+    define<py_scatter>("scatter_cells"),     define<py_embed>("embedding_lookup"),
+    define<py_norm>("group_norm_act"),       define<py_attention>("cross_attention"),
 };
 // entry(name, op): the native entry `name` for the registered op `op` ("namespace::name")
 PyObject* py_entry(PyObject*, PyObject* args) {

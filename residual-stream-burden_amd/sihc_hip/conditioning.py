@@ -32,6 +32,7 @@ from torch.library import custom_op, register_autograd
 
 from . import launch
 from ._lib import MAX_HEAD_DIM
+from ._native import native
 from .sublayer_kernels import _require_packed
 
 _TYPES = (torch.float32, torch.bfloat16)
@@ -91,6 +92,7 @@ def _embedding_autograd(ctx, grad):
 
 
 register_autograd(_embedding_lookup, _embedding_autograd, setup_context=_embedding_setup)
+native(_embedding_lookup, "embedding_lookup")
 
 
 def embedding_lookup(table: Tensor, ids: Tensor, scale: float = 1.0, padding_idx: Optional[int] = None, *,
@@ -166,6 +168,7 @@ def _norm_autograd(ctx, grad, _):
 
 
 register_autograd(_group_norm_act, _norm_autograd, setup_context=_norm_setup)
+native(_group_norm_act, "group_norm_act")
 
 
 def group_norm_act(x: Tensor, weight: Tensor, bias: Tensor, groups: int = 32, eps: float = 1e-6,
@@ -239,6 +242,7 @@ def _attention_autograd(ctx, grad, _):
 
 
 register_autograd(_cross_attention, _attention_autograd, setup_context=_attention_setup)
+native(_cross_attention, "cross_attention")
 
 
 def cross_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor] = None,
