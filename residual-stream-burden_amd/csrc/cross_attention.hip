@@ -41,8 +41,14 @@ struct Args {
   int64_t batch;
   int queries, keys, heads, shared, each, dim;
   int64_t rows;   // query rows of a key head: each * queries
-  int64_t tiles;  // blocks of a key head
+  int64_t tiles;  // blocks of a key head (in the forward, of one part of its keys)
+  int splits, span;  // the forward's parts of the keys, and their keys (a multiple of PIECE)
+  float* part_o;     // [splits][batch, key head][rows][dim] sums, where there are several parts
+  float2* part_s;    // their largest scores and sums
   float scale;
+  bool fast;               // (Piece)
+  uint32_t magic;  // r / queries is the high word of r * magic, shifted right (0: r shifted right)
+  int shift;
 };
 
 // ------------------------------------------------------------------------------ fragments
@@ -143,16 +149,46 @@ __device__ __forceinline__ void columns_product(f32x16* acc, const float* piece,
                                                     acc[t], 0, 0, 0);
 }
 
-// PIECE rows into LDS: row(r) is the address of row r < valid; zeros past them.
-template <typename T, int DP, int THREADS, typename Row>
-__device__ __forceinline__ void stage(T* lds, Row row, int valid, int dim) {
-  constexpr int N = 16 / int(sizeof(T)), VECS = DP / N;
-  for (int i = int(threadIdx.x); i < PIECE * VECS; i += THREADS) {
-    const int r = i / VECS, c = (i - r * VECS) * N;
-    const Vec<T, N> v = r < valid ? load_some<T, N>(row(r) + c, dim - c) : Vec<T, N>::zero();
-    *reinterpret_cast<u32x4*>(lds + r * Lds<T, DP>::STRIDE + c) = v.raw;
+// PIECE rows on their way to LDS: loaded into registers while the piece before is worked on. Heads of
+// whole 16-byte vectors whose rows lie within 32-bit offsets of `base` (Args::fast) load without
+// branches, from places that exist, so that all loads are in flight at once; others are loaded when
+// they are stored. offset(r) is the byte offset of row r of the piece; rows past `valid` and channels
+// past dim are zeros.
+template <typename T, int DP, int THREADS>
+struct Piece {
+  static constexpr int N = 16 / int(sizeof(T)), VECS = DP / N, COUNT = (PIECE * VECS + THREADS - 1) / THREADS;
+  Vec<T, N> v[COUNT];
+  template <typename Offset>
+  __device__ __forceinline__ void fetch(const void* base, Offset offset, int valid, int dim) {
+    const char* from = static_cast<const char*>(base);
+#pragma unroll
+    for (int k = 0; k < COUNT; ++k) {
+      const int i = int(threadIdx.x) + k * THREADS, r = i / VECS, c = (i - r * VECS) * N;
+      const uint32_t at = offset(min(r, valid - 1)) + uint32_t(min(c, dim - N)) * uint32_t(sizeof(T));
+      v[k] = load<T, N>(reinterpret_cast<const T*>(from + at));
+    }
+#pragma unroll
+    for (int k = 0; k < COUNT; ++k) {
+      const int i = int(threadIdx.x) + k * THREADS, r = i / VECS, c = (i - r * VECS) * N;
+      if (r >= valid || c >= dim) v[k] = Vec<T, N>::zero();
+    }
   }
-}
+  __device__ __forceinline__ void commit(T* lds) const {
+#pragma unroll
+    for (int k = 0; k < COUNT; ++k) {
+      const int i = int(threadIdx.x) + k * THREADS, r = i / VECS, c = (i - r * VECS) * N;
+      if (PIECE * VECS % THREADS == 0 || r < PIECE) *reinterpret_cast<u32x4*>(lds + r * Lds<T, DP>::STRIDE + c) = v[k].raw;
+    }
+  }
+  template <typename Row>
+  __device__ static void copy(T* lds, Row row, int valid, int dim) {
+    for (int i = int(threadIdx.x); i < PIECE * VECS; i += THREADS) {
+      const int r = i / VECS, c = (i - r * VECS) * N;
+      const Vec<T, N> v = r < valid ? load_some<T, N>(row(r) + c, dim - c) : Vec<T, N>::zero();
+      *reinterpret_cast<u32x4*>(lds + r * Lds<T, DP>::STRIDE + c) = v.raw;
+    }
+  }
+};
 
 // A lane's row of sums (its registers hold 4 adjacent channels each), times f.
 template <typename T, int DP>
@@ -178,14 +214,16 @@ __device__ __forceinline__ void store_row(T* row, const f32x16* acc, float f, in
 // ------------------------------------------------------------------------------ addresses
 struct Unit {  // what a block works on
   int64_t b, tile;
+  int split;
   int g;    // key head
   int len;  // keys of the batch row
 };
 __device__ __forceinline__ Unit unit_of(const Args& a) {
   const int64_t block = xcd_block(int(blockIdx.x), int(gridDim.x));
   Unit u;
-  const int64_t bg = block / a.tiles;
-  u.tile = block - bg * a.tiles;
+  const int64_t part = block / a.tiles, bg = part / a.splits;
+  u.tile = block - part * a.tiles;
+  u.split = int(part - bg * a.splits);
   u.b = bg / a.shared;
   u.g = int(bg - u.b * a.shared);
   u.len = a.lengths ? min(max(a.lengths[u.b], 0), a.keys) : a.keys;
@@ -197,6 +235,10 @@ struct QueryRow {
 __device__ __forceinline__ QueryRow query_row(const Args& a, const Unit& u, int64_t r) {
   const uint32_t h = uint32_t(r) / uint32_t(a.queries);
   return {u.g * a.each + int(h), int(uint32_t(r) - h * uint32_t(a.queries))};
+}
+// r / queries, without a division.
+__device__ __forceinline__ uint32_t fast_query_head(const Args& a, uint32_t r) {
+  return a.magic ? uint32_t((uint64_t(r) * a.magic) >> 32) >> a.shift : r >> a.shift;
 }
 template <typename T>
 __device__ __forceinline__ const T* q_at(const Args& a, const Unit& u, QueryRow r) {
@@ -217,9 +259,11 @@ __device__ __forceinline__ const T* v_at(const Args& a, const Unit& u, int64_t k
   return static_cast<const T*>(a.v) + u.b * a.vs[0] + key * a.vs[1] + u.g * a.vs[2];
 }
 
+// Blocks of several waves are compiled for two waves on a SIMD where their tiles fit 256 registers: the
+// softmax of one wave then runs beside the products of the other.
 // -------------------------------------------------------------------------------- forward
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64) void k_attend(Args a) {
+__global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 384 ? 2 : 1) void k_attend(Args a) {
   __shared__ __attribute__((aligned(16))) T lds_k[Lds<T, DP>::SIZE], lds_v[Lds<T, DP>::SIZE];
   const Unit u = unit_of(a);
   const int lane = int(threadIdx.x & 31), half = int(threadIdx.x >> 5 & 1), wave = int(threadIdx.x >> 6);
@@ -228,34 +272,56 @@ __global__ __launch_bounds__(NW * 64) void k_attend(Args a) {
   const QueryRow qr = query_row(a, u, valid ? r : 0);
   Own<T, DP> q;
   load_own<T, DP>(q, q_at<T>(a, u, qr), valid, a.dim, half);
+  const float c = a.scale * LOG2E;
   f32x16 o[d_tiles<DP>()] = {};
   float top = -INFINITY, sum = 0.f;  // sum: of the keys of this lane's half
-  const float c = a.scale * LOG2E;
-  for (int k0 = 0; k0 < u.len; k0 += PIECE) {
-    const int here = min(PIECE, u.len - k0);
+  const int begin = u.split * a.span, end = min(u.len, begin + a.span);
+  Piece<T, DP, NW * 64> pk, pv;
+  auto fetch = [&](int k0) {
+    const int here = min(PIECE, end - k0);
+    const uint32_t ks = uint32_t(a.ks[1]) * uint32_t(sizeof(T)), vs = uint32_t(a.vs[1]) * uint32_t(sizeof(T));
+    pk.fetch(k_at<T>(a, u, k0), [&](int i) { return uint32_t(i) * ks; }, here, a.dim);
+    pv.fetch(v_at<T>(a, u, k0), [&](int i) { return uint32_t(i) * vs; }, here, a.dim);
+  };
+  if (a.fast && begin < end) fetch(begin);
+  for (int k0 = begin; k0 < end; k0 += PIECE) {
+    const int here = min(PIECE, end - k0);
     __syncthreads();
-    stage<T, DP, NW * 64>(lds_k, [&](int i) { return k_at<T>(a, u, k0 + i); }, here, a.dim);
-    stage<T, DP, NW * 64>(lds_v, [&](int i) { return v_at<T>(a, u, k0 + i); }, here, a.dim);
+    if (a.fast) {
+      pk.commit(lds_k);
+      pv.commit(lds_v);
+    } else {
+      Piece<T, DP, NW * 64>::copy(lds_k, [&](int i) { return k_at<T>(a, u, k0 + i); }, here, a.dim);
+      Piece<T, DP, NW * 64>::copy(lds_v, [&](int i) { return v_at<T>(a, u, k0 + i); }, here, a.dim);
+    }
     __syncthreads();
+    if (a.fast && k0 + PIECE < end) fetch(k0 + PIECE);
     f32x16 s[2];
     float most = -INFINITY;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       s[t] = rows_product<DP>(lds_k + t * 32 * Lds<T, DP>::STRIDE, q, lane, half);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[t][i] = t * 32 + row_of(i, half) < here ? s[t][i] * c : -INFINITY;
-        most = fmaxf(most, s[t][i]);
-      }
+      s[t] *= c;
     }
-    most = fmaxf(most, __shfl_xor(most, 32));
-    const float now = fmaxf(top, most);
-    const float base = now == -INFINITY ? 0.f : now;  // (every score so far is -inf)
-    const float keep = __builtin_amdgcn_exp2f(top - base);
-    top = now;
-    sum *= keep;
+    if (here < PIECE) {
 #pragma unroll
-    for (int t = 0; t < d_tiles<DP>(); ++t) o[t] *= keep;
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (t * 32 + row_of(i, half) >= here) s[t][i] = -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) most = fmaxf(most, fmaxf(s[0][i], s[1][i]));
+    most = fmaxf(most, __shfl_xor(most, 32));
+    if (__any(most > top)) {  // a new largest score: rescale what was summed under the old one
+      const float now = fmaxf(top, most);
+      const float keep = __builtin_amdgcn_exp2f(now == -INFINITY ? 0.f : top - now);
+      top = now;
+      sum *= keep;
+#pragma unroll
+      for (int t = 0; t < d_tiles<DP>(); ++t) o[t] *= keep;
+    }
+    const float base = top == -INFINITY ? 0.f : top;  // (every score so far is -inf)
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
@@ -268,14 +334,62 @@ __global__ __launch_bounds__(NW * 64) void k_attend(Args a) {
   }
   sum += __shfl_xor(sum, 32);
   if (!valid) return;
+  if (a.splits > 1) {
+    const int64_t row = ((int64_t(u.split) * a.batch + u.b) * a.shared + u.g) * a.rows + r;
+    if (half == 0) a.part_s[row] = {top, sum};
+    if (begin < end) store_row<float, DP>(a.part_o + row * a.dim, o, 1.f, a.dim, half);
+    return;
+  }
   const float inverse = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // (NaN stays NaN)
   store_row<T, DP>(static_cast<T*>(a.o) + packed_q(a, u, qr), o, inverse, a.dim, half);
   if (a.stats && half == 0) a.stats[stat_at(a, u, qr)] = {top == -INFINITY ? 0.f : top, inverse};
 }
 
+// The parts of a row, brought under their largest score and summed in ascending order; one wave a row.
+template <typename T>
+__global__ __launch_bounds__(256) void k_attend_join(Args a, int64_t total) {
+  const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (row >= total) return;
+  const int lane = int(threadIdx.x & 63);
+  const int64_t bg = row / a.rows;
+  Unit u;
+  u.b = bg / a.shared;
+  u.g = int(bg - u.b * a.shared);
+  const QueryRow qr = query_row(a, u, row - bg * a.rows);
+  // a lane's parts: their largest score, and what each one's sums are worth under it
+  float top = -INFINITY;
+  for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, a.part_s[s * total + row].x);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+  const float base = top == -INFINITY ? 0.f : top;
+  float sum = 0.f, o[2] = {};
+  for (int s0 = 0; s0 < a.splits; s0 += 64) {
+    const int mine = s0 + lane;
+    const float2 p = mine < a.splits ? a.part_s[mine * total + row] : float2{-INFINITY, 0.f};
+    const float worth = p.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(p.x - base);
+    const int here = min(64, a.splits - s0);
+#pragma unroll 4
+    for (int k = 0; k < here; ++k) {
+      const float w = __shfl(worth, k), part = __shfl(p.y, k);
+      sum += w * part;
+      if (part == 0.f) continue;  // (a part past the length: its sums were not written)
+      const float* from = a.part_o + ((s0 + k) * total + row) * a.dim;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (lane + e * 64 < a.dim) o[e] = fmaf(w, from[lane + e * 64], o[e]);
+    }
+  }
+  const float inverse = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+  T* to = static_cast<T*>(a.o) + packed_q(a, u, qr);
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (lane + e * 64 < a.dim) to[lane + e * 64] = from_f32<T>(o[e] * inverse);
+  if (a.stats && lane == 0) a.stats[stat_at(a, u, qr)] = {base, inverse};
+}
+
 // ------------------------------------------------------------------ gradient of the queries
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64) void k_attend_dq(Args a) {
+__global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 320 ? 2 : 1) void k_attend_dq(Args a) {
   __shared__ __attribute__((aligned(16))) T lds_k[Lds<T, DP>::SIZE], lds_v[Lds<T, DP>::SIZE];
   const Unit u = unit_of(a);
   const int lane = int(threadIdx.x & 31), half = int(threadIdx.x >> 5 & 1), wave = int(threadIdx.x >> 6);
@@ -300,12 +414,26 @@ __global__ __launch_bounds__(NW * 64) void k_attend_dq(Args a) {
   if (valid && half == 0) a.delta[stat_at(a, u, qr)] = delta;
   f32x16 dq[d_tiles<DP>()] = {};
   const float c = a.scale * LOG2E;
+  Piece<T, DP, NW * 64> pk, pv;
+  auto fetch = [&](int k0) {
+    const int here = min(PIECE, u.len - k0);
+    const uint32_t ks = uint32_t(a.ks[1]) * uint32_t(sizeof(T)), vs = uint32_t(a.vs[1]) * uint32_t(sizeof(T));
+    pk.fetch(k_at<T>(a, u, k0), [&](int i) { return uint32_t(i) * ks; }, here, a.dim);
+    pv.fetch(v_at<T>(a, u, k0), [&](int i) { return uint32_t(i) * vs; }, here, a.dim);
+  };
+  if (a.fast && u.len) fetch(0);
   for (int k0 = 0; k0 < u.len; k0 += PIECE) {
     const int here = min(PIECE, u.len - k0);
     __syncthreads();
-    stage<T, DP, NW * 64>(lds_k, [&](int i) { return k_at<T>(a, u, k0 + i); }, here, a.dim);
-    stage<T, DP, NW * 64>(lds_v, [&](int i) { return v_at<T>(a, u, k0 + i); }, here, a.dim);
+    if (a.fast) {
+      pk.commit(lds_k);
+      pv.commit(lds_v);
+    } else {
+      Piece<T, DP, NW * 64>::copy(lds_k, [&](int i) { return k_at<T>(a, u, k0 + i); }, here, a.dim);
+      Piece<T, DP, NW * 64>::copy(lds_v, [&](int i) { return v_at<T>(a, u, k0 + i); }, here, a.dim);
+    }
     __syncthreads();
+    if (a.fast && k0 + PIECE < u.len) fetch(k0 + PIECE);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const T* kp = lds_k + t * 32 * Lds<T, DP>::STRIDE;
@@ -324,7 +452,7 @@ __global__ __launch_bounds__(NW * 64) void k_attend_dq(Args a) {
 
 // --------------------------------------------------------- gradients of the keys and values
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64) void k_attend_dkv(Args a) {
+__global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= (sizeof(T) == 2 ? 192 : 256) ? 2 : 1) void k_attend_dkv(Args a) {
   __shared__ __attribute__((aligned(16))) T lds_q[Lds<T, DP>::SIZE], lds_g[Lds<T, DP>::SIZE];
   __shared__ __attribute__((aligned(16))) float lds_top[PIECE], lds_inverse[PIECE], lds_delta[PIECE];
   const Unit u = unit_of(a);
@@ -337,26 +465,51 @@ __global__ __launch_bounds__(NW * 64) void k_attend_dkv(Args a) {
   f32x16 dk[d_tiles<DP>()] = {}, dv[d_tiles<DP>()] = {};
   const float c = a.scale * LOG2E;
   if (u.tile * (NW * 32) < u.len) {
+    Piece<T, DP, NW * 64> pq, pg;
+    float2 st = {0.f, 0.f};  // the statistics of the row that this thread stages
+    float delta = 0.f;
+    const T* grad = static_cast<const T*>(a.grad);
+    const void* q0 = q_at<T>(a, u, {u.g * a.each, 0});
+    const void* g0 = grad + packed_q(a, u, {u.g * a.each, 0});
+    const uint32_t size = sizeof(T), qt = uint32_t(a.qs[1]) * size, qh = uint32_t(a.qs[2]) * size,
+                   gt = uint32_t(a.heads * a.dim) * size, gh = uint32_t(a.dim) * size;
+    auto fetch = [&](int64_t r0) {
+      const int here = int(min(int64_t(PIECE), a.rows - r0));
+      auto offset = [&](int i, uint32_t token, uint32_t head) {
+        const uint32_t r = uint32_t(r0) + uint32_t(i), h = fast_query_head(a, r);
+        return (r - h * uint32_t(a.queries)) * token + h * head;
+      };
+      pq.fetch(q0, [&](int i) { return offset(i, qt, qh); }, here, a.dim);
+      pg.fetch(g0, [&](int i) { return offset(i, gt, gh); }, here, a.dim);
+    };
+    if (a.fast && a.rows) fetch(0);
     for (int64_t r0 = 0; r0 < a.rows; r0 += PIECE) {
       const int here = int(min(int64_t(PIECE), a.rows - r0));
-      __syncthreads();
-      stage<T, DP, NW * 64>(lds_q, [&](int i) { return q_at<T>(a, u, query_row(a, u, r0 + i)); }, here, a.dim);
-      stage<T, DP, NW * 64>(
-          lds_g, [&](int i) { return static_cast<const T*>(a.grad) + packed_q(a, u, query_row(a, u, r0 + i)); }, here,
-          a.dim);
-      for (int i = int(threadIdx.x); i < PIECE; i += NW * 64) {
-        float2 st = {0.f, 0.f};
-        float delta = 0.f;
-        if (i < here) {
-          const int64_t at = stat_at(a, u, query_row(a, u, r0 + i));
+      if (threadIdx.x < PIECE) {
+        st = {0.f, 0.f};
+        delta = 0.f;
+        if (int(threadIdx.x) < here) {
+          const int64_t at = stat_at(a, u, query_row(a, u, r0 + threadIdx.x));
           st = a.stats[at];
           delta = a.delta[at];
         }
-        lds_top[i] = st.x;
-        lds_inverse[i] = st.y;
-        lds_delta[i] = delta;
       }
       __syncthreads();
+      if (a.fast) {
+        pq.commit(lds_q);
+        pg.commit(lds_g);
+      } else {
+        Piece<T, DP, NW * 64>::copy(lds_q, [&](int i) { return q_at<T>(a, u, query_row(a, u, r0 + i)); }, here, a.dim);
+        Piece<T, DP, NW * 64>::copy(
+            lds_g, [&](int i) { return grad + packed_q(a, u, query_row(a, u, r0 + i)); }, here, a.dim);
+      }
+      if (threadIdx.x < PIECE) {
+        lds_top[threadIdx.x] = st.x;
+        lds_inverse[threadIdx.x] = st.y;
+        lds_delta[threadIdx.x] = delta;
+      }
+      __syncthreads();
+      if (a.fast && r0 + PIECE < a.rows) fetch(r0 + PIECE);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const T *qp = lds_q + t * 32 * Lds<T, DP>::STRIDE, *gp = lds_g + t * 32 * Lds<T, DP>::STRIDE;
@@ -422,8 +575,37 @@ Args args_of(const sihc_attention* s) {
   a.dim = s->dim;
   a.rows = int64_t(a.each) * a.queries;
   a.scale = s->scale;
+  a.splits = 1;
+  a.span = INT32_MAX - PIECE;
+  // Rows of whole vectors, and offsets within an image's queries, and within a piece of keys, below 2^31.
+  const int64_t size = s->dtype == SIHC_DTYPE_F32 ? 4 : 2, most = (int64_t(1) << 31) / size - s->dim;
+  auto within = [&](int64_t tokens, int64_t token, int64_t heads, int64_t head) {
+    return token >= 0 && head >= 0 && (token == 0 || tokens <= most / token) && (head == 0 || heads <= most / head) &&
+           tokens * token + heads * head < most;
+  };
+  a.fast = s->dim * size % 16 == 0 && within(s->queries, s->q_stride[1], s->heads, s->q_stride[2]) &&
+           within(s->queries, int64_t(s->heads) * s->dim, s->heads, s->dim) &&
+           within(PIECE, s->k_stride[1], 0, 0) && within(PIECE, s->v_stride[1], 0, 0);
+  // r / queries for r < 2^31 (Granlund and Montgomery 1994, as in sihc_kernels.hip): with 2^l the next
+  // power of two, magic = ceil(2^(31 + l) / queries) is exact; powers of two are a shift.
+  int l = 0;
+  while ((int64_t(1) << l) < a.queries) ++l;
+  if (a.queries > 0 && (int64_t(1) << l) != a.queries) {
+    a.magic = uint32_t(((uint64_t(1) << (31 + l)) + uint64_t(a.queries) - 1) / uint64_t(a.queries));
+    a.shift = l - 1;
+  } else {
+    a.shift = l;
+  }
   return a;
 }
+// Few rows leave most of the card idle: then the keys are cut into parts of at least 128, for about
+// 1024 blocks.
+int splits_of(const sihc_attention* s) {
+  const int64_t blocks = s->batch * s->kv_heads * ceil_div(int64_t(s->queries) * (s->heads / s->kv_heads), 32);
+  if (blocks <= 0 || blocks >= 512) return 1;
+  return int(std::max<int64_t>(1, std::min<int64_t>(s->keys / 128, ceil_div(1024, blocks))));
+}
+int64_t query_rows(const sihc_attention* s) { return s->batch * s->heads * int64_t(s->queries); }
 // Calls f(T, DP): the smallest compiled width of a head.
 template <typename F>
 int by_width(const sihc_attention* s, F&& f) {
@@ -435,26 +617,42 @@ int by_width(const sihc_attention* s, F&& f) {
     return f(t, IC<128>{});
   });
 }
-// Calls f(NW) with the waves of a block over `rows` rows of its own side.
+// Calls f(NW) with the waves of a block over `rows` rows of its own side, `heads` times: blocks of one
+// wave where larger ones would leave most of the card idle.
 template <typename F>
-int by_waves(int64_t rows, F&& f) {
-  return rows <= 32 ? f(IC<1>{}) : f(IC<4>{});
+int by_waves(int64_t rows, int64_t heads, F&& f) {
+  return rows <= 32 || ceil_div(rows, 128) * heads < 256 ? f(IC<1>{}) : f(IC<4>{});
 }
 
 }  // namespace
 
 extern "C" {
 
-size_t sihc_cross_attention_workspace_size(const sihc_attention*) { return 0; }
+size_t sihc_cross_attention_workspace_size(const sihc_attention* s) {
+  if (check_args("sihc_cross_attention", s)) return 0;
+  const int splits = splits_of(s);
+  return splits > 1 ? size_t(splits) * size_t(query_rows(s)) * size_t(s->dim + 2) * 4 : 0;
+}
 
 int sihc_cross_attention(const sihc_attention* s, const void* q, const void* k, const void* v, const int32_t* lengths,
-                         void* out, float* stats, void*, size_t, void* stream) {
+                         void* out, float* stats, void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "sihc_cross_attention";
   if (int rc = check_args(what, s)) return rc;
   if (s->batch == 0 || s->queries == 0) return SIHC_OK;
   if (!q || !out || (s->keys && (!k || !v))) return fail(SIHC_ERR_INVALID, "%s: null pointer", what);
-  if (!aligned(stats, 8)) return fail(SIHC_ERR_INVALID, "%s: misaligned stats", what);
+  const size_t need = sihc_cross_attention_workspace_size(s);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(SIHC_ERR_INVALID, "%s: workspace of %zu bytes required, got %zu", what, need, workspace_bytes);
+  if (!aligned(stats, 8) || !aligned(workspace, 16))
+    return fail(SIHC_ERR_INVALID, "%s: misaligned workspace or stats", what);
   Args a = args_of(s);
+  const int64_t total = query_rows(s);
+  a.splits = splits_of(s);
+  if (a.splits > 1) {
+    a.span = int(ceil_div(ceil_div(s->keys, a.splits), PIECE) * PIECE);
+    a.part_s = static_cast<float2*>(workspace);
+    a.part_o = reinterpret_cast<float*>(a.part_s + a.splits * total);
+  }
   a.q = q;
   a.k = k;
   a.v = v;
@@ -462,12 +660,16 @@ int sihc_cross_attention(const sihc_attention* s, const void* q, const void* k, 
   a.o = out;
   a.stats = reinterpret_cast<float2*>(stats);
   return by_width(s, [&](auto t, auto dp) {
-    return by_waves(a.rows, [&](auto nw) {
+    using T = decltype(t);
+    return by_waves(a.rows, a.batch * a.shared * a.splits, [&](auto nw) {
       constexpr int NW = decltype(nw)::value;
       a.tiles = ceil_div(a.rows, NW * 32);
-      hipLaunchKernelGGL((k_attend<decltype(t), decltype(dp)::value, NW>),
-                         dim3(unsigned(a.tiles * a.batch * a.shared)), dim3(NW * 64), 0,
+      hipLaunchKernelGGL((k_attend<T, decltype(dp)::value, NW>),
+                         dim3(unsigned(a.tiles * a.batch * a.shared * a.splits)), dim3(NW * 64), 0,
                          static_cast<hipStream_t>(stream), a);
+      if (a.splits > 1)
+        hipLaunchKernelGGL(k_attend_join<T>, dim3(unsigned(ceil_div(total, 4))), dim3(256), 0,
+                           static_cast<hipStream_t>(stream), a, total);
       return check_launch(what);
     });
   });
@@ -513,7 +715,7 @@ int sihc_cross_attention_backward(const sihc_attention* s, const void* grad, con
     constexpr int DP = decltype(dp)::value;
     int rc = SIHC_OK;
     if (a.queries)
-      rc = by_waves(a.rows, [&](auto nw) {
+      rc = by_waves(a.rows, a.batch * a.shared, [&](auto nw) {
         constexpr int NW = decltype(nw)::value;
         a.tiles = ceil_div(a.rows, NW * 32);
         hipLaunchKernelGGL((k_attend_dq<T, DP, NW>), dim3(unsigned(a.tiles * a.batch * a.shared)), dim3(NW * 64), 0, st,
@@ -521,7 +723,7 @@ int sihc_cross_attention_backward(const sihc_attention* s, const void* grad, con
         return check_launch(what);
       });
     if (rc || !a.keys) return rc;
-    return by_waves(a.keys, [&](auto nw) {
+    return by_waves(a.keys, a.batch * a.shared, [&](auto nw) {
       constexpr int NW = decltype(nw)::value;
       a.tiles = ceil_div(a.keys, NW * 32);
       hipLaunchKernelGGL((k_attend_dkv<T, DP, NW>), dim3(unsigned(a.tiles * a.batch * a.shared)), dim3(NW * 64), 0, st,
