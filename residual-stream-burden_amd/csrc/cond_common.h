@@ -94,9 +94,19 @@ __device__ __forceinline__ void load_f32(const T* p, float* o) {
   for (int k = 0; k < V; k += PIECE) load<T, PIECE>(p + k).to(o + k);
 }
 
+// Sum over a wave, in every lane: within rows of 16 lanes by data-parallel moves (quad permutations
+// and mirrors), then across the rows.
+template <int CONTROL>
+__device__ __forceinline__ float moved(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CONTROL, 0xf, 0xf, true));
+}
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+  v += moved<0xb1>(v);   // quad_perm [1,0,3,2]
+  v += moved<0x4e>(v);   // quad_perm [2,3,0,1]
+  v += moved<0x141>(v);  // row_half_mirror
+  v += moved<0x140>(v);  // row_mirror
+  v += __shfl_xor(v, 16);
+  v += __shfl_xor(v, 32);
   return v;
 }
 

@@ -337,7 +337,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 384 ? 2 : 1) v
   if (a.splits > 1) {
     const int64_t row = ((int64_t(u.split) * a.batch + u.b) * a.shared + u.g) * a.rows + r;
     if (half == 0) a.part_s[row] = {top, sum};
-    if (begin < end) store_row<float, DP>(a.part_o + row * a.dim, o, 1.f, a.dim, half);
+    store_row<float, DP>(a.part_o + row * a.dim, o, 1.f, a.dim, half);  // (zeros past the length)
     return;
   }
   const float inverse = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // (NaN stays NaN)
@@ -345,45 +345,51 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 384 ? 2 : 1) v
   if (a.stats && half == 0) a.stats[stat_at(a, u, qr)] = {top == -INFINITY ? 0.f : top, inverse};
 }
 
-// The parts of a row, brought under their largest score and summed in ascending order; one wave a row.
+// The parts of a row, brought under their largest score and summed: a block a row, of 8 groups of 32
+// lanes that take every eighth part, 4 channels a lane, and whose sums are added in order.
 template <typename T>
 __global__ __launch_bounds__(256) void k_attend_join(Args a, int64_t total) {
-  const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (row >= total) return;
-  const int lane = int(threadIdx.x & 63);
+  __shared__ f32x4 lds_o[8][32];
+  __shared__ float lds_sum[8];
+  const int64_t row = blockIdx.x;
+  const int lane = int(threadIdx.x & 31), group = int(threadIdx.x >> 5);
   const int64_t bg = row / a.rows;
   Unit u;
   u.b = bg / a.shared;
   u.g = int(bg - u.b * a.shared);
   const QueryRow qr = query_row(a, u, row - bg * a.rows);
-  // a lane's parts: their largest score, and what each one's sums are worth under it
   float top = -INFINITY;
-  for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, a.part_s[s * total + row].x);
+  for (int s = int(threadIdx.x & 63); s < a.splits; s += 64) top = fmaxf(top, a.part_s[s * total + row].x);
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
   const float base = top == -INFINITY ? 0.f : top;
-  float sum = 0.f, o[2] = {};
-  for (int s0 = 0; s0 < a.splits; s0 += 64) {
-    const int mine = s0 + lane;
-    const float2 p = mine < a.splits ? a.part_s[mine * total + row] : float2{-INFINITY, 0.f};
-    const float worth = p.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(p.x - base);
-    const int here = min(64, a.splits - s0);
+  float sum = 0.f;
+  f32x4 o = {};
+  const int c = min(lane * 4, max(a.dim - 4, 0)), n = min(4, a.dim);
 #pragma unroll 4
-    for (int k = 0; k < here; ++k) {
-      const float w = __shfl(worth, k), part = __shfl(p.y, k);
-      sum += w * part;
-      if (part == 0.f) continue;  // (a part past the length: its sums were not written)
-      const float* from = a.part_o + ((s0 + k) * total + row) * a.dim;
+  for (int s = group; s < a.splits; s += 8) {
+    const float2 p = a.part_s[s * total + row];
+    const float worth = __builtin_amdgcn_exp2f(p.x - base);
+    sum += worth * p.y;
+    const float* from = a.part_o + (s * total + row) * a.dim + c;
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        if (lane + e * 64 < a.dim) o[e] = fmaf(w, from[lane + e * 64], o[e]);
-    }
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(worth, from[min(e, n - 1)], o[e]);
+  }
+  lds_o[group][lane] = o;
+  if (lane == 0) lds_sum[group] = sum;
+  __syncthreads();
+  if (group) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) {
+    o += lds_o[k][lane];
+    sum += lds_sum[k];
   }
   const float inverse = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-  T* to = static_cast<T*>(a.o) + packed_q(a, u, qr);
+  T* to = static_cast<T*>(a.o) + packed_q(a, u, qr) + c;
+  if (lane * 4 < a.dim)
 #pragma unroll
-  for (int e = 0; e < 2; ++e)
-    if (lane + e * 64 < a.dim) to[lane + e * 64] = from_f32<T>(o[e] * inverse);
+    for (int e = 0; e < 4; ++e)
+      if (e < n) to[e] = from_f32<T>(o[e] * inverse);
   if (a.stats && lane == 0) a.stats[stat_at(a, u, qr)] = {base, inverse};
 }
 
@@ -668,7 +674,7 @@ int sihc_cross_attention(const sihc_attention* s, const void* q, const void* k, 
                          dim3(unsigned(a.tiles * a.batch * a.shared * a.splits)), dim3(NW * 64), 0,
                          static_cast<hipStream_t>(stream), a);
       if (a.splits > 1)
-        hipLaunchKernelGGL(k_attend_join<T>, dim3(unsigned(ceil_div(total, 4))), dim3(256), 0,
+        hipLaunchKernelGGL(k_attend_join<T>, dim3(unsigned(total)), dim3(256), 0,
                            static_cast<hipStream_t>(stream), a, total);
       return check_launch(what);
     });

@@ -18,10 +18,9 @@
 namespace {
 using namespace sihc_cond;
 
-constexpr int TILE = 2048;        // keys a block sorts in one pass, 8 a thread
-constexpr int CHUNK = 32;         // sorted tokens a wave sums
+constexpr int OWN_SCAN = 64;      // up to so many tiles the scattering blocks add the counts up themselves
 constexpr int FEW_TOKENS = 1024;  // up to here the rows' tokens are listed by scanning all ids
-constexpr int FEW_ROWS = 8;       // table rows of a block there
+constexpr int FEW_ROWS = 8;       // table rows of a block there, at most
 
 template <typename I>
 __device__ __forceinline__ uint32_t id_at(const I* ids, int64_t n, uint32_t rows) {
@@ -30,20 +29,34 @@ __device__ __forceinline__ uint32_t id_at(const I* ids, int64_t n, uint32_t rows
 }
 
 // ------------------------------------------------------------------------------- lookup
-// One vector a thread; the last vector of a row that V does not divide moves back to end with it.
-template <typename T, typename I, int V>
+// UNROLL vectors a thread, a block apart, so that a thread's ids, then its rows, are in flight together;
+// the last vector of a row that V does not divide moves back to end with it.
+template <typename T, typename I, int V, int UNROLL>
 __global__ __launch_bounds__(256) void k_embed(const T* __restrict__ table, const I* __restrict__ ids,
                                                T* __restrict__ out, int64_t items, uint32_t rows, int C, int vecs,
                                                float scale) {
-  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= items) return;
-  const int64_t n = items <= 0x7fffffff ? int64_t(uint32_t(i) / uint32_t(vecs)) : i / vecs;
-  const int c = min(int(i - n * vecs) * V, C - V);
-  float v[V];
-  load<T, V>(table + int64_t(id_at(ids, n, rows)) * C + c).to(v);
+  const int64_t first = int64_t(blockIdx.x) * (256 * UNROLL) + threadIdx.x;
+  const T* from[UNROLL];
+  int64_t to[UNROLL];
 #pragma unroll
-  for (int k = 0; k < V; ++k) v[k] *= scale;
-  store<T, V>(out + n * C + c, Vec<T, V>::of(v));
+  for (int k = 0; k < UNROLL; ++k) {
+    const int64_t i = min(first + k * 256, items - 1);  // (threads past the end repeat the last vector)
+    const int64_t n = items <= 0x7fffffff ? int64_t(uint32_t(i) / uint32_t(vecs)) : i / vecs;
+    const int c = min(int(i - n * vecs) * V, C - V);
+    from[k] = table + int64_t(id_at(ids, n, rows)) * C + c;
+    to[k] = n * C + c;
+  }
+  Vec<T, V> row[UNROLL];
+#pragma unroll
+  for (int k = 0; k < UNROLL; ++k) row[k] = load<T, V>(from[k]);
+#pragma unroll
+  for (int k = 0; k < UNROLL; ++k) {
+    float v[V];
+    row[k].to(v);
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] *= scale;
+    store<T, V>(out + to[k], Vec<T, V>::of(v));
+  }
 }
 
 // ------------------------------------------------------------------- gradient, few tokens
@@ -52,11 +65,11 @@ __global__ __launch_bounds__(256) void k_embed(const T* __restrict__ table, cons
 template <typename T, typename I, int V>
 __global__ __launch_bounds__(256) void k_embed_grad_few(const T* __restrict__ grad, const I* __restrict__ ids,
                                                         T* __restrict__ out, int tokens, uint32_t rows, int C, int vecs,
-                                                        float scale, int64_t padding) {
+                                                        float scale, int64_t padding, int per_block) {
   __shared__ uint32_t list[FEW_TOKENS];  // token << 3 | row of the block
   __shared__ int wave_total[4];
   const int tid = int(threadIdx.x);
-  const uint32_t r0 = blockIdx.x * FEW_ROWS;
+  const uint32_t r0 = blockIdx.x * uint32_t(per_block);
   const int per = (tokens + 255) / 256, begin = min(tokens, tid * per), end = min(tokens, begin + per);
   uint32_t found[FEW_TOKENS / 256];
   int count = 0;
@@ -65,7 +78,7 @@ __global__ __launch_bounds__(256) void k_embed_grad_few(const T* __restrict__ gr
     found[k] = ~0u;
     if (begin + k < end) {
       const uint32_t id = id_at(ids, begin + k, rows);
-      if (id - r0 < uint32_t(FEW_ROWS) && int64_t(id) != padding) {
+      if (id - r0 < uint32_t(per_block) && int64_t(id) != padding) {
         found[k] = uint32_t(begin + k) << 3 | (id - r0);
         ++count;
       }
@@ -90,7 +103,7 @@ __global__ __launch_bounds__(256) void k_embed_grad_few(const T* __restrict__ gr
   for (int k = 0; k < FEW_TOKENS / 256; ++k)
     if (found[k] != ~0u) list[before++] = found[k];
   __syncthreads();
-  const int here = min(FEW_ROWS, int(rows - r0));
+  const int here = min(per_block, int(rows - r0));
   for (int item = tid; item < here * vecs; item += 256) {
     const int row = item / vecs, c = min((item - row * vecs) * V, C - V);
     float sum[V] = {};
@@ -124,15 +137,28 @@ struct PairKeys {
   __device__ __forceinline__ u32x2 operator()(int64_t n) const { return pairs[n]; }
 };
 
-// hist[tile][digit]: keys of the tile with that digit.
-template <typename K>
-__global__ __launch_bounds__(256) void k_sort_count(K keys, uint32_t* __restrict__ hist, int64_t n, int shift, int bins) {
+// n16 vectors and what is left of `bytes`, by `blocks` blocks.
+__device__ __forceinline__ void clear(u32x4* p, int64_t bytes, int64_t block, int64_t blocks) {
+  const int64_t n16 = bytes / 16;
+#pragma unroll 4
+  for (int64_t i = block * 256 + threadIdx.x; i < n16; i += blocks * 256) p[i] = u32x4{};
+  if (block == 0 && threadIdx.x < (bytes & 15)) reinterpret_cast<uint8_t*>(p + n16)[threadIdx.x] = 0;
+}
+
+// hist[tile][digit]: keys of the tile (256 x STEPS keys) with that digit. Blocks past the tiles clear the table's
+// gradient, of which a sort of few blocks leaves the memory's time free.
+template <typename K, int STEPS>
+__global__ __launch_bounds__(256) void k_sort_count(K keys, uint32_t* __restrict__ hist, int64_t n, int shift, int bins,
+                                                    int tiles, u32x4* __restrict__ table, int64_t table_bytes,
+                                                    uint32_t* __restrict__ crossing) {
   __shared__ uint32_t h[1024];
+  if (blockIdx.x == 0 && threadIdx.x == 0) *crossing = 0;
+  if (int(blockIdx.x) >= tiles) return clear(table, table_bytes, blockIdx.x - tiles, gridDim.x - tiles);
   for (int b = int(threadIdx.x); b < bins; b += 256) h[b] = 0;
   __syncthreads();
-  const int64_t base = int64_t(blockIdx.x) * TILE;
+  const int64_t base = int64_t(blockIdx.x) * (256 * STEPS);
 #pragma unroll
-  for (int k = 0; k < TILE / 256; ++k) {
+  for (int k = 0; k < STEPS; ++k) {
     const int64_t i = base + k * 256 + threadIdx.x;
     if (i < n) atomicAdd(&h[(keys(i).x >> shift) & uint32_t(bins - 1)], 1u);
   }
@@ -146,12 +172,22 @@ __global__ __launch_bounds__(1024) void k_sort_scan(uint32_t* __restrict__ hist,
   __shared__ uint32_t wave_total[16];
   const int b = int(threadIdx.x), wave = b >> 6;
   uint32_t total = 0;
-  if (b < bins)
-    for (int t = 0; t < tiles; ++t) {
-      const uint32_t c = hist[int64_t(t) * bins + b];
-      hist[int64_t(t) * bins + b] = total;
-      total += c;
-    }
+  auto each_tile = [&](auto f) {  // f(count) is the new value; 8 tiles' counts are in flight at a time
+    if (b < bins)
+      for (int t0 = 0; t0 < tiles; t0 += 8) {
+        uint32_t c[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) c[k] = hist[int64_t(min(t0 + k, tiles - 1)) * bins + b];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (t0 + k < tiles) hist[int64_t(t0 + k) * bins + b] = f(c[k]);
+      }
+  };
+  each_tile([&](uint32_t c) {
+    const uint32_t had = total;
+    total += c;
+    return had;
+  });
   uint32_t before = total;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -162,21 +198,60 @@ __global__ __launch_bounds__(1024) void k_sort_scan(uint32_t* __restrict__ hist,
   __syncthreads();
   before -= total;
   for (int w = 0; w < wave; ++w) before += wave_total[w];
-  if (b < bins)
-    for (int t = 0; t < tiles; ++t) hist[int64_t(t) * bins + b] += before;
+  each_tile([&](uint32_t c) { return c + before; });
+}
+
+// The same for one tile, by every block for itself: bin b of a thread, b < bins <= 1024.
+__device__ __forceinline__ void own_scan(const uint32_t* hist, uint32_t* at, int tile, int tiles, int bins) {
+  __shared__ uint32_t wave_total[4];
+  const int tid = int(threadIdx.x), wave = tid >> 6;
+  const int per = (bins + 255) / 256;  // adjacent bins of a thread
+  uint32_t total[4] = {}, earlier[4] = {}, all = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (k < per && tid * per + k < bins)
+      for (int t0 = 0; t0 < tiles; t0 += 16) {  // 16 tiles' counts in flight at a time
+        uint32_t c[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) c[j] = hist[int64_t(min(t0 + j, tiles - 1)) * bins + tid * per + k];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          if (t0 + j < tile) earlier[k] += c[j];
+          if (t0 + j < tiles) total[k] += c[j];
+        }
+      }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) all += total[k];
+  uint32_t before = all;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t o = __shfl_up(before, d);
+    if ((tid & 63) >= d) before += o;
+  }
+  if ((tid & 63) == 63) wave_total[wave] = before;
+  __syncthreads();
+  before -= all;
+  for (int w = 0; w < wave; ++w) before += wave_total[w];
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (k < per && tid * per + k < bins) {
+      at[tid * per + k] = before + earlier[k];
+      before += total[k];
+    }
+  __syncthreads();
 }
 
 // Stable scatter of a tile: a wave takes 64 keys at a time in ascending order; a key's place among
 // its equals is the waves before, the wave's steps before, and the lanes before (a ballot a bit).
-template <typename K>
+template <typename K, int STEPS>
 __global__ __launch_bounds__(256) void k_sort_scatter(K keys, const uint32_t* __restrict__ start,
-                                                      u32x2* __restrict__ out, int64_t n, int shift, int bits) {
-  __shared__ uint32_t count[4][1024];
+                                                      u32x2* __restrict__ out, int64_t n, int shift, int bits,
+                                                      int tiles) {
+  __shared__ uint32_t count[4][1024], own[1024];
   const int tid = int(threadIdx.x), wave = tid >> 6, lane = tid & 63, bins = 1 << bits;
   for (int b = tid; b < 4 * 1024; b += 256) (&count[0][0])[b] = 0;
   __syncthreads();
-  constexpr int STEPS = TILE / 256;
-  const int64_t base = int64_t(blockIdx.x) * TILE + wave * (TILE / 4);
+  const int64_t base = (int64_t(blockIdx.x) * 4 + wave) * (64 * STEPS);
   u32x2 key[STEPS];
   uint32_t rank[STEPS];
 #pragma unroll
@@ -202,8 +277,10 @@ __global__ __launch_bounds__(256) void k_sort_scatter(K keys, const uint32_t* __
     __builtin_amdgcn_wave_barrier();
   }
   __syncthreads();
+  const bool counts = tiles <= OWN_SCAN;  // `start` holds the counts
+  if (counts) own_scan(start, own, int(blockIdx.x), tiles, bins);
   for (int b = tid; b < bins; b += 256) {
-    uint32_t at = start[int64_t(blockIdx.x) * bins + b];
+    uint32_t at = counts ? own[b] : start[int64_t(blockIdx.x) * bins + b];
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const uint32_t c = count[w][b];
@@ -218,18 +295,13 @@ __global__ __launch_bounds__(256) void k_sort_scatter(K keys, const uint32_t* __
 }
 
 // ----------------------------------------------------------------- gradient, sorted tokens
-__global__ __launch_bounds__(256) void k_zero(u32x4* __restrict__ p, int64_t n16, int64_t bytes) {
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n16; i += int64_t(gridDim.x) * 256) p[i] = u32x4{};
-  if (blockIdx.x == 0 && threadIdx.x < (bytes & 15)) reinterpret_cast<uint8_t*>(p + n16)[threadIdx.x] = 0;
-}
-
-// One wave: CHUNK sorted tokens x 64 vectors of the row. partial[chunk][0]: the run that the chunk
+// One wave: CHUNK (8 or 32) sorted tokens x 64 vectors of the row. partial[chunk][0]: the run that the chunk
 // before began; [1]: the run that begins here and goes on in the next chunk. A run through the whole
 // chunk is [0].
-template <typename T, int V>
+template <typename T, int V, int CHUNK>
 __global__ __launch_bounds__(256) void k_embed_grad(const T* __restrict__ grad, const u32x2* __restrict__ sorted,
-                                                    T* __restrict__ out, float* __restrict__ partial, int64_t n,
-                                                    int64_t chunks, uint32_t rows, int C, int slices, float scale) {
+                                                    T* __restrict__ out, float* __restrict__ partial,
+                                                    uint32_t* __restrict__ crossing, int64_t n, int64_t chunks, uint32_t rows, int C, int slices, float scale) {
   const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
   const int64_t chunk = item / slices;
   if (chunk >= chunks) return;
@@ -263,6 +335,7 @@ __global__ __launch_bounds__(256) void k_embed_grad(const T* __restrict__ grad, 
       const uint32_t after = last ? next : __shfl(mine.x, min(k + 1, 63));
       if (after == row && !last) continue;
       const bool goes_on = last && after == row;
+      if (goes_on && !head && row < rows && cb == 0) crossing[1 + atomicAdd(crossing, 1u)] = uint32_t(chunk);
       if (on && row < rows) {
         if (head || goes_on) {
           float* p = partial + (chunk * 2 + (head ? 0 : 1)) * C + c;
@@ -281,39 +354,43 @@ __global__ __launch_bounds__(256) void k_embed_grad(const T* __restrict__ grad, 
   }
 }
 
-// The runs that cross chunks. A block looks at one chunk: where a run begins in it and goes on, its
-// partial rows of this chunk and the following ones are summed, by 4 thread rows over ascending
-// quarters of the run's chunks, then the quarters in order.
+// The runs that cross chunks, of the listed chunks in which they begin: their partial rows of this chunk
+// and the following ones are summed, by 4 thread rows over ascending quarters of the run's chunks, then
+// the quarters in order. blockIdx.y: 64 channels.
 template <typename T>
 __global__ __launch_bounds__(256) void k_embed_grad_runs(const u32x2* __restrict__ sorted,
-                                                         const float* __restrict__ partial, T* __restrict__ out,
-                                                         int64_t n, uint32_t rows, int C, float scale) {
+                                                         const float* __restrict__ partial,
+                                                         const uint32_t* __restrict__ crossing, T* __restrict__ out,
+                                                         int64_t n, int C, float scale, int CHUNK) {
   __shared__ float quarter[4][64];
-  const int64_t chunk = blockIdx.x, edge = (chunk + 1) * CHUNK;
-  if (edge >= n) return;
-  const uint32_t row = sorted[edge - 1].x;
-  if (row >= rows || sorted[edge].x != row) return;                            // no run goes on
-  if (sorted[chunk * CHUNK].x == row && chunk && sorted[chunk * CHUNK - 1].x == row) return;  // it began before
-  int64_t low = edge + 1, high = n;  // first position past the run
-  while (low < high) {
-    const int64_t mid = (low + high) / 2;
-    if (sorted[mid].x == row) low = mid + 1;
-    else high = mid;
-  }
-  const int64_t last = (low - 1) / CHUNK, parts = last - chunk, each = (parts + 3) / 4;
   const int lane = int(threadIdx.x & 63), q = int(threadIdx.x >> 6);
-  for (int c0 = 0; c0 < C; c0 += 64) {
-    const int c = min(c0 + lane, C - 1);
-    float sum = q == 0 ? partial[(chunk * 2 + 1) * C + c] : 0.f;
-    const int64_t begin = chunk + 1 + q * each, end = min(last + 1, begin + each);
+  const int listed = int(crossing[0]);
+  for (int item = int(blockIdx.x); item < listed; item += int(gridDim.x)) {
+    const int64_t chunk = crossing[1 + item];
+    const uint32_t row = sorted[(chunk + 1) * CHUNK].x;
+    int64_t parts = 1;  // chunks after this one that the run reaches: 64 of their ends at a time
+    for (;; parts += 64) {
+      const int64_t end = (chunk + 1 + parts + lane) * CHUNK;
+      const uint64_t stops = __ballot(end >= n || sorted[min(end, n - 1)].x != row);
+      if (stops) {
+        parts += __builtin_ctzll(stops);
+        break;
+      }
+    }
+    const int64_t last = chunk + parts, each = (parts + 3) / 4;
+    for (int c0 = int(blockIdx.y) * 64; c0 < C; c0 += int(gridDim.y) * 64) {
+      const int c = min(c0 + lane, C - 1);
+      float sum = q == 0 ? partial[(chunk * 2 + 1) * C + c] : 0.f;
+      const int64_t begin = chunk + 1 + q * each, end = min(last + 1, begin + each);
 #pragma unroll 8
-    for (int64_t k = begin; k < end; ++k) sum += partial[k * 2 * C + c];
-    quarter[q][lane] = sum;
-    __syncthreads();
-    if (q == 0 && c0 + lane < C)
-      out[int64_t(row) * C + c] =
-          from_f32<T>(scale * (((quarter[0][lane] + quarter[1][lane]) + quarter[2][lane]) + quarter[3][lane]));
-    __syncthreads();
+      for (int64_t k = begin; k < end; ++k) sum += partial[k * 2 * C + c];
+      quarter[q][lane] = sum;
+      __syncthreads();
+      if (q == 0 && c0 + lane < C)
+        out[int64_t(row) * C + c] =
+            from_f32<T>(scale * (((quarter[0][lane] + quarter[1][lane]) + quarter[2][lane]) + quarter[3][lane]));
+      __syncthreads();
+    }
   }
 }
 
@@ -340,9 +417,11 @@ int by_id(int id_bits, F&& f) {
 
 struct SortPlan {
   int passes, bits;  // of at most 10 bits each
+  int steps;         // keys a thread sorts in one pass
+  int chunk;         // sorted tokens a wave sums
   int64_t tiles, chunks;
-  size_t pairs_bytes, hist_bytes, partial_bytes;  // two pair arrays, one histogram, the partial rows
-  size_t total() const { return 2 * pairs_bytes + hist_bytes + partial_bytes; }
+  size_t pairs_bytes, hist_bytes, list_bytes, partial_bytes;  // two pair arrays, counts, runs, partial rows
+  size_t total() const { return 2 * pairs_bytes + hist_bytes + list_bytes + partial_bytes; }
 };
 SortPlan sort_plan(int64_t tokens, int64_t rows, int C) {
   SortPlan p{};
@@ -350,10 +429,14 @@ SortPlan sort_plan(int64_t tokens, int64_t rows, int C) {
   while ((int64_t(1) << bits) < rows + 1) ++bits;
   p.passes = (bits + 9) / 10;
   p.bits = (bits + p.passes - 1) / p.passes;
-  p.tiles = ceil_div(tokens, TILE);
-  p.chunks = ceil_div(tokens, CHUNK);
+  p.steps = tokens <= 1024 * OWN_SCAN ? 4 : 16;
+  p.tiles = ceil_div(tokens, 256 * p.steps);
+  // short chunks where long ones would be fewer than 16 waves to a CU (rows of 64 vectors a wave)
+  p.chunk = ceil_div(tokens, 32) * ceil_div(C, 512) < 256 * 16 ? 8 : 32;
+  p.chunks = ceil_div(tokens, p.chunk);
   p.pairs_bytes = size_t(ceil_div(tokens * 8, 256)) * 256;
   p.hist_bytes = size_t(ceil_div(p.tiles * (int64_t(4) << p.bits), 256)) * 256;
+  p.list_bytes = size_t(ceil_div((p.chunks + 1) * 4, 256)) * 256;
   p.partial_bytes = size_t(p.chunks) * 2 * size_t(C) * 4;
   return p;
 }
@@ -384,11 +467,19 @@ int sihc_embedding(const void* table, const void* ids, void* out, int64_t tokens
         constexpr int V = decltype(v)::value;
         if constexpr (V * sizeof(T) <= 16) {
           const int vecs = int(ceil_div(channels, V));
-          const int64_t items = tokens * vecs, blocks = ceil_div(items, 256);
-          if (blocks > 0x7fffffff) return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
-          hipLaunchKernelGGL((k_embed<T, I, V>), dim3(unsigned(blocks)), dim3(256), 0, static_cast<hipStream_t>(stream),
-                             static_cast<const T*>(table), static_cast<const I*>(ids), static_cast<T*>(out), items,
-                             uint32_t(rows), channels, vecs, scale);
+          const int64_t items = tokens * vecs;
+          auto launch = [&](auto unroll) {
+            constexpr int U = decltype(unroll)::value;
+            const int64_t blocks = ceil_div(items, 256 * U);
+            if (blocks > 0x7fffffff) return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
+            hipLaunchKernelGGL((k_embed<T, I, V, U>), dim3(unsigned(blocks)), dim3(256), 0,
+                               static_cast<hipStream_t>(stream), static_cast<const T*>(table),
+                               static_cast<const I*>(ids), static_cast<T*>(out), items, uint32_t(rows), channels, vecs,
+                               scale);
+            return check_launch(what);
+          };
+          // several vectors a thread once that leaves 4 blocks to a CU
+          return items >= 256 * 4 * 1024 ? launch(IC<4>{}) : launch(IC<1>{});
         }
         return check_launch(what);
       });
@@ -425,26 +516,34 @@ int sihc_embedding_backward(const void* grad, const void* ids, void* grad_table,
           const I* id = static_cast<const I*>(ids);
           T* out = static_cast<T*>(grad_table);
           if (tokens <= FEW_TOKENS) {
-            hipLaunchKernelGGL((k_embed_grad_few<T, I, V>), dim3(unsigned(ceil_div(rows, FEW_ROWS))), dim3(256), 0, st, g,
-                               id, out, int(tokens), uint32_t(rows), channels, vecs, scale, padding);
+            // about two vectors a thread: more rows would follow one another
+            const int per_block = std::max(1, std::min(FEW_ROWS, 512 / vecs));
+            hipLaunchKernelGGL((k_embed_grad_few<T, I, V>), dim3(unsigned(ceil_div(rows, per_block))), dim3(256), 0, st, g,
+                               id, out, int(tokens), uint32_t(rows), channels, vecs, scale, padding, per_block);
             return check_launch(what);
           }
           const SortPlan p = sort_plan(tokens, rows, channels);
           char* w = static_cast<char*>(workspace);
           u32x2* pairs[2] = {reinterpret_cast<u32x2*>(w), reinterpret_cast<u32x2*>(w + p.pairs_bytes)};
           uint32_t* hist = reinterpret_cast<uint32_t*>(w + 2 * p.pairs_bytes);
-          float* partial = reinterpret_cast<float*>(w + 2 * p.pairs_bytes + p.hist_bytes);
+          uint32_t* crossing = reinterpret_cast<uint32_t*>(w + 2 * p.pairs_bytes + p.hist_bytes);
+          float* partial = reinterpret_cast<float*>(w + 2 * p.pairs_bytes + p.hist_bytes + p.list_bytes);
           const int64_t bytes = rows * channels * int64_t(sizeof(T));
-          // (an output that is not 16-byte aligned is cleared by its leading bytes first)
           if (!aligned(out, 16)) return fail(SIHC_ERR_INVALID, "%s: grad_table must be 16-byte aligned", what);
-          hipLaunchKernelGGL(k_zero, dim3(unsigned(std::min<int64_t>(ceil_div(bytes, 4096) + 1, 256 * 16))), dim3(256), 0,
-                             st, reinterpret_cast<u32x4*>(out), bytes / 16, bytes);
-          const dim3 grid(static_cast<unsigned>(p.tiles));
-          auto pass = [&](auto keys, u32x2* to, int shift) {
+          const unsigned tiles = unsigned(p.tiles), clearing = unsigned(std::min<int64_t>(ceil_div(bytes, 16384) + 1, 2048));
+          auto tiled_pass = [&](auto keys, auto n, u32x2* to, int shift) {
             using K = decltype(keys);
-            hipLaunchKernelGGL(k_sort_count<K>, grid, dim3(256), 0, st, keys, hist, tokens, shift, 1 << p.bits);
-            hipLaunchKernelGGL(k_sort_scan, dim3(1), dim3(1024), 0, st, hist, int(p.tiles), 1 << p.bits);
-            hipLaunchKernelGGL(k_sort_scatter<K>, grid, dim3(256), 0, st, keys, hist, to, tokens, shift, p.bits);
+            constexpr int STEPS = decltype(n)::value;
+            hipLaunchKernelGGL((k_sort_count<K, STEPS>), dim3(tiles + (shift ? 0 : clearing)), dim3(256), 0, st, keys, hist,
+                               tokens, shift, 1 << p.bits, int(tiles), reinterpret_cast<u32x4*>(out), bytes, crossing);
+            if (p.tiles > OWN_SCAN)
+              hipLaunchKernelGGL(k_sort_scan, dim3(1), dim3(1024), 0, st, hist, int(tiles), 1 << p.bits);
+            hipLaunchKernelGGL((k_sort_scatter<K, STEPS>), dim3(tiles), dim3(256), 0, st, keys, hist, to, tokens, shift,
+                               p.bits, int(tiles));
+          };
+          auto pass = [&](auto keys, u32x2* to, int shift) {
+            if (p.steps == 4) tiled_pass(keys, IC<4>{}, to, shift);
+            else tiled_pass(keys, IC<16>{}, to, shift);
           };
           pass(IdKeys<I>{id, uint32_t(rows), padding}, pairs[0], 0);
           for (int k = 1; k < p.passes; ++k) pass(PairKeys{pairs[(k + 1) & 1]}, pairs[k & 1], k * p.bits);
@@ -452,10 +551,16 @@ int sihc_embedding_backward(const void* grad, const void* ids, void* grad_table,
           const int slices = int(ceil_div(vecs, 64));
           const int64_t blocks = ceil_div(p.chunks * slices, 4);
           if (blocks > 0x7fffffff) return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
-          hipLaunchKernelGGL((k_embed_grad<T, V>), dim3(unsigned(blocks)), dim3(256), 0, st, g, sorted, out, partial,
-                             tokens, p.chunks, uint32_t(rows), channels, slices, scale);
-          hipLaunchKernelGGL(k_embed_grad_runs<T>, dim3(unsigned(p.chunks)), dim3(256), 0, st, sorted, partial, out,
-                             tokens, uint32_t(rows), channels, scale);
+          auto sum = [&](auto chunk) {
+            hipLaunchKernelGGL((k_embed_grad<T, V, decltype(chunk)::value>), dim3(unsigned(blocks)), dim3(256), 0, st, g,
+                               sorted, out, partial, crossing, tokens, p.chunks, uint32_t(rows), channels, slices, scale);
+          };
+          if (p.chunk == 8) sum(IC<8>{});
+          else sum(IC<32>{});
+          const unsigned listed = unsigned(std::min<int64_t>(p.chunks, 1024)),
+                         columns = unsigned(std::min<int64_t>(ceil_div(channels, 64), 64));
+          hipLaunchKernelGGL(k_embed_grad_runs<T>, dim3(listed, columns), dim3(256), 0, st, sorted, partial, crossing, out,
+                             tokens, channels, scale, p.chunk);
         }
         return check_launch(what);
       });

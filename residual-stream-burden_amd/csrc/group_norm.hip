@@ -17,12 +17,11 @@
 namespace {
 using namespace sihc_cond;
 
-constexpr int THREADS = 1024;
-
 struct Shape {
   int64_t batch, pixels;
   int C, groups, per_group;  // channels, groups, channels of a group
   int slice_groups, W;       // groups and channels of a block's slice
+  int threads;               // of a block
   int lanes, rows;           // vectors of a slice's pixel; pixels a block loads at once
   int chunks;                // blocks that share a slice
   int64_t chunk_pixels;
@@ -36,8 +35,8 @@ __device__ __forceinline__ float rounded_product(float a, float b) {
   return a * b;
 }
 
-// What a launch does: all of it, or the two halves of a slice in chunks.
-enum { WHOLE, STATS, APPLY };
+// The two launches over slices in chunks.
+enum { STATS, APPLY };
 
 // Sum of v over the threads of each group of the slice, left in out[group] (and visible to all).
 __device__ __forceinline__ void group_sums(float v, const Shape& s, float* scratch, float* out) {
@@ -72,6 +71,12 @@ __device__ __forceinline__ void convert(Vec<T, V>& held, float* v) {
   asm volatile("" : "+v"(held.raw));
   held.to(v);
 }
+// A thread's Place::reach, for one phase: kept from one phase to the next, the comparisons with it would
+// take the scalar registers.
+__device__ __forceinline__ int for_phase(int reach) {
+  asm volatile("" : "+v"(reach));
+  return reach;
+}
 __device__ __forceinline__ void one_vector() { __builtin_amdgcn_sched_barrier(0); }
 
 __device__ __forceinline__ float sigmoid(float u) { return __builtin_amdgcn_rcpf(1.f + __expf(-u)); }
@@ -80,16 +85,18 @@ struct Place {
   int64_t b;
   int slice, chunk, lane, row, group;  // group: of the slice
   bool on;
+  int reach;  // pixels of the chunk from this thread's first on (0 for a thread without pixels)
   int64_t first;  // first pixel of the chunk
   int pixels;     // pixels of the chunk
 };
+// Of block `block` among `blocks`; neighbouring slices share lines, so they go to one XCD.
 template <int V>
-__device__ __forceinline__ Place place(const Shape& s) {
+__device__ __forceinline__ Place place(const Shape& s, int block, int blocks) {
   Place p;
   const int slices = s.groups / s.slice_groups;
-  const int64_t block = xcd_block(int(blockIdx.x), int(gridDim.x));
-  const int64_t unit = block / s.chunks;
-  p.chunk = int(block - unit * s.chunks);
+  const int64_t at = xcd_block(block, blocks);
+  const int64_t unit = at / s.chunks;
+  p.chunk = int(at - unit * s.chunks);
   p.b = unit / slices;
   p.slice = int(unit - p.b * slices);
   p.row = int(threadIdx.x) / s.lanes;
@@ -98,6 +105,7 @@ __device__ __forceinline__ Place place(const Shape& s) {
   p.group = p.on ? p.lane * V / s.per_group : 0;
   p.first = p.chunk * s.chunk_pixels;
   p.pixels = int(min(s.chunk_pixels, s.pixels - p.first));
+  p.reach = p.on ? p.pixels - p.row : 0;
   return p;
 }
 
@@ -116,22 +124,187 @@ __device__ __forceinline__ float2 merge(const float2* part, const Shape& s, int 
   return {mean, squares};
 }
 
-// stats: [batch, groups] of (mean, rstd), may be null. part: [batch, chunks, groups] of (mean, squares).
-template <typename T, typename TW, int V, int NV, int MODE>
-__global__ __launch_bounds__(THREADS) void k_group_norm(const T* __restrict__ x, const TW* __restrict__ weight,
+// Threads of a block, at most, and the blocks of 1024 threads on a CU that a kernel is compiled for: two
+// where what a thread holds, and works with beside it, fits 64 registers, so that one loads while
+// the other computes.
+constexpr int MOST_THREADS = 1024;
+constexpr int large_blocks(int held, int V, bool backward) {
+  return (backward ? held + 4 * V <= 22 : held + 2 * V <= 28) ? 2 : 1;
+}
+constexpr int simd_waves(int TB, int held, int V, bool backward) {
+  return TB < MOST_THREADS ? 1 : 4 * large_blocks(held, V, backward);
+}
+template <typename T, int V>
+constexpr int words() { return V * int(sizeof(T)) < 4 ? 1 : V * int(sizeof(T)) / 4; }
+
+// Sums of two values over the threads of each group of the slice, for every thread its own group's.
+// lds: 2 x TB floats, not in use since the last barrier but one.
+template <int TB>
+__device__ __forceinline__ float2 two_sums(float2 v, const Shape& s, int group, float* lds) {
+  const int tid = int(threadIdx.x), wave = tid >> 6, lane = tid & 63;
+  float2 out = {0.f, 0.f};
+  if (s.slice_groups == 1) {
+    v = {wave_sum(v.x), wave_sum(v.y)};
+    if (lane == 0) {
+      lds[wave] = v.x;
+      lds[TB + wave] = v.y;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < TB / 64; ++k) {
+      out.x += lds[k];
+      out.y += lds[TB + k];
+    }
+    return out;
+  }
+  lds[tid] = v.x;
+  lds[TB + tid] = v.y;
+  __syncthreads();
+  const int span = s.lanes / s.slice_groups, count = s.rows * span;
+  float2 mine[2];  // (a slice has at most 2 groups a wave: 32 of 1024 threads)
+  for (int g = wave, k = 0; g < s.slice_groups; g += TB / 64, ++k) {
+    float2 t = {0.f, 0.f};
+    for (int i = lane; i < count; i += 64) {
+      const int at = (i / span) * s.lanes + g * span + i % span;
+      t.x += lds[at];
+      t.y += lds[TB + at];
+    }
+    mine[k & 1] = {wave_sum(t.x), wave_sum(t.y)};
+  }
+  __syncthreads();
+  for (int g = wave, k = 0; g < s.slice_groups; g += TB / 64, ++k)
+    if (lane == 0) {
+      lds[g] = mine[k & 1].x;
+      lds[TB + g] = mine[k & 1].y;
+    }
+  __syncthreads();
+  return {lds[group], lds[TB + group]};
+}
+
+// Sums of the V elements of a vector and of their squares. bf16: two elements an instruction, the
+// products exact and the sums fp32.
+template <typename T, int V>
+__device__ __forceinline__ void add_moments(const Vec<T, V>& v, float2& sum) {
+  if constexpr (sizeof(T) == 2 && V >= 2) {
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+    constexpr uint32_t ONES = 0x3f803f80u;
+    uint32_t w[V / 2];
+    __builtin_memcpy(w, &v.raw, sizeof(w));
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      const pair x = __builtin_bit_cast(pair, w[k]);
+      sum.x = __builtin_amdgcn_fdot2_f32_bf16(x, __builtin_bit_cast(pair, ONES), sum.x, false);
+      sum.y = __builtin_amdgcn_fdot2_f32_bf16(x, x, sum.y, false);
+    }
+  } else {
+    float f[V];
+    v.to(f);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      sum.x += f[e];
+      sum.y = fmaf(f[e], f[e], sum.y);
+    }
+  }
+}
+
+// u sigmoid(u) from u and -u log2(e).
+__device__ __forceinline__ float silu(float u, float minus_u2) {
+  return u * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(minus_u2));
+}
+constexpr float LOG2E = 1.4426950408889634f;
+
+// Whole slices, one a block. The variance is first taken from the sums of x and of x^2; where that loses
+// digits (a mean above 8 deviations, or any fp32 input) from the squares about the mean. stats:
+// [batch, groups] of (mean, rstd), may be null.
+template <typename T, typename TW, int V, int NV, int TB>
+__global__ __launch_bounds__(TB, (simd_waves(TB, NV * words<T, V>(), V, false))) void k_group_norm(
+    const T* __restrict__ x, const TW* __restrict__ weight, const TW* __restrict__ bias, T* __restrict__ y,
+    float2* __restrict__ stats, Shape s) {
+  __shared__ float lds[2][2 * TB];
+  const Place p = place<V>(s, int(blockIdx.x), int(gridDim.x));
+  const int64_t at = (p.b * s.pixels + p.row) * s.C + p.slice * s.W + p.lane * V, step = int64_t(s.rows) * s.C;
+  Vec<T, V> held[NV];
+  int reach = for_phase(p.reach);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) held[k] = k * s.rows < reach ? load<T, V>(x + at + k * step) : Vec<T, V>::zero();
+  const float inverse_n = 1.f / (float(s.pixels) * float(s.per_group));
+  float2 sum = {0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < NV; ++k) add_moments(held[k], sum);
+  sum = two_sums<TB>(p.on ? sum : float2{0.f, 0.f}, s, p.group, lds[0]);
+  const float mean = sum.x * inverse_n;
+  float var = sum.y * inverse_n - mean * mean;
+  bool lost = sizeof(T) == 4 || !(mean * mean <= 64.f * var);
+  for (int g = 0; s.slice_groups > 1 && g < s.slice_groups; ++g) {  // (the same answer for every thread)
+    const float m = lds[0][g] * inverse_n, v = lds[0][TB + g] * inverse_n - m * m;
+    lost |= !(m * m <= 64.f * v);
+  }
+  if (lost) {
+    float2 squares = {0.f, 0.f};
+    reach = for_phase(p.reach);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      one_vector();
+      if (k * s.rows < reach) {
+        float v[V];
+        convert(held[k], v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) squares.x += (v[e] - mean) * (v[e] - mean);
+      }
+    }
+    var = two_sums<TB>(squares, s, p.group, lds[1]).x * inverse_n;
+  }
+  const float rstd = 1.f / sqrtf(var + s.eps);
+  if (stats && p.row == 0 && p.on && p.lane * V % s.per_group == 0)
+    stats[p.b * s.groups + p.slice * s.slice_groups + p.group] = {mean, rstd};
+  // u = (x - shift) a + d. bf16: shift = 0, a = weight rstd, d = bias - mean a, whose rounding is far below
+  // the output's; fp32: the mean is subtracted first.
+  const int c = p.on ? p.slice * s.W + p.lane * V : 0;
+  float a[V], d[V];
+  load_f32<TW, V>(weight + c, a);
+  load_f32<TW, V>(bias + c, d);
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    a[e] *= rstd;
+    if (sizeof(T) == 2) d[e] = fmaf(-mean, a[e], d[e]);
+  }
+  T* dst = y + at;
+  reach = for_phase(p.reach);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    one_vector();
+    if (k * s.rows < reach) {
+      float v[V];
+      convert(held[k], v);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float u = fmaf(sizeof(T) == 4 ? v[e] - mean : v[e], a[e], d[e]);
+        v[e] = s.silu ? silu(u, -LOG2E * u) : u;
+      }
+      store<T, V>(dst, Vec<T, V>::of(v));
+    }
+    dst += step;
+  }
+}
+
+// The same over slices in chunks. stats: [batch, groups] of (mean, rstd), may be null. part: [batch, chunks, groups] of (mean, squares).
+template <typename T, typename TW, int V, int NV, int TB, int MODE>
+__global__ __launch_bounds__(TB, (simd_waves(TB, NV * words<T, V>(), V, false))) void k_group_norm_chunk(const T* __restrict__ x, const TW* __restrict__ weight,
                                                         const TW* __restrict__ bias, T* __restrict__ y,
                                                         float2* __restrict__ stats, float2* __restrict__ part,
                                                         Shape s) {
-  __shared__ float scratch[THREADS], sums[THREADS], sums2[THREADS];
-  const Place p = place<V>(s);
+  __shared__ float scratch[TB], sums[TB], sums2[TB];
+  const Place p = place<V>(s, int(blockIdx.x), int(gridDim.x));
+  int reach;
   const int c = p.slice * s.W + p.lane * V;
   const int64_t at = (p.b * s.pixels + p.first + p.row) * s.C + c;
   const T* src = x + at;
   const int64_t step = int64_t(s.rows) * s.C;
   Vec<T, V> held[NV];
+  reach = for_phase(p.reach);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    held[k] = p.on && k * s.rows + p.row < p.pixels ? load<T, V>(src + k * step) : Vec<T, V>::zero();
+    held[k] = k * s.rows < reach ? load<T, V>(src + k * step) : Vec<T, V>::zero();
   }
   float mean, rstd;
   if constexpr (MODE != APPLY) {
@@ -148,10 +321,11 @@ __global__ __launch_bounds__(THREADS) void k_group_norm(const T* __restrict__ x,
     const float n = float(p.pixels) * float(s.per_group);
     mean = sums[p.group] / n;
     float squares = 0.f;
+    reach = for_phase(p.reach);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       one_vector();
-      if (p.on && k * s.rows + p.row < p.pixels) {
+      if (k * s.rows < reach) {
         float v[V];
         convert(held[k], v);
 #pragma unroll
@@ -166,10 +340,6 @@ __global__ __launch_bounds__(THREADS) void k_group_norm(const T* __restrict__ x,
       }
       return;
     }
-    rstd = 1.f / sqrtf(sums2[p.group] / n + s.eps);
-    if (stats && int(threadIdx.x) < s.slice_groups)
-      stats[p.b * s.groups + p.slice * s.slice_groups + int(threadIdx.x)] = {
-          sums[threadIdx.x] / n, 1.f / sqrtf(sums2[threadIdx.x] / n + s.eps)};
   } else {
     if (int(threadIdx.x) < s.slice_groups) {
       const int g = p.slice * s.slice_groups + int(threadIdx.x);
@@ -204,21 +374,158 @@ __global__ __launch_bounds__(THREADS) void k_group_norm(const T* __restrict__ x,
   }
 }
 
-// part: [batch * chunks][2][C] sums over the chunk's pixels of g and of g h.
-template <typename T, typename TW, int V, int NV, int MODE>
-__global__ __launch_bounds__(THREADS) void k_group_norm_grad(const T* __restrict__ dy, const T* __restrict__ x,
+// Sums over the block's rows of each channel's two values, left in channel[2][W]. lds: 2 x rows x W floats,
+// then 2 x W for `channel`.
+template <int V, int TB>
+__device__ __forceinline__ float* channel_sums(const float* sg, const float* sh, const Place& p, const Shape& s,
+                                               float* lds) {
+  const int tid = int(threadIdx.x), size = s.rows * s.W;
+  float* channel = lds + 2 * size;
+  if (p.on)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      lds[p.row * s.W + p.lane * V + e] = sg[e];
+      lds[size + p.row * s.W + p.lane * V + e] = sh[e];
+    }
+  __syncthreads();
+  // the threads' first step adds rows a stride apart, the second the strides, in ascending order
+  const int stride = max(1, min(s.rows, TB / (2 * s.W)));
+  for (int i = tid; i < 2 * s.W * stride; i += TB) {
+    const int which = i / (s.W * stride), rest = i - which * s.W * stride, first = rest / s.W, k = rest - first * s.W;
+    float sum = 0.f;
+    for (int r = first; r < s.rows; r += stride) sum += lds[which * size + r * s.W + k];
+    lds[which * size + first * s.W + k] = sum;  // (of these rows, which no other thread reads)
+  }
+  __syncthreads();
+  for (int i = tid; i < 2 * s.W; i += TB) {
+    const int which = i / s.W, k = i - which * s.W;
+    float sum = 0.f;
+    for (int r = 0; r < stride; ++r) sum += lds[which * size + r * s.W + k];
+    channel[i] = sum;
+  }
+  __syncthreads();
+  return channel;
+}
+
+// h and g = dy act'(u) of an element.
+__device__ __forceinline__ void element(float x, float dy, float2 st, float w, float b, bool act, float& h, float& g) {
+  h = (x - st.x) * st.y;
+  g = dy;
+  if (act) {
+    const float u = fmaf(h, w, b), q = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-LOG2E * u));
+    g *= q * fmaf(u, 1.f - q, 1.f);
+  }
+}
+
+// The means of w g and of w g h over a group, from its channels' sums; one wave a group.
+template <typename TW, int TB>
+__device__ __forceinline__ void group_means(const TW* weight, const float* channel, const Place& p, const Shape& s,
+                                            float2* means) {
+  const int tid = int(threadIdx.x);
+  const float inverse_n = 1.f / (float(s.pixels) * float(s.per_group));
+  for (int g = tid >> 6; g < s.slice_groups; g += TB / 64) {
+    float a = 0.f, d = 0.f;
+    for (int k = tid & 63; k < s.per_group; k += 64) {
+      const float wk = to_f32(weight[p.slice * s.W + g * s.per_group + k]);
+      a += wk * channel[g * s.per_group + k];
+      d += wk * channel[s.W + g * s.per_group + k];
+    }
+    a = wave_sum(a);
+    d = wave_sum(d);
+    if ((tid & 63) == 0) means[g] = {a * inverse_n, d * inverse_n};
+  }
+  __syncthreads();
+}
+
+// Whole slices, one a block. g takes the registers that dy came in, as fp32, so that the second pass needs
+// no exponentials; part: [batch][2][C] sums over the pixels of g and of g h.
+template <typename T, typename TW, int V, int NV, int TB>
+__global__ __launch_bounds__(TB, (simd_waves(TB, NV * (words<T, V>() + V), V, true))) void k_group_norm_grad(
+    const T* __restrict__ dy, const T* __restrict__ x, const TW* __restrict__ weight, const TW* __restrict__ bias,
+    const float2* __restrict__ stats, T* __restrict__ dx, float* __restrict__ part, Shape s) {
+  extern __shared__ float lds[];
+  __shared__ float2 means[TB];
+  const int tid = int(threadIdx.x);
+  const Place p = place<V>(s, int(blockIdx.x), int(gridDim.x));
+  const int64_t at = (p.b * s.pixels + p.row) * s.C + p.slice * s.W + p.lane * V, step = int64_t(s.rows) * s.C;
+  Vec<T, V> hx[NV], hg[NV];
+  int reach = for_phase(p.reach);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const bool in = k * s.rows < reach;
+    hx[k] = in ? load<T, V>(x + at + k * step) : Vec<T, V>::zero();
+    hg[k] = in ? load<T, V>(dy + at + k * step) : Vec<T, V>::zero();
+  }
+  const int c = p.on ? p.slice * s.W + p.lane * V : 0;
+  const float2 st = stats[p.b * s.groups + p.slice * s.slice_groups + p.group];
+  float g[NV][V], w[V], sg[V] = {}, sh[V] = {};
+  load_f32<TW, V>(weight + c, w);
+  {
+    float b[V];
+    load_f32<TW, V>(bias + c, b);
+    reach = for_phase(p.reach);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      one_vector();
+      if (k * s.rows < reach) {
+        float xv[V], gv[V];
+        convert(hx[k], xv);
+        hg[k].to(gv);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          float h;
+          element(xv[e], gv[e], st, w[e], b[e], s.silu, h, g[k][e]);
+          sg[e] += g[k][e];
+          sh[e] = fmaf(g[k][e], h, sh[e]);
+        }
+      }
+    }
+  }
+  const float* channel = channel_sums<V, TB>(sg, sh, p, s, lds);
+  for (int i = tid; i < 2 * s.W; i += TB) {
+    const int which = i / s.W;
+    part[(p.b * 2 + which) * s.C + p.slice * s.W + i - which * s.W] = channel[i];
+  }
+  group_means<TW, TB>(weight, channel, p, s, means);
+  // dx = rstd (w g - mean_g - h mean_gh), h = (x - mean) rstd
+  const float2 m = means[p.group];
+  T* dst = dx + at;
+  reach = for_phase(p.reach);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    one_vector();
+    if (k * s.rows < reach) {
+      float xv[V];
+      convert(hx[k], xv);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float h = (xv[e] - st.x) * st.y;
+        xv[e] = st.y * (rounded_product(w[e], g[k][e]) - m.x - h * m.y);
+      }
+      store<T, V>(dst, Vec<T, V>::of(xv));
+    }
+    dst += step;
+  }
+}
+
+// The same over slices in chunks. part: [batch * chunks][2][C] sums over the chunk's pixels of g and of g h.
+template <typename T, typename TW, int V, int NV, int TB, int MODE>
+__global__ __launch_bounds__(TB, (simd_waves(TB, 2 * NV * words<T, V>(), V, true))) void k_group_norm_grad_chunk(const T* __restrict__ dy, const T* __restrict__ x,
                                                              const TW* __restrict__ weight,
                                                              const TW* __restrict__ bias,
                                                              const float2* __restrict__ stats, T* __restrict__ dx,
                                                              float* __restrict__ part, Shape s) {
-  extern __shared__ float lds[];  // [rows][W], twice the slice's channel sums
-  const Place p = place<V>(s);
+  extern __shared__ float lds[];
+  __shared__ float2 means[TB];
+  const Place p = place<V>(s, int(blockIdx.x), int(gridDim.x));
+  int reach;
   const int tid = int(threadIdx.x), c = p.slice * s.W + p.lane * V;
   const int64_t at = (p.b * s.pixels + p.first + p.row) * s.C + c, step = int64_t(s.rows) * s.C;
   Vec<T, V> hx[NV], hg[NV];
+  reach = for_phase(p.reach);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const bool in = p.on && k * s.rows + p.row < p.pixels;
+    const bool in = k * s.rows < reach;
     hx[k] = in ? load<T, V>(x + at + k * step) : Vec<T, V>::zero();
     hg[k] = in ? load<T, V>(dy + at + k * step) : Vec<T, V>::zero();
   }
@@ -228,96 +535,61 @@ __global__ __launch_bounds__(THREADS) void k_group_norm_grad(const T* __restrict
     load_f32<TW, V>(weight + c, w);
     load_f32<TW, V>(bias + c, b);
   }
-  // h and g of an element
-  auto element = [&](float xv, float gv, int e, float& h, float& g) {
-    h = (xv - st.x) * st.y;
-    g = gv;
-    if (s.silu) {
-      const float u = fmaf(h, w[e], b[e]), q = sigmoid(u);
-      g *= q * (1.f + u * (1.f - q));
-    }
-  };
-  float* channel = lds + s.rows * s.W;  // [2][W]
-  if constexpr (MODE != APPLY) {
+  if constexpr (MODE == STATS) {
     float sg[V] = {}, sh[V] = {};
+    reach = for_phase(p.reach);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       one_vector();
-      if (k * s.rows + p.row < p.pixels) {
+      if (k * s.rows < reach) {
         float xv[V], gv[V];
         convert(hx[k], xv);
         convert(hg[k], gv);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           float h, g;
-          element(xv[e], gv[e], e, h, g);
+          element(xv[e], gv[e], st, w[e], b[e], s.silu, h, g);
           sg[e] += g;
-          sh[e] += g * h;
+          sh[e] = fmaf(g, h, sh[e]);
         }
       }
     }
-    for (int which = 0; which < 2; ++which) {
-      __syncthreads();
-      if (p.on)
-#pragma unroll
-        for (int e = 0; e < V; ++e) lds[p.row * s.W + p.lane * V + e] = which ? sh[e] : sg[e];
-      __syncthreads();
-      for (int k = tid; k < s.W; k += THREADS) {
-        float sum = 0.f;
-        for (int r = 0; r < s.rows; ++r) sum += lds[r * s.W + k];
-        channel[which * s.W + k] = sum;
-        part[((p.b * s.chunks + p.chunk) * 2 + which) * s.C + p.slice * s.W + k] = sum;
-      }
+    const float* channel = channel_sums<V, TB>(sg, sh, p, s, lds);
+    for (int i = tid; i < 2 * s.W; i += TB) {
+      const int which = i / s.W;
+      part[((p.b * s.chunks + p.chunk) * 2 + which) * s.C + p.slice * s.W + i - which * s.W] = channel[i];
     }
-    if constexpr (MODE == STATS) return;
-    __syncthreads();
   } else {
-    for (int k = tid; k < 2 * s.W; k += THREADS) {
-      const int which = k / s.W, cc = k - which * s.W;
+    float* channel = lds;
+    for (int i = tid; i < 2 * s.W; i += TB) {
+      const int which = i / s.W;
       float sum = 0.f;
       for (int q = 0; q < s.chunks; ++q)
-        sum += part[((p.b * s.chunks + q) * 2 + which) * s.C + p.slice * s.W + cc];
-      channel[k] = sum;
+        sum += part[((p.b * s.chunks + q) * 2 + which) * s.C + p.slice * s.W + i - which * s.W];
+      channel[i] = sum;
     }
     __syncthreads();
-  }
-  // the two group means
-  __shared__ float means[2][THREADS];
-  const float inv_n = 1.f / (float(s.pixels) * float(s.per_group));
-  for (int g = tid >> 6; g < s.slice_groups; g += THREADS / 64) {
-    float a = 0.f, d = 0.f;
-    for (int k = tid & 63; k < s.per_group; k += 64) {
-      const float wk = to_f32(weight[p.slice * s.W + g * s.per_group + k]);
-      a += wk * channel[g * s.per_group + k];
-      d += wk * channel[s.W + g * s.per_group + k];
-    }
-    a = wave_sum(a);
-    d = wave_sum(d);
-    if ((tid & 63) == 0) {
-      means[0][g] = a * inv_n;
-      means[1][g] = d * inv_n;
-    }
-  }
-  __syncthreads();
-  if (!p.on) return;
-  const float ma = means[0][p.group], md = means[1][p.group];
-  T* dst = dx + at;
+    group_means<TW, TB>(weight, channel, p, s, means);
+    const float2 m = means[p.group];
+    T* dst = dx + at;
+    reach = for_phase(p.reach);
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    one_vector();
-    if (k * s.rows + p.row < p.pixels) {
-      float xv[V], gv[V];
-      convert(hx[k], xv);
-      convert(hg[k], gv);
+    for (int k = 0; k < NV; ++k) {
+      one_vector();
+      if (k * s.rows < reach) {
+        float xv[V], gv[V];
+        convert(hx[k], xv);
+        convert(hg[k], gv);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        float h, g;
-        element(xv[e], gv[e], e, h, g);
-        xv[e] = st.y * (rounded_product(w[e], g) - ma - h * md);
+        for (int e = 0; e < V; ++e) {
+          float h, g;
+          element(xv[e], gv[e], st, w[e], b[e], s.silu, h, g);
+          xv[e] = st.y * (rounded_product(w[e], g) - m.x - h * m.y);
+        }
+        store<T, V>(dst, Vec<T, V>::of(xv));
       }
-      store<T, V>(dst, Vec<T, V>::of(xv));
+      dst += step;
     }
-    dst += step;
   }
 }
 
@@ -339,8 +611,8 @@ __global__ __launch_bounds__(256) void k_channel_sums(const float* __restrict__ 
 }
 
 // ---------------------------------------------------------------------------------- host
-// The register words a thread holds of a tensor, at most; NV vectors of V elements.
-constexpr int WORDS = 64;
+// The register words a thread holds, at most.
+constexpr int WORDS = 80;
 struct Plan {
   Shape s;
   int V, NV;
@@ -351,8 +623,8 @@ int vec_of(int per_group, int elem) {
     if (v * elem <= 16 && per_group % v == 0) return v;
   return 1;
 }
-// arrays: tensors a block holds (1 forward, 2 backward).
-Plan plan(int64_t batch, int64_t pixels, int C, int groups, float eps, bool silu, int elem, int arrays) {
+// backward: a block holds x and the output's gradient, and that in fp32.
+Plan plan(int64_t batch, int64_t pixels, int C, int groups, float eps, bool silu, int elem, bool backward) {
   Plan p{};
   Shape& s = p.s;
   s.batch = batch;
@@ -363,23 +635,26 @@ Plan plan(int64_t batch, int64_t pixels, int C, int groups, float eps, bool silu
   s.eps = eps;
   s.silu = silu;
   p.V = vec_of(s.per_group, elem);
-  // whole groups until a pixel's piece is a line of 128 bytes, as long as the slice fits
-  const int word_vec = std::max(1, p.V * elem / 4), most = WORDS / arrays / word_vec;
-  auto vectors = [&](int g) {
+  // whole groups until a pixel's piece is a line of 128 bytes, as long as the slice fits and the grid fills
+  // the card (64 x 32 x 32 x 1152, 36 channels a group: pieces of 72 bytes 88 us, writing 1.17 times the
+  // output, of 144 bytes 82 us and 1.00)
+  const int most = WORDS / (std::max(1, p.V * elem / 4) + (backward ? p.V : 0));
+  auto vectors = [&](int g, int threads) {
     const int lanes = g * s.per_group / p.V;
-    return lanes > THREADS ? int64_t(1) << 40 : ceil_div(pixels, THREADS / lanes);
+    return lanes > threads ? int64_t(1) << 40 : ceil_div(pixels, threads / lanes);
   };
   s.slice_groups = 1;
-  for (int g = 1; g <= groups; ++g) {
-    if (groups % g || g * s.per_group / p.V > THREADS) continue;
-    if (g > 1 && (vectors(g) > most || s.slice_groups * s.per_group * elem >= 128)) break;
+  for (int g = 2; g <= groups; ++g) {
+    if (groups % g || g * s.per_group / p.V > MOST_THREADS) continue;
+    if (vectors(g, MOST_THREADS) > most || s.slice_groups * s.per_group * elem >= 128 || batch * (groups / g) < 512) break;
     s.slice_groups = g;
   }
+  // small slices: blocks of 256 threads, several to a CU
+  s.threads = vectors(s.slice_groups, 256) <= 8 ? 256 : MOST_THREADS;
   s.W = s.slice_groups * s.per_group;
   s.lanes = s.W / p.V;
-  s.rows = THREADS / s.lanes;
-  const int64_t need = vectors(s.slice_groups);
-  s.chunks = int(ceil_div(need, most));
+  s.rows = s.threads / s.lanes;
+  s.chunks = int(ceil_div(vectors(s.slice_groups, s.threads), most));
   s.chunk_pixels = ceil_div(pixels, s.chunks);
   p.NV = int(ceil_div(s.chunk_pixels, s.rows));
   return p;
@@ -389,7 +664,7 @@ int check_sizes(const char* what, int64_t batch, int64_t pixels, int C, int grou
   if (batch < 0 || pixels < 0 || C <= 0 || (pixels && batch > SIHC_MAX_TOKENS / pixels))
     return fail(SIHC_ERR_INVALID, "%s: bad sizes", what);
   if (groups <= 0 || C % groups) return fail(SIHC_ERR_INVALID, "%s: %d channels are not %d groups", what, C, groups);
-  if (C / groups / vec_of(C / groups, dtype == SIHC_DTYPE_F32 ? 4 : 2) > THREADS)
+  if (C / groups / vec_of(C / groups, dtype == SIHC_DTYPE_F32 ? 4 : 2) > MOST_THREADS)
     return fail(SIHC_ERR_INVALID, "%s: groups of %d channels are too wide", what, C / groups);
   if (act != SIHC_ACT_NONE && act != SIHC_ACT_SILU) return fail(SIHC_ERR_INVALID, "%s: bad activation %d", what, act);
   if (!valid_dtype(dtype) || !valid_dtype(w_dtype)) return fail(SIHC_ERR_INVALID, "%s: bad dtype", what);
@@ -399,28 +674,32 @@ int check_sizes(const char* what, int64_t batch, int64_t pixels, int C, int grou
 }
 int elem_size(int dtype) { return dtype == SIHC_DTYPE_F32 ? 4 : 2; }
 
-// Calls f<T, TW, V, NV> with NV the smallest compiled count of at least p.NV vectors.
-template <int ARRAYS, typename F>
+// Calls f(T, TW, V, NV, TB, whole) with NV the smallest compiled count of at least p.NV vectors; slices in
+// chunks (whole = false) take the largest.
+template <bool BACKWARD, typename F>
 int by_plan(const Plan& p, int dtype, int w_dtype, F&& f) {
   return by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     auto with = [&](auto tw, auto v) {
-      constexpr int V = decltype(v)::value, words = V * int(sizeof(T)) / 4 > 0 ? V * int(sizeof(T)) / 4 : 1;
-      int rc = SIHC_ERR_INVALID;
-      auto attempt = [&](auto nv) {
+      constexpr int V = decltype(v)::value, MOST = WORDS / (words<T, V>() + (BACKWARD ? V : 0));
+      int rc = SIHC_OK;
+      auto attempt = [&](auto nv, auto tb) {
         constexpr int NV = decltype(nv)::value;
-        if constexpr (NV * words * ARRAYS <= WORDS) {
-          if (p.NV <= NV) {
-            rc = f(t, tw, v, nv);
+        if constexpr (NV <= MOST) {
+          if (p.s.threads == decltype(tb)::value && p.s.chunks == 1 && p.NV <= NV) {
+            rc = f(t, tw, v, nv, tb, std::true_type{});
             return true;
           }
         }
         return false;
       };
-      if (attempt(IC<1>{}) || attempt(IC<2>{}) || attempt(IC<4>{}) || attempt(IC<8>{}) || attempt(IC<16>{}) ||
-          attempt(IC<32>{}) || attempt(IC<64>{}))
+      constexpr IC<256> small{};
+      constexpr IC<1024> large{};
+      if (attempt(IC<1>{}, small) || attempt(IC<2>{}, small) || attempt(IC<4>{}, small) || attempt(IC<8>{}, small) ||
+          attempt(IC<4>{}, large) || attempt(IC<7>{}, large) || attempt(IC<10>{}, large) || attempt(IC<14>{}, large) ||
+          attempt(IC<20>{}, large) || attempt(IC<28>{}, large) || attempt(IC<40>{}, large) || attempt(IC<80>{}, large))
         return rc;
-      return fail(SIHC_ERR_INVALID, "group norm: internal plan");
+      return f(t, tw, v, IC<MOST>{}, large, std::false_type{});
     };
     auto by_v = [&](auto tw) {
       switch (p.V) {
@@ -441,7 +720,7 @@ extern "C" {
 
 size_t sihc_group_norm_workspace_size(int64_t batch, int64_t pixels, int channels, int groups, int dtype) {
   if (batch <= 0 || pixels <= 0 || channels <= 0 || groups <= 0 || channels % groups || !valid_dtype(dtype)) return 0;
-  const Plan p = plan(batch, pixels, channels, groups, 0.f, false, elem_size(dtype), 1);
+  const Plan p = plan(batch, pixels, channels, groups, 0.f, false, elem_size(dtype), false);
   return p.s.chunks > 1 ? size_t(batch) * size_t(p.s.chunks) * size_t(groups) * 8 : 0;
 }
 
@@ -456,23 +735,25 @@ int sihc_group_norm(const void* x, const void* weight, const void* bias, void* y
   if (need && (!workspace || workspace_bytes < need))
     return fail(SIHC_ERR_INVALID, "%s: workspace of %zu bytes required, got %zu", what, need, workspace_bytes);
   if (!aligned(workspace, 8) || !aligned(stats, 8)) return fail(SIHC_ERR_INVALID, "%s: misaligned workspace or stats", what);
-  const Plan p = plan(batch, pixels, channels, groups, eps, act == SIHC_ACT_SILU, elem_size(dtype), 1);
+  const Plan p = plan(batch, pixels, channels, groups, eps, act == SIHC_ACT_SILU, elem_size(dtype), false);
   const int64_t blocks = batch * (groups / p.s.slice_groups) * p.s.chunks;
   if (blocks > 0x7fffffff) return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
   const dim3 grid(static_cast<unsigned>(blocks));
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return by_plan<1>(p, dtype, w_dtype, [&](auto t, auto tw, auto v, auto nv) {
+  return by_plan<false>(p, dtype, w_dtype, [&](auto t, auto tw, auto v, auto nv, auto tb, auto whole) {
     using T = decltype(t);
     using TW = decltype(tw);
-    constexpr int V = decltype(v)::value, NV = decltype(nv)::value;
-    auto launch = [&](auto mode) {
-      hipLaunchKernelGGL((k_group_norm<T, TW, V, NV, decltype(mode)::value>), grid, dim3(THREADS), 0, st,
-                         static_cast<const T*>(x), static_cast<const TW*>(weight), static_cast<const TW*>(bias),
-                         static_cast<T*>(y), reinterpret_cast<float2*>(stats), static_cast<float2*>(workspace), p.s);
-    };
-    if (p.s.chunks == 1) {
-      launch(IC<WHOLE>{});
+    constexpr int V = decltype(v)::value, NV = decltype(nv)::value, TB = decltype(tb)::value;
+    if constexpr (decltype(whole)::value) {
+      hipLaunchKernelGGL((k_group_norm<T, TW, V, NV, TB>), grid, dim3(TB), 0, st, static_cast<const T*>(x),
+                         static_cast<const TW*>(weight), static_cast<const TW*>(bias), static_cast<T*>(y),
+                         reinterpret_cast<float2*>(stats), p.s);
     } else {
+      auto launch = [&](auto mode) {
+        hipLaunchKernelGGL((k_group_norm_chunk<T, TW, V, NV, TB, decltype(mode)::value>), grid, dim3(TB), 0, st,
+                           static_cast<const T*>(x), static_cast<const TW*>(weight), static_cast<const TW*>(bias),
+                           static_cast<T*>(y), reinterpret_cast<float2*>(stats), static_cast<float2*>(workspace), p.s);
+      };
       launch(IC<STATS>{});
       launch(IC<APPLY>{});
     }
@@ -482,7 +763,7 @@ int sihc_group_norm(const void* x, const void* weight, const void* bias, void* y
 
 size_t sihc_group_norm_backward_workspace_size(int64_t batch, int64_t pixels, int channels, int groups, int dtype) {
   if (batch <= 0 || pixels <= 0 || channels <= 0 || groups <= 0 || channels % groups || !valid_dtype(dtype)) return 0;
-  const Plan p = plan(batch, pixels, channels, groups, 0.f, false, elem_size(dtype), 2);
+  const Plan p = plan(batch, pixels, channels, groups, 0.f, false, elem_size(dtype), true);
   return size_t(batch) * size_t(p.s.chunks) * 2 * size_t(channels) * 4;
 }
 
@@ -506,25 +787,28 @@ int sihc_group_norm_backward(const void* grad, const void* x, const void* weight
       return fail(SIHC_ERR_INVALID, "%s: workspace of %zu bytes required, got %zu", what, need, workspace_bytes);
     if (!aligned(workspace, 8) || !aligned(stats, 8))
       return fail(SIHC_ERR_INVALID, "%s: misaligned workspace or stats", what);
-    const Plan p = plan(batch, pixels, channels, groups, 0.f, act == SIHC_ACT_SILU, elem_size(dtype), 2);
+    const Plan p = plan(batch, pixels, channels, groups, 0.f, act == SIHC_ACT_SILU, elem_size(dtype), true);
     const int64_t blocks = batch * (groups / p.s.slice_groups) * p.s.chunks;
     if (blocks > 0x7fffffff) return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
     parts = batch * p.s.chunks;
     const dim3 grid(static_cast<unsigned>(blocks));
-    const unsigned lds = unsigned(p.s.rows + 2) * unsigned(p.s.W) * 4u;
-    const int rc = by_plan<2>(p, dtype, w_dtype, [&](auto t, auto tw, auto v, auto nv) {
+    const unsigned lds = 2u * unsigned(p.s.rows + 1) * unsigned(p.s.W) * 4u;
+    const int rc = by_plan<true>(p, dtype, w_dtype, [&](auto t, auto tw, auto v, auto nv, auto tb, auto whole) {
       using T = decltype(t);
       using TW = decltype(tw);
-      constexpr int V = decltype(v)::value, NV = decltype(nv)::value;
-      auto launch = [&](auto mode) {
-        hipLaunchKernelGGL((k_group_norm_grad<T, TW, V, NV, decltype(mode)::value>), grid, dim3(THREADS), lds, st,
-                           static_cast<const T*>(grad), static_cast<const T*>(x), static_cast<const TW*>(weight),
-                           static_cast<const TW*>(bias), reinterpret_cast<const float2*>(stats),
-                           static_cast<T*>(grad_x), static_cast<float*>(workspace), p.s);
-      };
-      if (p.s.chunks == 1) {
-        launch(IC<WHOLE>{});
+      constexpr int V = decltype(v)::value, NV = decltype(nv)::value, TB = decltype(tb)::value;
+      if constexpr (decltype(whole)::value) {
+        hipLaunchKernelGGL((k_group_norm_grad<T, TW, V, NV, TB>), grid, dim3(TB), lds, st, static_cast<const T*>(grad),
+                           static_cast<const T*>(x), static_cast<const TW*>(weight), static_cast<const TW*>(bias),
+                           reinterpret_cast<const float2*>(stats), static_cast<T*>(grad_x),
+                           static_cast<float*>(workspace), p.s);
       } else {
+        auto launch = [&](auto mode) {
+          hipLaunchKernelGGL((k_group_norm_grad_chunk<T, TW, V, NV, TB, decltype(mode)::value>), grid, dim3(TB), lds, st,
+                             static_cast<const T*>(grad), static_cast<const T*>(x), static_cast<const TW*>(weight),
+                             static_cast<const TW*>(bias), reinterpret_cast<const float2*>(stats),
+                             static_cast<T*>(grad_x), static_cast<float*>(workspace), p.s);
+        };
         launch(IC<STATS>{});
         launch(IC<APPLY>{});
       }
