@@ -666,6 +666,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
                                int64_t groups, double eps, const std::string& act) {
     variable_list out = run_norm(x, weight, bias, groups, eps, act);
     ctx->mark_non_differentiable({out[1]});
+    ctx->set_materialize_grads(false);  // (zeros for the statistics' gradient would be a launch)
     ctx->save_for_backward({x, weight, bias, out[1]});
     ctx->saved_data["groups"] = groups;
     ctx->saved_data["act"] = act;
@@ -674,6 +675,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &stats = saved[3];
+    if (!grads[0].defined()) return variable_list(6);
     const Tensor grad = grads[0].contiguous();
     const int64_t groups = ctx->saved_data["groups"].toInt();
     const std::string act = ctx->saved_data["act"].toStringRef();
@@ -740,6 +742,7 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
     const Tensor n = lengths.value_or(Tensor());
     variable_list out = run_attention(q, k, v, n, scale);
     ctx->mark_non_differentiable({out[1]});
+    ctx->set_materialize_grads(false);
     ctx->save_for_backward({q, k, v, n, out[0], out[1]});
     ctx->saved_data["scale"] = scale;
     return out;
@@ -747,6 +750,7 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &n = saved[3], &out = saved[4], &stats = saved[5];
+    if (!grads[0].defined()) return variable_list(5);
     const Tensor grad = grads[0].contiguous();
     const double scale = ctx->saved_data["scale"].toDouble();
     Tensor dq, dk, dv;

@@ -158,10 +158,13 @@ def _group_norm_act_backward_fake(grad, x, weight, bias, stats, groups, act):
 def _norm_setup(ctx, inputs, output):
     x, weight, bias, ctx.groups, _, ctx.act = inputs
     ctx.mark_non_differentiable(output[1])
+    ctx.set_materialize_grads(False)  # zeros for the statistics' gradient would be a launch
     ctx.save_for_backward(x, weight, bias, output[1])
 
 
 def _norm_autograd(ctx, grad, _):
+    if grad is None:
+        return (None,) * 6
     x, weight, bias, stats = ctx.saved_tensors
     return (*_group_norm_act_backward(grad.contiguous(), x, weight, bias, stats, ctx.groups, ctx.act), None, None,
             None)
@@ -233,10 +236,13 @@ def _cross_attention_backward_fake(grad, q, k, v, lengths, out, stats, scale):
 def _attention_setup(ctx, inputs, output):
     q, k, v, lengths, ctx.scale = inputs
     ctx.mark_non_differentiable(output[1])
+    ctx.set_materialize_grads(False)
     ctx.save_for_backward(q, k, v, lengths, *output)
 
 
 def _attention_autograd(ctx, grad, _):
+    if grad is None:
+        return (None,) * 5
     q, k, v, lengths, out, stats = ctx.saved_tensors
     return (*_cross_attention_backward(grad.contiguous(), q, k, v, lengths, out, stats, ctx.scale), None, None)
 
