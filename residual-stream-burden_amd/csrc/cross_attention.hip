@@ -92,10 +92,10 @@ __device__ __forceinline__ void load_own(Own<T, DP>& own, const T* row, bool val
   }
 }
 
-// acc[r, own] = sum over channels of piece[r, c] own[c], r one of 32 rows from `piece`.
+// acc[r, own] + sum over channels of piece[r, c] own[c], r one of 32 rows from `piece`.
 template <int DP>
-__device__ __forceinline__ f32x16 rows_product(const bf16* piece, const Own<bf16, DP>& own, int lane, int half) {
-  f32x16 acc = {};
+__device__ __forceinline__ f32x16 rows_product(const bf16* piece, const Own<bf16, DP>& own, int lane, int half,
+                                               f32x16 acc = f32x16{}) {
   const bf16* p = piece + lane * Lds<bf16, DP>::STRIDE + half * 8;
 #pragma unroll
   for (int k = 0; k < DP / 16; ++k)
@@ -103,8 +103,8 @@ __device__ __forceinline__ f32x16 rows_product(const bf16* piece, const Own<bf16
   return acc;
 }
 template <int DP>
-__device__ __forceinline__ f32x16 rows_product(const float* piece, const Own<float, DP>& own, int lane, int half) {
-  f32x16 acc = {};
+__device__ __forceinline__ f32x16 rows_product(const float* piece, const Own<float, DP>& own, int lane, int half,
+                                               f32x16 acc = f32x16{}) {
   const float* p = piece + lane * Lds<float, DP>::STRIDE + half * 4;
 #pragma unroll
   for (int k = 0; k < DP / 8; ++k) {
@@ -117,35 +117,67 @@ __device__ __forceinline__ f32x16 rows_product(const float* piece, const Own<flo
 // Row of a tile that register i of a lane's half holds.
 __device__ __forceinline__ constexpr int row_of(int i, int half) { return (i / 4) * 8 + half * 4 + i % 4; }
 
+// A tile of probabilities or score gradients as the right operand of a product over its rows.
+template <typename T>
+struct Tile;
+template <>
+struct Tile<bf16> {
+  bf16x8 v[2];  // registers 0..7 and 8..15
+  __device__ __forceinline__ explicit Tile(const f32x16& p) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[k][i] = static_cast<__bf16>(p[k * 8 + i]);
+  }
+  // Sum of the lane's 16 values as rounded: the weights that the values are multiplied by.
+  __device__ __forceinline__ float add_to(float sum) const {
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+    const pair ones = __builtin_bit_cast(pair, 0x3f803f80u);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; i += 2)
+        sum = __builtin_amdgcn_fdot2_f32_bf16(pair{v[k][i], v[k][i + 1]}, ones, sum, false);
+    return sum;
+  }
+};
+template <>
+struct Tile<float> {
+  f32x16 v;
+  __device__ __forceinline__ explicit Tile(const f32x16& p) : v(p) {}
+  __device__ __forceinline__ float add_to(float sum) const {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += v[i];
+    return sum;
+  }
+};
+
 // acc[t][c, own] += sum over the 32 rows r from `piece` of piece[r, 32 t + c] p[r, own].
 template <int DP>
-__device__ __forceinline__ void columns_product(f32x16* acc, const bf16* piece, const f32x16& p, int lane, int half) {
+__device__ __forceinline__ void columns_product(f32x16* acc, const bf16* piece, const Tile<bf16>& p, int lane, int half) {
   constexpr int S = Lds<bf16, DP>::STRIDE;
   typedef __attribute__((address_space(3))) s16x4* LdsPtr;
   const int j = lane & 15;
   const bf16* at = piece + (half * 4 + j / 4) * S + (lane & 16) + (j % 4) * 4;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    bf16x8 b;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] = static_cast<__bf16>(p[k * 8 + i]);
 #pragma unroll
     for (int t = 0; t < d_tiles<DP>(); ++t) {
       const bf16* low = at + k * 16 * S + t * 32;
       const s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)low);
       const s16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(low + 8 * S));
       const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
-      acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc[t], 0, 0, 0);
+      acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, p.v[k], acc[t], 0, 0, 0);
     }
   }
 }
 template <int DP>
-__device__ __forceinline__ void columns_product(f32x16* acc, const float* piece, const f32x16& p, int lane, int half) {
+__device__ __forceinline__ void columns_product(f32x16* acc, const float* piece, const Tile<float>& p, int lane, int half) {
 #pragma unroll
   for (int i = 0; i < 16; ++i)
 #pragma unroll
     for (int t = 0; t < d_tiles<DP>(); ++t)
-      acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(piece[row_of(i, half) * Lds<float, DP>::STRIDE + t * 32 + lane], p[i],
+      acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(piece[row_of(i, half) * Lds<float, DP>::STRIDE + t * 32 + lane], p.v[i],
                                                     acc[t], 0, 0, 0);
 }
 
@@ -167,17 +199,14 @@ struct Piece {
       const uint32_t at = offset(min(r, valid - 1)) + uint32_t(min(c, dim - N)) * uint32_t(sizeof(T));
       v[k] = load<T, N>(reinterpret_cast<const T*>(from + at));
     }
-#pragma unroll
-    for (int k = 0; k < COUNT; ++k) {
-      const int i = int(threadIdx.x) + k * THREADS, r = i / VECS, c = (i - r * VECS) * N;
-      if (r >= valid || c >= dim) v[k] = Vec<T, N>::zero();
-    }
   }
-  __device__ __forceinline__ void commit(T* lds) const {
+  // (the zeros are put in here: in fetch() they would wait for the loads)
+  __device__ __forceinline__ void commit(T* lds, int valid, int dim) const {
 #pragma unroll
     for (int k = 0; k < COUNT; ++k) {
       const int i = int(threadIdx.x) + k * THREADS, r = i / VECS, c = (i - r * VECS) * N;
-      if (PIECE * VECS % THREADS == 0 || r < PIECE) *reinterpret_cast<u32x4*>(lds + r * Lds<T, DP>::STRIDE + c) = v[k].raw;
+      const u32x4 w = r >= valid || c >= dim ? u32x4{} : v[k].raw;
+      if (PIECE * VECS % THREADS == 0 || r < PIECE) *reinterpret_cast<u32x4*>(lds + r * Lds<T, DP>::STRIDE + c) = w;
     }
   }
   template <typename Row>
@@ -288,48 +317,58 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 384 ? 2 : 1) v
     const int here = min(PIECE, end - k0);
     __syncthreads();
     if (a.fast) {
-      pk.commit(lds_k);
-      pv.commit(lds_v);
+      pk.commit(lds_k, here, a.dim);
+      pv.commit(lds_v, here, a.dim);
     } else {
       Piece<T, DP, NW * 64>::copy(lds_k, [&](int i) { return k_at<T>(a, u, k0 + i); }, here, a.dim);
       Piece<T, DP, NW * 64>::copy(lds_v, [&](int i) { return v_at<T>(a, u, k0 + i); }, here, a.dim);
     }
     __syncthreads();
     if (a.fast && k0 + PIECE < end) fetch(k0 + PIECE);
-    f32x16 s[2];
-    float most = -INFINITY;
+    // Scores under the base of earlier pieces need no maximum as long as their powers stay small: a base
+    // is a scale, and sums keep their digits under any. The first piece, and one whose powers grow
+    // past 2^40, take their maximum as the new base, on scores computed again.
+    bool anew = __any(top == -INFINITY);
+    for (;;) {
+      f32x16 s[2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      s[t] = rows_product<DP>(lds_k + t * 32 * Lds<T, DP>::STRIDE, q, lane, half);
-      s[t] *= c;
-    }
-    if (here < PIECE) {
+      for (int t = 0; t < 2; ++t) s[t] = rows_product<DP>(lds_k + t * 32 * Lds<T, DP>::STRIDE, q, lane, half);
+      if (anew) {
+        float most = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (t * 32 + row_of(i, half) < here) most = fmaxf(most, s[t][i] * c);
+        most = fmaxf(most, __shfl_xor(most, 32));
+        const float now = fmaxf(top, most), keep = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - now);
+        top = now;
+        sum *= keep;
+#pragma unroll
+        for (int t = 0; t < d_tiles<DP>(); ++t) o[t] *= keep;
+      }
+      const float base = top == -INFINITY ? 0.f : top;  // (every score so far is -inf)
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (t * 32 + row_of(i, half) >= here) s[t][i] = -INFINITY;
-    }
+        for (int i = 0; i < 16; ++i) s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], c, -base));
+      if (here < PIECE) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) most = fmaxf(most, fmaxf(s[0][i], s[1][i]));
-    most = fmaxf(most, __shfl_xor(most, 32));
-    if (__any(most > top)) {  // a new largest score: rescale what was summed under the old one
-      const float now = fmaxf(top, most);
-      const float keep = __builtin_amdgcn_exp2f(now == -INFINITY ? 0.f : top - now);
-      top = now;
-      sum *= keep;
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int t = 0; t < d_tiles<DP>(); ++t) o[t] *= keep;
-    }
-    const float base = top == -INFINITY ? 0.f : top;  // (every score so far is -inf)
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - base);
-        sum += s[t][i];
+          for (int i = 0; i < 16; ++i)
+            if (t * 32 + row_of(i, half) >= here) s[t][i] = 0.f;
       }
-      columns_product<DP>(o, lds_v + t * 32 * Lds<T, DP>::STRIDE, s[t], lane, half);
+      const Tile<T> p0(s[0]), p1(s[1]);
+      const float more = p1.add_to(p0.add_to(0.f));
+      if (!anew && __any(more > 0x1p40f)) {
+        anew = true;
+        continue;
+      }
+      sum += more;
+      columns_product<DP>(o, lds_v, p0, lane, half);
+      columns_product<DP>(o, lds_v + 32 * Lds<T, DP>::STRIDE, p1, lane, half);
+      break;
     }
   }
   sum += __shfl_xor(sum, 32);
@@ -393,6 +432,18 @@ __global__ __launch_bounds__(256) void k_attend_join(Args a, int64_t total) {
   if (a.stats && lane == 0) a.stats[stat_at(a, u, qr)] = {base, inverse};
 }
 
+// The statistics of a row as a gradient's kernel takes them: bf16 folds the sum into the exponent, whose
+// rounding (2^-24 of about 10) is far below the inputs'; fp32 keeps the factor.
+template <typename T>
+__device__ __forceinline__ float2 exponent(float2 st) {
+  return sizeof(T) == 2 ? float2{st.x - __builtin_amdgcn_logf(st.y), 1.f} : st;  // (log2; no key: +inf, P = 0)
+}
+template <typename T>
+__device__ __forceinline__ float probability(float s, float c, float2 st) {
+  const float p = __builtin_amdgcn_exp2f(fmaf(s, c, -st.x));
+  return sizeof(T) == 2 ? p : p * st.y;
+}
+
 // ------------------------------------------------------------------ gradient of the queries
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 320 ? 2 : 1) void k_attend_dq(Args a) {
@@ -416,8 +467,11 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 320 ? 2 : 1) v
       for (int i = 0; i < N; ++i) delta = fmaf(float(g.v[k][i]), float(o.v[k][i]), delta);
     delta += __shfl_xor(delta, 32);
   }
-  const float2 st = valid ? a.stats[stat_at(a, u, qr)] : float2{0.f, 0.f};
+  const float2 st = exponent<T>(valid ? a.stats[stat_at(a, u, qr)] : float2{0.f, 0.f});
   if (valid && half == 0) a.delta[stat_at(a, u, qr)] = delta;
+  f32x16 minus_delta;  // where dP starts from, so that P times it is dS
+#pragma unroll
+  for (int i = 0; i < 16; ++i) minus_delta[i] = -delta;
   f32x16 dq[d_tiles<DP>()] = {};
   const float c = a.scale * LOG2E;
   Piece<T, DP, NW * 64> pk, pv;
@@ -432,8 +486,8 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 320 ? 2 : 1) v
     const int here = min(PIECE, u.len - k0);
     __syncthreads();
     if (a.fast) {
-      pk.commit(lds_k);
-      pv.commit(lds_v);
+      pk.commit(lds_k, here, a.dim);
+      pv.commit(lds_v, here, a.dim);
     } else {
       Piece<T, DP, NW * 64>::copy(lds_k, [&](int i) { return k_at<T>(a, u, k0 + i); }, here, a.dim);
       Piece<T, DP, NW * 64>::copy(lds_v, [&](int i) { return v_at<T>(a, u, k0 + i); }, here, a.dim);
@@ -444,13 +498,15 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 320 ? 2 : 1) v
     for (int t = 0; t < 2; ++t) {
       const T* kp = lds_k + t * 32 * Lds<T, DP>::STRIDE;
       f32x16 s = rows_product<DP>(kp, q, lane, half);
-      const f32x16 dp = rows_product<DP>(lds_v + t * 32 * Lds<T, DP>::STRIDE, g, lane, half);
+      const f32x16 dp = rows_product<DP>(lds_v + t * 32 * Lds<T, DP>::STRIDE, g, lane, half, minus_delta);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float p = __builtin_amdgcn_exp2f(s[i] * c - st.x) * st.y;
-        s[i] = t * 32 + row_of(i, half) < here ? p * (dp[i] - delta) : 0.f;
+      for (int i = 0; i < 16; ++i) s[i] = probability<T>(s[i], c, st) * dp[i];
+      if (here < PIECE) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (t * 32 + row_of(i, half) >= here) s[i] = 0.f;
       }
-      columns_product<DP>(dq, kp, s, lane, half);
+      columns_product<DP>(dq, kp, Tile<T>(s), lane, half);
     }
   }
   if (valid) store_row<T, DP>(static_cast<T*>(a.dq) + packed_q(a, u, qr), dq, a.scale, a.dim, half);
@@ -502,39 +558,47 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= (sizeof(T) == 
       }
       __syncthreads();
       if (a.fast) {
-        pq.commit(lds_q);
-        pg.commit(lds_g);
+        pq.commit(lds_q, here, a.dim);
+        pg.commit(lds_g, here, a.dim);
       } else {
         Piece<T, DP, NW * 64>::copy(lds_q, [&](int i) { return q_at<T>(a, u, query_row(a, u, r0 + i)); }, here, a.dim);
         Piece<T, DP, NW * 64>::copy(
             lds_g, [&](int i) { return grad + packed_q(a, u, query_row(a, u, r0 + i)); }, here, a.dim);
       }
       if (threadIdx.x < PIECE) {
-        lds_top[threadIdx.x] = st.x;
-        lds_inverse[threadIdx.x] = st.y;
-        lds_delta[threadIdx.x] = delta;
+        const float2 e = exponent<T>(st);
+        lds_top[threadIdx.x] = e.x;
+        lds_inverse[threadIdx.x] = e.y;
+        lds_delta[threadIdx.x] = -delta;
       }
       __syncthreads();
       if (a.fast && r0 + PIECE < a.rows) fetch(r0 + PIECE);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const T *qp = lds_q + t * 32 * Lds<T, DP>::STRIDE, *gp = lds_g + t * 32 * Lds<T, DP>::STRIDE;
+        f32x16 dp;
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const f32x4 d = *reinterpret_cast<const f32x4*>(lds_delta + t * 32 + row_of(i, half));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) dp[i + j] = d[j];
+        }
         f32x16 s = rows_product<DP>(qp, k, lane, half);
-        f32x16 dp = rows_product<DP>(gp, v, lane, half);
+        dp = rows_product<DP>(gp, v, lane, half, dp);
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
           const int row = t * 32 + row_of(i, half);
           const f32x4 top = *reinterpret_cast<const f32x4*>(lds_top + row);
-          const f32x4 inverse = *reinterpret_cast<const f32x4*>(lds_inverse + row);
-          const f32x4 delta = *reinterpret_cast<const f32x4*>(lds_delta + row);
+          f32x4 inverse = {};
+          if (sizeof(T) == 4) inverse = *reinterpret_cast<const f32x4*>(lds_inverse + row);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            s[i + j] = __builtin_amdgcn_exp2f(s[i + j] * c - top[j]) * inverse[j];
-            dp[i + j] = s[i + j] * (dp[i + j] - delta[j]);
+            s[i + j] = probability<T>(s[i + j], c, {top[j], inverse[j]});
+            dp[i + j] *= s[i + j];
           }
         }
-        columns_product<DP>(dv, gp, s, lane, half);
-        columns_product<DP>(dk, qp, dp, lane, half);
+        columns_product<DP>(dv, gp, Tile<T>(s), lane, half);
+        columns_product<DP>(dk, qp, Tile<T>(dp), lane, half);
       }
     }
   }
