@@ -42,9 +42,11 @@ struct Args {
   int queries, keys, heads, shared, each, dim;
   int64_t rows;   // query rows of a key head: each * queries
   int64_t tiles;  // blocks of a key head (in the forward, of one part of its keys)
-  int splits, span;  // the forward's parts of the keys, and their keys (a multiple of PIECE)
-  float* part_o;     // [splits][batch, key head][rows][dim] sums, where there are several parts
-  float2* part_s;    // their largest scores and sums
+  int splits;        // parts of a key head's keys (forward) or query rows (key and value gradients)
+  int64_t span;      // keys or rows of a part, a multiple of PIECE
+  float* part_o;     // where there are several: [splits][batch, key head][rows][dim] sums (forward), or
+                     // [splits][2][batch, keys, key heads, dim] (gradients of keys and values)
+  float2* part_s;    // (forward) their bases and sums of powers
   float scale;
   bool fast;               // (Piece)
   uint32_t magic;  // r / queries is the high word of r * magic, shifted right (0: r shifted right)
@@ -84,6 +86,17 @@ template <typename T, int DP>
 __device__ __forceinline__ void load_own(Own<T, DP>& own, const T* row, bool valid, int dim, int half) {
   constexpr int N = 16 / int(sizeof(T));  // 8 or 4: the lane's channels of one step
   constexpr int STEPS = DP / (2 * N);
+  if (dim % N == 0) {  // all loads from places that exist, then the zeros: no branch waits for one
+    Vec<T, N> v[STEPS];
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) v[k] = load<T, N>(row + min(k * 2 * N + half * N, dim - N));
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) {
+      if (!valid || k * 2 * N + half * N >= dim) v[k] = Vec<T, N>::zero();
+      __builtin_memcpy(&own.v[k], &v[k].raw, 16);
+    }
+    return;
+  }
 #pragma unroll
   for (int k = 0; k < STEPS; ++k) {
     const int c = k * 2 * N + half * N;
@@ -189,6 +202,7 @@ __device__ __forceinline__ void columns_product(f32x16* acc, const float* piece,
 template <typename T, int DP, int THREADS>
 struct Piece {
   static constexpr int N = 16 / int(sizeof(T)), VECS = DP / N, COUNT = (PIECE * VECS + THREADS - 1) / THREADS;
+  static constexpr bool HELD = COUNT <= 16;  // (fp32 pieces of one wave would fill its registers)
   Vec<T, N> v[COUNT];
   template <typename Offset>
   __device__ __forceinline__ void fetch(const void* base, Offset offset, int valid, int dim) {
@@ -211,33 +225,80 @@ struct Piece {
   }
   template <typename Row>
   __device__ static void copy(T* lds, Row row, int valid, int dim) {
+    constexpr int UNROLL = HELD ? 1 : 4;  // (4 loads in flight where this is the only way in)
+#pragma unroll UNROLL
     for (int i = int(threadIdx.x); i < PIECE * VECS; i += THREADS) {
       const int r = i / VECS, c = (i - r * VECS) * N;
-      const Vec<T, N> v = r < valid ? load_some<T, N>(row(r) + c, dim - c) : Vec<T, N>::zero();
+      Vec<T, N> v;
+      if (!HELD && dim % N == 0) {
+        v = load<T, N>(row(min(r, valid - 1)) + min(c, dim - N));
+        if (r >= valid || c >= dim) v = Vec<T, N>::zero();
+      } else {
+        v = r < valid ? load_some<T, N>(row(r) + c, dim - c) : Vec<T, N>::zero();
+      }
       *reinterpret_cast<u32x4*>(lds + r * Lds<T, DP>::STRIDE + c) = v.raw;
     }
   }
 };
 
-// A lane's row of sums (its registers hold 4 adjacent channels each), times f.
-template <typename T, int DP>
-__device__ __forceinline__ void store_row(T* row, const f32x16* acc, float f, int dim, int half) {
+// A wave's 32 rows of sums, times f, to `to` + the rows' offsets (each lane's own). They pass through the
+// wave's part of LDS (32 rows of a piece), so that a store writes whole 16-byte vectors of adjacent
+// channels: straight from the registers it would write 8 bytes of each of 64 rows. Every wave of the
+// block calls it, with `rows` in use by none.
+template <typename T, int DP, typename TO>
+__device__ __forceinline__ void store_rows(TO* to, int64_t offset, bool valid, T* rows, const f32x16* acc, float f, int dim,
+                                           int lane, int half) {
+  constexpr int N = 16 / int(sizeof(TO)), VECS = DP / N;
+  if constexpr (sizeof(TO) == sizeof(T)) {
+    constexpr int S = Lds<T, DP>::STRIDE;
 #pragma unroll
-  for (int t = 0; t < d_tiles<DP>(); ++t)
+    for (int t = 0; t < d_tiles<DP>(); ++t)
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const int c = t * 32 + row_of(i, half);
-      float e[4];
+      for (int i = 0; i < 16; i += 4) {
+        if (t * 32 + (i / 4) * 8 >= DP) continue;
+        float e[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) e[j] = acc[t][i + j] * f;
-      if (c + 4 <= dim) {
-        store<T, 4>(row + c, Vec<T, 4>::of(e));
+        for (int j = 0; j < 4; ++j) e[j] = acc[t][i + j] * f;
+        const Vec<T, 4> v = Vec<T, 4>::of(e);
+        __builtin_memcpy(rows + lane * S + t * 32 + row_of(i, half), &v.raw, sizeof(v.raw));
+      }
+    __syncthreads();
+    const int lane64 = half * 32 + lane, mine = valid ? 1 : 0;
+    for (int i = lane64; i < 32 * VECS; i += 64) {
+      const int r = i / VECS, c = (i - r * VECS) * N;
+      const int64_t at = (int64_t(__shfl(int(offset >> 32), r)) << 32) | uint32_t(__shfl(int(offset), r));
+      if (!__shfl(mine, r) || c >= dim) continue;
+      Vec<T, N> v;
+      __builtin_memcpy(&v.raw, rows + r * S + c, 16);
+      if (c + N <= dim) {
+        store<T, N>(to + at + c, v);
       } else {
+        T e[N];
+        __builtin_memcpy(e, &v.raw, 16);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (c + j < dim) row[c + j] = from_f32<T>(e[j]);
+        for (int j = 0; j < N; ++j)
+          if (c + j < dim) to[at + c + j] = e[j];
       }
     }
+    __syncthreads();
+  } else if (valid) {  // fp32 parts of bf16 inputs: 16 bytes from each lane
+#pragma unroll
+    for (int t = 0; t < d_tiles<DP>(); ++t)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const int c = t * 32 + row_of(i, half);
+        float e[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e[j] = acc[t][i + j] * f;
+        if (c + 4 <= dim) {
+          store<TO, 4>(to + offset + c, Vec<TO, 4>::of(e));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (c + j < dim) to[offset + c + j] = e[j];
+        }
+      }
+  }
 }
 
 // ------------------------------------------------------------------------------ addresses
@@ -247,12 +308,24 @@ struct Unit {  // what a block works on
   int g;    // key head
   int len;  // keys of the batch row
 };
+// Blocks of a key head share its keys (or its queries), so they go to one XCD, whose L2 they meet in; key
+// heads go to the XCDs in turn, so that the heads of a long row of the batch are spread over all of
+// them. Heads of many blocks are spread themselves: what they share is small against their work.
 __device__ __forceinline__ Unit unit_of(const Args& a) {
-  const int64_t block = xcd_block(int(blockIdx.x), int(gridDim.x));
+  const int64_t block = blockIdx.x, parts = a.batch * a.shared * a.splits;
+  int64_t part = block / a.tiles;
   Unit u;
-  const int64_t part = block / a.tiles, bg = part / a.splits;
   u.tile = block - part * a.tiles;
-  u.split = int(part - bg * a.splits);
+  const int64_t whole = parts & ~int64_t(7);  // (the last parts of a count that 8 does not divide: in order)
+  if (a.tiles < 8 && block < whole * a.tiles) {
+    const int64_t i = block >> 3, row = i / a.tiles;
+    part = row * 8 + (block & 7);
+    u.tile = i - row * a.tiles;
+  }
+  // (parts of the sums are the slowest, so that neighbours are of one batch row and other heads)
+  const int64_t heads = a.batch * a.shared;
+  u.split = int(part / heads);
+  const int64_t bg = part - u.split * heads;
   u.b = bg / a.shared;
   u.g = int(bg - u.b * a.shared);
   u.len = a.lengths ? min(max(a.lengths[u.b], 0), a.keys) : a.keys;
@@ -288,35 +361,43 @@ __device__ __forceinline__ const T* v_at(const Args& a, const Unit& u, int64_t k
   return static_cast<const T*>(a.v) + u.b * a.vs[0] + key * a.vs[1] + u.g * a.vs[2];
 }
 
+// Where a wave's 32 rows lie in the two pieces' LDS (SIZE is not less than 64 rows).
+template <typename T, int DP>
+__device__ __forceinline__ int wave_rows() { return int(threadIdx.x >> 6) * 32 * Lds<T, DP>::STRIDE; }
+
 // Blocks of several waves are compiled for two waves on a SIMD where their tiles fit 256 registers: the
 // softmax of one wave then runs beside the products of the other.
 // -------------------------------------------------------------------------------- forward
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 384 ? 2 : 1) void k_attend(Args a) {
-  __shared__ __attribute__((aligned(16))) T lds_k[Lds<T, DP>::SIZE], lds_v[Lds<T, DP>::SIZE];
+  __shared__ __attribute__((aligned(16))) T lds[2 * Lds<T, DP>::SIZE];
+  T *const lds_k = lds, *const lds_v = lds + Lds<T, DP>::SIZE, *const mine = lds + wave_rows<T, DP>();
   const Unit u = unit_of(a);
   const int lane = int(threadIdx.x & 31), half = int(threadIdx.x >> 5 & 1), wave = int(threadIdx.x >> 6);
   const int64_t r = u.tile * (NW * 32) + wave * 32 + lane;
   const bool valid = r < a.rows;
   const QueryRow qr = query_row(a, u, valid ? r : 0);
-  Own<T, DP> q;
-  load_own<T, DP>(q, q_at<T>(a, u, qr), valid, a.dim, half);
   const float c = a.scale * LOG2E;
   f32x16 o[d_tiles<DP>()] = {};
   float top = -INFINITY, sum = 0.f;  // sum: of the keys of this lane's half
-  const int begin = u.split * a.span, end = min(u.len, begin + a.span);
+  const int begin = int(u.split * a.span), end = int(min(int64_t(u.len), begin + a.span));
   Piece<T, DP, NW * 64> pk, pv;
+  const bool fast = pk.HELD && a.fast;
   auto fetch = [&](int k0) {
     const int here = min(PIECE, end - k0);
     const uint32_t ks = uint32_t(a.ks[1]) * uint32_t(sizeof(T)), vs = uint32_t(a.vs[1]) * uint32_t(sizeof(T));
     pk.fetch(k_at<T>(a, u, k0), [&](int i) { return uint32_t(i) * ks; }, here, a.dim);
     pv.fetch(v_at<T>(a, u, k0), [&](int i) { return uint32_t(i) * vs; }, here, a.dim);
   };
-  if (a.fast && begin < end) fetch(begin);
+  Own<T, DP> q;
+  if (begin < end) {
+    if (fast) fetch(begin);
+    load_own<T, DP>(q, q_at<T>(a, u, qr), valid, a.dim, half);
+  }
   for (int k0 = begin; k0 < end; k0 += PIECE) {
     const int here = min(PIECE, end - k0);
     __syncthreads();
-    if (a.fast) {
+    if (fast) {
       pk.commit(lds_k, here, a.dim);
       pv.commit(lds_v, here, a.dim);
     } else {
@@ -324,12 +405,13 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 384 ? 2 : 1) v
       Piece<T, DP, NW * 64>::copy(lds_v, [&](int i) { return v_at<T>(a, u, k0 + i); }, here, a.dim);
     }
     __syncthreads();
-    if (a.fast && k0 + PIECE < end) fetch(k0 + PIECE);
+    if (fast && k0 + PIECE < end) fetch(k0 + PIECE);
     // Scores under the base of earlier pieces need no maximum as long as their powers stay small: a base
     // is a scale, and sums keep their digits under any. The first piece, and one whose powers grow
     // past 2^40, take their maximum as the new base, on scores computed again.
     bool anew = __any(top == -INFINITY);
     for (;;) {
+      asm volatile("" ::: "memory");  // (operands are read in every turn, not held across them)
       f32x16 s[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) s[t] = rows_product<DP>(lds_k + t * 32 * Lds<T, DP>::STRIDE, q, lane, half);
@@ -372,16 +454,16 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 384 ? 2 : 1) v
     }
   }
   sum += __shfl_xor(sum, 32);
-  if (!valid) return;
+  __syncthreads();
   if (a.splits > 1) {
     const int64_t row = ((int64_t(u.split) * a.batch + u.b) * a.shared + u.g) * a.rows + r;
-    if (half == 0) a.part_s[row] = {top, sum};
-    store_row<float, DP>(a.part_o + row * a.dim, o, 1.f, a.dim, half);  // (zeros past the length)
+    if (valid && half == 0) a.part_s[row] = {top, sum};
+    store_rows<T, DP>(a.part_o, row * a.dim, valid, mine, o, 1.f, a.dim, lane, half);  // (zeros past the length)
     return;
   }
   const float inverse = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // (NaN stays NaN)
-  store_row<T, DP>(static_cast<T*>(a.o) + packed_q(a, u, qr), o, inverse, a.dim, half);
-  if (a.stats && half == 0) a.stats[stat_at(a, u, qr)] = {top == -INFINITY ? 0.f : top, inverse};
+  if (valid && a.stats && half == 0) a.stats[stat_at(a, u, qr)] = {top == -INFINITY ? 0.f : top, inverse};
+  store_rows<T, DP>(static_cast<T*>(a.o), packed_q(a, u, qr), valid, mine, o, inverse, a.dim, lane, half);
 }
 
 // The parts of a row, brought under their largest score and summed: a block a row, of 8 groups of 32
@@ -447,7 +529,8 @@ __device__ __forceinline__ float probability(float s, float c, float2 st) {
 // ------------------------------------------------------------------ gradient of the queries
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 320 ? 2 : 1) void k_attend_dq(Args a) {
-  __shared__ __attribute__((aligned(16))) T lds_k[Lds<T, DP>::SIZE], lds_v[Lds<T, DP>::SIZE];
+  __shared__ __attribute__((aligned(16))) T lds[2 * Lds<T, DP>::SIZE];
+  T *const lds_k = lds, *const lds_v = lds + Lds<T, DP>::SIZE, *const mine = lds + wave_rows<T, DP>();
   const Unit u = unit_of(a);
   const int lane = int(threadIdx.x & 31), half = int(threadIdx.x >> 5 & 1), wave = int(threadIdx.x >> 6);
   const int64_t r = u.tile * (NW * 32) + wave * 32 + lane;
@@ -468,24 +551,26 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 320 ? 2 : 1) v
     delta += __shfl_xor(delta, 32);
   }
   const float2 st = exponent<T>(valid ? a.stats[stat_at(a, u, qr)] : float2{0.f, 0.f});
-  if (valid && half == 0) a.delta[stat_at(a, u, qr)] = delta;
+  if (valid && half == 0 && u.split == 0) a.delta[stat_at(a, u, qr)] = delta;
   f32x16 minus_delta;  // where dP starts from, so that P times it is dS
 #pragma unroll
   for (int i = 0; i < 16; ++i) minus_delta[i] = -delta;
   f32x16 dq[d_tiles<DP>()] = {};
   const float c = a.scale * LOG2E;
   Piece<T, DP, NW * 64> pk, pv;
+  const bool fast = pk.HELD && a.fast;
+  const int begin = int(u.split * a.span), end = int(min(int64_t(u.len), begin + a.span));
   auto fetch = [&](int k0) {
-    const int here = min(PIECE, u.len - k0);
+    const int here = min(PIECE, end - k0);
     const uint32_t ks = uint32_t(a.ks[1]) * uint32_t(sizeof(T)), vs = uint32_t(a.vs[1]) * uint32_t(sizeof(T));
     pk.fetch(k_at<T>(a, u, k0), [&](int i) { return uint32_t(i) * ks; }, here, a.dim);
     pv.fetch(v_at<T>(a, u, k0), [&](int i) { return uint32_t(i) * vs; }, here, a.dim);
   };
-  if (a.fast && u.len) fetch(0);
-  for (int k0 = 0; k0 < u.len; k0 += PIECE) {
-    const int here = min(PIECE, u.len - k0);
+  if (fast && begin < end) fetch(begin);
+  for (int k0 = begin; k0 < end; k0 += PIECE) {
+    const int here = min(PIECE, end - k0);
     __syncthreads();
-    if (a.fast) {
+    if (fast) {
       pk.commit(lds_k, here, a.dim);
       pv.commit(lds_v, here, a.dim);
     } else {
@@ -493,7 +578,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 320 ? 2 : 1) v
       Piece<T, DP, NW * 64>::copy(lds_v, [&](int i) { return v_at<T>(a, u, k0 + i); }, here, a.dim);
     }
     __syncthreads();
-    if (a.fast && k0 + PIECE < u.len) fetch(k0 + PIECE);
+    if (fast && k0 + PIECE < end) fetch(k0 + PIECE);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const T* kp = lds_k + t * 32 * Lds<T, DP>::STRIDE;
@@ -509,13 +594,20 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 320 ? 2 : 1) v
       columns_product<DP>(dq, kp, Tile<T>(s), lane, half);
     }
   }
-  if (valid) store_row<T, DP>(static_cast<T*>(a.dq) + packed_q(a, u, qr), dq, a.scale, a.dim, half);
+  __syncthreads();
+  if (a.splits > 1) {
+    float* part = a.part_o + u.split * (a.batch * a.queries * a.heads * a.dim);
+    store_rows<T, DP>(part, packed_q(a, u, qr), valid, mine, dq, a.scale, a.dim, lane, half);
+    return;
+  }
+  store_rows<T, DP>(static_cast<T*>(a.dq), packed_q(a, u, qr), valid, mine, dq, a.scale, a.dim, lane, half);
 }
 
 // --------------------------------------------------------- gradients of the keys and values
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= (sizeof(T) == 2 ? 192 : 256) ? 2 : 1) void k_attend_dkv(Args a) {
-  __shared__ __attribute__((aligned(16))) T lds_q[Lds<T, DP>::SIZE], lds_g[Lds<T, DP>::SIZE];
+  __shared__ __attribute__((aligned(16))) T lds[2 * Lds<T, DP>::SIZE];
+  T *const lds_q = lds, *const lds_g = lds + Lds<T, DP>::SIZE, *const mine = lds + wave_rows<T, DP>();
   __shared__ __attribute__((aligned(16))) float lds_top[PIECE], lds_inverse[PIECE], lds_delta[PIECE];
   const Unit u = unit_of(a);
   const int lane = int(threadIdx.x & 31), half = int(threadIdx.x >> 5 & 1), wave = int(threadIdx.x >> 6);
@@ -528,6 +620,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= (sizeof(T) == 
   const float c = a.scale * LOG2E;
   if (u.tile * (NW * 32) < u.len) {
     Piece<T, DP, NW * 64> pq, pg;
+    const bool fast = pq.HELD && a.fast;
     float2 st = {0.f, 0.f};  // the statistics of the row that this thread stages
     float delta = 0.f;
     const T* grad = static_cast<const T*>(a.grad);
@@ -544,9 +637,10 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= (sizeof(T) == 
       pq.fetch(q0, [&](int i) { return offset(i, qt, qh); }, here, a.dim);
       pg.fetch(g0, [&](int i) { return offset(i, gt, gh); }, here, a.dim);
     };
-    if (a.fast && a.rows) fetch(0);
-    for (int64_t r0 = 0; r0 < a.rows; r0 += PIECE) {
-      const int here = int(min(int64_t(PIECE), a.rows - r0));
+    const int64_t begin = u.split * a.span, end = min(a.rows, begin + a.span);
+    if (fast && begin < end) fetch(begin);
+    for (int64_t r0 = begin; r0 < end; r0 += PIECE) {
+      const int here = int(min(int64_t(PIECE), end - r0));
       if (threadIdx.x < PIECE) {
         st = {0.f, 0.f};
         delta = 0.f;
@@ -557,7 +651,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= (sizeof(T) == 
         }
       }
       __syncthreads();
-      if (a.fast) {
+      if (fast) {
         pq.commit(lds_q, here, a.dim);
         pg.commit(lds_g, here, a.dim);
       } else {
@@ -572,7 +666,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= (sizeof(T) == 
         lds_delta[threadIdx.x] = -delta;
       }
       __syncthreads();
-      if (a.fast && r0 + PIECE < a.rows) fetch(r0 + PIECE);
+      if (fast && r0 + PIECE < end) fetch(r0 + PIECE);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const T *qp = lds_q + t * 32 * Lds<T, DP>::STRIDE, *gp = lds_g + t * 32 * Lds<T, DP>::STRIDE;
@@ -602,14 +696,45 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= (sizeof(T) == 
       }
     }
   }
-  if (key >= a.keys) return;
   if (!valid) {  // past the length: the sums of this lane's column mean nothing
 #pragma unroll
     for (int t = 0; t < d_tiles<DP>(); ++t) dk[t] = dv[t] = f32x16{};
   }
+  const bool row = key < a.keys;
   const int64_t at = ((u.b * a.keys + key) * a.shared + u.g) * a.dim;
-  store_row<T, DP>(static_cast<T*>(a.dk) + at, dk, a.scale, a.dim, half);
-  store_row<T, DP>(static_cast<T*>(a.dv) + at, dv, 1.f, a.dim, half);
+  __syncthreads();
+  if (a.splits > 1) {
+    const int64_t all = a.batch * a.keys * a.shared * a.dim;
+    store_rows<T, DP>(a.part_o + 2 * u.split * all, at, row, mine, dk, a.scale, a.dim, lane, half);
+    store_rows<T, DP>(a.part_o + (2 * u.split + 1) * all, at, row, mine, dv, 1.f, a.dim, lane, half);
+    return;
+  }
+  store_rows<T, DP>(static_cast<T*>(a.dk), at, row, mine, dk, a.scale, a.dim, lane, half);
+  store_rows<T, DP>(static_cast<T*>(a.dv), at, row, mine, dv, 1.f, a.dim, lane, half);
+}
+
+// Parts of one tensor's gradient (blockIdx.y: of two), added in ascending order: out[i] = sum over s of
+// part[s * tensors * n + i].
+template <typename T>
+__global__ __launch_bounds__(256) void k_attend_sum(const float* __restrict__ part, T* __restrict__ first,
+                                                    T* __restrict__ second, int64_t n, int splits) {
+  const int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 4, stride = n * gridDim.y;
+  if (i >= n) return;
+  const float* from = part + blockIdx.y * n + i;
+  T* to = (blockIdx.y ? second : first) + i;
+  if (n % 4 == 0) {
+    f32x4 sum = {};
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) sum += *reinterpret_cast<const f32x4*>(from + s * stride);
+    const float e[4] = {sum[0], sum[1], sum[2], sum[3]};
+    store<T, 4>(to, Vec<T, 4>::of(e));
+    return;
+  }
+  for (int j = 0; j < 4 && i + j < n; ++j) {
+    float sum = 0.f;
+    for (int s = 0; s < splits; ++s) sum += from[s * stride + j];
+    to[j] = from_f32<T>(sum);
+  }
 }
 
 // ---------------------------------------------------------------------------------- host
@@ -625,7 +750,7 @@ int check_args(const char* what, const sihc_attention* a) {
   // row lists and tiles are counted in int32; stats and packed offsets in int64
   const int64_t rows = int64_t(a->queries) * (a->heads / a->kv_heads);
   if (rows >= SIHC_MAX_TOKENS || a->keys >= SIHC_MAX_TOKENS ||
-      (a->batch && (rows / 32 + a->keys / 32 + 2) > 0x7fffffff / (a->batch * a->kv_heads)))
+      (a->batch && (rows / 32 + a->keys / 32 + 2) > (0x7fffffff >> 8) / (a->batch * a->kv_heads)))
     return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
   return SIHC_OK;
 }
@@ -646,7 +771,7 @@ Args args_of(const sihc_attention* s) {
   a.rows = int64_t(a.each) * a.queries;
   a.scale = s->scale;
   a.splits = 1;
-  a.span = INT32_MAX - PIECE;
+  a.span = int64_t(1) << 40;
   // Rows of whole vectors, and offsets within an image's queries, and within a piece of keys, below 2^31.
   const int64_t size = s->dtype == SIHC_DTYPE_F32 ? 4 : 2, most = (int64_t(1) << 31) / size - s->dim;
   auto within = [&](int64_t tokens, int64_t token, int64_t heads, int64_t head) {
@@ -668,12 +793,32 @@ Args args_of(const sihc_attention* s) {
   }
   return a;
 }
-// Few rows leave most of the card idle: then the keys are cut into parts of at least 128, for about
-// 1024 blocks.
-int splits_of(const sihc_attention* s) {
-  const int64_t blocks = s->batch * s->kv_heads * ceil_div(int64_t(s->queries) * (s->heads / s->kv_heads), 32);
-  if (blocks <= 0 || blocks >= 512) return 1;
-  return int(std::max<int64_t>(1, std::min<int64_t>(s->keys / 128, ceil_div(1024, blocks))));
+// Parts of `length` keys or rows for `blocks` blocks of one wave: none where `full` of them fill the card,
+// otherwise for about that many, of at least `least`.
+struct Parts {
+  int count;
+  int64_t span;  // a multiple of PIECE
+};
+Parts parts_of(int64_t length, int64_t blocks, int64_t full, int64_t target, int64_t least) {
+  Parts p{1, ceil_div(std::max<int64_t>(length, 1), PIECE) * PIECE};
+  if (blocks <= 0 || blocks >= full || length <= least) return p;
+  const int64_t most = std::min<int64_t>({ceil_div(target, blocks), ceil_div(length, least), int64_t(256)});
+  p.span = ceil_div(ceil_div(length, most), PIECE) * PIECE;
+  p.count = int(ceil_div(length, p.span));
+  return p;
+}
+int64_t row_count(const sihc_attention* s) { return int64_t(s->queries) * (s->heads / s->kv_heads); }
+int64_t row_blocks(const sihc_attention* s) { return s->batch * s->kv_heads * ceil_div(row_count(s), 32); }
+// fp32 products take 8 times the time of bf16 ones, so parts of one piece are worth their joining.
+int64_t least_part(const sihc_attention* s) { return s->dtype == SIHC_DTYPE_F32 ? PIECE : 2 * PIECE; }
+// Few query rows: the keys in parts, for the forward and for the gradient of the queries.
+Parts forward_parts(const sihc_attention* s) { return parts_of(s->keys, row_blocks(s), 512, 1024, least_part(s)); }
+Parts dq_parts(const sihc_attention* s) { return parts_of(s->keys, row_blocks(s), 256, 512, least_part(s)); }
+// Few keys and many query rows: the rows in parts, for the gradients of keys and values (4 x 16 heads x
+// 4,096 rows over 2,048 keys and 4 key heads, 1024 waves of 32 keys: 463 us in one part, 329 in two,
+// 338 in four).
+Parts dkv_parts(const sihc_attention* s) {
+  return parts_of(row_count(s), s->batch * s->kv_heads * ceil_div(s->keys, 32), 2048, 2048, 2 * least_part(s));
 }
 int64_t query_rows(const sihc_attention* s) { return s->batch * s->heads * int64_t(s->queries); }
 // Calls f(T, DP): the smallest compiled width of a head.
@@ -700,7 +845,7 @@ extern "C" {
 
 size_t sihc_cross_attention_workspace_size(const sihc_attention* s) {
   if (check_args("sihc_cross_attention", s)) return 0;
-  const int splits = splits_of(s);
+  const int splits = forward_parts(s).count;
   return splits > 1 ? size_t(splits) * size_t(query_rows(s)) * size_t(s->dim + 2) * 4 : 0;
 }
 
@@ -717,9 +862,10 @@ int sihc_cross_attention(const sihc_attention* s, const void* q, const void* k, 
     return fail(SIHC_ERR_INVALID, "%s: misaligned workspace or stats", what);
   Args a = args_of(s);
   const int64_t total = query_rows(s);
-  a.splits = splits_of(s);
+  const Parts parts = forward_parts(s);
+  a.splits = parts.count;
+  a.span = parts.span;
   if (a.splits > 1) {
-    a.span = int(ceil_div(ceil_div(s->keys, a.splits), PIECE) * PIECE);
     a.part_s = static_cast<float2*>(workspace);
     a.part_o = reinterpret_cast<float*>(a.part_s + a.splits * total);
   }
@@ -745,9 +891,17 @@ int sihc_cross_attention(const sihc_attention* s, const void* q, const void* k, 
   });
 }
 
+static size_t delta_bytes(const sihc_attention* s) { return size_t(ceil_div(query_rows(s) * 4, 256)) * 256; }
+
 size_t sihc_cross_attention_backward_workspace_size(const sihc_attention* s) {
-  if (!s || s->batch <= 0 || s->queries <= 0 || s->heads <= 0) return 0;
-  return size_t(s->batch) * size_t(s->queries) * size_t(s->heads) * 4;
+  if (check_args("sihc_cross_attention_backward", s)) return 0;
+  // the two gradients' parts follow one another
+  const int q = dq_parts(s).count, kv = dkv_parts(s).count;
+  const size_t q_bytes = q > 1 ? size_t(q) * size_t(query_rows(s)) * size_t(s->dim) * 4 : 0;
+  const size_t kv_bytes =
+      kv > 1 ? size_t(kv) * 2 * size_t(s->batch) * size_t(s->keys) * size_t(s->kv_heads) * size_t(s->dim) * 4 : 0;
+  const size_t sums = std::max(q_bytes, kv_bytes);
+  return delta_bytes(s) + sums;
 }
 
 int sihc_cross_attention_backward(const sihc_attention* s, const void* grad, const void* q, const void* k,
@@ -784,20 +938,35 @@ int sihc_cross_attention_backward(const sihc_attention* s, const void* grad, con
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
     int rc = SIHC_OK;
-    if (a.queries)
-      rc = by_waves(a.rows, a.batch * a.shared, [&](auto nw) {
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(s));
+    auto sum = [&](void* first, void* second, int64_t n) {
+      if (a.splits > 1)
+        hipLaunchKernelGGL(k_attend_sum<T>, dim3(unsigned(ceil_div(n, 1024)), second ? 2 : 1), dim3(256), 0, st, a.part_o,
+                           static_cast<T*>(first), static_cast<T*>(second), n, a.splits);
+    };
+    if (a.queries) {
+      const Parts parts = dq_parts(s);
+      a.splits = parts.count;
+      a.span = parts.span;
+      rc = by_waves(a.rows, a.batch * a.shared * a.splits, [&](auto nw) {
         constexpr int NW = decltype(nw)::value;
         a.tiles = ceil_div(a.rows, NW * 32);
-        hipLaunchKernelGGL((k_attend_dq<T, DP, NW>), dim3(unsigned(a.tiles * a.batch * a.shared)), dim3(NW * 64), 0, st,
-                           a);
+        hipLaunchKernelGGL((k_attend_dq<T, DP, NW>), dim3(unsigned(a.tiles * a.batch * a.shared * a.splits)),
+                           dim3(NW * 64), 0, st, a);
+        sum(grad_q, nullptr, query_rows(s) * a.dim);
         return check_launch(what);
       });
+    }
     if (rc || !a.keys) return rc;
-    return by_waves(a.keys, a.batch * a.shared, [&](auto nw) {
+    const Parts parts = dkv_parts(s);
+    a.splits = parts.count;
+    a.span = parts.span;
+    return by_waves(a.keys, a.batch * a.shared * a.splits, [&](auto nw) {
       constexpr int NW = decltype(nw)::value;
       a.tiles = ceil_div(a.keys, NW * 32);
-      hipLaunchKernelGGL((k_attend_dkv<T, DP, NW>), dim3(unsigned(a.tiles * a.batch * a.shared)), dim3(NW * 64), 0, st,
-                         a);
+      hipLaunchKernelGGL((k_attend_dkv<T, DP, NW>), dim3(unsigned(a.tiles * a.batch * a.shared * a.splits)),
+                         dim3(NW * 64), 0, st, a);
+      sum(grad_k, grad_v, a.batch * a.keys * a.shared * a.dim);
       return check_launch(what);
     });
   });
