@@ -369,21 +369,23 @@ size_t sihc_cross_attention_workspace_size(const sihc_attention *a);
  * with g the key and value head of h. q is [batch, queries, heads, dim], k and v are [batch, keys,
  * kv_heads, dim], strided; out is packed. lengths (int32 [batch], NULL: all keys) are clamped to
  * [0, keys]; a row of length 0 gives zeros, and what k and v hold past a length is not used.
- * stats, if given, receives [batch, heads, queries] pairs (the largest scaled score in units of
- * log 2, the reciprocal of the sum of 2^(score - largest)) for the backward. */
+ * For the backward: stats, if given, receives [batch, heads, queries] pairs (a base of the row's
+ * scaled scores in units of log 2, the reciprocal of the sum of 2^(score - base)); low, if given
+ * (bf16 only), receives what out lost when it was rounded, like out. */
 int sihc_cross_attention(const sihc_attention *a, const void *q, const void *k, const void *v,
-                         const int32_t *lengths, void *out, float *stats, void *workspace,
-                         size_t workspace_bytes, void *stream);
+                         const int32_t *lengths, void *out, float *stats, void *low,
+                         void *workspace, size_t workspace_bytes, void *stream);
 
 size_t sihc_cross_attention_backward_workspace_size(const sihc_attention *a);
-/* Adjoint of sihc_cross_attention from its inputs, output and stats. grad, out and grad_q are
- * packed [batch, queries, heads, dim], grad_k and grad_v packed [batch, keys, kv_heads, dim];
+/* Adjoint of sihc_cross_attention from its inputs, output, stats and low (bf16: required; the row
+ * sums of grad * out are differences' small terms, and out alone carries them to 2^-9 only). grad,
+ * out, low and grad_q are packed [batch, queries, heads, dim], grad_k and grad_v packed [batch, keys, kv_heads, dim];
  * keys past a length get zero gradients. Sums in fp32 in a fixed order, without atomics. */
 int sihc_cross_attention_backward(const sihc_attention *a, const void *grad, const void *q,
                                   const void *k, const void *v, const int32_t *lengths,
-                                  const void *out, const float *stats, void *grad_q, void *grad_k,
-                                  void *grad_v, void *workspace, size_t workspace_bytes,
-                                  void *stream);
+                                  const void *out, const float *stats, const void *low,
+                                  void *grad_q, void *grad_k, void *grad_v, void *workspace,
+                                  size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -32,8 +32,8 @@ constexpr int PIECE = 64;  // rows of the other side in LDS at a time
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Args {
-  const void *q, *k, *v, *grad, *out;
-  void *o, *dq, *dk, *dv;
+  const void *q, *k, *v, *grad, *out, *low;
+  void *o, *o_low, *dq, *dk, *dv;
   const int32_t* lengths;
   float2* stats;
   float* delta;  // [batch, heads, queries] rowsum(dO O)
@@ -82,28 +82,35 @@ __device__ __forceinline__ Vec<T, N> load_some(const T* p, int left) {
   __builtin_memcpy(&v.raw, e, sizeof(e));
   return v;
 }
+// The loads are apart from their use, so that those of several tensors are in flight together: heads of
+// whole vectors load without branches, from places that exist, and take their zeros in own().
 template <typename T, int DP>
-__device__ __forceinline__ void load_own(Own<T, DP>& own, const T* row, bool valid, int dim, int half) {
-  constexpr int N = 16 / int(sizeof(T));  // 8 or 4: the lane's channels of one step
-  constexpr int STEPS = DP / (2 * N);
-  if (dim % N == 0) {  // all loads from places that exist, then the zeros: no branch waits for one
-    Vec<T, N> v[STEPS];
+struct OwnLoads {
+  static constexpr int N = 16 / int(sizeof(T));  // 8 or 4: the lane's channels of one step
+  static constexpr int STEPS = DP / (2 * N);
+  Vec<T, N> v[STEPS];
+  __device__ __forceinline__ OwnLoads(const T* row, bool valid, int dim, int half) {
+    if (dim % N == 0) {
 #pragma unroll
-    for (int k = 0; k < STEPS; ++k) v[k] = load<T, N>(row + min(k * 2 * N + half * N, dim - N));
+      for (int k = 0; k < STEPS; ++k) v[k] = load<T, N>(row + min(k * 2 * N + half * N, dim - N));
+    } else {
+#pragma unroll
+      for (int k = 0; k < STEPS; ++k) {
+        const int c = k * 2 * N + half * N;
+        v[k] = valid ? load_some<T, N>(row + c, dim - c) : Vec<T, N>::zero();
+      }
+    }
+  }
+  __device__ __forceinline__ Own<T, DP> own(bool valid, int dim, int half) const {
+    Own<T, DP> out;
 #pragma unroll
     for (int k = 0; k < STEPS; ++k) {
-      if (!valid || k * 2 * N + half * N >= dim) v[k] = Vec<T, N>::zero();
-      __builtin_memcpy(&own.v[k], &v[k].raw, 16);
+      const u32x4 w = !valid || k * 2 * N + half * N >= dim ? u32x4{} : v[k].raw;
+      __builtin_memcpy(&out.v[k], &w, 16);
     }
-    return;
+    return out;
   }
-#pragma unroll
-  for (int k = 0; k < STEPS; ++k) {
-    const int c = k * 2 * N + half * N;
-    const Vec<T, N> v = valid ? load_some<T, N>(row + c, dim - c) : Vec<T, N>::zero();
-    __builtin_memcpy(&own.v[k], &v.raw, 16);
-  }
-}
+};
 
 // acc[r, own] + sum over channels of piece[r, c] own[c], r one of 32 rows from `piece`.
 template <int DP>
@@ -361,6 +368,13 @@ __device__ __forceinline__ const T* v_at(const Args& a, const Unit& u, int64_t k
   return static_cast<const T*>(a.v) + u.b * a.vs[0] + key * a.vs[1] + u.g * a.vs[2];
 }
 
+// What a value loses when it is stored (an infinity or NaN loses nothing that could be added back).
+template <typename T>
+__device__ __forceinline__ float lost(float v) {
+  const float d = v - to_f32(from_f32<T>(v));
+  return fabsf(d) < INFINITY ? d : 0.f;
+}
+
 // Where a wave's 32 rows lie in the two pieces' LDS (SIZE is not less than 64 rows).
 template <typename T, int DP>
 __device__ __forceinline__ int wave_rows() { return int(threadIdx.x >> 6) * 32 * Lds<T, DP>::STRIDE; }
@@ -391,8 +405,9 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 384 ? 2 : 1) v
   };
   Own<T, DP> q;
   if (begin < end) {
+    const OwnLoads<T, DP> lq(q_at<T>(a, u, qr), valid, a.dim, half);
     if (fast) fetch(begin);
-    load_own<T, DP>(q, q_at<T>(a, u, qr), valid, a.dim, half);
+    q = lq.own(valid, a.dim, half);
   }
   for (int k0 = begin; k0 < end; k0 += PIECE) {
     const int here = min(PIECE, end - k0);
@@ -464,6 +479,13 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 384 ? 2 : 1) v
   const float inverse = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // (NaN stays NaN)
   if (valid && a.stats && half == 0) a.stats[stat_at(a, u, qr)] = {top == -INFINITY ? 0.f : top, inverse};
   store_rows<T, DP>(static_cast<T*>(a.o), packed_q(a, u, qr), valid, mine, o, inverse, a.dim, lane, half);
+  if (sizeof(T) == 2 && a.o_low) {
+#pragma unroll
+    for (int t = 0; t < d_tiles<DP>(); ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[t][i] = lost<T>(o[t][i] * inverse);
+    store_rows<T, DP>(static_cast<T*>(a.o_low), packed_q(a, u, qr), valid, mine, o, 1.f, a.dim, lane, half);
+  }
 }
 
 // The parts of a row, brought under their largest score and summed: a block a row, of 8 groups of 32
@@ -507,10 +529,14 @@ __global__ __launch_bounds__(256) void k_attend_join(Args a, int64_t total) {
   }
   const float inverse = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
   T* to = static_cast<T*>(a.o) + packed_q(a, u, qr) + c;
+  T* low = a.o_low ? static_cast<T*>(a.o_low) + packed_q(a, u, qr) + c : nullptr;
   if (lane * 4 < a.dim)
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (e < n) to[e] = from_f32<T>(o[e] * inverse);
+      if (e < n) {
+        to[e] = from_f32<T>(o[e] * inverse);
+        if (sizeof(T) == 2 && low) low[e] = from_f32<T>(lost<T>(o[e] * inverse));
+      }
   if (a.stats && lane == 0) a.stats[stat_at(a, u, qr)] = {base, inverse};
 }
 
@@ -536,26 +562,12 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 320 ? 2 : 1) v
   const int64_t r = u.tile * (NW * 32) + wave * 32 + lane;
   const bool valid = r < a.rows;
   const QueryRow qr = query_row(a, u, valid ? r : 0);
-  Own<T, DP> q, g;
-  load_own<T, DP>(q, q_at<T>(a, u, qr), valid, a.dim, half);
-  load_own<T, DP>(g, static_cast<const T*>(a.grad) + packed_q(a, u, qr), valid, a.dim, half);
-  float delta = 0.f;
-  {
-    Own<T, DP> o;
-    load_own<T, DP>(o, static_cast<const T*>(a.out) + packed_q(a, u, qr), valid, a.dim, half);
-    constexpr int N = 16 / int(sizeof(T));
-#pragma unroll
-    for (int k = 0; k < DP / (2 * N); ++k)
-#pragma unroll
-      for (int i = 0; i < N; ++i) delta = fmaf(float(g.v[k][i]), float(o.v[k][i]), delta);
-    delta += __shfl_xor(delta, 32);
-  }
-  const float2 st = exponent<T>(valid ? a.stats[stat_at(a, u, qr)] : float2{0.f, 0.f});
-  if (valid && half == 0 && u.split == 0) a.delta[stat_at(a, u, qr)] = delta;
-  f32x16 minus_delta;  // where dP starts from, so that P times it is dS
-#pragma unroll
-  for (int i = 0; i < 16; ++i) minus_delta[i] = -delta;
-  f32x16 dq[d_tiles<DP>()] = {};
+  // everything that the row needs, and the first piece, in flight together
+  const OwnLoads<T, DP> lq(q_at<T>(a, u, qr), valid, a.dim, half);
+  const OwnLoads<T, DP> lg(static_cast<const T*>(a.grad) + packed_q(a, u, qr), valid, a.dim, half);
+  const OwnLoads<T, DP> lo(static_cast<const T*>(a.out) + packed_q(a, u, qr), valid, a.dim, half);
+  const OwnLoads<T, DP> ll(static_cast<const T*>(sizeof(T) == 2 ? a.low : a.out) + packed_q(a, u, qr), valid, a.dim, half);
+  float2 st = valid ? a.stats[stat_at(a, u, qr)] : float2{0.f, 0.f};
   const float c = a.scale * LOG2E;
   Piece<T, DP, NW * 64> pk, pv;
   const bool fast = pk.HELD && a.fast;
@@ -567,6 +579,28 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 320 ? 2 : 1) v
     pv.fetch(v_at<T>(a, u, k0), [&](int i) { return uint32_t(i) * vs; }, here, a.dim);
   };
   if (fast && begin < end) fetch(begin);
+  const Own<T, DP> q = lq.own(valid, a.dim, half), g = lg.own(valid, a.dim, half);
+  float delta = 0.f;
+  {
+    // dP - delta is small where one key has most of a row, so delta is summed over the output as it was
+    // before its rounding
+    const Own<T, DP> o = lo.own(valid, a.dim, half), low = ll.own(valid, a.dim, half);
+    constexpr int N = 16 / int(sizeof(T));
+#pragma unroll
+    for (int k = 0; k < DP / (2 * N); ++k)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float whole = sizeof(T) == 2 ? float(o.v[k][i]) + float(low.v[k][i]) : float(o.v[k][i]);
+        delta = fmaf(float(g.v[k][i]), whole, delta);
+      }
+    delta += __shfl_xor(delta, 32);
+  }
+  st = exponent<T>(st);
+  if (valid && half == 0 && u.split == 0) a.delta[stat_at(a, u, qr)] = delta;
+  f32x16 minus_delta;  // where dP starts from, so that P times it is dS
+#pragma unroll
+  for (int i = 0; i < 16; ++i) minus_delta[i] = -delta;
+  f32x16 dq[d_tiles<DP>()] = {};
   for (int k0 = begin; k0 < end; k0 += PIECE) {
     const int here = min(PIECE, end - k0);
     __syncthreads();
@@ -613,9 +647,9 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= (sizeof(T) == 
   const int lane = int(threadIdx.x & 31), half = int(threadIdx.x >> 5 & 1), wave = int(threadIdx.x >> 6);
   const int64_t key = u.tile * (NW * 32) + wave * 32 + lane;
   const bool valid = key < u.len;
-  Own<T, DP> k, v;
-  load_own<T, DP>(k, k_at<T>(a, u, valid ? key : 0), valid, a.dim, half);
-  load_own<T, DP>(v, v_at<T>(a, u, valid ? key : 0), valid, a.dim, half);
+  const OwnLoads<T, DP> lk(k_at<T>(a, u, valid ? key : 0), valid, a.dim, half);
+  const OwnLoads<T, DP> lv(v_at<T>(a, u, valid ? key : 0), valid, a.dim, half);
+  const Own<T, DP> k = lk.own(valid, a.dim, half), v = lv.own(valid, a.dim, half);
   f32x16 dk[d_tiles<DP>()] = {}, dv[d_tiles<DP>()] = {};
   const float c = a.scale * LOG2E;
   if (u.tile * (NW * 32) < u.len) {
@@ -850,7 +884,7 @@ size_t sihc_cross_attention_workspace_size(const sihc_attention* s) {
 }
 
 int sihc_cross_attention(const sihc_attention* s, const void* q, const void* k, const void* v, const int32_t* lengths,
-                         void* out, float* stats, void* workspace, size_t workspace_bytes, void* stream) {
+                         void* out, float* stats, void* low, void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "sihc_cross_attention";
   if (int rc = check_args(what, s)) return rc;
   if (s->batch == 0 || s->queries == 0) return SIHC_OK;
@@ -874,6 +908,7 @@ int sihc_cross_attention(const sihc_attention* s, const void* q, const void* k, 
   a.v = v;
   a.lengths = lengths;
   a.o = out;
+  a.o_low = low;
   a.stats = reinterpret_cast<float2*>(stats);
   return by_width(s, [&](auto t, auto dp) {
     using T = decltype(t);
@@ -906,14 +941,14 @@ size_t sihc_cross_attention_backward_workspace_size(const sihc_attention* s) {
 
 int sihc_cross_attention_backward(const sihc_attention* s, const void* grad, const void* q, const void* k,
                                   const void* v, const int32_t* lengths, const void* out, const float* stats,
-                                  void* grad_q, void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes,
-                                  void* stream) {
+                                  const void* low, void* grad_q, void* grad_k, void* grad_v, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
   const char* what = "sihc_cross_attention_backward";
   if (int rc = check_args(what, s)) return rc;
   if (s->batch == 0) return SIHC_OK;
-  if (s->queries && (!grad || !q || !out || !stats || !grad_q)) return fail(SIHC_ERR_INVALID, "%s: null pointer", what);
+  if (s->queries && (!grad || !q || !out || !stats || !grad_q || (s->dtype == SIHC_DTYPE_BF16 && !low))) return fail(SIHC_ERR_INVALID, "%s: null pointer", what);
   if (s->keys && (!k || !v || !grad_k || !grad_v)) return fail(SIHC_ERR_INVALID, "%s: null pointer", what);
-  for (const void* in : {grad, q, k, v, out})
+  for (const void* in : {grad, q, k, v, out, low})
     for (const void* to : {grad_q, grad_k, grad_v})
       if (in && in == to) return fail(SIHC_ERR_INVALID, "%s: an output is one of the inputs", what);
   const size_t need = sihc_cross_attention_backward_workspace_size(s);
@@ -927,6 +962,7 @@ int sihc_cross_attention_backward(const sihc_attention* s, const void* grad, con
   a.v = v;
   a.grad = grad;
   a.out = out;
+  a.low = low;
   a.dq = grad_q;
   a.dk = grad_k;
   a.dv = grad_v;

@@ -722,42 +722,49 @@ sihc_attention attention_of(const Tensor& q, const Tensor& k, const Tensor& v, d
   a.dtype = dtype_code(q);
   return a;
 }
-variable_list run_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths, double scale) {
+// (out, statistics, what out lost in rounding): the latter two empty unless `train`
+variable_list run_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths, double scale,
+                            bool train) {
   const c10::DeviceGuard guard(q.device());
   const sihc_attention a = attention_of(q, k, v, scale);
+  const bool rounded = train && q.scalar_type() == at::kBFloat16;
   Tensor out = at::empty(q.sizes(), q.options()), ws;
-  Tensor stats = at::empty({q.size(0), q.size(2), q.size(1), 2}, q.options().dtype(at::kFloat));
+  Tensor stats = train ? at::empty({q.size(0), q.size(2), q.size(1), 2}, q.options().dtype(at::kFloat))
+                       : at::empty({0}, q.options().dtype(at::kFloat));
+  Tensor low = rounded ? at::empty(q.sizes(), q.options()) : at::empty({0}, q.options());
   const size_t bytes = sihc_cross_attention_workspace_size(&a);
   if (bytes) ws = workspace(bytes, q);
   check(sihc_cross_attention(&a, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), index_ptr(lengths),
-                             out.data_ptr(), stats.data_ptr<float>(), bytes ? ws.data_ptr() : nullptr, bytes,
-                             stream_of(q)),
+                             out.data_ptr(), train ? stats.data_ptr<float>() : nullptr,
+                             rounded ? low.data_ptr() : nullptr, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q)),
         true);
-  return {out, stats};
+  return {out, stats, low};
 }
 struct AttentionFn : torch::autograd::Function<AttentionFn> {
   static constexpr bool is_traceable = true;
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
-                               const std::optional<Tensor>& lengths, double scale) {
+                               const std::optional<Tensor>& lengths, double scale, bool train) {
     const Tensor n = lengths.value_or(Tensor());
-    variable_list out = run_attention(q, k, v, n, scale);
-    ctx->mark_non_differentiable({out[1]});
+    variable_list out = run_attention(q, k, v, n, scale, train);
+    ctx->mark_non_differentiable({out[1], out[2]});
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({q, k, v, n, out[0], out[1]});
+    ctx->save_for_backward({q, k, v, n, out[0], out[1], out[2]});
     ctx->saved_data["scale"] = scale;
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &n = saved[3], &out = saved[4], &stats = saved[5];
-    if (!grads[0].defined()) return variable_list(5);
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &n = saved[3], &out = saved[4], &stats = saved[5],
+                 &low = saved[6];
+    if (!grads[0].defined()) return variable_list(6);
     const Tensor grad = grads[0].contiguous();
     const double scale = ctx->saved_data["scale"].toDouble();
     Tensor dq, dk, dv;
     if (direct() && attention_fits(q, k, v, n) && same(grad, out) && grad.sizes().equals(q.sizes()) &&
         grad.scalar_type() == q.scalar_type() && grad.device() == q.device() &&
+        (q.scalar_type() == at::kFloat || same(low, out)) &&
         stats_fits(stats, {q.size(0), q.size(2), q.size(1), 2}, q)) {
-      RECORD_FUNCTION("sihc::cross_attention_backward", (Args{grad, q, k, v, maybe(n), out, stats, scale}));
+      RECORD_FUNCTION("sihc::cross_attention_backward", (Args{grad, q, k, v, maybe(n), out, stats, low, scale}));
       const c10::DeviceGuard device(q.device());
       const sihc_attention a = attention_of(q, k, v, scale);
       dq = at::empty(q.sizes(), q.options());
@@ -766,16 +773,18 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
       const Tensor ws = workspace(sihc_cross_attention_backward_workspace_size(&a), q);
       check(sihc_cross_attention_backward(&a, grad.const_data_ptr(), q.const_data_ptr(), k.const_data_ptr(),
                                           v.const_data_ptr(), index_ptr(n), out.const_data_ptr(),
-                                          stats.const_data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                                          ws.data_ptr(), size_t(ws.numel()) * 4, stream_of(q)),
+                                          stats.const_data_ptr<float>(),
+                                          q.scalar_type() == at::kFloat ? nullptr : low.const_data_ptr(),
+                                          dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(),
+                                          size_t(ws.numel()) * 4, stream_of(q)),
             false);
     } else {
       static auto op = registered<std::tuple<Tensor, Tensor, Tensor>(
           const Tensor&, const Tensor&, const Tensor&, const Tensor&, const std::optional<Tensor>&, const Tensor&,
-          const Tensor&, double)>("sihc::cross_attention_backward");
-      std::tie(dq, dk, dv) = op.call(grad, q, k, v, maybe(n), out, stats, scale);
+          const Tensor&, const Tensor&, double)>("sihc::cross_attention_backward");
+      std::tie(dq, dk, dv) = op.call(grad, q, k, v, maybe(n), out, stats, low, scale);
     }
-    return {dq, dk, dv, Tensor(), Tensor()};
+    return {dq, dk, dv, Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -967,10 +976,10 @@ bool unwrap_integer(PyObject* o, int64_t& v) {
   PyErr_Clear();
   return false;
 }
-PyObject* pair_of(const variable_list& ts) {
-  PyObject* pair = PyTuple_New(2);
-  for (int i = 0; pair && i < 2; ++i) PyTuple_SET_ITEM(pair, i, THPVariable_Wrap(ts[size_t(i)]));
-  return pair;
+PyObject* tuple_of(const variable_list& ts) {
+  PyObject* tuple = PyTuple_New(Py_ssize_t(ts.size()));
+  for (size_t i = 0; tuple && i < ts.size(); ++i) PyTuple_SET_ITEM(tuple, Py_ssize_t(i), THPVariable_Wrap(ts[i]));
+  return tuple;
 }
 PyObject* py_embed(PyObject* self, PyObject* const* args, Py_ssize_t n) {
   if (n != 4) return not_implemented();
@@ -998,14 +1007,15 @@ PyObject* py_norm(PyObject* self, PyObject* const* args, Py_ssize_t n) {
     if (!unwrap(args[0], x) || !unwrap(args[1], weight) || !unwrap(args[2], bias) ||
         !unwrap_integer(args[3], groups) || !unwrap_number(args[4], eps) || !norm_fits(x, weight, bias, groups))
       return not_implemented();
-    return pair_of(call(self, [&] { return Args{x, weight, bias, groups, eps, act}; }, [&] {
+    return tuple_of(call(self, [&] { return Args{x, weight, bias, groups, eps, act}; }, [&] {
       return unrecorded() ? run_norm(x, weight, bias, groups, eps, act)
                           : NormFn::apply(x, weight, bias, groups, eps, act);
     }));
   });
 }
 PyObject* py_attention(PyObject* self, PyObject* const* args, Py_ssize_t n) {
-  if (n != 5) return not_implemented();
+  if (n != 6 || !PyBool_Check(args[5])) return not_implemented();
+  const bool train = args[5] == Py_True;
   return guarded(self, [&]() -> PyObject* {
     Tensor q, k, v, lengths;
     double scale;
@@ -1013,9 +1023,9 @@ PyObject* py_attention(PyObject* self, PyObject* const* args, Py_ssize_t n) {
         (args[3] != Py_None && !unwrap(args[3], lengths)) || !unwrap_number(args[4], scale) ||
         !attention_fits(q, k, v, lengths))
       return not_implemented();
-    return pair_of(call(self, [&] { return Args{q, k, v, maybe(lengths), scale}; }, [&] {
-      return unrecorded() ? run_attention(q, k, v, lengths, scale)
-                          : AttentionFn::apply(q, k, v, maybe(lengths), scale);
+    return tuple_of(call(self, [&] { return Args{q, k, v, maybe(lengths), scale, train}; }, [&] {
+      return unrecorded() || !train ? run_attention(q, k, v, lengths, scale, train)
+                                    : AttentionFn::apply(q, k, v, maybe(lengths), scale, train);
     }));
   });
 }

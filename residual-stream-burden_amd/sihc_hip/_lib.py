@@ -84,10 +84,10 @@ PROTOTYPES: dict[str, tuple] = {
     "sihc_group_norm_backward": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _i32,
                                         _i32, _vp, _sz, _vp]),
     "sihc_cross_attention_workspace_size": (_sz, [_attp]),
-    "sihc_cross_attention": (_i32, [_attp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "sihc_cross_attention": (_i32, [_attp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "sihc_cross_attention_backward_workspace_size": (_sz, [_attp]),
-    "sihc_cross_attention_backward": (_i32, [_attp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
-                                             _vp]),
+    "sihc_cross_attention_backward": (_i32, [_attp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                             _sz, _vp]),
     "sihc_fma_rate": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp]),
 }
 

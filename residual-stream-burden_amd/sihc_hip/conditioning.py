@@ -204,47 +204,51 @@ def _check_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor])
 
 
 @custom_op("sihc::cross_attention", mutates_args=())
-def _cross_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor],
-                     scale: float) -> tuple[Tensor, Tensor]:
+def _cross_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor], scale: float,
+                     train: bool) -> tuple[Tensor, Tensor, Tensor]:
     _check_attention(q, k, v, lengths)
-    return launch.cross_attention(q, k, v, lengths, scale)
+    return launch.cross_attention(q, k, v, lengths, scale, train)
 
 
 @_cross_attention.register_fake
-def _cross_attention_fake(q, k, v, lengths, scale):
+def _cross_attention_fake(q, k, v, lengths, scale, train):
     b, n, h, _ = q.shape
-    return q.new_empty(q.shape), q.new_empty((b, h, n, 2), dtype=torch.float32)
+    return (q.new_empty(q.shape), q.new_empty((b, h, n, 2) if train else (0,), dtype=torch.float32),
+            q.new_empty(q.shape if train and q.dtype == torch.bfloat16 else (0,)))
 
 
 @custom_op("sihc::cross_attention_backward", mutates_args=())
 def _cross_attention_backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor], out: Tensor,
-                              stats: Tensor, scale: float) -> tuple[Tensor, Tensor, Tensor]:
+                              stats: Tensor, low: Tensor, scale: float) -> tuple[Tensor, Tensor, Tensor]:
     _check_attention(q, k, v, lengths)  # saved tensors come back through the caller's hooks
-    _require_packed("cross_attention backward", grad=grad, out=out, stats=stats)
+    _require_packed("cross_attention backward", grad=grad, out=out, stats=stats, low=low)
     b, n, h, _ = q.shape
-    if any(t.shape != q.shape or t.dtype != q.dtype for t in (grad, out)) or stats.shape != (b, h, n, 2):
-        raise ValueError("cross_attention backward: the output gradient must match the output")
-    _require_gpu("cross_attention backward", q, grad=grad, out=out, stats=stats)
-    return launch.cross_attention_backward(grad, q, k, v, lengths, out, stats, scale)
+    like = (grad, out, low) if q.dtype == torch.bfloat16 else (grad, out)
+    if any(t.shape != q.shape or t.dtype != q.dtype for t in like) or stats.shape != (b, h, n, 2):
+        raise ValueError("cross_attention backward: the gradient and the saved tensors must match the output of a "
+                         "call with train=True")
+    _require_gpu("cross_attention backward", q, grad=grad, out=out, stats=stats, low=low)
+    return launch.cross_attention_backward(grad, q, k, v, lengths, out, stats, low, scale)
 
 
 @_cross_attention_backward.register_fake
-def _cross_attention_backward_fake(grad, q, k, v, lengths, out, stats, scale):
+def _cross_attention_backward_fake(grad, q, k, v, lengths, out, stats, low, scale):
     return tuple(t.new_empty(t.shape) for t in (q, k, v))
 
 
 def _attention_setup(ctx, inputs, output):
-    q, k, v, lengths, ctx.scale = inputs
-    ctx.mark_non_differentiable(output[1])
+    q, k, v, lengths, ctx.scale, _ = inputs
+    ctx.mark_non_differentiable(output[1], output[2])
     ctx.set_materialize_grads(False)
     ctx.save_for_backward(q, k, v, lengths, *output)
 
 
-def _attention_autograd(ctx, grad, _):
+def _attention_autograd(ctx, grad, _, __):
     if grad is None:
-        return (None,) * 5
-    q, k, v, lengths, out, stats = ctx.saved_tensors
-    return (*_cross_attention_backward(grad.contiguous(), q, k, v, lengths, out, stats, ctx.scale), None, None)
+        return (None,) * 6
+    q, k, v, lengths, out, stats, low = ctx.saved_tensors
+    return (*_cross_attention_backward(grad.contiguous(), q, k, v, lengths, out, stats, low, ctx.scale), None, None,
+            None)
 
 
 register_autograd(_cross_attention, _attention_autograd, setup_context=_attention_setup)
@@ -261,7 +265,8 @@ def cross_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor] =
             low, high = int(lengths.min()), int(lengths.max())
             if low < 0 or high > k.shape[1]:
                 raise ValueError(f"lengths must lie in [0, {k.shape[1]}], got [{low}, {high}]")
-    return _cross_attention(q, k, v, lengths, 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale)[0]
+    train = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    return _cross_attention(q, k, v, lengths, 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale, train)[0]
 
 
 __all__ = ["embedding_lookup", "cross_attention", "group_norm_act"]

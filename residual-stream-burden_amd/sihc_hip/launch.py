@@ -362,29 +362,33 @@ def _attention(q: Tensor, k: Tensor, v: Tensor, scale: float) -> Attention:
 
 
 @_on_tensor_device
-def cross_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor],
-                    scale: float) -> tuple[Tensor, Tensor]:
-    """(attention of q [B,Lq,H,D] over k, v [B,Lk,KH,D], [B,H,Lq,2] softmax statistics)."""
+def cross_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor], scale: float,
+                    train: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """(attention of q [B,Lq,H,D] over k, v [B,Lk,KH,D], and for the backward [B,H,Lq,2] softmax statistics
+    and, in bf16, what the output lost in rounding; both empty unless `train`)."""
     out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    stats = torch.empty((q.shape[0], q.shape[2], q.shape[1], 2), device=q.device, dtype=torch.float32)
+    stats = torch.empty((q.shape[0], q.shape[2], q.shape[1], 2) if train else (0,), device=q.device,
+                        dtype=torch.float32)
+    low = torch.empty(q.shape if train and q.dtype == torch.bfloat16 else (0,), device=q.device, dtype=q.dtype)
     L, a = lib(), _attention(q, k, v, scale)
     nbytes = L.sihc_cross_attention_workspace_size(ctypes.byref(a))
     ws = _workspace(nbytes, q.device) if nbytes else None
     check(L.sihc_cross_attention(ctypes.byref(a), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(lengths),
-                                 out.data_ptr(), stats.data_ptr(), _ptr(ws), nbytes, _stream(q.device)))
-    return out, stats
+                                 out.data_ptr(), stats.data_ptr() or None, low.data_ptr() or None, _ptr(ws), nbytes,
+                                 _stream(q.device)))
+    return out, stats, low
 
 
 @_on_tensor_device
 def cross_attention_backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, lengths: Optional[Tensor], out: Tensor,
-                             stats: Tensor, scale: float) -> tuple[Tensor, Tensor, Tensor]:
+                             stats: Tensor, low: Tensor, scale: float) -> tuple[Tensor, Tensor, Tensor]:
     """(query, key, value gradients) of cross_attention, packed."""
     dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
     L, a = lib(), _attention(q, k, v, scale)
     ws = _workspace(L.sihc_cross_attention_backward_workspace_size(ctypes.byref(a)), q.device)
     check(L.sihc_cross_attention_backward(ctypes.byref(a), grad.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                                          _ptr(lengths), out.data_ptr(), stats.data_ptr(), dq.data_ptr(),
-                                          dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws.numel() * 4,
+                                          _ptr(lengths), out.data_ptr(), stats.data_ptr(), low.data_ptr() or None,
+                                          dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws.numel() * 4,
                                           _stream(q.device)))
     return dq, dk, dv
 

@@ -61,7 +61,7 @@ def test_cross_attention_arguments():
                       v_stride=three, scale=1.0, dtype=1)
         return ctypes.byref(_lib.Attention(*{**values, **over}.values()))
 
-    call = lambda a, q=FAKE: L.sihc_cross_attention(a, q, FAKE, FAKE, None, FAKE, None, None, 0, None)  # noqa: E731
+    call = lambda a, q=FAKE: L.sihc_cross_attention(a, q, FAKE, FAKE, None, FAKE, None, None, None, 0, None)  # noqa: E731
     refused(call(sizes(heads=3)), b"do not share")
     refused(call(sizes(dim=129)), b"at most 128")
     refused(call(sizes(dtype=3)), b"bad dtype")
@@ -70,8 +70,8 @@ def test_cross_attention_arguments():
     refused(call(sizes(), None), b"null pointer")
     refused(call(None), b"null sizes")
     assert call(sizes(batch=0)) == 0
-    back = lambda a, dq, n: L.sihc_cross_attention_backward(a, FAKE, FAKE, FAKE, FAKE, None, FAKE, FAKE, dq,  # noqa: E731
-                                                            FAKE * 2, FAKE * 3, FAKE, n, None)
+    back = lambda a, dq, n: L.sihc_cross_attention_backward(a, FAKE, FAKE, FAKE, FAKE, None, FAKE, FAKE, FAKE,  # noqa: E731
+                                                            dq, FAKE * 2, FAKE * 3, FAKE, n, None)
     need = L.sihc_cross_attention_backward_workspace_size(sizes())
     assert need >= 2 * 4 * 4 * 4
     refused(back(sizes(), FAKE * 4, need - 1), b"workspace of")

@@ -25,8 +25,8 @@ def cases():
     yield conditioning._embedding_lookup, [normal(50, 24, dtype=torch.bfloat16)], (ids.int(), 2, -1)
     yield conditioning._group_norm_act, [normal(2, 5, 5, 24, dtype=torch.bfloat16), normal(24), normal(24)], (4, 1e-6, "silu")
     yield conditioning._group_norm_act, [normal(2, 25, 24), normal(24), normal(24)], (4, 1e-6, "none")
-    yield conditioning._cross_attention, [normal(2, 11, 4, 40, dtype=torch.bfloat16), kv[:, :, 0], kv[:, :, 1]], (n, 0.2)
-    yield conditioning._cross_attention, [normal(2, 11, 4, 40), normal(2, 3, 2, 40), normal(2, 3, 2, 40)], (None, 0.2)
+    yield conditioning._cross_attention, [normal(2, 11, 4, 40, dtype=torch.bfloat16), kv[:, :, 0], kv[:, :, 1]], (n, 0.2, True)
+    yield conditioning._cross_attention, [normal(2, 11, 4, 40), normal(2, 3, 2, 40), normal(2, 3, 2, 40)], (None, 0.2, True)
 
 
 def passed(op, leaves, rest, call):
@@ -47,7 +47,7 @@ def test_same_bits_as_the_registered_ops(monkeypatch):
         assert taken and taken[0] is not NotImplemented, op
         plain = passed(op, leaves, rest, lambda *a: CustomOpDef.__call__(op, *a))
         assert len(native) == len(plain) and all(torch.equal(a, b) for a, b in zip(native, plain)), op
-        with torch.no_grad():
+        with torch.no_grad():  # (train=True: all outputs are filled)
             again = op(*leaves, *rest)
         again = again if isinstance(again, tuple) else (again,)
         assert all(torch.equal(a, b) for a, b in zip(again, native))
@@ -61,8 +61,11 @@ def test_stats_carry_no_gradient_and_unused_inputs_none():
     assert y.requires_grad and not stats.requires_grad
     assert torch.autograd.grad(y.sum(), x)[0].shape == x.shape  # (only x asks for a gradient)
     q = torch.randn(1, 2, 1, 8, device="cuda", requires_grad=True)
-    out, stats = conditioning._cross_attention(q, q.detach(), q.detach(), None, 1.0)
-    assert out.requires_grad and not stats.requires_grad
+    out, stats, low = conditioning._cross_attention(q, q.detach(), q.detach(), None, 1.0, True)
+    assert out.requires_grad and not stats.requires_grad and not low.requires_grad
+    # a call that is not to be differentiated keeps nothing, and says so when it is
+    out, stats, low = conditioning._cross_attention(q.detach(), q.detach(), q.detach(), None, 1.0, False)
+    assert not out.requires_grad and not stats.numel() and not low.numel()
 
 
 def test_modes_hooks_and_bad_arguments_reach_the_registered_ops():
