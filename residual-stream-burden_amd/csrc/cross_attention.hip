@@ -42,6 +42,7 @@ struct Args {
   int queries, keys, heads, shared, each, dim;
   int64_t rows;   // query rows of a key head: each * queries
   int64_t tiles;  // blocks of a key head (in the forward, of one part of its keys)
+  int cluster;       // (unit_of)
   int splits;        // parts of a key head's keys (forward) or query rows (key and value gradients)
   int64_t span;      // keys or rows of a part, a multiple of PIECE
   float* part_o;     // where there are several: [splits][batch, key head][rows][dim] sums (forward), or
@@ -315,19 +316,20 @@ struct Unit {  // what a block works on
   int g;    // key head
   int len;  // keys of the batch row
 };
-// Blocks of a key head share its keys (or its queries), so they go to one XCD, whose L2 they meet in; key
-// heads go to the XCDs in turn, so that the heads of a long row of the batch are spread over all of
-// them. Heads of many blocks are spread themselves: what they share is small against their work.
+// Blocks of a key head share its keys (or its queries), and neighbouring heads the lines at the ends of
+// their rows' pieces, so `cluster` heads go to one XCD, whose L2 they meet in; the clusters go to the
+// XCDs in turn, so that the rows of the batch, of different lengths, are spread over all of them.
+// Heads of many blocks are spread themselves: what they share is small against their work.
 __device__ __forceinline__ Unit unit_of(const Args& a) {
   const int64_t block = blockIdx.x, parts = a.batch * a.shared * a.splits;
   int64_t part = block / a.tiles;
   Unit u;
   u.tile = block - part * a.tiles;
-  const int64_t whole = parts & ~int64_t(7);  // (the last parts of a count that 8 does not divide: in order)
+  const int64_t round = 8 * a.cluster, whole = parts - parts % round;  // (the last parts: in order)
   if (a.tiles < 8 && block < whole * a.tiles) {
-    const int64_t i = block >> 3, row = i / a.tiles;
-    part = row * 8 + (block & 7);
-    u.tile = i - row * a.tiles;
+    const int64_t i = block >> 3, in = i / a.tiles, row = in / a.cluster;  // of this XCD: part and round
+    part = row * round + (block & 7) * a.cluster + (in - row * a.cluster);
+    u.tile = i - in * a.tiles;
   }
   // (parts of the sums are the slowest, so that neighbours are of one batch row and other heads)
   const int64_t heads = a.batch * a.shared;
@@ -379,11 +381,11 @@ __device__ __forceinline__ float lost(float v) {
 template <typename T, int DP>
 __device__ __forceinline__ int wave_rows() { return int(threadIdx.x >> 6) * 32 * Lds<T, DP>::STRIDE; }
 
-// Blocks of several waves are compiled for two waves on a SIMD where their tiles fit 256 registers: the
-// softmax of one wave then runs beside the products of the other.
+// Blocks of several waves are compiled for two waves on a SIMD where their tiles fit 256 registers, three
+// where they fit 168: the softmax of one wave then runs beside the products of another.
 // -------------------------------------------------------------------------------- forward
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 384 ? 2 : 1) void k_attend(Args a) {
+__global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 384 ? (sizeof(T) * DP <= 160 && sizeof(T) == 2 ? 3 : 2) : 1) void k_attend(Args a) {
   __shared__ __attribute__((aligned(16))) T lds[2 * Lds<T, DP>::SIZE];
   T *const lds_k = lds, *const lds_v = lds + Lds<T, DP>::SIZE, *const mine = lds + wave_rows<T, DP>();
   const Unit u = unit_of(a);
@@ -671,19 +673,19 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= (sizeof(T) == 
       pq.fetch(q0, [&](int i) { return offset(i, qt, qh); }, here, a.dim);
       pg.fetch(g0, [&](int i) { return offset(i, gt, gh); }, here, a.dim);
     };
+    // the statistics of the piece's row that this thread stages, from a row that exists
+    auto fetch_stats = [&](int64_t r0) {
+      const int64_t at = stat_at(a, u, query_row(a, u, min(r0 + int(threadIdx.x), a.rows - 1)));
+      st = a.stats[at];
+      delta = a.delta[at];
+    };
     const int64_t begin = u.split * a.span, end = min(a.rows, begin + a.span);
-    if (fast && begin < end) fetch(begin);
+    if (begin < end) {
+      if (fast) fetch(begin);
+      fetch_stats(begin);
+    }
     for (int64_t r0 = begin; r0 < end; r0 += PIECE) {
       const int here = int(min(int64_t(PIECE), end - r0));
-      if (threadIdx.x < PIECE) {
-        st = {0.f, 0.f};
-        delta = 0.f;
-        if (int(threadIdx.x) < here) {
-          const int64_t at = stat_at(a, u, query_row(a, u, r0 + threadIdx.x));
-          st = a.stats[at];
-          delta = a.delta[at];
-        }
-      }
       __syncthreads();
       if (fast) {
         pq.commit(lds_q, here, a.dim);
@@ -694,13 +696,18 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= (sizeof(T) == 
             lds_g, [&](int i) { return grad + packed_q(a, u, query_row(a, u, r0 + i)); }, here, a.dim);
       }
       if (threadIdx.x < PIECE) {
-        const float2 e = exponent<T>(st);
+        // (a row past the end: no probability)
+        const bool in = int(threadIdx.x) < here;
+        const float2 e = exponent<T>(in ? st : float2{0.f, 0.f});
         lds_top[threadIdx.x] = e.x;
         lds_inverse[threadIdx.x] = e.y;
-        lds_delta[threadIdx.x] = -delta;
+        lds_delta[threadIdx.x] = in ? -delta : 0.f;
       }
       __syncthreads();
-      if (fast && r0 + PIECE < end) fetch(r0 + PIECE);
+      if (r0 + PIECE < end) {
+        if (fast) fetch(r0 + PIECE);
+        fetch_stats(r0 + PIECE);
+      }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const T *qp = lds_q + t * 32 * Lds<T, DP>::STRIDE, *gp = lds_g + t * 32 * Lds<T, DP>::STRIDE;
@@ -804,6 +811,14 @@ Args args_of(const sihc_attention* s) {
   a.dim = s->dim;
   a.rows = int64_t(a.each) * a.queries;
   a.scale = s->scale;
+  a.cluster = 1;
+  // as long as every XCD takes 16 clusters (64 x 16 heads of 72 channels, 256 rows over up to 256 keys:
+  // forward and gradients 237 us by single heads, 224 by 2, 215 by 4, 227 by 8)
+  for (int n : {4, 2})
+    if (s->kv_heads % n == 0 && s->batch * s->kv_heads / n >= 128) {
+      a.cluster = n;
+      break;
+    }
   a.splits = 1;
   a.span = int64_t(1) << 40;
   // Rows of whole vectors, and offsets within an image's queries, and within a piece of keys, below 2^31.
