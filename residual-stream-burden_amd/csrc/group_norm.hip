@@ -23,8 +23,9 @@ struct Shape {
   int slice_groups, W;       // groups and channels of a block's slice
   int threads;               // of a block
   int lanes, rows;           // vectors of a slice's pixel; pixels a block loads at once
-  int chunks;                // blocks that share a slice
-  int64_t chunk_pixels;
+  // rows of whole pixels (the streaming kernels): an image in chunks, a pixel in `widths` of W channels
+  int widths, chunks;
+  int64_t span;  // pixels of a chunk
   float eps;
   bool silu;
 };
@@ -33,35 +34,6 @@ struct Shape {
 __device__ __forceinline__ float rounded_product(float a, float b) {
 #pragma clang fp contract(off)
   return a * b;
-}
-
-// The two launches over slices in chunks.
-enum { STATS, APPLY };
-
-// Sum of v over the threads of each group of the slice, left in out[group] (and visible to all).
-__device__ __forceinline__ void group_sums(float v, const Shape& s, float* scratch, float* out) {
-  const int tid = int(threadIdx.x);
-  __syncthreads();  // earlier readers of scratch and out are done
-  if (s.slice_groups == 1) {
-    const float t = wave_sum(v);
-    if ((tid & 63) == 0) scratch[tid >> 6] = t;
-    __syncthreads();
-    if (tid < 64) {
-      const float sum = wave_sum(tid < int(blockDim.x >> 6) ? scratch[tid] : 0.f);
-      if (tid == 0) out[0] = sum;
-    }
-  } else {
-    scratch[tid] = v;
-    __syncthreads();
-    const int wave = tid >> 6, lane = tid & 63, waves = int(blockDim.x >> 6), span = s.lanes / s.slice_groups;
-    for (int g = wave; g < s.slice_groups; g += waves) {
-      float t = 0.f;
-      for (int k = lane; k < s.rows * span; k += 64) t += scratch[(k / span) * s.lanes + g * span + k % span];
-      t = wave_sum(t);
-      if (lane == 0) out[g] = t;
-    }
-  }
-  __syncthreads();
 }
 
 // The vectors that a thread holds are worked on one after another, and converted anew in each phase:
@@ -79,15 +51,11 @@ __device__ __forceinline__ int for_phase(int reach) {
 }
 __device__ __forceinline__ void one_vector() { __builtin_amdgcn_sched_barrier(0); }
 
-__device__ __forceinline__ float sigmoid(float u) { return __builtin_amdgcn_rcpf(1.f + __expf(-u)); }
-
 struct Place {
   int64_t b;
-  int slice, chunk, lane, row, group;  // group: of the slice
+  int slice, lane, row, group;  // group: of the slice
   bool on;
-  int reach;  // pixels of the chunk from this thread's first on (0 for a thread without pixels)
-  int64_t first;  // first pixel of the chunk
-  int pixels;     // pixels of the chunk
+  int reach;  // pixels from this thread's first on (0 for a thread without pixels)
 };
 // Of block `block` among `blocks`; neighbouring slices share lines, so they go to one XCD.
 template <int V>
@@ -95,33 +63,14 @@ __device__ __forceinline__ Place place(const Shape& s, int block, int blocks) {
   Place p;
   const int slices = s.groups / s.slice_groups;
   const int64_t at = xcd_block(block, blocks);
-  const int64_t unit = at / s.chunks;
-  p.chunk = int(at - unit * s.chunks);
-  p.b = unit / slices;
-  p.slice = int(unit - p.b * slices);
+  p.b = at / slices;
+  p.slice = int(at - p.b * slices);
   p.row = int(threadIdx.x) / s.lanes;
   p.lane = int(threadIdx.x) - p.row * s.lanes;
   p.on = p.row < s.rows;
   p.group = p.on ? p.lane * V / s.per_group : 0;
-  p.first = p.chunk * s.chunk_pixels;
-  p.pixels = int(min(s.chunk_pixels, s.pixels - p.first));
-  p.reach = p.on ? p.pixels - p.row : 0;
+  p.reach = p.on ? int(s.pixels) - p.row : 0;
   return p;
-}
-
-// The mean and the sum of squares about it of a group from its chunks' (chunks x [mean, squares]).
-__device__ __forceinline__ float2 merge(const float2* part, const Shape& s, int stride) {
-  float mean = 0.f, squares = 0.f;
-  for (int k = 0; k < s.chunks; ++k) {
-    const float n = float(min(s.chunk_pixels, s.pixels - k * s.chunk_pixels)) / float(s.pixels);
-    mean += n * part[int64_t(k) * stride].x;
-  }
-  for (int k = 0; k < s.chunks; ++k) {
-    const float n = float(min(s.chunk_pixels, s.pixels - k * s.chunk_pixels)) * float(s.per_group);
-    const float2 p = part[int64_t(k) * stride];
-    squares += p.y + n * (p.x - mean) * (p.x - mean);
-  }
-  return {mean, squares};
 }
 
 // Threads of a block, at most, and the blocks of 1024 threads on a CU that a kernel is compiled for: two
@@ -131,7 +80,7 @@ constexpr int MOST_THREADS = 1024;
 constexpr int large_blocks(int held, int V, bool backward) {
   return (backward ? held + 4 * V <= 22 : held + 2 * V <= 28) ? 2 : 1;
 }
-constexpr int simd_waves(int TB, int held, int V, bool backward) {
+[[maybe_unused]] constexpr int simd_waves(int TB, int held, int V, bool backward) {
   return TB < MOST_THREADS ? 1 : 4 * large_blocks(held, V, backward);
 }
 template <typename T, int V>
@@ -287,90 +236,159 @@ __global__ __launch_bounds__(TB, (simd_waves(TB, NV * words<T, V>(), V, false)))
   }
 }
 
-// The same over slices in chunks. stats: [batch, groups] of (mean, rstd), may be null. part: [batch, chunks, groups] of (mean, squares).
-template <typename T, typename TW, int V, int NV, int TB, int MODE>
-__global__ __launch_bounds__(TB, (simd_waves(TB, NV * words<T, V>(), V, false))) void k_group_norm_chunk(const T* __restrict__ x, const TW* __restrict__ weight,
-                                                        const TW* __restrict__ bias, T* __restrict__ y,
-                                                        float2* __restrict__ stats, float2* __restrict__ part,
-                                                        Shape s) {
-  __shared__ float scratch[TB], sums[TB], sums2[TB];
-  const Place p = place<V>(s, int(blockIdx.x), int(gridDim.x));
-  int reach;
-  const int c = p.slice * s.W + p.lane * V;
-  const int64_t at = (p.b * s.pixels + p.first + p.row) * s.C + c;
-  const T* src = x + at;
-  const int64_t step = int64_t(s.rows) * s.C;
-  Vec<T, V> held[NV];
-  reach = for_phase(p.reach);
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    held[k] = k * s.rows < reach ? load<T, V>(src + k * step) : Vec<T, V>::zero();
-  }
-  float mean, rstd;
-  if constexpr (MODE != APPLY) {
-    float sum = 0.f;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      one_vector();
-      float v[V];
-      convert(held[k], v);
-#pragma unroll
-      for (int e = 0; e < V; ++e) sum += v[e];
-    }
-    group_sums(p.on ? sum : 0.f, s, scratch, sums);
-    const float n = float(p.pixels) * float(s.per_group);
-    mean = sums[p.group] / n;
-    float squares = 0.f;
-    reach = for_phase(p.reach);
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      one_vector();
-      if (k * s.rows < reach) {
-        float v[V];
-        convert(held[k], v);
-#pragma unroll
-        for (int e = 0; e < V; ++e) squares += (v[e] - mean) * (v[e] - mean);
-      }
-    }
-    group_sums(squares, s, scratch, sums2);
-    if constexpr (MODE == STATS) {
-      if (int(threadIdx.x) < s.slice_groups) {
-        const int g = p.slice * s.slice_groups + int(threadIdx.x);
-        part[(p.b * s.chunks + p.chunk) * s.groups + g] = {sums[threadIdx.x] / n, sums2[threadIdx.x]};
-      }
-      return;
-    }
-  } else {
-    if (int(threadIdx.x) < s.slice_groups) {
-      const int g = p.slice * s.slice_groups + int(threadIdx.x);
-      const float2 m = merge(part + p.b * s.chunks * s.groups + g, s, s.groups);
-      sums[threadIdx.x] = m.x;
-      sums2[threadIdx.x] = 1.f / sqrtf(m.y / (float(s.pixels) * float(s.per_group)) + s.eps);
-      if (stats && p.chunk == 0) stats[p.b * s.groups + g] = {m.x, sums2[threadIdx.x]};
-    }
-    __syncthreads();
-    mean = sums[p.group];
-    rstd = sums2[p.group];
-  }
-  if (!p.on) return;
-  float w[V], b[V];
-  load_f32<TW, V>(weight + c, w);
-  load_f32<TW, V>(bias + c, b);
-  T* dst = y + at;
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    one_vector();
-    if (k * s.rows + p.row < p.pixels) {
-      float v[V];
-      convert(held[k], v);
+// ----------------------------------------------------------------------- whole rows, twice
+// Where a slice does not fit a block, and where images are large: the pixels pass in whole rows, in 16-byte
+// vectors whatever the groups' width, once for the statistics and once for the result, which the last
+// level cache has in part (the second pass takes the images in reverse). A block takes a chunk of an
+// image's pixels; a thread holds V channels and walks the chunk's pixels.
+struct Stream {
+  int64_t b, first;  // image, first pixel of the chunk
+  int chunk, row, c, pixels;
+  bool on;
+};
+template <int V>
+__device__ __forceinline__ Stream stream_of(const Shape& s, int block) {
+  Stream p;
+  const int width = block % s.widths;
+  const int64_t unit = block / s.widths;
+  p.b = unit / s.chunks;
+  p.chunk = int(unit - p.b * s.chunks);
+  p.row = int(threadIdx.x) / s.lanes;
+  p.c = width * s.W + (int(threadIdx.x) - p.row * s.lanes) * V;
+  p.first = p.chunk * s.span;
+  p.pixels = int(min(s.span, s.pixels - p.first));
+  p.on = p.row < s.rows && p.c < s.C;
+  return p;
+}
+// f(k, ahead) over the thread's pixels, `ahead` of them loaded at once.
+constexpr int AHEAD = 4;
+
+// part: [batch, chunks, groups] of (mean, squares about it) of the chunk's pixels. A thread sums about its
+// channel's first value, the block about the first value of the group, so that no digits are lost to a mean.
+template <typename T, int V>
+__global__ __launch_bounds__(1024) void k_norm_moments(const T* __restrict__ x, float2* __restrict__ part, Shape s) {
+  extern __shared__ float lds[];  // [2][rows][W], then the groups' first values
+  const Stream p = stream_of<V>(s, int(blockIdx.x));
+  const int tid = int(threadIdx.x), size = s.rows * s.W, groups = s.W / s.per_group, first_group = p.c / s.W * groups;
+  float* first = lds + 2 * size;
+  const int64_t at = (p.b * s.pixels + p.first + p.row) * s.C + p.c, step = int64_t(s.rows) * s.C;
+  const int cl = p.c % s.W, g0 = cl / s.per_group, in0 = cl - g0 * s.per_group;  // group, channel of the group
+  float shift[V] = {}, sum[V] = {}, squares[V] = {};
+  if (p.on && p.row < p.pixels) {
+    load<T, V>(x + at).to(shift);
+    if (p.row == 0) {
+      int in = in0, g = g0;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float u = fmaf((v[e] - mean) * rstd, w[e], b[e]);
-        v[e] = s.silu ? u * sigmoid(u) : u;
+        if (in == 0) first[g] = shift[e];
+        if (++in == s.per_group) in = 0, ++g;
       }
-      store<T, V>(dst, Vec<T, V>::of(v));
     }
-    dst += step;
+    const int count = (p.pixels - p.row + s.rows - 1) / s.rows;
+    for (int k0 = 0; k0 < count; k0 += AHEAD) {
+      Vec<T, V> v[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) v[j] = load<T, V>(x + at + min(k0 + j, count - 1) * step);
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        if (k0 + j >= count) break;
+        float f[V];
+        v[j].to(f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float d = f[e] - shift[e];
+          sum[e] += d;
+          squares[e] = fmaf(d, d, squares[e]);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (p.on) {
+    const float n = p.row < p.pixels ? float((p.pixels - p.row + s.rows - 1) / s.rows) : 0.f;
+    int in = in0, g = g0;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float d = n > 0.f ? shift[e] - first[g] : 0.f;
+      if (++in == s.per_group) in = 0, ++g;
+      lds[p.row * s.W + cl + e] = fmaf(n, d, sum[e]);
+      lds[size + p.row * s.W + cl + e] = squares[e] + d * (2.f * sum[e] + n * d);
+    }
+  }
+  __syncthreads();
+  const float n = float(p.pixels) * float(s.per_group);
+  for (int g = tid >> 6; g < groups; g += int(blockDim.x) >> 6) {
+    if (first_group + g >= s.groups) break;
+    float a = 0.f, d = 0.f;
+    for (int r = 0; r < s.rows; ++r)
+      for (int k = tid & 63; k < s.per_group; k += 64) {
+        a += lds[r * s.W + g * s.per_group + k];
+        d += lds[size + r * s.W + g * s.per_group + k];
+      }
+    a = wave_sum(a);
+    d = wave_sum(d);
+    if ((tid & 63) == 0)
+      part[(p.b * s.chunks + p.chunk) * s.groups + first_group + g] = {first[g] + a / n, fmaxf(d - a * (a / n), 0.f)};
+  }
+}
+
+// stats: [batch, groups] of (mean, rstd) from the chunks' moments; a wave a group.
+__global__ __launch_bounds__(256) void k_norm_stats(const float2* __restrict__ part, float2* __restrict__ stats,
+                                                    float2* __restrict__ out, Shape s) {
+  const int64_t i = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (i >= s.batch * s.groups) return;
+  const int64_t b = i / s.groups;
+  const float2* from = part + b * s.chunks * s.groups + (i - b * s.groups);
+  const int lane = int(threadIdx.x & 63);
+  float mean = 0.f, squares = 0.f;
+  for (int k = lane; k < s.chunks; k += 64)
+    mean += float(min(s.span, s.pixels - k * s.span)) / float(s.pixels) * from[int64_t(k) * s.groups].x;
+  mean = wave_sum(mean);
+  for (int k = lane; k < s.chunks; k += 64) {
+    const float2 p = from[int64_t(k) * s.groups];
+    squares += p.y + float(min(s.span, s.pixels - k * s.span)) * float(s.per_group) * (p.x - mean) * (p.x - mean);
+  }
+  squares = wave_sum(squares);
+  if (lane) return;
+  const float2 st = {mean, 1.f / sqrtf(squares / (float(s.pixels) * float(s.per_group)) + s.eps)};
+  stats[i] = st;
+  if (out) out[i] = st;
+}
+
+template <typename T, typename TW, int V>
+__global__ __launch_bounds__(1024) void k_norm_apply(const T* __restrict__ x, const TW* __restrict__ weight,
+                                                     const TW* __restrict__ bias, const float2* __restrict__ stats,
+                                                     T* __restrict__ y, Shape s) {
+  const Stream p = stream_of<V>(s, int(gridDim.x) - 1 - int(blockIdx.x));
+  if (!p.on || p.row >= p.pixels) return;
+  const int64_t at = (p.b * s.pixels + p.first + p.row) * s.C + p.c, step = int64_t(s.rows) * s.C;
+  float a[V], d[V], mean[V];
+  load_f32<TW, V>(weight + p.c, a);
+  load_f32<TW, V>(bias + p.c, d);
+#pragma unroll
+  for (int e = 0; e < V; ++e) {  // u = (x - mean) a + d, as k_group_norm
+    const float2 st = stats[p.b * s.groups + (p.c + e) / s.per_group];
+    a[e] *= st.y;
+    mean[e] = st.x;
+    if (sizeof(T) == 2) d[e] = fmaf(-st.x, a[e], d[e]);
+  }
+  const int count = (p.pixels - p.row + s.rows - 1) / s.rows;
+  for (int k0 = 0; k0 < count; k0 += AHEAD) {
+    Vec<T, V> v[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) v[j] = load<T, V>(x + at + min(k0 + j, count - 1) * step);
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (k0 + j >= count) break;
+      float f[V];
+      v[j].to(f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float u = fmaf(sizeof(T) == 4 ? f[e] - mean[e] : f[e], a[e], d[e]);
+        f[e] = s.silu ? silu(u, -LOG2E * u) : u;
+      }
+      store<T, V>(y + at + (k0 + j) * step, Vec<T, V>::of(f));
+    }
   }
 }
 
@@ -508,88 +526,104 @@ __global__ __launch_bounds__(TB, (simd_waves(TB, NV * (words<T, V>() + V), V, tr
   }
 }
 
-// The same over slices in chunks. part: [batch * chunks][2][C] sums over the chunk's pixels of g and of g h.
-template <typename T, typename TW, int V, int NV, int TB, int MODE>
-__global__ __launch_bounds__(TB, (simd_waves(TB, 2 * NV * words<T, V>(), V, true))) void k_group_norm_grad_chunk(const T* __restrict__ dy, const T* __restrict__ x,
-                                                             const TW* __restrict__ weight,
-                                                             const TW* __restrict__ bias,
-                                                             const float2* __restrict__ stats, T* __restrict__ dx,
-                                                             float* __restrict__ part, Shape s) {
-  extern __shared__ float lds[];
-  __shared__ float2 means[TB];
-  const Place p = place<V>(s, int(blockIdx.x), int(gridDim.x));
-  int reach;
-  const int tid = int(threadIdx.x), c = p.slice * s.W + p.lane * V;
-  const int64_t at = (p.b * s.pixels + p.first + p.row) * s.C + c, step = int64_t(s.rows) * s.C;
-  Vec<T, V> hx[NV], hg[NV];
-  reach = for_phase(p.reach);
+// Whole rows, as the forward's: the channels' sums of g and g h over a chunk, part [batch, chunks][2][C].
+template <typename T, typename TW, int V, bool DX>
+__global__ __launch_bounds__(1024) void k_norm_grad_rows(const T* __restrict__ dy, const T* __restrict__ x,
+                                                        const TW* __restrict__ weight, const TW* __restrict__ bias,
+                                                        const float2* __restrict__ stats, const float2* __restrict__ means,
+                                                        T* __restrict__ dx, float* __restrict__ part, Shape s) {
+  extern __shared__ float lds[];  // [2][rows][W]
+  const Stream p = stream_of<V>(s, DX ? int(gridDim.x) - 1 - int(blockIdx.x) : int(blockIdx.x));
+  const bool on = p.on && p.row < p.pixels;
+  if (DX && !on) return;
+  const int64_t at = (p.b * s.pixels + p.first + p.row) * s.C + p.c, step = int64_t(s.rows) * s.C;
+  const int tid = int(threadIdx.x), size = s.rows * s.W, cl = p.c % s.W;
+  float w[V] = {}, b[V] = {}, sg[V] = {}, sh[V] = {};
+  float2 st[V] = {}, m[V] = {};
+  if (on) {
+    load_f32<TW, V>(weight + p.c, w);
+    load_f32<TW, V>(bias + p.c, b);
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const bool in = k * s.rows < reach;
-    hx[k] = in ? load<T, V>(x + at + k * step) : Vec<T, V>::zero();
-    hg[k] = in ? load<T, V>(dy + at + k * step) : Vec<T, V>::zero();
-  }
-  const float2 st = stats[p.b * s.groups + p.slice * s.slice_groups + p.group];
-  float w[V] = {}, b[V] = {};
-  if (p.on) {
-    load_f32<TW, V>(weight + c, w);
-    load_f32<TW, V>(bias + c, b);
-  }
-  if constexpr (MODE == STATS) {
-    float sg[V] = {}, sh[V] = {};
-    reach = for_phase(p.reach);
+    for (int e = 0; e < V; ++e) {
+      const int64_t group = p.b * s.groups + (p.c + e) / s.per_group;
+      st[e] = stats[group];
+      if (DX) m[e] = means[group];
+    }
+    const int count = (p.pixels - p.row + s.rows - 1) / s.rows;
+    constexpr int N = AHEAD / 2;
+    for (int k0 = 0; k0 < count; k0 += N) {
+      Vec<T, V> vx[N], vg[N];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      one_vector();
-      if (k * s.rows < reach) {
-        float xv[V], gv[V];
-        convert(hx[k], xv);
-        convert(hg[k], gv);
+      for (int j = 0; j < N; ++j) {
+        vx[j] = load<T, V>(x + at + min(k0 + j, count - 1) * step);
+        vg[j] = load<T, V>(dy + at + min(k0 + j, count - 1) * step);
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        if (k0 + j >= count) break;
+        float f[V], g0[V];
+        vx[j].to(f);
+        vg[j].to(g0);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           float h, g;
-          element(xv[e], gv[e], st, w[e], b[e], s.silu, h, g);
-          sg[e] += g;
-          sh[e] = fmaf(g, h, sh[e]);
+          element(f[e], g0[e], st[e], w[e], b[e], s.silu, h, g);
+          if (DX) {
+            f[e] = st[e].y * (rounded_product(w[e], g) - m[e].x - h * m[e].y);
+          } else {
+            sg[e] += g;
+            sh[e] = fmaf(g, h, sh[e]);
+          }
         }
+        if (DX) store<T, V>(dx + at + (k0 + j) * step, Vec<T, V>::of(f));
       }
     }
-    const float* channel = channel_sums<V, TB>(sg, sh, p, s, lds);
-    for (int i = tid; i < 2 * s.W; i += TB) {
-      const int which = i / s.W;
-      part[((p.b * s.chunks + p.chunk) * 2 + which) * s.C + p.slice * s.W + i - which * s.W] = channel[i];
-    }
-  } else {
-    float* channel = lds;
-    for (int i = tid; i < 2 * s.W; i += TB) {
-      const int which = i / s.W;
-      float sum = 0.f;
-      for (int q = 0; q < s.chunks; ++q)
-        sum += part[((p.b * s.chunks + q) * 2 + which) * s.C + p.slice * s.W + i - which * s.W];
-      channel[i] = sum;
-    }
+  }
+  if constexpr (!DX) {
+    if (p.on)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        lds[p.row * s.W + cl + e] = sg[e];
+        lds[size + p.row * s.W + cl + e] = sh[e];
+      }
     __syncthreads();
-    group_means<TW, TB>(weight, channel, p, s, means);
-    const float2 m = means[p.group];
-    T* dst = dx + at;
-    reach = for_phase(p.reach);
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      one_vector();
-      if (k * s.rows < reach) {
-        float xv[V], gv[V];
-        convert(hx[k], xv);
-        convert(hg[k], gv);
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          float h, g;
-          element(xv[e], gv[e], st, w[e], b[e], s.silu, h, g);
-          xv[e] = st.y * (rounded_product(w[e], g) - m.x - h * m.y);
-        }
-        store<T, V>(dst, Vec<T, V>::of(xv));
-      }
-      dst += step;
+    const int c0 = p.c - cl;  // of the block's width (a thread past the rows has its own c, of the same width)
+    for (int i = tid; i < 2 * s.W; i += int(blockDim.x)) {
+      const int which = i / s.W, k = i - which * s.W;
+      if (c0 + k >= s.C) continue;
+      float sum = 0.f;
+      for (int r = 0; r < s.rows; ++r) sum += lds[which * size + r * s.W + k];
+      part[((p.b * s.chunks + p.chunk) * 2 + which) * s.C + c0 + k] = sum;
     }
+  }
+}
+
+// One image: the channels' sums over its chunks, total [batch][2][C], and the groups' means of w g and w g h.
+template <typename TW>
+__global__ __launch_bounds__(1024) void k_norm_grad_means(const float* __restrict__ part, const TW* __restrict__ weight,
+                                                          float* __restrict__ total, float2* __restrict__ means, Shape s) {
+  const int64_t b = blockIdx.x;
+  float* sums = total + b * 2 * s.C;
+  for (int i = int(threadIdx.x); i < 2 * s.C; i += 1024) {
+    float sum = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < s.chunks; ++k) sum += part[(b * s.chunks + k) * 2 * s.C + i];
+    sums[i] = sum;
+  }
+  __threadfence_block();
+  __syncthreads();
+  const float inverse_n = 1.f / (float(s.pixels) * float(s.per_group));
+  for (int g = int(threadIdx.x) >> 6; g < s.groups; g += 16) {
+    float a = 0.f, d = 0.f;
+    for (int k = int(threadIdx.x) & 63; k < s.per_group; k += 64) {
+      const int c = g * s.per_group + k;
+      const float wk = to_f32(weight[c]);
+      a += wk * sums[c];
+      d += wk * sums[s.C + c];
+    }
+    a = wave_sum(a);
+    d = wave_sum(d);
+    if ((threadIdx.x & 63) == 0) means[b * s.groups + g] = {a * inverse_n, d * inverse_n};
   }
 }
 
@@ -613,8 +647,12 @@ __global__ __launch_bounds__(256) void k_channel_sums(const float* __restrict__ 
 // ---------------------------------------------------------------------------------- host
 // The register words a thread holds, at most.
 constexpr int WORDS = 80;
+// Images from so many bytes on pass in whole rows though their slices fit (64 images of 64 x 64 x 1152,
+// 9.4 MB each: 362 us, by slices 392; of 32 x 32 x 1152, 2.4 MB: 106 and 80, the gradients 168 and 154).
+constexpr int64_t STREAM_FROM = int64_t(4) << 20;
 struct Plan {
   Shape s;
+  bool whole;  // one slice a block; else whole rows
   int V, NV;
 };
 // The widest vector of at most 16 bytes that divides a group, so that each lies in one group.
@@ -623,6 +661,8 @@ int vec_of(int per_group, int elem) {
     if (v * elem <= 16 && per_group % v == 0) return v;
   return 1;
 }
+// Vectors of a pixel that a block takes in whole rows, at most: LDS holds two sums of each channel.
+int most_lanes(int V) { return V >= 4 ? 512 : MOST_THREADS; }
 // backward: a block holds x and the output's gradient, and that in fp32.
 Plan plan(int64_t batch, int64_t pixels, int C, int groups, float eps, bool silu, int elem, bool backward) {
   Plan p{};
@@ -650,13 +690,31 @@ Plan plan(int64_t batch, int64_t pixels, int C, int groups, float eps, bool silu
     s.slice_groups = g;
   }
   // small slices: blocks of 256 threads, several to a CU
-  s.threads = vectors(s.slice_groups, 256) <= 8 ? 256 : MOST_THREADS;
+  s.threads = vectors(s.slice_groups, 256) <= std::min(8, most) ? 256 : MOST_THREADS;
   s.W = s.slice_groups * s.per_group;
   s.lanes = s.W / p.V;
   s.rows = s.threads / s.lanes;
-  s.chunks = int(ceil_div(vectors(s.slice_groups, s.threads), most));
-  s.chunk_pixels = ceil_div(pixels, s.chunks);
-  p.NV = int(ceil_div(s.chunk_pixels, s.rows));
+  p.NV = int(std::min<int64_t>(ceil_div(pixels, s.rows), most + 1));
+  p.whole = p.NV <= most && pixels * C * elem < STREAM_FROM;
+  if (p.whole) return p;
+  // whole rows: 16-byte vectors where a pixel's fit a block, else whole groups of them
+  p.V = vec_of(C, elem);
+  int threads = most_lanes(p.V);
+  s.W = C;
+  s.widths = 1;
+  if (C / p.V > threads) {
+    p.V = vec_of(s.per_group, elem);
+    threads = most_lanes(p.V);
+    s.W = std::max(1, threads * p.V / s.per_group) * s.per_group;
+    s.widths = int(ceil_div(C, s.W));
+  }
+  s.lanes = s.W / p.V;
+  s.rows = std::max(1, 512 / s.lanes);
+  s.threads = int(ceil_div(int64_t(s.rows) * s.lanes, 64) * 64);
+  // 32 pixels a thread, fewer for 32 chunks of an image (its results do not depend on the batch)
+  const int64_t steps = std::max<int64_t>(4, std::min<int64_t>(32, pixels / (int64_t(s.rows) * 32)));
+  s.span = steps * s.rows;
+  s.chunks = int(ceil_div(pixels, s.span));
   return p;
 }
 
@@ -664,7 +722,8 @@ int check_sizes(const char* what, int64_t batch, int64_t pixels, int C, int grou
   if (batch < 0 || pixels < 0 || C <= 0 || (pixels && batch > SIHC_MAX_TOKENS / pixels))
     return fail(SIHC_ERR_INVALID, "%s: bad sizes", what);
   if (groups <= 0 || C % groups) return fail(SIHC_ERR_INVALID, "%s: %d channels are not %d groups", what, C, groups);
-  if (C / groups / vec_of(C / groups, dtype == SIHC_DTYPE_F32 ? 4 : 2) > MOST_THREADS)
+  const int V = vec_of(C / groups, dtype == SIHC_DTYPE_F32 ? 4 : 2);
+  if (C / groups / V > most_lanes(V))
     return fail(SIHC_ERR_INVALID, "%s: groups of %d channels are too wide", what, C / groups);
   if (act != SIHC_ACT_NONE && act != SIHC_ACT_SILU) return fail(SIHC_ERR_INVALID, "%s: bad activation %d", what, act);
   if (!valid_dtype(dtype) || !valid_dtype(w_dtype)) return fail(SIHC_ERR_INVALID, "%s: bad dtype", what);
@@ -674,20 +733,21 @@ int check_sizes(const char* what, int64_t batch, int64_t pixels, int C, int grou
 }
 int elem_size(int dtype) { return dtype == SIHC_DTYPE_F32 ? 4 : 2; }
 
-// Calls f(T, TW, V, NV, TB, whole) with NV the smallest compiled count of at least p.NV vectors; slices in
-// chunks (whole = false) take the largest.
-template <bool BACKWARD, typename F>
-int by_plan(const Plan& p, int dtype, int w_dtype, F&& f) {
+// Calls f(T, TW, V, NV, TB) with NV the smallest compiled count of at least p.NV vectors, or, for whole
+// rows, rows(T, TW, V).
+template <bool BACKWARD, typename F, typename R>
+int by_plan(const Plan& p, int dtype, int w_dtype, F&& f, R&& rows) {
   return by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     auto with = [&](auto tw, auto v) {
+      if (!p.whole) return rows(t, tw, v);
       constexpr int V = decltype(v)::value, MOST = WORDS / (words<T, V>() + (BACKWARD ? V : 0));
       int rc = SIHC_OK;
       auto attempt = [&](auto nv, auto tb) {
         constexpr int NV = decltype(nv)::value;
         if constexpr (NV <= MOST) {
-          if (p.s.threads == decltype(tb)::value && p.s.chunks == 1 && p.NV <= NV) {
-            rc = f(t, tw, v, nv, tb, std::true_type{});
+          if (p.s.threads == decltype(tb)::value && p.NV <= NV) {
+            rc = f(t, tw, v, nv, tb);
             return true;
           }
         }
@@ -695,11 +755,13 @@ int by_plan(const Plan& p, int dtype, int w_dtype, F&& f) {
       };
       constexpr IC<256> small{};
       constexpr IC<1024> large{};
-      if (attempt(IC<1>{}, small) || attempt(IC<2>{}, small) || attempt(IC<4>{}, small) || attempt(IC<8>{}, small) ||
+      if (attempt(IC<1>{}, small) || attempt(IC<2>{}, small) || attempt(IC<4>{}, small) || attempt(IC<6>{}, small) ||
+          attempt(IC<8>{}, small) ||
           attempt(IC<4>{}, large) || attempt(IC<7>{}, large) || attempt(IC<10>{}, large) || attempt(IC<14>{}, large) ||
-          attempt(IC<20>{}, large) || attempt(IC<28>{}, large) || attempt(IC<40>{}, large) || attempt(IC<80>{}, large))
+          attempt(IC<20>{}, large) || attempt(IC<28>{}, large) || attempt(IC<40>{}, large) || attempt(IC<80>{}, large) ||
+          attempt(IC<MOST>{}, large))
         return rc;
-      return f(t, tw, v, IC<MOST>{}, large, std::false_type{});
+      return fail(SIHC_ERR_INVALID, "group norm: internal plan");
     };
     auto by_v = [&](auto tw) {
       switch (p.V) {
@@ -719,9 +781,11 @@ int by_plan(const Plan& p, int dtype, int w_dtype, F&& f) {
 extern "C" {
 
 size_t sihc_group_norm_workspace_size(int64_t batch, int64_t pixels, int channels, int groups, int dtype) {
-  if (batch <= 0 || pixels <= 0 || channels <= 0 || groups <= 0 || channels % groups || !valid_dtype(dtype)) return 0;
+  if (check_sizes("sihc_group_norm", batch, pixels, channels, groups, SIHC_ACT_NONE, dtype, dtype) || batch == 0 ||
+      pixels == 0)
+    return 0;
   const Plan p = plan(batch, pixels, channels, groups, 0.f, false, elem_size(dtype), false);
-  return p.s.chunks > 1 ? size_t(batch) * size_t(p.s.chunks) * size_t(groups) * 8 : 0;
+  return p.whole ? 0 : size_t(batch) * size_t(p.s.chunks + 1) * size_t(groups) * 8;  // the chunks' moments, the statistics
 }
 
 int sihc_group_norm(const void* x, const void* weight, const void* bias, void* y, float* stats, int64_t batch,
@@ -736,35 +800,44 @@ int sihc_group_norm(const void* x, const void* weight, const void* bias, void* y
     return fail(SIHC_ERR_INVALID, "%s: workspace of %zu bytes required, got %zu", what, need, workspace_bytes);
   if (!aligned(workspace, 8) || !aligned(stats, 8)) return fail(SIHC_ERR_INVALID, "%s: misaligned workspace or stats", what);
   const Plan p = plan(batch, pixels, channels, groups, eps, act == SIHC_ACT_SILU, elem_size(dtype), false);
-  const int64_t blocks = batch * (groups / p.s.slice_groups) * p.s.chunks;
+  const int64_t blocks = p.whole ? batch * (groups / p.s.slice_groups) : batch * p.s.chunks * p.s.widths;
   if (blocks > 0x7fffffff) return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
-  const dim3 grid(static_cast<unsigned>(blocks));
+  const dim3 grid(static_cast<unsigned>(blocks)), threads(static_cast<unsigned>(p.s.threads));
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return by_plan<false>(p, dtype, w_dtype, [&](auto t, auto tw, auto v, auto nv, auto tb, auto whole) {
-    using T = decltype(t);
-    using TW = decltype(tw);
-    constexpr int V = decltype(v)::value, NV = decltype(nv)::value, TB = decltype(tb)::value;
-    if constexpr (decltype(whole)::value) {
-      hipLaunchKernelGGL((k_group_norm<T, TW, V, NV, TB>), grid, dim3(TB), 0, st, static_cast<const T*>(x),
-                         static_cast<const TW*>(weight), static_cast<const TW*>(bias), static_cast<T*>(y),
-                         reinterpret_cast<float2*>(stats), p.s);
-    } else {
-      auto launch = [&](auto mode) {
-        hipLaunchKernelGGL((k_group_norm_chunk<T, TW, V, NV, TB, decltype(mode)::value>), grid, dim3(TB), 0, st,
-                           static_cast<const T*>(x), static_cast<const TW*>(weight), static_cast<const TW*>(bias),
-                           static_cast<T*>(y), reinterpret_cast<float2*>(stats), static_cast<float2*>(workspace), p.s);
-      };
-      launch(IC<STATS>{});
-      launch(IC<APPLY>{});
-    }
-    return check_launch(what);
-  });
+  return by_plan<false>(
+      p, dtype, w_dtype,
+      [&](auto t, auto tw, auto v, auto nv, auto tb) {
+        using T = decltype(t);
+        using TW = decltype(tw);
+        constexpr int V = decltype(v)::value, NV = decltype(nv)::value, TB = decltype(tb)::value;
+        hipLaunchKernelGGL((k_group_norm<T, TW, V, NV, TB>), grid, threads, 0, st, static_cast<const T*>(x),
+                           static_cast<const TW*>(weight), static_cast<const TW*>(bias), static_cast<T*>(y),
+                           reinterpret_cast<float2*>(stats), p.s);
+        return check_launch(what);
+      },
+      [&](auto t, auto tw, auto v) {
+        using T = decltype(t);
+        using TW = decltype(tw);
+        constexpr int V = decltype(v)::value;
+        float2 *part = static_cast<float2*>(workspace), *own = part + batch * p.s.chunks * groups;
+        const unsigned lds = (2u * unsigned(p.s.rows) * unsigned(p.s.W) + unsigned(p.s.W / p.s.per_group)) * 4u;
+        hipLaunchKernelGGL((k_norm_moments<T, V>), grid, threads, lds, st, static_cast<const T*>(x), part, p.s);
+        hipLaunchKernelGGL(k_norm_stats, dim3(unsigned(ceil_div(batch * groups, 4))), dim3(256), 0, st, part, own,
+                           reinterpret_cast<float2*>(stats), p.s);
+        hipLaunchKernelGGL((k_norm_apply<T, TW, V>), grid, threads, 0, st, static_cast<const T*>(x),
+                           static_cast<const TW*>(weight), static_cast<const TW*>(bias), own, static_cast<T*>(y), p.s);
+        return check_launch(what);
+      });
 }
 
 size_t sihc_group_norm_backward_workspace_size(int64_t batch, int64_t pixels, int channels, int groups, int dtype) {
-  if (batch <= 0 || pixels <= 0 || channels <= 0 || groups <= 0 || channels % groups || !valid_dtype(dtype)) return 0;
+  if (check_sizes("sihc_group_norm_backward", batch, pixels, channels, groups, SIHC_ACT_NONE, dtype, dtype) ||
+      batch == 0 || pixels == 0)
+    return 0;
   const Plan p = plan(batch, pixels, channels, groups, 0.f, false, elem_size(dtype), true);
-  return size_t(batch) * size_t(p.s.chunks) * 2 * size_t(channels) * 4;
+  // the images' channel sums; whole rows: and the chunks', and the groups' means
+  const size_t rows = size_t(batch) * 2 * size_t(channels) * 4;
+  return p.whole ? rows : rows * size_t(p.s.chunks + 1) + size_t(batch) * size_t(groups) * 8;
 }
 
 int sihc_group_norm_backward(const void* grad, const void* x, const void* weight, const void* bias, const float* stats,
@@ -788,32 +861,43 @@ int sihc_group_norm_backward(const void* grad, const void* x, const void* weight
     if (!aligned(workspace, 8) || !aligned(stats, 8))
       return fail(SIHC_ERR_INVALID, "%s: misaligned workspace or stats", what);
     const Plan p = plan(batch, pixels, channels, groups, 0.f, act == SIHC_ACT_SILU, elem_size(dtype), true);
-    const int64_t blocks = batch * (groups / p.s.slice_groups) * p.s.chunks;
+    const int64_t blocks = p.whole ? batch * (groups / p.s.slice_groups) : batch * p.s.chunks * p.s.widths;
     if (blocks > 0x7fffffff) return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
-    parts = batch * p.s.chunks;
-    const dim3 grid(static_cast<unsigned>(blocks));
-    const unsigned lds = 2u * unsigned(p.s.rows + 1) * unsigned(p.s.W) * 4u;
-    const int rc = by_plan<true>(p, dtype, w_dtype, [&](auto t, auto tw, auto v, auto nv, auto tb, auto whole) {
-      using T = decltype(t);
-      using TW = decltype(tw);
-      constexpr int V = decltype(v)::value, NV = decltype(nv)::value, TB = decltype(tb)::value;
-      if constexpr (decltype(whole)::value) {
-        hipLaunchKernelGGL((k_group_norm_grad<T, TW, V, NV, TB>), grid, dim3(TB), lds, st, static_cast<const T*>(grad),
-                           static_cast<const T*>(x), static_cast<const TW*>(weight), static_cast<const TW*>(bias),
-                           reinterpret_cast<const float2*>(stats), static_cast<T*>(grad_x),
-                           static_cast<float*>(workspace), p.s);
-      } else {
-        auto launch = [&](auto mode) {
-          hipLaunchKernelGGL((k_group_norm_grad_chunk<T, TW, V, NV, TB, decltype(mode)::value>), grid, dim3(TB), lds, st,
-                             static_cast<const T*>(grad), static_cast<const T*>(x), static_cast<const TW*>(weight),
-                             static_cast<const TW*>(bias), reinterpret_cast<const float2*>(stats),
-                             static_cast<T*>(grad_x), static_cast<float*>(workspace), p.s);
-        };
-        launch(IC<STATS>{});
-        launch(IC<APPLY>{});
-      }
-      return check_launch(what);
-    });
+    parts = batch;
+    const dim3 grid(static_cast<unsigned>(blocks)), threads(static_cast<unsigned>(p.s.threads));
+    const int rc = by_plan<true>(
+        p, dtype, w_dtype,
+        [&](auto t, auto tw, auto v, auto nv, auto tb) {
+          using T = decltype(t);
+          using TW = decltype(tw);
+          constexpr int V = decltype(v)::value, NV = decltype(nv)::value, TB = decltype(tb)::value;
+          const unsigned lds = 2u * unsigned(p.s.rows + 1) * unsigned(p.s.W) * 4u;
+          hipLaunchKernelGGL((k_group_norm_grad<T, TW, V, NV, TB>), grid, threads, lds, st, static_cast<const T*>(grad),
+                             static_cast<const T*>(x), static_cast<const TW*>(weight), static_cast<const TW*>(bias),
+                             reinterpret_cast<const float2*>(stats), static_cast<T*>(grad_x),
+                             static_cast<float*>(workspace), p.s);
+          return check_launch(what);
+        },
+        [&](auto t, auto tw, auto v) {
+          using T = decltype(t);
+          using TW = decltype(tw);
+          constexpr int V = decltype(v)::value;
+          float *total = static_cast<float*>(workspace), *part = total + batch * 2 * channels;
+          float2* means = reinterpret_cast<float2*>(part + batch * p.s.chunks * 2 * channels);
+          const unsigned lds = 2u * unsigned(p.s.rows) * unsigned(p.s.W) * 4u;
+          auto pass = [&](auto dx) {
+            constexpr bool DX = decltype(dx)::value;
+            hipLaunchKernelGGL((k_norm_grad_rows<T, TW, V, DX>), grid, threads, DX ? 0 : lds, st,
+                               static_cast<const T*>(grad), static_cast<const T*>(x), static_cast<const TW*>(weight),
+                               static_cast<const TW*>(bias), reinterpret_cast<const float2*>(stats), means,
+                               static_cast<T*>(grad_x), part, p.s);
+          };
+          pass(std::false_type{});
+          hipLaunchKernelGGL(k_norm_grad_means<TW>, dim3(unsigned(batch)), dim3(1024), 0, st, part,
+                             static_cast<const TW*>(weight), total, means, p.s);
+          pass(std::true_type{});
+          return check_launch(what);
+        });
     if (rc) return rc;
   }
   auto sums = [&](auto tw) {
