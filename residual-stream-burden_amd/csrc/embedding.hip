@@ -355,8 +355,8 @@ __global__ __launch_bounds__(256) void k_embed_grad(const T* __restrict__ grad, 
 }
 
 // The runs that cross chunks, of the listed chunks in which they begin: their partial rows of this chunk
-// and the following ones are summed, by 4 thread rows over ascending quarters of the run's chunks, then
-// the quarters in order. blockIdx.y: 64 channels.
+// and the following ones are summed, 256 channels a block (blockIdx.y), in ascending order; of a long
+// run by 4 thread rows over ascending quarters of the run's chunks, then the quarters in order.
 template <typename T>
 __global__ __launch_bounds__(256) void k_embed_grad_runs(const u32x2* __restrict__ sorted,
                                                          const float* __restrict__ partial,
@@ -378,18 +378,30 @@ __global__ __launch_bounds__(256) void k_embed_grad_runs(const u32x2* __restrict
       }
     }
     const int64_t last = chunk + parts, each = (parts + 3) / 4;
-    for (int c0 = int(blockIdx.y) * 64; c0 < C; c0 += int(gridDim.y) * 64) {
-      const int c = min(c0 + lane, C - 1);
-      float sum = q == 0 ? partial[(chunk * 2 + 1) * C + c] : 0.f;
-      const int64_t begin = chunk + 1 + q * each, end = min(last + 1, begin + each);
+    const float* own = partial + (chunk * 2 + 1) * C;
+    for (int base = int(blockIdx.y) * 256; base < C; base += int(gridDim.y) * 256) {
+      if (parts <= 16) {
+        const int c = base + int(threadIdx.x);
+        if (c >= C) continue;
+        float sum = own[c];
+#pragma unroll 4
+        for (int64_t k = chunk + 1; k <= last; ++k) sum += partial[k * 2 * C + c];
+        out[int64_t(row) * C + c] = from_f32<T>(scale * sum);
+        continue;
+      }
+      for (int c0 = base; c0 < min(C, base + 256); c0 += 64) {
+        const int c = min(c0 + lane, C - 1);
+        float sum = q == 0 ? own[c] : 0.f;
+        const int64_t begin = chunk + 1 + q * each, end = min(last + 1, begin + each);
 #pragma unroll 8
-      for (int64_t k = begin; k < end; ++k) sum += partial[k * 2 * C + c];
-      quarter[q][lane] = sum;
-      __syncthreads();
-      if (q == 0 && c0 + lane < C)
-        out[int64_t(row) * C + c] =
-            from_f32<T>(scale * (((quarter[0][lane] + quarter[1][lane]) + quarter[2][lane]) + quarter[3][lane]));
-      __syncthreads();
+        for (int64_t k = begin; k < end; ++k) sum += partial[k * 2 * C + c];
+        quarter[q][lane] = sum;
+        __syncthreads();
+        if (q == 0 && c0 + lane < C)
+          out[int64_t(row) * C + c] =
+              from_f32<T>(scale * (((quarter[0][lane] + quarter[1][lane]) + quarter[2][lane]) + quarter[3][lane]));
+        __syncthreads();
+      }
     }
   }
 }
@@ -558,7 +570,7 @@ int sihc_embedding_backward(const void* grad, const void* ids, void* grad_table,
           if (p.chunk == 8) sum(IC<8>{});
           else sum(IC<32>{});
           const unsigned listed = unsigned(std::min<int64_t>(p.chunks, 1024)),
-                         columns = unsigned(std::min<int64_t>(ceil_div(channels, 64), 64));
+                         columns = unsigned(std::min<int64_t>(ceil_div(channels, 256), 64));
           hipLaunchKernelGGL(k_embed_grad_runs<T>, dim3(listed, columns), dim3(256), 0, st, sorted, partial, crossing, out,
                              tokens, channels, scale, p.chunk);
         }
