@@ -4,7 +4,9 @@
 //   grad[r, :] = scale * sum over n ascending with id_n = r of dout[n, :]
 //
 // Both are bound by memory: the lookup reads a row and writes a row per token, the gradient
-// reads the tokens' rows and writes the whole table's. Ids outside the table select its last
+// reads the tokens' rows and writes the whole table's. (Of 32,768 tokens of 1152 bf16 channels over
+// 32,768 rows, half of them padding and the others' ids as frequent as their cube roots fall: lookup
+// 23 us, gradient 54 us, of which its sort takes 32 beside clearing the table.) Ids outside the table select its last
 // row in both (the host wrappers reject them), so no access can leave it.
 //
 // The gradient takes no atomics on values. Few tokens: every block owns a few table rows, lists
@@ -18,9 +20,14 @@
 namespace {
 using namespace sihc_cond;
 
-constexpr int OWN_SCAN = 64;      // up to so many tiles the scattering blocks add the counts up themselves
-constexpr int FEW_TOKENS = 1024;  // up to here the rows' tokens are listed by scanning all ids
-constexpr int FEW_ROWS = 8;       // table rows of a block there, at most
+// Up to so many tiles the scattering blocks add the counts up themselves, past them one block does for all
+// (whole gradients of 64 channels: 16, 32 and 64 tiles 33, 49 and 92 us, with that block 38, 56 and 107).
+constexpr int OWN_SCAN = 64;
+// Up to so many tokens the rows' tokens are listed by scanning all ids (1152 bf16 channels, 1001 rows: 256 and
+// 1024 tokens 4.7 and 5.9 us, by the sort 19.5 and 21.5; 32,768 rows: 1024 tokens 24 and 36, 2048 more than
+// 40 and 36). A row that all tokens select is then summed by one block: 256 tokens 42 us, by the sort 25.
+constexpr int FEW_TOKENS = 1024;
+constexpr int FEW_ROWS = 8;  // table rows of a block there, at most
 
 template <typename I>
 __device__ __forceinline__ uint32_t id_at(const I* ids, int64_t n, uint32_t rows) {
@@ -29,7 +36,8 @@ __device__ __forceinline__ uint32_t id_at(const I* ids, int64_t n, uint32_t rows
 }
 
 // ------------------------------------------------------------------------------- lookup
-// UNROLL vectors a thread, a block apart, so that a thread's ids, then its rows, are in flight together;
+// 32,768 rows of 1152 bf16 channels from 32,768: 23.5 us, 6.4 TB/s of the rows read (in part from the caches)
+// and written. UNROLL vectors a thread, a block apart, so that a thread's ids, then its rows, are in flight together;
 // the last vector of a row that V does not divide moves back to end with it.
 template <typename T, typename I, int V, int UNROLL>
 __global__ __launch_bounds__(256) void k_embed(const T* __restrict__ table, const I* __restrict__ ids,
@@ -60,7 +68,8 @@ __global__ __launch_bounds__(256) void k_embed(const T* __restrict__ table, cons
 }
 
 // ------------------------------------------------------------------- gradient, few tokens
-// Each thread owns an ascending run of the ids, so a prefix sum of the threads' matches lists the
+// Latency: 256 fp32 tokens of 1152 channels over 1001 rows 4.8 us, half of it the scan of the ids. Each thread
+// owns an ascending run of the ids, so a prefix sum of the threads' matches lists the
 // block's tokens in ascending order.
 template <typename T, typename I, int V>
 __global__ __launch_bounds__(256) void k_embed_grad_few(const T* __restrict__ grad, const I* __restrict__ ids,
@@ -107,13 +116,27 @@ __global__ __launch_bounds__(256) void k_embed_grad_few(const T* __restrict__ gr
   for (int item = tid; item < here * vecs; item += 256) {
     const int row = item / vecs, c = min((item - row * vecs) * V, C - V);
     float sum[V] = {};
-    for (int k = 0; k < total; ++k) {
-      if (int(list[k] & 7u) != row) continue;
-      float v[V];
-      load<T, V>(grad + int64_t(list[k] >> 3) * C + c).to(v);
+    auto add = [&](int k0, auto n) {  // n tokens' rows in flight, the block's other rows' among them
+      constexpr int N = decltype(n)::value;
+      uint32_t at[N];
+      Vec<T, V> v[N];
 #pragma unroll
-      for (int e = 0; e < V; ++e) sum[e] += v[e];
-    }
+      for (int j = 0; j < N; ++j) at[j] = list[min(k0 + j, total - 1)];
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = load<T, V>(grad + int64_t(at[j] >> 3) * C + c);
+      __builtin_amdgcn_sched_barrier(0);  // (the loads would be taken apart to save registers)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const bool own = int(at[j] & 7u) == row && (N == 8 || k0 + j < total);
+        float f[V];
+        v[j].to(f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum[e] += own ? f[e] : 0.f;
+      }
+    };
+    int k = 0;
+    for (; k + 8 <= total; k += 8) add(k, IC<8>{});
+    for (; k < total; k += 2) add(k, IC<2>{});
 #pragma unroll
     for (int e = 0; e < V; ++e) sum[e] *= scale;
     store<T, V>(out + (int64_t(r0) + row) * C + c, Vec<T, V>::of(sum));
@@ -145,6 +168,8 @@ __device__ __forceinline__ void clear(u32x4* p, int64_t bytes, int64_t block, in
   if (block == 0 && threadIdx.x < (bytes & 15)) reinterpret_cast<uint8_t*>(p + n16)[threadIdx.x] = 0;
 }
 
+// One pass of a sort of 32,768 tokens: count 3.7 us (14.0 beside the clearing of 75 MB, 5.4 TB/s), scatter 7.5,
+// most of it launch and latency.
 // hist[tile][digit]: keys of the tile (256 x STEPS keys) with that digit. Blocks past the tiles clear the table's
 // gradient, of which a sort of few blocks leaves the memory's time free.
 template <typename K, int STEPS>
@@ -295,7 +320,7 @@ __global__ __launch_bounds__(256) void k_sort_scatter(K keys, const uint32_t* __
 }
 
 // ----------------------------------------------------------------- gradient, sorted tokens
-// One wave: CHUNK (8 or 32) sorted tokens x 64 vectors of the row. partial[chunk][0]: the run that the chunk
+// One wave: CHUNK (8 or 32) sorted tokens x 64 vectors of the row, 8 of them in flight. partial[chunk][0]: the run that the chunk
 // before began; [1]: the run that begins here and goes on in the next chunk. A run through the whole
 // chunk is [0].
 template <typename T, int V, int CHUNK>
@@ -441,10 +466,12 @@ SortPlan sort_plan(int64_t tokens, int64_t rows, int C) {
   while ((int64_t(1) << bits) < rows + 1) ++bits;
   p.passes = (bits + 9) / 10;
   p.bits = (bits + p.passes - 1) / p.passes;
+  // (whole gradients of 64 channels: 32,768 tokens 48 us by 4 steps, 65 by 16; 131,072: 111, 96)
   p.steps = tokens <= 1024 * OWN_SCAN ? 4 : 16;
   p.tiles = ceil_div(tokens, 256 * p.steps);
-  // short chunks where long ones would be fewer than 16 waves to a CU (rows of 64 vectors a wave)
-  p.chunk = ceil_div(tokens, 32) * ceil_div(C, 512) < 256 * 16 ? 8 : 32;
+  // short chunks where long ones would leave most of the card idle (bf16, 1152 channels, 32,768 rows, the whole
+  // gradient: 4,096 tokens 39 us by chunks of 8, 46 of 32; 16,384: 49, 48; 32,768: 70, 58; 256 channels alike)
+  p.chunk = tokens <= 16384 ? 8 : 32;
   p.chunks = ceil_div(tokens, p.chunk);
   p.pairs_bytes = size_t(ceil_div(tokens * 8, 256)) * 256;
   p.hist_bytes = size_t(ceil_div(p.tiles * (int64_t(4) << p.bits), 256)) * 256;
@@ -490,7 +517,8 @@ int sihc_embedding(const void* table, const void* ids, void* out, int64_t tokens
                                scale);
             return check_launch(what);
           };
-          // several vectors a thread once that leaves 4 blocks to a CU
+          // several vectors a thread once that leaves 4 blocks to a CU (8,192 rows of 1152 bf16 channels: 6.8 us,
+          // one vector a thread 7.1; 2,048: 4.0 and 3.8)
           return items >= 256 * 4 * 1024 ? launch(IC<4>{}) : launch(IC<1>{});
         }
         return check_launch(what);
@@ -528,7 +556,8 @@ int sihc_embedding_backward(const void* grad, const void* ids, void* grad_table,
           const I* id = static_cast<const I*>(ids);
           T* out = static_cast<T*>(grad_table);
           if (tokens <= FEW_TOKENS) {
-            // about two vectors a thread: more rows would follow one another
+            // about two vectors a thread: more rows would follow one another (64 fp32 tokens of 1152 channels:
+            // one row 5.0 us, 8 rows 7.7)
             const int per_block = std::max(1, std::min(FEW_ROWS, 512 / vecs));
             hipLaunchKernelGGL((k_embed_grad_few<T, I, V>), dim3(unsigned(ceil_div(rows, per_block))), dim3(256), 0, st, g,
                                id, out, int(tokens), uint32_t(rows), channels, vecs, scale, padding, per_block);
