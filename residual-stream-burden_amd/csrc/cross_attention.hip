@@ -842,15 +842,15 @@ Args args_of(const sihc_attention* s) {
   }
   return a;
 }
-// Parts of `length` keys or rows for `blocks` blocks of one wave: none where `full` of them fill the card,
-// otherwise for about that many, of at least `least`.
+// Parts of `length` keys or rows for `blocks` blocks of one wave: none where `full` of them fill the card or
+// `length` is `alone` at most, otherwise for about `target` blocks, of at least `least`.
 struct Parts {
   int count;
   int64_t span;  // a multiple of PIECE
 };
-Parts parts_of(int64_t length, int64_t blocks, int64_t full, int64_t target, int64_t least) {
+Parts parts_of(int64_t length, int64_t blocks, int64_t full, int64_t target, int64_t alone, int64_t least) {
   Parts p{1, ceil_div(std::max<int64_t>(length, 1), PIECE) * PIECE};
-  if (blocks <= 0 || blocks >= full || length <= least) return p;
+  if (blocks <= 0 || blocks >= full || length <= alone) return p;
   const int64_t most = std::min<int64_t>({ceil_div(target, blocks), ceil_div(length, least), int64_t(256)});
   p.span = ceil_div(ceil_div(length, most), PIECE) * PIECE;
   p.count = int(ceil_div(length, p.span));
@@ -858,16 +858,20 @@ Parts parts_of(int64_t length, int64_t blocks, int64_t full, int64_t target, int
 }
 int64_t row_count(const sihc_attention* s) { return int64_t(s->queries) * (s->heads / s->kv_heads); }
 int64_t row_blocks(const sihc_attention* s) { return s->batch * s->kv_heads * ceil_div(row_count(s), 32); }
-// fp32 products take 8 times the time of bf16 ones, so parts of one piece are worth their joining.
-int64_t least_part(const sihc_attention* s) { return s->dtype == SIHC_DTYPE_F32 ? PIECE : 2 * PIECE; }
-// Few query rows: the keys in parts, for the forward and for the gradient of the queries.
-Parts forward_parts(const sihc_attention* s) { return parts_of(s->keys, row_blocks(s), 512, 1024, least_part(s)); }
-Parts dq_parts(const sihc_attention* s) { return parts_of(s->keys, row_blocks(s), 256, 512, least_part(s)); }
+// fp32 products take 8 times the time of bf16 ones, so parts of one piece are worth their joining where those
+// of bf16 are not (8 heads of 64, one query over 128 keys: 9.2 us in two parts, 8.4 in one).
+int64_t alone(const sihc_attention* s) { return s->dtype == SIHC_DTYPE_F32 ? PIECE : 2 * PIECE; }
+// Few query rows: the keys in parts, for the forward (one query over 4,096 keys, 4 key heads of 128: batches of
+// 8, 32, 64 and 128 take 24, 52, 106 and 203 us in parts for 1024 blocks, 175, 177, 180 and 190 in one) and
+// for the gradient of the queries (32 queries over 2,048 keys, 8 heads of 64: all gradients of batches of 1,
+// 16, 32, 48 18, 54, 90 and 135 us in parts for 512 blocks, 57, 84, 108 and 141 in one).
+Parts forward_parts(const sihc_attention* s) { return parts_of(s->keys, row_blocks(s), 512, 1024, alone(s), PIECE); }
+Parts dq_parts(const sihc_attention* s) { return parts_of(s->keys, row_blocks(s), 512, 512, alone(s), PIECE); }
 // Few keys and many query rows: the rows in parts, for the gradients of keys and values (4 x 16 heads x
 // 4,096 rows over 2,048 keys and 4 key heads, 1024 waves of 32 keys: 463 us in one part, 329 in two,
-// 338 in four).
+// 338 in four; 8 x 16 heads of 72, 256 rows over 256 keys: all gradients 42 us in parts of 128 rows, 30 in one).
 Parts dkv_parts(const sihc_attention* s) {
-  return parts_of(row_count(s), s->batch * s->kv_heads * ceil_div(s->keys, 32), 2048, 2048, 2 * least_part(s));
+  return parts_of(row_count(s), s->batch * s->kv_heads * ceil_div(s->keys, 32), 2048, 2048, 2 * alone(s), 2 * alone(s));
 }
 int64_t query_rows(const sihc_attention* s) { return s->batch * s->heads * int64_t(s->queries); }
 // Calls f(T, DP): the smallest compiled width of a head.
@@ -881,11 +885,12 @@ int by_width(const sihc_attention* s, F&& f) {
     return f(t, IC<128>{});
   });
 }
-// Calls f(NW) with the waves of a block over `rows` rows of its own side, `heads` times: blocks of one
-// wave where larger ones would leave most of the card idle.
+// Calls f(NW) with the waves of a block over `rows` rows of its own side: four share the other side's pieces
+// (4 x 16 heads of 72, 256 rows over 256 keys: forward 15.3 us, by blocks of one wave 17.8, gradients 27 and
+// 33) unless there is work for one alone (64 x 16 heads of 72, 32 rows: 33 and 22).
 template <typename F>
-int by_waves(int64_t rows, int64_t heads, F&& f) {
-  return rows <= 32 || ceil_div(rows, 128) * heads < 256 ? f(IC<1>{}) : f(IC<4>{});
+int by_waves(int64_t rows, F&& f) {
+  return rows <= 32 ? f(IC<1>{}) : f(IC<4>{});
 }
 
 }  // namespace
@@ -927,7 +932,7 @@ int sihc_cross_attention(const sihc_attention* s, const void* q, const void* k, 
   a.stats = reinterpret_cast<float2*>(stats);
   return by_width(s, [&](auto t, auto dp) {
     using T = decltype(t);
-    return by_waves(a.rows, a.batch * a.shared * a.splits, [&](auto nw) {
+    return by_waves(a.rows, [&](auto nw) {
       constexpr int NW = decltype(nw)::value;
       a.tiles = ceil_div(a.rows, NW * 32);
       hipLaunchKernelGGL((k_attend<T, decltype(dp)::value, NW>),
@@ -999,7 +1004,7 @@ int sihc_cross_attention_backward(const sihc_attention* s, const void* grad, con
       const Parts parts = dq_parts(s);
       a.splits = parts.count;
       a.span = parts.span;
-      rc = by_waves(a.rows, a.batch * a.shared * a.splits, [&](auto nw) {
+      rc = by_waves(a.rows, [&](auto nw) {
         constexpr int NW = decltype(nw)::value;
         a.tiles = ceil_div(a.rows, NW * 32);
         hipLaunchKernelGGL((k_attend_dq<T, DP, NW>), dim3(unsigned(a.tiles * a.batch * a.shared * a.splits)),
@@ -1012,7 +1017,7 @@ int sihc_cross_attention_backward(const sihc_attention* s, const void* grad, con
     const Parts parts = dkv_parts(s);
     a.splits = parts.count;
     a.span = parts.span;
-    return by_waves(a.keys, a.batch * a.shared * a.splits, [&](auto nw) {
+    return by_waves(a.keys, [&](auto nw) {
       constexpr int NW = decltype(nw)::value;
       a.tiles = ceil_div(a.keys, NW * 32);
       hipLaunchKernelGGL((k_attend_dkv<T, DP, NW>), dim3(unsigned(a.tiles * a.batch * a.shared * a.splits)),
