@@ -731,6 +731,13 @@ int check_sizes(const char* what, int64_t batch, int64_t pixels, int C, int grou
     return fail(SIHC_ERR_INVALID, "%s: weights must be fp32 or share the input's type", what);
   return SIHC_OK;
 }
+// The chunks of a pass that leaves no sums: short, their length changes no result (64 x 64 x 64 x 1152, 32 steps
+// in the chunks of the moments: the forward 341 us by 4 steps, 353 by 8, 367 by 32; one image 21, 21 and 31).
+Shape short_chunks(Shape s) {
+  s.span = AHEAD * s.rows;
+  s.chunks = int(ceil_div(s.pixels, s.span));
+  return s;
+}
 int elem_size(int dtype) { return dtype == SIHC_DTYPE_F32 ? 4 : 2; }
 
 // Calls f(T, TW, V, NV, TB) with NV the smallest compiled count of at least p.NV vectors, or, for whole
@@ -801,7 +808,8 @@ int sihc_group_norm(const void* x, const void* weight, const void* bias, void* y
   if (!aligned(workspace, 8) || !aligned(stats, 8)) return fail(SIHC_ERR_INVALID, "%s: misaligned workspace or stats", what);
   const Plan p = plan(batch, pixels, channels, groups, eps, act == SIHC_ACT_SILU, elem_size(dtype), false);
   const int64_t blocks = p.whole ? batch * (groups / p.s.slice_groups) : batch * p.s.chunks * p.s.widths;
-  if (blocks > 0x7fffffff) return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
+  if (blocks > 0x7fffffff || batch * short_chunks(p.s).chunks * p.s.widths > 0x7fffffff)
+    return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
   const dim3 grid(static_cast<unsigned>(blocks)), threads(static_cast<unsigned>(p.s.threads));
   hipStream_t st = static_cast<hipStream_t>(stream);
   return by_plan<false>(
@@ -824,8 +832,10 @@ int sihc_group_norm(const void* x, const void* weight, const void* bias, void* y
         hipLaunchKernelGGL((k_norm_moments<T, V>), grid, threads, lds, st, static_cast<const T*>(x), part, p.s);
         hipLaunchKernelGGL(k_norm_stats, dim3(unsigned(ceil_div(batch * groups, 4))), dim3(256), 0, st, part, own,
                            reinterpret_cast<float2*>(stats), p.s);
-        hipLaunchKernelGGL((k_norm_apply<T, TW, V>), grid, threads, 0, st, static_cast<const T*>(x),
-                           static_cast<const TW*>(weight), static_cast<const TW*>(bias), own, static_cast<T*>(y), p.s);
+        const Shape s = short_chunks(p.s);
+        hipLaunchKernelGGL((k_norm_apply<T, TW, V>), dim3(unsigned(batch * s.chunks * s.widths)), threads, 0, st,
+                           static_cast<const T*>(x), static_cast<const TW*>(weight), static_cast<const TW*>(bias), own,
+                           static_cast<T*>(y), s);
         return check_launch(what);
       });
 }
@@ -862,7 +872,8 @@ int sihc_group_norm_backward(const void* grad, const void* x, const void* weight
       return fail(SIHC_ERR_INVALID, "%s: misaligned workspace or stats", what);
     const Plan p = plan(batch, pixels, channels, groups, 0.f, act == SIHC_ACT_SILU, elem_size(dtype), true);
     const int64_t blocks = p.whole ? batch * (groups / p.s.slice_groups) : batch * p.s.chunks * p.s.widths;
-    if (blocks > 0x7fffffff) return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
+    if (blocks > 0x7fffffff || batch * short_chunks(p.s).chunks * p.s.widths > 0x7fffffff)
+      return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
     parts = batch;
     const dim3 grid(static_cast<unsigned>(blocks)), threads(static_cast<unsigned>(p.s.threads));
     const int rc = by_plan<true>(
@@ -887,10 +898,12 @@ int sihc_group_norm_backward(const void* grad, const void* x, const void* weight
           const unsigned lds = 2u * unsigned(p.s.rows) * unsigned(p.s.W) * 4u;
           auto pass = [&](auto dx) {
             constexpr bool DX = decltype(dx)::value;
-            hipLaunchKernelGGL((k_norm_grad_rows<T, TW, V, DX>), grid, threads, DX ? 0 : lds, st,
+            const Shape s = DX ? short_chunks(p.s) : p.s;
+            hipLaunchKernelGGL((k_norm_grad_rows<T, TW, V, DX>), dim3(unsigned(batch * s.chunks * s.widths)), threads,
+                               DX ? 0 : lds, st,
                                static_cast<const T*>(grad), static_cast<const T*>(x), static_cast<const TW*>(weight),
                                static_cast<const TW*>(bias), reinterpret_cast<const float2*>(stats), means,
-                               static_cast<T*>(grad_x), part, p.s);
+                               static_cast<T*>(grad_x), part, s);
           };
           pass(std::false_type{});
           hipLaunchKernelGGL(k_norm_grad_means<TW>, dim3(unsigned(batch)), dim3(1024), 0, st, part,
