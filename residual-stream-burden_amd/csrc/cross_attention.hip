@@ -15,8 +15,18 @@
 // The query rows of all heads that share a key head are one list of rows (head by head), so shared
 // heads fill tiles together, and their key gradients are one sum.
 //
-// Rounding: probabilities and score gradients enter their products in the inputs' type; scores,
-// statistics, sums and the row sums of dO O stay in fp32.
+// What bounds it, at 4 images, 16 heads of 64 over 4 key heads, 4,096 rows over up to 2,048 keys (bf16): the
+// matrix and vector instructions between them. The forward takes 168-176 us (587 TFLOP/s), the query gradient
+// 195-209, the key and value gradients 305-319; all three 530-560 us, half the rate of a large matrix
+// product, because a wave's exponentials and its products share one SIMD and its tiles leave it one to
+// two other waves to run beside. At 256 rows over 256 keys (64 images, 16 heads of 72) the blocks live for
+// a few pieces only, and their loads' latency bounds them: 61, 72 and 73 us, about 2.5 times the time of
+// the bytes. One row over 4,096 keys (8 images, 16 heads of 128 over 4): 17 us of 67 MB, and 4 us to join.
+//
+// Rounding: probabilities and score gradients enter their products in the inputs' type (a bf16 gradient is
+// then 1.4 times as far from the exact one as its own rounding puts it: two products' operands are rounded,
+// and fp32 operands would take eight times the matrix time); scores, statistics, sums and the row sums of
+// dO O stay in fp32.
 #include "cond_common.h"
 
 namespace {
@@ -384,8 +394,11 @@ __device__ __forceinline__ int wave_rows() { return int(threadIdx.x >> 6) * 32 *
 // Blocks of several waves are compiled for two waves on a SIMD where their tiles fit 256 registers, three
 // where they fit 168: the softmax of one wave then runs beside the products of another.
 // -------------------------------------------------------------------------------- forward
+constexpr int forward_waves(int bytes, bool halves, int NW) {  // waves of a SIMD; bytes of a head's row
+  return NW == 1 || bytes > 384 ? 1 : halves && bytes <= 160 ? 3 : 2;
+}
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 384 ? (sizeof(T) * DP <= 160 && sizeof(T) == 2 ? 3 : 2) : 1) void k_attend(Args a) {
+__global__ __launch_bounds__(NW * 64, forward_waves(sizeof(T) * DP, sizeof(T) == 2, NW)) void k_attend(Args a) {
   __shared__ __attribute__((aligned(16))) T lds[2 * Lds<T, DP>::SIZE];
   T *const lds_k = lds, *const lds_v = lds + Lds<T, DP>::SIZE, *const mine = lds + wave_rows<T, DP>();
   const Unit u = unit_of(a);
@@ -490,7 +503,7 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 384 ? (sizeof(
   }
 }
 
-// The parts of a row, brought under their largest score and summed: a block a row, of 8 groups of 32
+// Latency: 4.3 us for 128 rows of 17 parts. The parts of a row, brought under their largest score and summed: a block a row, of 8 groups of 32
 // lanes that take every eighth part, 4 channels a lane, and whose sums are added in order.
 template <typename T>
 __global__ __launch_bounds__(256) void k_attend_join(Args a, int64_t total) {
@@ -640,8 +653,9 @@ __global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= 320 ? 2 : 1) v
 }
 
 // --------------------------------------------------------- gradients of the keys and values
+constexpr int keys_waves(int bytes, bool halves, int NW) { return NW > 1 && bytes <= (halves ? 192 : 256) ? 2 : 1; }
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, NW > 1 && sizeof(T) * DP <= (sizeof(T) == 2 ? 192 : 256) ? 2 : 1) void k_attend_dkv(Args a) {
+__global__ __launch_bounds__(NW * 64, keys_waves(sizeof(T) * DP, sizeof(T) == 2, NW)) void k_attend_dkv(Args a) {
   __shared__ __attribute__((aligned(16))) T lds[2 * Lds<T, DP>::SIZE];
   T *const lds_q = lds, *const lds_g = lds + Lds<T, DP>::SIZE, *const mine = lds + wave_rows<T, DP>();
   __shared__ __attribute__((aligned(16))) float lds_top[PIECE], lds_inverse[PIECE], lds_delta[PIECE];
@@ -966,7 +980,8 @@ int sihc_cross_attention_backward(const sihc_attention* s, const void* grad, con
   const char* what = "sihc_cross_attention_backward";
   if (int rc = check_args(what, s)) return rc;
   if (s->batch == 0) return SIHC_OK;
-  if (s->queries && (!grad || !q || !out || !stats || !grad_q || (s->dtype == SIHC_DTYPE_BF16 && !low))) return fail(SIHC_ERR_INVALID, "%s: null pointer", what);
+  if (s->queries && (!grad || !q || !out || !stats || !grad_q || (s->dtype == SIHC_DTYPE_BF16 && !low)))
+    return fail(SIHC_ERR_INVALID, "%s: null pointer", what);
   if (s->keys && (!k || !v || !grad_k || !grad_v)) return fail(SIHC_ERR_INVALID, "%s: null pointer", what);
   for (const void* in : {grad, q, k, v, out, low})
     for (const void* to : {grad_q, grad_k, grad_v})

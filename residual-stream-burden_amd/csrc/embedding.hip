@@ -320,13 +320,14 @@ __global__ __launch_bounds__(256) void k_sort_scatter(K keys, const uint32_t* __
 }
 
 // ----------------------------------------------------------------- gradient, sorted tokens
-// One wave: CHUNK (8 or 32) sorted tokens x 64 vectors of the row, 8 of them in flight. partial[chunk][0]: the run that the chunk
-// before began; [1]: the run that begins here and goes on in the next chunk. A run through the whole
-// chunk is [0].
+// One wave: CHUNK (8 or 32) sorted tokens x 64 vectors of the row, 8 of them in flight. partial[chunk][0]:
+// the run that the chunk before began; [1]: the run that begins here and goes on in the next chunk. A run
+// through the whole chunk is [0].
 template <typename T, int V, int CHUNK>
 __global__ __launch_bounds__(256) void k_embed_grad(const T* __restrict__ grad, const u32x2* __restrict__ sorted,
                                                     T* __restrict__ out, float* __restrict__ partial,
-                                                    uint32_t* __restrict__ crossing, int64_t n, int64_t chunks, uint32_t rows, int C, int slices, float scale) {
+                                                    uint32_t* __restrict__ crossing, int64_t n, int64_t chunks,
+                                                    uint32_t rows, int C, int slices, float scale) {
   const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
   const int64_t chunk = item / slices;
   if (chunk >= chunks) return;

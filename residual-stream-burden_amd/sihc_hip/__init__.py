@@ -8,6 +8,7 @@ Modules
   indexed            spatially indexed (int32 state index) gather/scatter and read/write
   conditioning       embedding lookup, cross attention and group norm with an activation: what
                      conditions a denoiser on an encoder's states
+  text_denoiser      a text-conditioned SiHC denoiser on them
   launch             tensor-level launchers over the C ABI (include/sihc_hip.h)
 """
 from ._lib import LIB_PATH, lib  # noqa: F401
