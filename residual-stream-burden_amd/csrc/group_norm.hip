@@ -97,9 +97,9 @@ template <typename T, int V>
 constexpr int words() { return V * int(sizeof(T)) < 4 ? 1 : V * int(sizeof(T)) / 4; }
 
 // Sums of two values over the threads of each group of the slice, for every thread its own group's.
-// lds: 2 x TB floats, not in use since the last barrier but one.
+// lds: 2 x TB floats, not in use since the last barrier but one. of: the groups' sums, where there are several.
 template <int TB>
-__device__ __forceinline__ float2 two_sums(float2 v, const Shape& s, int group, float* lds) {
+__device__ __forceinline__ float2 two_sums(float2 v, const Shape& s, int group, float* lds, float2* of) {
   const int tid = int(threadIdx.x), wave = tid >> 6, lane = tid & 63;
   float2 out = {0.f, 0.f};
   if (s.slice_groups == 1) {
@@ -120,24 +120,18 @@ __device__ __forceinline__ float2 two_sums(float2 v, const Shape& s, int group, 
   lds[TB + tid] = v.y;
   __syncthreads();
   const int span = s.lanes / s.slice_groups, count = s.rows * span;
-  float2 mine[2];  // (a slice has at most 2 groups a wave: 32 of 1024 threads)
-  for (int g = wave, k = 0; g < s.slice_groups; g += TB / 64, ++k) {
+  for (int g = wave; g < s.slice_groups; g += TB / 64) {
     float2 t = {0.f, 0.f};
     for (int i = lane; i < count; i += 64) {
       const int at = (i / span) * s.lanes + g * span + i % span;
       t.x += lds[at];
       t.y += lds[TB + at];
     }
-    mine[k & 1] = {wave_sum(t.x), wave_sum(t.y)};
+    t = {wave_sum(t.x), wave_sum(t.y)};
+    if (lane == 0) of[g] = t;
   }
   __syncthreads();
-  for (int g = wave, k = 0; g < s.slice_groups; g += TB / 64, ++k)
-    if (lane == 0) {
-      lds[g] = mine[k & 1].x;
-      lds[TB + g] = mine[k & 1].y;
-    }
-  __syncthreads();
-  return {lds[group], lds[TB + group]};
+  return of[group];
 }
 
 // Sums of the V elements of a vector and of their squares. bf16: two elements an instruction, the
@@ -180,6 +174,7 @@ __global__ __launch_bounds__(TB, (simd_waves(TB, NV * words<T, V>(), V, false)))
     const T* __restrict__ x, const TW* __restrict__ weight, const TW* __restrict__ bias, T* __restrict__ y,
     float2* __restrict__ stats, Shape s) {
   __shared__ float lds[2][2 * TB];
+  __shared__ float2 sums[TB];
   const Place p = place<V>(s, int(blockIdx.x), int(gridDim.x));
   const int64_t at = (p.b * s.pixels + p.row) * s.C + p.slice * s.W + p.lane * V, step = int64_t(s.rows) * s.C;
   Vec<T, V> held[NV];
@@ -190,12 +185,12 @@ __global__ __launch_bounds__(TB, (simd_waves(TB, NV * words<T, V>(), V, false)))
   float2 sum = {0.f, 0.f};
 #pragma unroll
   for (int k = 0; k < NV; ++k) add_moments(held[k], sum);
-  sum = two_sums<TB>(p.on ? sum : float2{0.f, 0.f}, s, p.group, lds[0]);
+  sum = two_sums<TB>(p.on ? sum : float2{0.f, 0.f}, s, p.group, lds[0], sums);
   const float mean = sum.x * inverse_n;
   float var = sum.y * inverse_n - mean * mean;
   bool lost = sizeof(T) == 4 || !(mean * mean <= 64.f * var);
   for (int g = 0; s.slice_groups > 1 && g < s.slice_groups; ++g) {  // (the same answer for every thread)
-    const float m = lds[0][g] * inverse_n, v = lds[0][TB + g] * inverse_n - m * m;
+    const float m = sums[g].x * inverse_n, v = sums[g].y * inverse_n - m * m;
     lost |= !(m * m <= 64.f * v);
   }
   if (lost) {
@@ -211,7 +206,7 @@ __global__ __launch_bounds__(TB, (simd_waves(TB, NV * words<T, V>(), V, false)))
         for (int e = 0; e < V; ++e) squares.x += (v[e] - mean) * (v[e] - mean);
       }
     }
-    var = two_sums<TB>(squares, s, p.group, lds[1]).x * inverse_n;
+    var = two_sums<TB>(squares, s, p.group, lds[1], sums).x * inverse_n;
   }
   const float rstd = 1.f / sqrtf(var + s.eps);
   if (stats && p.row == 0 && p.on && p.lane * V % s.per_group == 0)

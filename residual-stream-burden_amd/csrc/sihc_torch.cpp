@@ -630,10 +630,11 @@ struct EmbedFn : torch::autograd::Function<EmbedFn> {
       const c10::DeviceGuard device(grad.device());
       const int c = int(grad.size(-1));
       out = at::empty({rows, c}, grad.options());
-      const Tensor ws = workspace(sihc_embedding_backward_workspace_size(ids.numel(), rows, c), grad);
+      const size_t bytes = sihc_embedding_backward_workspace_size(ids.numel(), rows, c);
+      const Tensor ws = bytes ? workspace(bytes, grad) : Tensor();
       check(sihc_embedding_backward(grad.const_data_ptr(), ids.const_data_ptr(), out.data_ptr(), ids.numel(), rows, c,
-                                    float(scale), padding, id_bits(ids), dtype_code(grad), ws.data_ptr(),
-                                    size_t(ws.numel()) * 4, stream_of(grad)),
+                                    float(scale), padding, id_bits(ids), dtype_code(grad),
+                                    bytes ? ws.data_ptr() : nullptr, bytes, stream_of(grad)),
             false);
     } else {
       static auto op = registered<Tensor(const Tensor&, const Tensor&, int64_t, double, int64_t)>(

@@ -162,3 +162,18 @@ def test_drawn_sizes():
         want, dwant = embed_oracle(table, ids, 1.5, padding, grad)
         assert rel_l2(out.cpu(), want) <= 1.5 * (3.3e-3 if dtype == BF16 else 1e-5)
         assert rel_l2(dt.cpu(), dwant) <= 1.5 * (3.3e-3 if dtype == BF16 else 1e-5) if dwant.any() else not dt.any()
+
+
+# batches that leave a block many groups: 16 of one channel and 4 waves, 32 and 16 waves, 64, and a prime number
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("batch,pixels,channels,groups", [
+    (300, 16, 32, 32), (600, 9, 64, 64), (600, 200, 32, 32), (520, 5, 97, 97), (300, 30, 128, 32), (1100, 40, 64, 64)])
+def test_group_norm_of_many_narrow_groups(batch, pixels, channels, groups, dtype):
+    announce(f"group norm {batch}x{pixels}x{channels} groups={groups} {dtype}")
+    x = normal((batch, pixels, channels), dtype, 31, mean=0.4).requires_grad_()
+    w, b = normal((channels,), dtype, 32, mean=1.0, std=0.3).requires_grad_(), normal((channels,), dtype, 33).requires_grad_()
+    grad = normal(x.shape, dtype, 34)
+    y = group_norm_act(x, w, b, groups, 1e-5, "silu")
+    got = (y, *torch.autograd.grad(y, (x, w, b), grad))
+    for g, e, name in zip(got, norm_oracle(x, w, b, groups, 1e-5, "silu", grad), ("y", "dx", "dw", "db")):
+        assert rel_l2(g.cpu(), e) <= (1e-5 if dtype is F32 else 3.3e-3), name
