@@ -86,12 +86,12 @@ __device__ __forceinline__ Place place(const Shape& s, int block, int blocks) {
 // Threads of a block, at most, and the blocks of 1024 threads on a CU that a kernel is compiled for: two
 // where what a thread holds, and works with beside it, fits 64 registers, so that one loads while
 // the other computes.
-constexpr int MOST_THREADS = 1024;
+constexpr int MOST_THREADS = 1024, MIDDLE = 512, MIDDLE_VECTORS = 20;
 constexpr int large_blocks(int held, int V, bool backward) {
   return (backward ? held + 4 * V <= 22 : held + 2 * V <= 28) ? 2 : 1;
 }
 [[maybe_unused]] constexpr int simd_waves(int TB, int held, int V, bool backward) {
-  return TB < MOST_THREADS ? 1 : 4 * large_blocks(held, V, backward);
+  return TB == MIDDLE ? 4 : TB < MOST_THREADS ? 1 : 4 * large_blocks(held, V, backward);
 }
 template <typename T, int V>
 constexpr int words() { return V * int(sizeof(T)) < 4 ? 1 : V * int(sizeof(T)) / 4; }
@@ -696,6 +696,12 @@ Plan plan(int64_t batch, int64_t pixels, int C, int groups, float eps, bool silu
   // small slices: blocks of 256 threads, several to a CU (256 x 4 x 4 x 1152: 24 us, by 1024 threads 50; 64 x 7 x 7
   // x 136: 17.6 and 18.9)
   s.threads = vectors(s.slice_groups, 256) <= std::min(8, most) ? 256 : MOST_THREADS;
+  // forward: two blocks of 512 threads to a CU where the grid has them and a thread's 20 vectors hold the slice (32
+  // images of 32 x 32 x 768: 22 us, by 1024 threads 26; 128 of 16 x 16 x 1152: 29 and 35; fp32, 64 of 32 x 32 x
+  // 512: 45 and 56; by twice as many shorter vectors, 64 of 32 x 32 x 1152, 79 and 78; the gradients hold too much)
+  if (!backward && p.V * elem >= 8 && s.threads == MOST_THREADS &&
+      vectors(s.slice_groups, MIDDLE) <= std::min(MIDDLE_VECTORS, most) && batch * (groups / s.slice_groups) >= 512)
+    s.threads = MIDDLE;
   s.W = s.slice_groups * s.per_group;
   s.lanes = s.W / p.V;
   s.rows = s.threads / s.lanes;
@@ -768,6 +774,11 @@ int by_plan(const Plan& p, int dtype, int w_dtype, F&& f, R&& rows) {
       };
       constexpr IC<256> small{};
       constexpr IC<1024> large{};
+      if constexpr (!BACKWARD && V * sizeof(T) >= 8) {
+        constexpr IC<MIDDLE> middle{};
+        if (attempt(IC<8>{}, middle) || attempt(IC<14>{}, middle) || attempt(IC<MIDDLE_VECTORS>{}, middle))
+          return rc;
+      }
       if (attempt(IC<1>{}, small) || attempt(IC<2>{}, small) || attempt(IC<4>{}, small) || attempt(IC<6>{}, small) ||
           attempt(IC<8>{}, small) ||
           attempt(IC<4>{}, large) || attempt(IC<7>{}, large) || attempt(IC<10>{}, large) || attempt(IC<14>{}, large) ||
