@@ -16,12 +16,12 @@
 // heads fill tiles together, and their key gradients are one sum.
 //
 // What bounds it, at 4 images, 16 heads of 64 over 4 key heads, 4,096 rows over up to 2,048 keys (bf16): the
-// matrix and vector instructions between them. The forward takes 168-176 us (587 TFLOP/s), the query gradient
-// 195-209, the key and value gradients 305-319; all three 530-560 us, half the rate of a large matrix
-// product, because a wave's exponentials and its products share one SIMD and its tiles leave it one to
+// matrix and vector instructions between them. All three take 500-560 us, half the rate of a large matrix
+// product (the forward 157-172, the query gradient 190-204, the key and value gradients 290-316 when each
+// is traced), because a wave's exponentials and its products share one SIMD and its tiles leave it one to
 // two other waves to run beside. At 256 rows over 256 keys (64 images, 16 heads of 72) the blocks live for
-// a few pieces only, and their loads' latency bounds them: 61, 72 and 73 us, about 2.5 times the time of
-// the bytes. One row over 4,096 keys (8 images, 16 heads of 128 over 4): 17 us of 67 MB, and 4 us to join.
+// a few pieces only, and their loads' latency bounds them: 60, 70 and 72 us, 194 together, 2.4 times the
+// time of the bytes. One row over 4,096 keys (8 images, 16 heads of 128 over 4): 17 us of 67 MB, and 4 us to join.
 //
 // Rounding: probabilities and score gradients enter their products in the inputs' type (a bf16 gradient is
 // then 1.4 times as far from the exact one as its own rounding puts it: two products' operands are rounded,
