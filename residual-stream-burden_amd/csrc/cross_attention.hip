@@ -503,8 +503,9 @@ __global__ __launch_bounds__(NW * 64, forward_waves(sizeof(T) * DP, sizeof(T) ==
   }
 }
 
-// Latency: 4.3 us for 128 rows of 17 parts. The parts of a row, brought under their largest score and summed: a block a row, of 8 groups of 32
-// lanes that take every eighth part, 4 channels a lane, and whose sums are added in order.
+// The parts of a row, brought under their largest score and summed: a block a row, of 8 groups of 32 lanes
+// that take every eighth part, 4 channels a lane, and whose sums are added in order. Latency: 4.4 us for 128
+// rows of 32 parts of 128 channels.
 template <typename T>
 __global__ __launch_bounds__(256) void k_attend_join(Args a, int64_t total) {
   __shared__ f32x4 lds_o[8][32];
