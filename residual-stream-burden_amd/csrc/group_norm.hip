@@ -19,8 +19,9 @@
 // moments and once for the result. 64 images of 64 x 64 x 1152: 341 us, 3.5 TB/s of the 1.2 GB in and
 // out (5.3 TB/s with the second reading); by slices 392.
 //
-// A mean is subtracted before squares are summed (over the block's own elements, or about a first value,
-// then over the chunks' means), so a large mean costs no digits. Channel sums are added in a fixed
+// A mean is subtracted before squares are summed (over the block's own elements, or about a middle value of
+// a thread's own, then about the threads' and the chunks' means), so neither a large mean nor a value far from
+// the others costs digits. Channel sums are added in a fixed
 // order, without atomics.
 #include "cond_common.h"
 
@@ -267,32 +268,31 @@ __device__ __forceinline__ Stream stream_of(const Shape& s, int block) {
 constexpr int AHEAD = 4;
 
 // One reading: 604 MB (64 images of 64 x 64 x 1152) in 135 us, 4.5 TB/s, the rest of the time the blocks' own sums.
-// part: [batch, chunks, groups] of (mean, squares about it) of the chunk's pixels. A thread sums about its
-// channel's first value, the block about the first value of the group, so that no digits are lost to a mean.
+// part: [batch, chunks, groups] of (mean, squares about it) of the chunk's pixels. A thread sums about the median
+// of its channel's first three values, so that neither a mean nor a single value far from the others costs
+// digits; the block then takes the mean of the threads' means, and their squares about that.
 template <typename T, int V>
 __global__ __launch_bounds__(1024) void k_norm_moments(const T* __restrict__ x, float2* __restrict__ part, Shape s) {
-  extern __shared__ float lds[];  // [2][rows][W], then the groups' first values
+  extern __shared__ float lds[];  // [2][rows][W]: the threads' means, and squares about them
   const Stream p = stream_of<V>(s, int(blockIdx.x));
   const int tid = int(threadIdx.x), size = s.rows * s.W, groups = s.W / s.per_group, first_group = p.c / s.W * groups;
-  float* first = lds + 2 * size;
   const int64_t at = (p.b * s.pixels + p.first + p.row) * s.C + p.c, step = int64_t(s.rows) * s.C;
-  const int cl = p.c % s.W, g0 = cl / s.per_group, in0 = cl - g0 * s.per_group;  // group, channel of the group
+  const int cl = p.c % s.W;
   float shift[V] = {}, sum[V] = {}, squares[V] = {};
+  int count = 0;
   if (p.on && p.row < p.pixels) {
-    load<T, V>(x + at).to(shift);
-    if (p.row == 0) {
-      int in = in0, g = g0;
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        if (in == 0) first[g] = shift[e];
-        if (++in == s.per_group) in = 0, ++g;
-      }
-    }
-    const int count = (p.pixels - p.row + s.rows - 1) / s.rows;
+    count = (p.pixels - p.row + s.rows - 1) / s.rows;
     for (int k0 = 0; k0 < count; k0 += AHEAD) {
       Vec<T, V> v[AHEAD];
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j) v[j] = load<T, V>(x + at + min(k0 + j, count - 1) * step);
+      if (k0 == 0) {
+        float f[3][V];
+#pragma unroll
+        for (int j = 0; j < 3; ++j) v[j].to(f[j]);
+#pragma unroll
+        for (int e = 0; e < V; ++e) shift[e] = __builtin_amdgcn_fmed3f(f[0][e], f[1][e], f[2][e]);
+      }
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j) {
         if (k0 + j >= count) break;
@@ -307,32 +307,36 @@ __global__ __launch_bounds__(1024) void k_norm_moments(const T* __restrict__ x, 
       }
     }
   }
-  __syncthreads();
   if (p.on) {
-    const float n = p.row < p.pixels ? float((p.pixels - p.row + s.rows - 1) / s.rows) : 0.f;
-    int in = in0, g = g0;
+    const float inverse = count ? 1.f / float(count) : 0.f;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const float d = n > 0.f ? shift[e] - first[g] : 0.f;
-      if (++in == s.per_group) in = 0, ++g;
-      lds[p.row * s.W + cl + e] = fmaf(n, d, sum[e]);
-      lds[size + p.row * s.W + cl + e] = squares[e] + d * (2.f * sum[e] + n * d);
+      lds[p.row * s.W + cl + e] = fmaf(sum[e], inverse, shift[e]);
+      lds[size + p.row * s.W + cl + e] = fmaxf(squares[e] - sum[e] * (sum[e] * inverse), 0.f);
     }
   }
   __syncthreads();
-  const float n = float(p.pixels) * float(s.per_group);
+  // (row r holds `each` pixels, or one more)
+  const int each = p.pixels / s.rows, more = p.pixels - each * s.rows, used = min(s.rows, p.pixels);
+  const float n = float(p.pixels) * float(s.per_group), inverse_n = 1.f / n;
   for (int g = tid >> 6; g < groups; g += int(blockDim.x) >> 6) {
     if (first_group + g >= s.groups) break;
-    float a = 0.f, d = 0.f;
-    for (int r = 0; r < s.rows; ++r)
+    float mean = 0.f, a = 0.f, d = 0.f;
+    for (int r = 0; r < used; ++r)
+      for (int k = tid & 63; k < s.per_group; k += 64)
+        mean = fmaf(float(each + (r < more)) * inverse_n, lds[r * s.W + g * s.per_group + k], mean);
+    mean = wave_sum(mean);
+    for (int r = 0; r < used; ++r)
       for (int k = tid & 63; k < s.per_group; k += 64) {
-        a += lds[r * s.W + g * s.per_group + k];
-        d += lds[size + r * s.W + g * s.per_group + k];
+        const float off = lds[r * s.W + g * s.per_group + k] - mean, count = float(each + (r < more));
+        a = fmaf(count, off, a);
+        d += fmaf(count * off, off, lds[size + r * s.W + g * s.per_group + k]);
       }
-    a = wave_sum(a);
+    a = wave_sum(a);  // (what rounding left of the mean)
     d = wave_sum(d);
     if ((tid & 63) == 0)
-      part[(p.b * s.chunks + p.chunk) * s.groups + first_group + g] = {first[g] + a / n, fmaxf(d - a * (a / n), 0.f)};
+      part[(p.b * s.chunks + p.chunk) * s.groups + first_group + g] = {fmaf(a, inverse_n, mean),
+                                                                       fmaxf(d - a * (a * inverse_n), 0.f)};
   }
 }
 
@@ -845,7 +849,7 @@ int sihc_group_norm(const void* x, const void* weight, const void* bias, void* y
         using TW = decltype(tw);
         constexpr int V = decltype(v)::value;
         float2 *part = static_cast<float2*>(workspace), *own = part + batch * p.s.chunks * groups;
-        const unsigned lds = (2u * unsigned(p.s.rows) * unsigned(p.s.W) + unsigned(p.s.W / p.s.per_group)) * 4u;
+        const unsigned lds = 2u * unsigned(p.s.rows) * unsigned(p.s.W) * 4u;
         hipLaunchKernelGGL((k_norm_moments<T, V>), grid, threads, lds, st, static_cast<const T*>(x), part, p.s);
         hipLaunchKernelGGL(k_norm_stats, dim3(unsigned(ceil_div(batch * groups, 4))), dim3(256), 0, st, part, own,
                            reinterpret_cast<float2*>(stats), p.s);

@@ -1,0 +1,39 @@
+"""GPU: group norm where a few values are far from the rest.
+
+Bounds: fp32 1e-5 in relative L2, as for ordinary inputs. A value D deviations away puts D^2 into its
+group's sum of squares, so sums that are taken about anything but an outlier lose no digits to it: a
+thread's 32 terms carry at most 32 * 2^-24 = 2e-6 of it."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from helpers import announce, rel_l2
+from sihc_hip import group_norm_act
+from test_gpu_conditioning import norm_oracle, normal
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+# slices of a block, and images in whole rows: 4.7 MB in 32 groups, one group of all, rows of odd width
+@pytest.mark.parametrize("far", [100.0, 3e2, 3e3, 3e4])
+@pytest.mark.parametrize("pixels,channels,groups", [(256, 64, 4), (1024, 1152, 32), (16384, 128, 4), (40000, 33, 1)])
+def test_group_norm_keeps_its_digits_beside_an_outlier(pixels, channels, groups, far):
+    announce(f"group norm of {pixels}x{channels} in {groups} groups, the first value of each {far:g} deviations away")
+    x = normal((2, pixels, channels), F32, 40)
+    x[:, 0, ::channels // groups] = far
+    x.requires_grad_()
+    w, b = normal((channels,), F32, 41, mean=1.0, std=0.2).requires_grad_(), normal((channels,), F32, 42).requires_grad_()
+    grad = normal(x.shape, F32, 43)
+    for act in ("none", "silu"):
+        y = group_norm_act(x, w, b, groups, 1e-6, act)
+        got = (y, *torch.autograd.grad(y, (x, w, b), grad))
+        for name, g, e in zip(("y", "dx", "dw", "db"), got, norm_oracle(x, w, b, groups, 1e-6, act, grad)):
+            assert rel_l2(g.cpu(), e) <= 1e-5, (act, name)
+    # the other values, which are small beside the outliers, by themselves and group by group
+    one, zero = torch.ones_like(w), torch.zeros_like(w)
+    y, want = (t.detach().double().cpu().reshape(2, pixels, groups, -1)[:, 1:]
+               for t in (group_norm_act(x, one, zero, groups, 1e-6, "none"),
+                         norm_oracle(x, one, zero, groups, 1e-6, "none", grad)[0]))
+    assert float(((y - want).square().sum((1, 3)) / want.square().sum((1, 3))).sqrt().max()) <= 1e-5
