@@ -189,8 +189,10 @@ __global__ __launch_bounds__(TB, (simd_waves(TB, NV * words<T, V>(), V, false)))
   sum = two_sums<TB>(p.on ? sum : float2{0.f, 0.f}, s, p.group, lds[0], sums);
   const float mean = sum.x * inverse_n;
   float var = sum.y * inverse_n - mean * mean;
-  bool lost = sizeof(T) == 4 || !(mean * mean <= 64.f * var);
-  for (int g = 0; s.slice_groups > 1 && g < s.slice_groups; ++g) {  // (the same answer for every thread)
+  // The same answer for every thread of the block, which meet at barriers below: each works out every group's from
+  // the same sums by the same instructions, and takes its own group's from nowhere else.
+  bool lost = sizeof(T) == 4 || (s.slice_groups == 1 && !(mean * mean <= 64.f * var));
+  for (int g = 0; sizeof(T) == 2 && s.slice_groups > 1 && g < s.slice_groups; ++g) {
     const float m = sums[g].x * inverse_n, v = sums[g].y * inverse_n - m * m;
     lost |= !(m * m <= 64.f * v);
   }

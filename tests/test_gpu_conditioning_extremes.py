@@ -37,3 +37,20 @@ def test_group_norm_keeps_its_digits_beside_an_outlier(pixels, channels, groups,
                for t in (group_norm_act(x, one, zero, groups, 1e-6, "none"),
                          norm_oracle(x, one, zero, groups, 1e-6, "none", grad)[0]))
     assert float(((y - want).square().sum((1, 3)) / want.square().sum((1, 3))).sqrt().max()) <= 1e-5
+
+
+# a mean of about 8 deviations is where the variance is taken again, about the mean; images and groups on both sides of
+# that line, in blocks of one group, of several, and of many
+@pytest.mark.parametrize("batch,pixels,channels,groups", [(600, 64, 128, 32), (600, 256, 128, 16), (300, 100, 64, 64),
+                                                          (8, 256, 64, 2)])
+def test_group_norm_of_means_about_eight_deviations(batch, pixels, channels, groups):
+    announce(f"group norm {batch}x{pixels}x{channels} in {groups} groups, means about 8 deviations")
+    mean = normal((batch, 1, groups, 1), F32, 48, mean=8.0, std=0.2).repeat_interleave(channels // groups, 3)
+    x = (normal((batch, pixels, channels), F32, 49) + mean.reshape(batch, 1, channels)).to(BF16).requires_grad_()
+    w, b = normal((channels,), BF16, 50, mean=1.0).requires_grad_(), normal((channels,), BF16, 51).requires_grad_()
+    grad = normal(x.shape, BF16, 52)
+    y = group_norm_act(x, w, b, groups)
+    got = (y, *torch.autograd.grad(y, (x, w, b), grad))
+    for name, g, e in zip(("y", "dx", "dw", "db"), got, norm_oracle(x, w, b, groups, 1e-6, "silu", grad)):
+        assert rel_l2(g.cpu(), e) <= 3.3e-3, name
+    assert torch.equal(group_norm_act(x, w, b, groups), y)
