@@ -54,3 +54,25 @@ def test_group_norm_of_means_about_eight_deviations(batch, pixels, channels, gro
     for name, g, e in zip(("y", "dx", "dw", "db"), got, norm_oracle(x, w, b, groups, 1e-6, "silu", grad)):
         assert rel_l2(g.cpu(), e) <= 3.3e-3, name
     assert torch.equal(group_norm_act(x, w, b, groups), y)
+
+
+# a deviation whose square passes fp32: the variance is infinite, its reciprocal root zero, and y = act(bias)
+@pytest.mark.parametrize("pixels,channels,groups", [(256, 36, 1), (16384, 36, 1), (1024, 1152, 32)])
+@pytest.mark.parametrize("half", [False, True], ids=["two", "half"])
+def test_group_norm_of_squares_past_fp32(pixels, channels, groups, half):
+    announce(f"group norm of {pixels}x{channels} in {groups} groups, squares past fp32")
+    x = normal((1, pixels, channels), F32, 44)
+    if half:
+        x[:, torch.arange(pixels, device="cuda") % 32 > 15] = 5e19
+    else:
+        x[:, 0, 1::channels // groups], x[:, 1, 5::channels // groups] = -2e19, 2e19
+    x.requires_grad_()
+    w, b = normal((channels,), F32, 45, mean=1.0).requires_grad_(), normal((channels,), F32, 46).requires_grad_()
+    grad = normal(x.shape, F32, 47)
+    y = group_norm_act(x, w, b, groups)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), grad)
+    bias = b.detach().double().requires_grad_()
+    want = torch.nn.functional.silu(bias).expand(x.shape)
+    assert rel_l2(y, want) <= 1e-6
+    assert not dx.any() and not dw.any()
+    assert rel_l2(db, torch.autograd.grad(want, bias, grad.double())[0]) <= 1e-5
