@@ -250,7 +250,17 @@ class SiHCDenoiser(nn.Module):
                 e += 1
         return x, context
 
+    def _context(self, y_emb, dtype, text):
+        """What travels with the workspace from update to update, so that a call keeps nothing in the
+        module: the in-context prefix tokens or None (model.py:674-676). `text` is a subclass's own."""
+        if not self.in_context_len:
+            return None
+        return (y_emb[:, None].expand(-1, self.in_context_len, -1) + self.in_context_posemb).to(dtype)
+
     def forward(self, x, t, y):
+        return self._denoise(x, t, y)
+
+    def _denoise(self, x, t, y, text=None):
         b = x.shape[0]
         p, hi = self.patch, self.image // self.patch
         half = self.freq_dim // 2
@@ -261,9 +271,7 @@ class SiHCDenoiser(nn.Module):
         cond = self.t_mlp(temb) + y_emb
         patches = x.reshape(b, 3, hi, p, hi, p).permute(0, 2, 4, 1, 3, 5).reshape(b, hi, hi, 3 * p * p)
         carrier = self.stem(patches.to(self.stem.weight.dtype)).contiguous()
-        context = None
-        if self.in_context_len:  # model.py:674-676
-            context = (y_emb[:, None].expand(-1, self.in_context_len, -1) + self.in_context_posemb).to(carrier.dtype)
+        context = self._context(y_emb, carrier.dtype, text)
         run = self._stage_schedule if self.schedule == "stage" else self._literal_schedule
         start = 0
         for size in self.stages:

@@ -68,27 +68,29 @@ class TextSiHCDenoiser(SiHCDenoiser):
         # replaceable, as the routing hooks: the operators, their host-side value checks left out
         self.lookup = lambda *a: embedding_lookup(*a, validate=False)
         self.attend = lambda *a: cross_attention(*a, validate=False)
-        self._text: Optional[tuple[Tensor, Tensor]] = None
+
+    # The states travel with the workspace, beside the prefix tokens: calls on several threads, and bodies
+    # that are computed again in the backward, each have their own.
+    def _context(self, y_emb, dtype, text):
+        return super()._context(y_emb, dtype, text), text
 
     def _update(self, block, part, z, mod, context, index):
-        dz, context = super()._update(block, part, z, mod, context, index)
-        if part == 0 and self._text is not None:
-            dz = dz + mod[2].unsqueeze(1) * self.cross[index](z, *self._text, self.attend)
-        return dz, context
+        prefix, text = context
+        dz, prefix = super()._update(block, part, z, mod, prefix, index)
+        if part == 0 and text is not None:
+            dz = dz + mod[2].unsqueeze(1) * self.cross[index](z, *text, self.attend)
+        return dz, (prefix, text)
 
     def forward(self, x: Tensor, t: Tensor, y: Tensor, tokens: Optional[Tensor] = None,
                 lengths: Optional[Tensor] = None) -> Tensor:
         """tokens [B, L] (int32 or int64), lengths [B] int32 (None: all L); no tokens: labels alone."""
-        if tokens is not None:
-            if tokens.shape[1] > self.positions.shape[0]:
-                raise ValueError(f"at most {self.positions.shape[0]} tokens, got {tokens.shape[1]}")
-            states = self.lookup(self.tokens, tokens, math.sqrt(self.state_dim), self.padding_idx)
-            states = self.state_norm(states + self.positions[:tokens.shape[1]])
-            self._text = (states, lengths)
-        try:
-            return super().forward(x, t, y)
-        finally:
-            self._text = None
+        if tokens is None:
+            return self._denoise(x, t, y)
+        if tokens.shape[1] > self.positions.shape[0]:
+            raise ValueError(f"at most {self.positions.shape[0]} tokens, got {tokens.shape[1]}")
+        states = self.lookup(self.tokens, tokens, math.sqrt(self.state_dim), self.padding_idx)
+        states = self.state_norm(states + self.positions[:tokens.shape[1]])
+        return self._denoise(x, t, y, (states, lengths))
 
 
 __all__ = ["TextSiHCDenoiser"]
