@@ -134,6 +134,8 @@ inline int check_launch(const char* what) {
 inline bool valid_dtype(int dtype) { return dtype == SIHC_DTYPE_F32 || dtype == SIHC_DTYPE_BF16; }
 inline bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % uintptr_t(bytes) == 0; }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// Threads of a launch: HIP takes fewer than 2^32 in a dimension (a block of 256 less, for counts rounded up to one).
+constexpr int64_t MOST_LAUNCHED = (int64_t(1) << 32) - 256;
 // Calls f with the element type of a dtype code.
 template <typename F>
 int by_dtype(int dtype, F&& f) {

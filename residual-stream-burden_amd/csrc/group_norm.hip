@@ -753,10 +753,40 @@ int check_sizes(const char* what, int64_t batch, int64_t pixels, int C, int grou
 // in the chunks of the moments: the forward 341 us by 4 steps, 353 by 8, 367 by 32; one image 21, 21 and 31).
 Shape short_chunks(Shape s) {
   s.span = AHEAD * s.rows;
+  // (longer ones where an image's would pass what a launch takes)
+  while (ceil_div(s.pixels, s.span) * s.widths * s.threads > MOST_LAUNCHED) s.span *= 2;
   s.chunks = int(ceil_div(s.pixels, s.span));
   return s;
 }
 int elem_size(int dtype) { return dtype == SIHC_DTYPE_F32 ? 4 : 2; }
+// Images whose blocks a launch takes, for the widest of the launches of a direction; 0: not one.
+int64_t images_of_launch(const Plan& p) {
+  const Shape& s = p.s;
+  int64_t most = 0;
+  if (p.whole) {
+    most = int64_t(s.groups / s.slice_groups) * s.threads;
+  } else {
+    const int64_t sums = int64_t(s.chunks) * s.widths * s.threads,
+                  result = int64_t(short_chunks(s).chunks) * s.widths * s.threads;
+    most = std::max({sums, result, int64_t(s.groups) * 64, int64_t(1024)});  // (a wave a group, a block an image)
+  }
+  return MOST_LAUNCHED / most;
+}
+// Calls f(first image, images) for as many images at a time as a launch takes: a million rows of few channels are
+// a million images of one pixel.
+template <typename F>
+int by_images(const char* what, const Plan& p, F&& f) {
+  const int64_t step = images_of_launch(p);
+  if (step == 0) return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
+  int rc = SIHC_OK;
+  for (int64_t b = 0; b < p.s.batch && !rc; b += step) rc = f(b, std::min(step, p.s.batch - b));
+  return rc;
+}
+template <typename P>
+P* advanced(P* p, int64_t elements, int size) {  // (the element type is known by its size alone)
+  using Byte = std::conditional_t<std::is_const_v<P>, const char, char>;
+  return p ? static_cast<P*>(static_cast<Byte*>(p) + elements * size) : nullptr;
+}
 
 // Calls f(T, TW, V, NV, TB) with NV the smallest compiled count of at least p.NV vectors, or, for whole
 // rows, rows(T, TW, V).
@@ -829,38 +859,46 @@ int sihc_group_norm(const void* x, const void* weight, const void* bias, void* y
   if (need && (!workspace || workspace_bytes < need))
     return fail(SIHC_ERR_INVALID, "%s: workspace of %zu bytes required, got %zu", what, need, workspace_bytes);
   if (!aligned(workspace, 8) || !aligned(stats, 8)) return fail(SIHC_ERR_INVALID, "%s: misaligned workspace or stats", what);
-  const Plan p = plan(batch, pixels, channels, groups, eps, act == SIHC_ACT_SILU, elem_size(dtype), false);
-  const int64_t blocks = p.whole ? batch * (groups / p.s.slice_groups) : batch * p.s.chunks * p.s.widths;
-  if (blocks > 0x7fffffff || batch * short_chunks(p.s).chunks * p.s.widths > 0x7fffffff)
-    return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
-  const dim3 grid(static_cast<unsigned>(blocks)), threads(static_cast<unsigned>(p.s.threads));
+  const Plan all = plan(batch, pixels, channels, groups, eps, act == SIHC_ACT_SILU, elem_size(dtype), false);
+  const void* const whole_x = x;
+  void* const whole_y = y;
+  float2* const whole_stats = reinterpret_cast<float2*>(stats);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return by_plan<false>(
-      p, dtype, w_dtype,
-      [&](auto t, auto tw, auto v, auto nv, auto tb) {
-        using T = decltype(t);
-        using TW = decltype(tw);
-        constexpr int V = decltype(v)::value, NV = decltype(nv)::value, TB = decltype(tb)::value;
-        hipLaunchKernelGGL((k_group_norm<T, TW, V, NV, TB>), grid, threads, 0, st, static_cast<const T*>(x),
-                           static_cast<const TW*>(weight), static_cast<const TW*>(bias), static_cast<T*>(y),
-                           reinterpret_cast<float2*>(stats), p.s);
-        return check_launch(what);
-      },
-      [&](auto t, auto tw, auto v) {
-        using T = decltype(t);
-        using TW = decltype(tw);
-        constexpr int V = decltype(v)::value;
-        float2 *part = static_cast<float2*>(workspace), *own = part + batch * p.s.chunks * groups;
-        const unsigned lds = 2u * unsigned(p.s.rows) * unsigned(p.s.W) * 4u;
-        hipLaunchKernelGGL((k_norm_moments<T, V>), grid, threads, lds, st, static_cast<const T*>(x), part, p.s);
-        hipLaunchKernelGGL(k_norm_stats, dim3(unsigned(ceil_div(batch * groups, 4))), dim3(256), 0, st, part, own,
-                           reinterpret_cast<float2*>(stats), p.s);
-        const Shape s = short_chunks(p.s);
-        hipLaunchKernelGGL((k_norm_apply<T, TW, V>), dim3(unsigned(batch * s.chunks * s.widths)), threads, 0, st,
-                           static_cast<const T*>(x), static_cast<const TW*>(weight), static_cast<const TW*>(bias), own,
-                           static_cast<T*>(y), s);
-        return check_launch(what);
-      });
+  return by_images(what, all, [&](int64_t first, int64_t images) {
+    Plan p = all;
+    p.s.batch = images;
+    const int64_t element = first * pixels * channels;
+    const void* x = advanced(whole_x, element, elem_size(dtype));
+    void* y = advanced(whole_y, element, elem_size(dtype));
+    float2* stats = whole_stats ? whole_stats + first * groups : nullptr;
+    const int64_t blocks = images * (p.whole ? groups / p.s.slice_groups : p.s.chunks * p.s.widths);
+    const dim3 grid(static_cast<unsigned>(blocks)), threads(static_cast<unsigned>(p.s.threads));
+    return by_plan<false>(
+        p, dtype, w_dtype,
+        [&](auto t, auto tw, auto v, auto nv, auto tb) {
+          using T = decltype(t);
+          using TW = decltype(tw);
+          constexpr int V = decltype(v)::value, NV = decltype(nv)::value, TB = decltype(tb)::value;
+          hipLaunchKernelGGL((k_group_norm<T, TW, V, NV, TB>), grid, threads, 0, st, static_cast<const T*>(x),
+                             static_cast<const TW*>(weight), static_cast<const TW*>(bias), static_cast<T*>(y), stats, p.s);
+          return check_launch(what);
+        },
+        [&](auto t, auto tw, auto v) {
+          using T = decltype(t);
+          using TW = decltype(tw);
+          constexpr int V = decltype(v)::value;
+          float2 *part = static_cast<float2*>(workspace), *own = part + images * p.s.chunks * groups;
+          const unsigned lds = 2u * unsigned(p.s.rows) * unsigned(p.s.W) * 4u;
+          hipLaunchKernelGGL((k_norm_moments<T, V>), grid, threads, lds, st, static_cast<const T*>(x), part, p.s);
+          hipLaunchKernelGGL(k_norm_stats, dim3(unsigned(ceil_div(images * groups, 4))), dim3(256), 0, st, part, own,
+                             stats, p.s);
+          const Shape s = short_chunks(p.s);
+          hipLaunchKernelGGL((k_norm_apply<T, TW, V>), dim3(unsigned(images * s.chunks * s.widths)), threads, 0, st,
+                             static_cast<const T*>(x), static_cast<const TW*>(weight), static_cast<const TW*>(bias), own,
+                             static_cast<T*>(y), s);
+          return check_launch(what);
+        });
+  });
 }
 
 size_t sihc_group_norm_backward_workspace_size(int64_t batch, int64_t pixels, int channels, int groups, int dtype) {
@@ -893,47 +931,54 @@ int sihc_group_norm_backward(const void* grad, const void* x, const void* weight
       return fail(SIHC_ERR_INVALID, "%s: workspace of %zu bytes required, got %zu", what, need, workspace_bytes);
     if (!aligned(workspace, 8) || !aligned(stats, 8))
       return fail(SIHC_ERR_INVALID, "%s: misaligned workspace or stats", what);
-    const Plan p = plan(batch, pixels, channels, groups, 0.f, act == SIHC_ACT_SILU, elem_size(dtype), true);
-    const int64_t blocks = p.whole ? batch * (groups / p.s.slice_groups) : batch * p.s.chunks * p.s.widths;
-    if (blocks > 0x7fffffff || batch * short_chunks(p.s).chunks * p.s.widths > 0x7fffffff)
-      return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
+    const Plan all = plan(batch, pixels, channels, groups, 0.f, act == SIHC_ACT_SILU, elem_size(dtype), true);
     parts = batch;
-    const dim3 grid(static_cast<unsigned>(blocks)), threads(static_cast<unsigned>(p.s.threads));
-    const int rc = by_plan<true>(
-        p, dtype, w_dtype,
-        [&](auto t, auto tw, auto v, auto nv, auto tb) {
-          using T = decltype(t);
-          using TW = decltype(tw);
-          constexpr int V = decltype(v)::value, NV = decltype(nv)::value, TB = decltype(tb)::value;
-          const unsigned lds = 2u * unsigned(p.s.rows + 1) * unsigned(p.s.W) * 4u;
-          hipLaunchKernelGGL((k_group_norm_grad<T, TW, V, NV, TB>), grid, threads, lds, st, static_cast<const T*>(grad),
-                             static_cast<const T*>(x), static_cast<const TW*>(weight), static_cast<const TW*>(bias),
-                             reinterpret_cast<const float2*>(stats), static_cast<T*>(grad_x),
-                             static_cast<float*>(workspace), p.s);
-          return check_launch(what);
-        },
-        [&](auto t, auto tw, auto v) {
-          using T = decltype(t);
-          using TW = decltype(tw);
-          constexpr int V = decltype(v)::value;
-          float *total = static_cast<float*>(workspace), *part = total + batch * 2 * channels;
-          float2* means = reinterpret_cast<float2*>(part + batch * p.s.chunks * 2 * channels);
-          const unsigned lds = 2u * unsigned(p.s.rows) * unsigned(p.s.W) * 4u;
-          auto pass = [&](auto dx) {
-            constexpr bool DX = decltype(dx)::value;
-            const Shape s = DX ? short_chunks(p.s) : p.s;
-            hipLaunchKernelGGL((k_norm_grad_rows<T, TW, V, DX>), dim3(unsigned(batch * s.chunks * s.widths)), threads,
-                               DX ? 0 : lds, st,
-                               static_cast<const T*>(grad), static_cast<const T*>(x), static_cast<const TW*>(weight),
-                               static_cast<const TW*>(bias), reinterpret_cast<const float2*>(stats), means,
-                               static_cast<T*>(grad_x), part, s);
-          };
-          pass(std::false_type{});
-          hipLaunchKernelGGL(k_norm_grad_means<TW>, dim3(unsigned(batch)), dim3(1024), 0, st, part,
-                             static_cast<const TW*>(weight), total, means, p.s);
-          pass(std::true_type{});
-          return check_launch(what);
-        });
+    const void *const whole_grad = grad, *const whole_x = x;
+    void* const whole_grad_x = grad_x;
+    const int rc = by_images(what, all, [&](int64_t first, int64_t images) {
+      Plan p = all;
+      p.s.batch = images;
+      const int64_t element = first * pixels * channels;
+      const void *grad = advanced(whole_grad, element, elem_size(dtype)), *x = advanced(whole_x, element, elem_size(dtype));
+      void* grad_x = advanced(whole_grad_x, element, elem_size(dtype));
+      const float2* st2 = reinterpret_cast<const float2*>(stats) + first * groups;
+      float* total = static_cast<float*>(workspace) + first * 2 * channels;  // every image's; the rest is used again
+      const int64_t blocks = images * (p.whole ? groups / p.s.slice_groups : p.s.chunks * p.s.widths);
+      const dim3 grid(static_cast<unsigned>(blocks)), threads(static_cast<unsigned>(p.s.threads));
+      return by_plan<true>(
+          p, dtype, w_dtype,
+          [&](auto t, auto tw, auto v, auto nv, auto tb) {
+            using T = decltype(t);
+            using TW = decltype(tw);
+            constexpr int V = decltype(v)::value, NV = decltype(nv)::value, TB = decltype(tb)::value;
+            const unsigned lds = 2u * unsigned(p.s.rows + 1) * unsigned(p.s.W) * 4u;
+            hipLaunchKernelGGL((k_group_norm_grad<T, TW, V, NV, TB>), grid, threads, lds, st, static_cast<const T*>(grad),
+                               static_cast<const T*>(x), static_cast<const TW*>(weight), static_cast<const TW*>(bias),
+                               st2, static_cast<T*>(grad_x), total, p.s);
+            return check_launch(what);
+          },
+          [&](auto t, auto tw, auto v) {
+            using T = decltype(t);
+            using TW = decltype(tw);
+            constexpr int V = decltype(v)::value;
+            float* part = static_cast<float*>(workspace) + batch * 2 * channels;
+            float2* means = reinterpret_cast<float2*>(part + images * p.s.chunks * 2 * channels);
+            const unsigned lds = 2u * unsigned(p.s.rows) * unsigned(p.s.W) * 4u;
+            auto pass = [&](auto dx) {
+              constexpr bool DX = decltype(dx)::value;
+              const Shape s = DX ? short_chunks(p.s) : p.s;
+              hipLaunchKernelGGL((k_norm_grad_rows<T, TW, V, DX>), dim3(unsigned(images * s.chunks * s.widths)), threads,
+                                 DX ? 0 : lds, st, static_cast<const T*>(grad), static_cast<const T*>(x),
+                                 static_cast<const TW*>(weight), static_cast<const TW*>(bias), st2, means,
+                                 static_cast<T*>(grad_x), part, s);
+            };
+            pass(std::false_type{});
+            hipLaunchKernelGGL(k_norm_grad_means<TW>, dim3(unsigned(images)), dim3(1024), 0, st, part,
+                               static_cast<const TW*>(weight), total, means, p.s);
+            pass(std::true_type{});
+            return check_launch(what);
+          });
+    });
     if (rc) return rc;
   }
   auto sums = [&](auto tw) {
