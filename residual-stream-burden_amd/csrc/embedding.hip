@@ -74,11 +74,12 @@ __global__ __launch_bounds__(256) void k_embed(const T* __restrict__ table, cons
 template <typename T, typename I, int V>
 __global__ __launch_bounds__(256) void k_embed_grad_few(const T* __restrict__ grad, const I* __restrict__ ids,
                                                         T* __restrict__ out, int tokens, uint32_t rows, int C, int vecs,
-                                                        float scale, int64_t padding, int per_block) {
+                                                        float scale, int64_t padding, int per_block,
+                                                        uint32_t first_row) {
   __shared__ uint32_t list[FEW_TOKENS];  // token << 3 | row of the block
   __shared__ int wave_total[4];
   const int tid = int(threadIdx.x);
-  const uint32_t r0 = blockIdx.x * uint32_t(per_block);
+  const uint32_t r0 = first_row + blockIdx.x * uint32_t(per_block);
   const int per = (tokens + 255) / 256, begin = min(tokens, tid * per), end = min(tokens, begin + per);
   uint32_t found[FEW_TOKENS / 256];
   int count = 0;
@@ -511,7 +512,7 @@ int sihc_embedding(const void* table, const void* ids, void* out, int64_t tokens
           auto launch = [&](auto unroll) {
             constexpr int U = decltype(unroll)::value;
             const int64_t blocks = ceil_div(items, 256 * U);
-            if (blocks > 0x7fffffff) return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
+            if (blocks > MOST_LAUNCHED / 256) return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
             hipLaunchKernelGGL((k_embed<T, I, V, U>), dim3(unsigned(blocks)), dim3(256), 0,
                                static_cast<hipStream_t>(stream), static_cast<const T*>(table),
                                static_cast<const I*>(ids), static_cast<T*>(out), items, uint32_t(rows), channels, vecs,
@@ -560,9 +561,16 @@ int sihc_embedding_backward(const void* grad, const void* ids, void* grad_table,
             // about two vectors a thread: more rows would follow one another (64 fp32 tokens of 1152 channels:
             // one row 5.0 us, 8 rows 7.7)
             const int per_block = std::max(1, std::min(FEW_ROWS, 512 / vecs));
-            hipLaunchKernelGGL((k_embed_grad_few<T, I, V>), dim3(unsigned(ceil_div(rows, per_block))), dim3(256), 0, st, g,
-                               id, out, int(tokens), uint32_t(rows), channels, vecs, scale, padding, per_block);
-            return check_launch(what);
+            // (134 million narrow rows are more blocks than one launch takes)
+            const int64_t step = MOST_LAUNCHED / 256 * per_block;
+            int rc = SIHC_OK;
+            for (int64_t r = 0; r < rows && !rc; r += step) {
+              hipLaunchKernelGGL((k_embed_grad_few<T, I, V>), dim3(unsigned(ceil_div(std::min(step, rows - r), per_block))),
+                                 dim3(256), 0, st, g, id, out, int(tokens), uint32_t(rows), channels, vecs, scale, padding,
+                                 per_block, uint32_t(r));
+              rc = check_launch(what);
+            }
+            return rc;
           }
           const SortPlan p = sort_plan(tokens, rows, channels);
           char* w = static_cast<char*>(workspace);
@@ -592,7 +600,7 @@ int sihc_embedding_backward(const void* grad, const void* ids, void* grad_table,
           const u32x2* sorted = pairs[(p.passes - 1) & 1];
           const int slices = int(ceil_div(vecs, 64));
           const int64_t blocks = ceil_div(p.chunks * slices, 4);
-          if (blocks > 0x7fffffff) return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
+          if (blocks > MOST_LAUNCHED / 256) return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
           auto sum = [&](auto chunk) {
             hipLaunchKernelGGL((k_embed_grad<T, V, decltype(chunk)::value>), dim3(unsigned(blocks)), dim3(256), 0, st, g,
                                sorted, out, partial, crossing, tokens, p.chunks, uint32_t(rows), channels, slices, scale);

@@ -1,11 +1,12 @@
-"""GPU: sizes that take more threads than one launch has (2^32 in a dimension)."""
+"""GPU: sizes that take more threads than one launch has (2^32 in a dimension): millions of images of a few
+pixels, and of table rows of one channel."""
 from __future__ import annotations
 
 import pytest
 import torch
 
 from helpers import announce, rel_l2
-from sihc_hip import group_norm_act
+from sihc_hip import embedding_lookup, group_norm_act
 
 pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
@@ -60,3 +61,14 @@ def test_group_norm_of_more_chunks_than_a_launch_takes():
     dx0, dw0, db0 = torch.autograd.grad(want, (few, w, b), few.detach())
     assert torch.equal(dx[some], dx0) and not dx[1:100].any()
     assert rel_l2(dw, dw0) <= 1e-5 and rel_l2(db, db0) <= 1e-5
+
+
+def test_embedding_gradient_of_more_rows_than_a_launch_takes():
+    rows = 2**27 + 11
+    announce(f"embedding of {rows} rows of one channel")
+    table = torch.zeros(rows, 1, dtype=BF16, device="cuda").requires_grad_()
+    ids = torch.tensor([0, 5, rows - 1, rows - 1, 2**27 - 8, 2**27 - 1, 2**27, rows - 2], device="cuda")
+    grad = torch.tensor([[1.0], [2], [3], [4], [5], [6], [7], [8]], dtype=BF16, device="cuda")
+    (dt,) = torch.autograd.grad(embedding_lookup(table, ids, 2.0), table, grad)
+    want = {0: 2.0, 5: 4.0, rows - 1: 14.0, 2**27 - 8: 10.0, 2**27 - 1: 12.0, 2**27: 14.0, rows - 2: 16.0}
+    assert {int(i): float(dt[i, 0]) for i in dt.flatten().nonzero().flatten()} == want
