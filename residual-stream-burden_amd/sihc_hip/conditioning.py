@@ -12,7 +12,8 @@ table, norms and self attention are plain PyTorch, sihc/models/sihc/components.p
   and nothing that k and v hold past a length has an effect, NaN included.
 * ``group_norm_act(x, weight, bias, groups, eps, act)``: over a channels-last tensor [B, ..., C],
   act(weight * (x - mean) * rstd + bias) with the mean and variance of each image's groups of
-  C / groups adjacent channels.
+  C / groups adjacent channels: at most 4,096 of them in bfloat16 where 8 divides the width, otherwise
+  2,048 of an even width and 1,024 of an odd one.
 
 All sums and statistics are fp32, in a fixed order without atomics on values: identical inputs
 give identical bits. float32 and bfloat16; the norm's weights may be float32 beside a bfloat16
@@ -111,6 +112,18 @@ def embedding_lookup(table: Tensor, ids: Tensor, scale: float = 1.0, padding_idx
 
 
 # ------------------------------------------------------------------------ group norm and act
+def _widest_group(width: int, dtype: torch.dtype) -> int:
+    """The most channels of a group of such a width: a block takes a pixel's part of one in vectors."""
+    return 4096 if dtype == torch.bfloat16 and width % 8 == 0 else 2048 if width % 2 == 0 else 1024
+
+
+def _check_group_width(x: Tensor, groups: int) -> None:
+    width = x.shape[-1] // max(groups, 1)
+    if width > _widest_group(width, x.dtype):
+        raise ValueError(f"group_norm_act: groups of {width} channels, at most {_widest_group(width, x.dtype)} of "
+                         f"that width and type")
+
+
 def _check_norm(x: Tensor, weight: Tensor, bias: Tensor, groups: int, act: str) -> None:
     _require_packed("group_norm_act", x=x, weight=weight, bias=bias)
     if x.ndim < 2:
@@ -118,6 +131,7 @@ def _check_norm(x: Tensor, weight: Tensor, bias: Tensor, groups: int, act: str) 
     channels = x.shape[-1]
     if groups < 1 or channels < 1 or channels % groups:
         raise ValueError(f"group_norm_act: {channels} channels cannot be cut into {groups} groups")
+    _check_group_width(x, groups)
     if weight.shape != (channels,) or bias.shape != (channels,):
         raise ValueError("group_norm_act: weight and bias must be [channels]")
     if x.dtype not in _TYPES or weight.dtype != bias.dtype or weight.dtype not in (x.dtype, torch.float32):
@@ -136,6 +150,7 @@ def _group_norm_act(x: Tensor, weight: Tensor, bias: Tensor, groups: int, eps: f
 
 @_group_norm_act.register_fake
 def _group_norm_act_fake(x, weight, bias, groups, eps, act):
+    _check_group_width(x, groups)
     return torch.empty_like(x), x.new_empty((x.shape[0], groups, 2), dtype=torch.float32)
 
 

@@ -1,0 +1,41 @@
+"""CPU: what the conditioning operators refuse by size, in the C entries and in the Python ones alike."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from sihc_hip import _lib, conditioning
+
+FAKE = 0x1000  # never dereferenced
+
+
+def refused(rc, text):
+    assert rc == 1 and text in _lib.lib().sihc_last_error()
+
+
+# channels of one group: the widest, and the next of the same divisors
+@pytest.mark.parametrize("dtype,code,most,more", [(torch.bfloat16, 1, 4096, 4104), (torch.bfloat16, 1, 2044, 2052),
+                                                  (torch.bfloat16, 1, 2046, 2050), (torch.bfloat16, 1, 1023, 1025),
+                                                  (torch.float32, 0, 2048, 2052), (torch.float32, 0, 2046, 2050),
+                                                  (torch.float32, 0, 1023, 1025), (torch.float32, 0, 1023, 4097)])
+@pytest.mark.parametrize("groups", [1, 3])
+def test_the_widest_groups(dtype, code, most, more, groups):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    L = _lib.lib()
+    assert conditioning._widest_group(most, dtype) >= most and conditioning._widest_group(more, dtype) < more
+    for width, taken in ((most, True), (more, False)):
+        need = L.sihc_group_norm_backward_workspace_size(2, 4, groups * width, groups, code)
+        assert (need > 0) == taken
+        with FakeTensorMode():
+            x, w = torch.empty(2, 4, groups * width, dtype=dtype, device="cuda"), torch.empty(groups * width, device="cuda")
+            if taken:
+                assert conditioning.group_norm_act(x, w, w, groups).shape == x.shape
+            else:
+                with pytest.raises(ValueError, match=f"groups of {width} channels"):
+                    conditioning.group_norm_act(x, w, w, groups)
+        if not taken:
+            refused(L.sihc_group_norm(FAKE, FAKE, FAKE, FAKE, None, 2, 4, groups * width, groups, 1e-6, 1, code, code, None,
+                                      0, None), b"too wide")
+            with pytest.raises(ValueError, match=f"groups of {width} channels"):  # (CPU tensors: sizes are looked at first)
+                conditioning._check_norm(torch.zeros(2, 1, groups * width, dtype=dtype), torch.zeros(groups * width),
+                                         torch.zeros(groups * width), groups, "silu")
