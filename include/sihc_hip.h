@@ -337,7 +337,7 @@ size_t sihc_group_norm_workspace_size(int64_t batch, int64_t pixels, int channel
  * and channels, y = act(weight * (x - m) * r + bias). weight and bias are [channels] in w_dtype
  * (fp32 or dtype). stats, if given, receives [batch, groups] pairs (m, r) for the backward.
  * The workspace may be NULL where its size is 0. A group has at most 4096 channels in bf16 where 8
- * divides its width, otherwise 2048 of an even width and 1024 of an odd one. */
+ * divides its width, otherwise 2048 of an even width and 1024 of an odd one; all groups 2^24. */
 int sihc_group_norm(const void *x, const void *weight, const void *bias, void *y, float *stats,
                     int64_t batch, int64_t pixels, int channels, int groups, float eps, int act,
                     int dtype, int w_dtype, void *workspace, size_t workspace_bytes, void *stream);

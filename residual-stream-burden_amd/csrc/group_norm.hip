@@ -737,7 +737,8 @@ Plan plan(int64_t batch, int64_t pixels, int C, int groups, float eps, bool silu
 }
 
 int check_sizes(const char* what, int64_t batch, int64_t pixels, int C, int groups, int act, int dtype, int w_dtype) {
-  if (batch < 0 || pixels < 0 || C <= 0 || (pixels && batch > SIHC_MAX_TOKENS / pixels))
+  // (channels are counted in int32, two sums of each)
+  if (batch < 0 || pixels < 0 || C <= 0 || C > (1 << 24) || (pixels && batch > SIHC_MAX_TOKENS / pixels))
     return fail(SIHC_ERR_INVALID, "%s: bad sizes", what);
   if (groups <= 0 || C % groups) return fail(SIHC_ERR_INVALID, "%s: %d channels are not %d groups", what, C, groups);
   const int V = vec_of(C / groups, dtype == SIHC_DTYPE_F32 ? 4 : 2);

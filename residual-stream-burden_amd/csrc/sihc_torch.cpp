@@ -176,7 +176,7 @@ bool embed_fits(const Tensor& table, const Tensor& ids) {
 bool norm_fits(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t groups) {
   if (!plain(x) || !plain(weight) || !plain(bias) || x.dim() < 2 || x.numel() == 0 || dtype_code(x) < 0) return false;
   const int64_t c = x.size(-1);
-  if (groups < 1 || c % groups || c >= (int64_t(1) << 31)) return false;
+  if (groups < 1 || c % groups || c > (int64_t(1) << 24)) return false;
   const int64_t width = c / groups;  // (wider groups: the registered op says what is taken)
   if (width > (x.scalar_type() == at::kBFloat16 && width % 8 == 0 ? 4096 : width % 2 == 0 ? 2048 : 1024)) return false;
   for (const Tensor* w : {&weight, &bias})

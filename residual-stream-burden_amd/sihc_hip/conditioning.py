@@ -13,7 +13,7 @@ table, norms and self attention are plain PyTorch, sihc/models/sihc/components.p
 * ``group_norm_act(x, weight, bias, groups, eps, act)``: over a channels-last tensor [B, ..., C],
   act(weight * (x - mean) * rstd + bias) with the mean and variance of each image's groups of
   C / groups adjacent channels: at most 4,096 of them in bfloat16 where 8 divides the width, otherwise
-  2,048 of an even width and 1,024 of an odd one.
+  2,048 of an even width and 1,024 of an odd one, and C at most 2^24.
 
 All sums and statistics are fp32, in a fixed order without atomics on values: identical inputs
 give identical bits. float32 and bfloat16; the norm's weights may be float32 beside a bfloat16
@@ -118,6 +118,8 @@ def _widest_group(width: int, dtype: torch.dtype) -> int:
 
 
 def _check_group_width(x: Tensor, groups: int) -> None:
+    if x.shape[-1] > 1 << 24:
+        raise ValueError(f"group_norm_act: at most {1 << 24} channels, got {x.shape[-1]}")
     width = x.shape[-1] // max(groups, 1)
     if width > _widest_group(width, x.dtype):
         raise ValueError(f"group_norm_act: groups of {width} channels, at most {_widest_group(width, x.dtype)} of "

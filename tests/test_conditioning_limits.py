@@ -39,3 +39,18 @@ def test_the_widest_groups(dtype, code, most, more, groups):
             with pytest.raises(ValueError, match=f"groups of {width} channels"):  # (CPU tensors: sizes are looked at first)
                 conditioning._check_norm(torch.zeros(2, 1, groups * width, dtype=dtype), torch.zeros(groups * width),
                                          torch.zeros(groups * width), groups, "silu")
+
+
+def test_the_most_channels_of_a_norm():
+    """A width whose two sums a channel pass int32 was taken."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    L = _lib.lib()
+    most = 1 << 24
+    assert L.sihc_group_norm_backward_workspace_size(1, 1, most, most // 8, 1) == 2 * most * 4 + 2 * most * 4 + most // 8 * 8
+    for channels in (2 * most, 1 << 30):
+        refused(L.sihc_group_norm(FAKE, FAKE, FAKE, FAKE, None, 1, 1, channels, channels // 8, 1e-6, 1, 1, 1, FAKE, 1 << 40,
+                                  None), b"bad sizes")
+        with FakeTensorMode():
+            x, w = torch.empty(1, channels, dtype=torch.bfloat16, device="cuda"), torch.empty(channels, device="cuda")
+            with pytest.raises(ValueError, match="at most 16777216 channels"):
+                conditioning.group_norm_act(x, w, w, channels // 8)
