@@ -806,7 +806,7 @@ int check_args(const char* what, const sihc_attention* a) {
   // row lists and tiles are counted in int32; stats and packed offsets in int64
   const int64_t rows = int64_t(a->queries) * (a->heads / a->kv_heads);
   if (rows >= SIHC_MAX_TOKENS || a->keys >= SIHC_MAX_TOKENS ||
-      (a->batch && (rows / 32 + a->keys / 32 + 2) > (0x7fffffff >> 8) / (a->batch * a->kv_heads)))
+      a->batch > (0x7fffffff >> 8) / (rows / 32 + a->keys / 32 + 2) / a->kv_heads)
     return fail(SIHC_ERR_INVALID, "%s: tensor too large", what);
   return SIHC_OK;
 }

@@ -1,6 +1,9 @@
 """CPU: what the conditioning operators refuse by size, in the C entries and in the Python ones alike."""
 from __future__ import annotations
 
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -54,3 +57,29 @@ def test_the_most_channels_of_a_norm():
             x, w = torch.empty(1, channels, dtype=torch.bfloat16, device="cuda"), torch.empty(channels, device="cuda")
             with pytest.raises(ValueError, match="at most 16777216 channels"):
                 conditioning.group_norm_act(x, w, w, channels // 8)
+
+
+# The library's answers to sizes that no tensor has, asked in a process of their own: such a call has ended
+# in an arithmetic fault and in a loop without end.
+ASK = """
+import ctypes, sys
+sys.path.insert(0, sys.argv[1])
+from sihc_hip import _lib
+three = (ctypes.c_int64 * 3)(1, 1, 1)
+L, a = _lib.lib(), lambda batch, kv: ctypes.byref(_lib.Attention(batch, 4, 6, 2 * kv, kv, 16, three, three, three, 1.0, 1))
+print({})
+"""
+
+
+def answer(call):
+    done = subprocess.run([sys.executable, "-c", ASK.format(call), str(_lib.LIB_PATH.parents[1])], capture_output=True,
+                          text=True, timeout=60)
+    assert done.returncode == 0, (done.returncode, done.stderr)
+    return done.stdout.split()
+
+
+def test_batches_past_64_bits_of_attention_blocks():
+    for batch, heads in ((1 << 62, 4), (1 << 61, 8), ((1 << 63) - 1, 2)):
+        assert answer(f"L.sihc_cross_attention_workspace_size(a({batch}, {heads})), "
+                      f"L.sihc_cross_attention_backward_workspace_size(a({batch}, {heads})), b'too large' in L.sihc_last_error()"
+                      ) == ["0", "0", "True"]
