@@ -530,7 +530,7 @@ int sihc_embedding(const void* table, const void* ids, void* out, int64_t tokens
 }
 
 size_t sihc_embedding_backward_workspace_size(int64_t tokens, int64_t rows, int channels) {
-  if (tokens <= FEW_TOKENS || rows <= 0 || channels <= 0) return 0;
+  if (check_sizes("sihc_embedding_backward", tokens, rows, channels, 32, SIHC_DTYPE_F32) || tokens <= FEW_TOKENS) return 0;
   return sort_plan(tokens, rows, channels).total();
 }
 

@@ -83,3 +83,10 @@ def test_batches_past_64_bits_of_attention_blocks():
         assert answer(f"L.sihc_cross_attention_workspace_size(a({batch}, {heads})), "
                       f"L.sihc_cross_attention_backward_workspace_size(a({batch}, {heads})), b'too large' in L.sihc_last_error()"
                       ) == ["0", "0", "True"]
+
+
+def test_workspaces_of_tables_that_no_memory_holds():
+    calls = [f"L.sihc_embedding_backward_workspace_size({tokens}, {rows}, {channels})"
+             for tokens, rows, channels in ((4096, (1 << 62) + 1, 64), (4096, (1 << 63) - 1, 64), (1 << 62, 100, 64),
+                                            (4096, 100, 1 << 30), (-1, 100, 64), (4096, 0, 64))]
+    assert answer(", ".join(calls)) == ["0"] * len(calls)
