@@ -663,22 +663,24 @@ variable_list run_norm(const Tensor& x, const Tensor& weight, const Tensor& bias
         true);
   return {y, stats};
 }
+// What a backward needs beside the result leaves by a pointer: an output marked as not differentiable ends
+// compiled autograd, which takes no such node.
 struct NormFn : torch::autograd::Function<NormFn> {
   static constexpr bool is_traceable = true;
-  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& bias,
-                               int64_t groups, double eps, const std::string& act) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& bias,
+                        int64_t groups, double eps, const std::string& act, Tensor* stats) {
     variable_list out = run_norm(x, weight, bias, groups, eps, act);
-    ctx->mark_non_differentiable({out[1]});
-    ctx->set_materialize_grads(false);  // (zeros for the statistics' gradient would be a launch)
+    ctx->set_materialize_grads(false);
     ctx->save_for_backward({x, weight, bias, out[1]});
     ctx->saved_data["groups"] = groups;
     ctx->saved_data["act"] = act;
-    return out;
+    *stats = out[1];
+    return out[0];
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &stats = saved[3];
-    if (!grads[0].defined()) return variable_list(6);
+    if (!grads[0].defined()) return variable_list(7);
     const Tensor grad = grads[0].contiguous();
     const int64_t groups = ctx->saved_data["groups"].toInt();
     const std::string act = ctx->saved_data["act"].toStringRef();
@@ -704,7 +706,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
           "sihc::group_norm_act_backward");
       std::tie(dx, dw, db) = op.call(grad, x, weight, bias, stats, groups, act);
     }
-    return {dx, dw, db, Tensor(), Tensor(), Tensor()};
+    return {dx, dw, db, Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -745,15 +747,16 @@ variable_list run_attention(const Tensor& q, const Tensor& k, const Tensor& v, c
 }
 struct AttentionFn : torch::autograd::Function<AttentionFn> {
   static constexpr bool is_traceable = true;
-  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
-                               const std::optional<Tensor>& lengths, double scale, bool train) {
+  // rest: the statistics, what the result lost in rounding (NormFn's pointer)
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                        const std::optional<Tensor>& lengths, double scale, variable_list* rest) {
     const Tensor n = lengths.value_or(Tensor());
-    variable_list out = run_attention(q, k, v, n, scale, train);
-    ctx->mark_non_differentiable({out[1], out[2]});
+    variable_list out = run_attention(q, k, v, n, scale, true);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({q, k, v, n, out[0], out[1], out[2]});
     ctx->saved_data["scale"] = scale;
-    return out;
+    *rest = {out[1], out[2]};
+    return out[0];
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
@@ -1011,8 +1014,10 @@ PyObject* py_norm(PyObject* self, PyObject* const* args, Py_ssize_t n) {
         !unwrap_integer(args[3], groups) || !unwrap_number(args[4], eps) || !norm_fits(x, weight, bias, groups))
       return not_implemented();
     return tuple_of(call(self, [&] { return Args{x, weight, bias, groups, eps, act}; }, [&] {
-      return unrecorded() ? run_norm(x, weight, bias, groups, eps, act)
-                          : NormFn::apply(x, weight, bias, groups, eps, act);
+      if (unrecorded()) return run_norm(x, weight, bias, groups, eps, act);
+      Tensor stats;
+      const Tensor out = NormFn::apply(x, weight, bias, groups, eps, act, &stats);
+      return variable_list{out, stats};
     }));
   });
 }
@@ -1027,8 +1032,10 @@ PyObject* py_attention(PyObject* self, PyObject* const* args, Py_ssize_t n) {
         !attention_fits(q, k, v, lengths))
       return not_implemented();
     return tuple_of(call(self, [&] { return Args{q, k, v, maybe(lengths), scale, train}; }, [&] {
-      return unrecorded() || !train ? run_attention(q, k, v, lengths, scale, train)
-                                    : AttentionFn::apply(q, k, v, maybe(lengths), scale, train);
+      if (unrecorded() || !train) return run_attention(q, k, v, lengths, scale, train);
+      variable_list rest;
+      const Tensor out = AttentionFn::apply(q, k, v, maybe(lengths), scale, &rest);
+      return variable_list{out, rest[0], rest[1]};
     }));
   });
 }
