@@ -16,12 +16,13 @@
 // heads fill tiles together, and their key gradients are one sum.
 //
 // What bounds it, at 4 images, 16 heads of 64 over 4 key heads, 4,096 rows over up to 2,048 keys (bf16): the
-// matrix and vector instructions between them. All three take 500-560 us, half the rate of a large matrix
-// product (the forward 157-172, the query gradient 190-204, the key and value gradients 290-316 when each
-// is traced), because a wave's exponentials and its products share one SIMD and its tiles leave it one to
-// two other waves to run beside. At 256 rows over 256 keys (64 images, 16 heads of 72) the blocks live for
-// a few pieces only, and their loads' latency bounds them: 60, 70 and 72 us, 194 together, 2.4 times the
-// time of the bytes. One row over 4,096 keys (8 images, 16 heads of 128 over 4): 17 us of 67 MB, and 4 us to join.
+// matrix and vector instructions between them. A training pass takes 570 us, half the rate of a large matrix
+// product, because a wave's exponentials and its products share one SIMD and its tiles leave it one to two
+// other waves to run beside. (Traced, where launches of this case are slower: the forward 172, the query
+// gradient 204, the key and value gradients 319, their parts' sum 8.) At 256 rows over 256 keys (64 images,
+// 16 heads of 72) the blocks live for a few pieces only, and their loads' latency bounds them: 198 us a
+// training pass, 2.4 times the time of the bytes (traced 64, 75 and 78). One row over 4,096 keys (8 images, 16
+// heads of 128 over 4): 17 us of 67 MB, and 4.5 us to join.
 //
 // Rounding: probabilities and score gradients enter their products in the inputs' type (a bf16 gradient is
 // then 1.4 times as far from the exact one as its own rounding puts it: two products' operands are rounded,
@@ -391,8 +392,11 @@ __device__ __forceinline__ float lost(float v) {
 template <typename T, int DP>
 __device__ __forceinline__ int wave_rows() { return int(threadIdx.x >> 6) * 32 * Lds<T, DP>::STRIDE; }
 
-// Blocks of several waves are compiled for two waves on a SIMD where their tiles fit 256 registers, three
-// where they fit 168: the softmax of one wave then runs beside the products of another.
+// Blocks of several waves are compiled for two waves on a SIMD where their tiles fit 256 registers, three where
+// they fit 168 or nearly: the softmax of one wave then runs beside the products of another. bf16 forwards over
+// heads of 64 and 80 channels spill 3 and 7 registers for the third wave (16 and 32 bytes a lane; fp32 ones of 96
+// 6, some query gradients 1), and all forwards keep 26 to 62 scalars in lanes of vector registers: both ways of
+// loading a piece live in one kernel.
 // -------------------------------------------------------------------------------- forward
 constexpr int forward_waves(int bytes, bool halves, int NW) {  // waves of a SIMD; bytes of a head's row
   return NW == 1 || bytes > 384 ? 1 : halves && bytes <= 160 ? 3 : 2;
@@ -438,7 +442,8 @@ __global__ __launch_bounds__(NW * 64, forward_waves(sizeof(T) * DP, sizeof(T) ==
     if (fast && k0 + PIECE < end) fetch(k0 + PIECE);
     // Scores under the base of earlier pieces need no maximum as long as their powers stay small: a base
     // is a scale, and sums keep their digits under any. The first piece, and one whose powers grow
-    // past 2^40, take their maximum as the new base, on scores computed again.
+    // past 2^40, take their maximum as the new base, on scores computed again. (So values may be as large as
+    // 2^128 / 2^40 over the pieces' number before a sum overflows whose quotient would not.)
     bool anew = __any(top == -INFINITY);
     for (;;) {
       asm volatile("" ::: "memory");  // (operands are read in every turn, not held across them)

@@ -6,7 +6,8 @@
 // Both are bound by memory: the lookup reads a row and writes a row per token, the gradient
 // reads the tokens' rows and writes the whole table's. (Of 32,768 tokens of 1152 bf16 channels over
 // 32,768 rows, half of them padding and the others' ids as frequent as their cube roots fall: lookup
-// 23 us, gradient 54 us, of which its sort takes 32 beside clearing the table.) Ids outside the table select its last
+// 23 us, gradient 60 us, of which its sort takes 34 beside clearing the table, and the sum 21 for twice the rows
+// that it needs: the padding tokens', which sort last, are read and dropped.) Ids outside the table select its last
 // row in both (the host wrappers reject them), so no access can leave it.
 //
 // The gradient takes no atomics on values. Few tokens: every block owns a few table rows, lists
@@ -25,7 +26,9 @@ using namespace sihc_cond;
 constexpr int OWN_SCAN = 64;
 // Up to so many tokens the rows' tokens are listed by scanning all ids (1152 bf16 channels, 1001 rows: 256 and
 // 1024 tokens 4.7 and 5.9 us, by the sort 19.5 and 21.5; 32,768 rows: 1024 tokens 24 and 36, 2048 more than
-// 40 and 36). A row that all tokens select is then summed by one block: 256 tokens 42 us, by the sort 25.
+// 40 and 36). A row that all tokens select is then summed by one block, whose threads add token after token: 256, 512
+// and 1024 tokens of one id 42, 82 and 160 us, by the sort 25, 26 and 31 (32,768 rows: 50, 94 and 183; 38, 40 and
+// 45). The line is drawn for spread ids; a prompt padded without a padding row is on the wrong side of it.
 constexpr int FEW_TOKENS = 1024;
 constexpr int FEW_ROWS = 8;  // table rows of a block there, at most
 

@@ -16,8 +16,12 @@
 //
 // Whole rows, twice: where a slice does not fit a block's registers, and where images are so large that
 // slices of a few groups read too short pieces of a pixel, the pixels pass in whole rows, once for the
-// moments and once for the result. 64 images of 64 x 64 x 1152: 341 us, 3.5 TB/s of the 1.2 GB in and
-// out (5.3 TB/s with the second reading); by slices 392.
+// moments and once for the result. 64 images of 64 x 64 x 1152: 343 us, 3.5 TB/s of the 1.2 GB in and
+// out (5.3 TB/s with the second reading); by slices 392. Their gradients 570 us, 3.2 TB/s of the 1.8 GB in and out
+// (5.3 TB/s with the second reading of x and dy).
+//
+// What this is not made for: images of one pixel ([rows, channels]). A block then holds one slice of a row, and the
+// weights' gradients are one chain of sums over the images: 262,144 rows of 1152 channels 5.8 ms and 13 ms.
 //
 // A mean is subtracted before squares are summed (over the block's own elements, or about a middle value of
 // a thread's own, then about the threads' and the chunks' means), so neither a large mean nor a value far from
@@ -269,7 +273,7 @@ __device__ __forceinline__ Stream stream_of(const Shape& s, int block) {
 }
 constexpr int AHEAD = 4;
 
-// One reading: 604 MB (64 images of 64 x 64 x 1152) in 135 us, 4.5 TB/s, the rest of the time the blocks' own sums.
+// One reading: 604 MB (64 images of 64 x 64 x 1152) in 136 us, 4.4 TB/s, the rest of the time the blocks' own sums.
 // part: [batch, chunks, groups] of (mean, squares about it) of the chunk's pixels. A thread sums about the median
 // of its channel's first three values, so that neither a mean nor a single value far from the others costs
 // digits; the block then takes the mean of the threads' means, and their squares about that.
@@ -658,7 +662,7 @@ __global__ __launch_bounds__(256) void k_channel_sums(const float* __restrict__ 
 // The register words a thread holds, at most.
 constexpr int WORDS = 80;
 // Images from so many bytes on pass in whole rows though their slices fit (64 images of 64 x 64 x 1152,
-// 9.4 MB each: 362 us, by slices 392; of 32 x 32 x 1152, 2.4 MB: 106 and 80, the gradients 168 and 154).
+// 9.4 MB each: 343 us, by slices 392; of 32 x 32 x 1152, 2.4 MB: 106 and 80, the gradients 168 and 154).
 constexpr int64_t STREAM_FROM = int64_t(4) << 20;
 struct Plan {
   Shape s;
