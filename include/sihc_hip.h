@@ -42,7 +42,7 @@ extern "C" {
 /* Tokens (batch*grid*grid) or workspace rows per call: fewer than 2^31 - 2^16, so a chunk's
  * end (chunks x tokens-per-chunk < tokens + chunks) and a thread's next token stay in int32. */
 #define SIHC_MAX_TOKENS (((int64_t)1 << 31) - ((int64_t)1 << 16))
-#define SIHC_ABI_VERSION 7
+#define SIHC_ABI_VERSION 8
 /* Bytes of the per-GPU scratch array of sihc_event_backward_noalloc (64 MiB). */
 #define SIHC_SCRATCH_BYTES (64u << 20)
 
@@ -387,6 +387,79 @@ int sihc_cross_attention_backward(const sihc_attention *a, const void *grad, con
                                   const void *out, const float *stats, const void *low,
                                   void *grad_q, void *grad_k, void *grad_v, void *workspace,
                                   size_t workspace_bytes, void *stream);
+
+/* ---- Operators of a block's body (since ABI 8). No reference counterpart: the reference's
+ * projections, head norms and rotation are plain PyTorch. ---- */
+
+enum { SIHC_ACT_SWIGLU = 2 }; /* sihc_linear_act alone */
+
+/* Sizes of a projection: x is [rows, inner] and the result [rows, outer], packed; weight is
+ * [outer, inner], with SIHC_ACT_SWIGLU [2 * outer, inner]. The gate is [rows / rows_per_gate,
+ * outer], its rows gate_stride elements apart; without one, rows_per_gate is any divisor of rows. */
+typedef struct {
+  int64_t rows;
+  int inner, outer, act, dtype;
+  int64_t rows_per_gate, gate_stride;
+} sihc_linear;
+
+size_t sihc_linear_act_workspace_size(const sihc_linear *l);
+/* h = x weight^T + bias; u = h, silu(h) or silu(h[:, :outer]) * h[:, outer:]; y = residual +
+ * gate * u, in fp32 sums, rounded once. bias, gate and residual may be NULL. h, if given,
+ * receives h in dtype for the backward. The workspace may be NULL where its size is 0. */
+int sihc_linear_act(const sihc_linear *l, const void *x, const void *weight, const void *bias,
+                    const void *gate, const void *residual, void *y, void *h, void *workspace,
+                    size_t workspace_bytes, void *stream);
+
+size_t sihc_linear_act_backward_workspace_size(const sihc_linear *l, int gated);
+/* Adjoint of sihc_linear_act (the residual's gradient is grad). h is needed where there is an
+ * activation or a gate. dx [rows, inner], dweight like weight, dbias [its rows] and dgate
+ * [rows / rows_per_gate, outer] are packed; each may be NULL if it is not wanted. Sums in fp32 in
+ * a fixed order, without atomics; the gradient of h is rounded to dtype as the products' operand. */
+int sihc_linear_act_backward(const sihc_linear *l, const void *grad, const void *x,
+                             const void *weight, const void *h, const void *gate, void *dx,
+                             void *dweight, void *dbias, void *dgate, void *workspace,
+                             size_t workspace_bytes, void *stream);
+
+#define SIHC_MAX_ROTARY_DIM 256
+#define SIHC_MAX_AXES 4
+enum { SIHC_POSITION_I32 = 0, SIHC_POSITION_F32 = 1 };
+/* Sizes of a norm of heads with rotation: q is [batch, tokens, heads, dim], k [batch, tokens,
+ * kv_heads, dim] (kv_heads 0: there is none), strides in elements between batch rows, tokens and
+ * heads, the channels of a head adjacent; dim is 1..SIHC_MAX_ROTARY_DIM. positions are [tokens,
+ * axes], position_batch_stride 0, or [batch, tokens, axes], position_batch_stride tokens (in
+ * positions). Axis i turns the pairs of the next widths[i] (even) channels of a head by position *
+ * theta^(-2 j / widths[i]), pair j; channels past the axes stay. inverse turns back. */
+typedef struct {
+  int64_t batch, tokens;
+  int heads, kv_heads, dim, axes;
+  int widths[SIHC_MAX_AXES];
+  int64_t q_stride[3], k_stride[3], position_batch_stride;
+  double theta;
+  float eps;
+  int dtype, w_dtype, position_dtype, inverse;
+} sihc_heads;
+
+/* y = R(position) (weight * x / sqrt(mean over the head of x^2 + eps)) of queries and keys in one
+ * pass; weights NULL: the rotation alone. Outputs are packed. */
+int sihc_qk_norm_rotary(const sihc_heads *h, const void *q, const void *k, const void *q_weight,
+                        const void *k_weight, const void *positions, void *q_out, void *k_out,
+                        void *stream);
+
+size_t sihc_qk_norm_rotary_backward_workspace_size(const sihc_heads *h);
+/* Adjoint of sihc_qk_norm_rotary with weights, from its inputs: grad_q, grad_k, dq and dk packed,
+ * the weights' gradients [dim] in w_dtype, summed in fp32 in a fixed order. (Without weights the
+ * adjoint is sihc_qk_norm_rotary itself with inverse set.) */
+int sihc_qk_norm_rotary_backward(const sihc_heads *h, const void *grad_q, const void *grad_k,
+                                 const void *q, const void *k, const void *q_weight,
+                                 const void *k_weight, const void *positions, void *dq, void *dk,
+                                 void *dq_weight, void *dk_weight, void *workspace,
+                                 size_t workspace_bytes, void *stream);
+
+/* y[i] = residual[i] + (word_i >= p 2^32 ? x[i] / (1 - p) : 0): word_i is part i % 4 of the Philox
+ * 4x32 block (10 rounds) of counter (i / 4, stream_id) under *key, which lies on the device. The
+ * residual may be NULL, y may be x or the residual. The adjoint is the same call on the gradient. */
+int sihc_dropout(const void *x, const void *residual, void *y, int64_t count, double p,
+                 const int64_t *key, int64_t stream_id, int dtype, void *stream);
 
 #ifdef __cplusplus
 }

@@ -20,7 +20,8 @@ from pathlib import Path
 PKG_ROOT = Path(__file__).resolve().parent
 REPO_ROOT = PKG_ROOT.parent
 SOURCES = [PKG_ROOT / "csrc" / name
-           for name in ("sihc_kernels.hip", "embedding.hip", "group_norm.hip", "cross_attention.hip")]
+           for name in ("sihc_kernels.hip", "embedding.hip", "group_norm.hip", "cross_attention.hip", "linear.hip",
+                        "head_norm.hip", "dropout.hip")]
 OUTPUT = PKG_ROOT / "sihc_hip" / "libsihc_hip.so"
 SELFTEST_SOURCE = PKG_ROOT / "csrc" / "abi_selftest.c"
 SELFTEST = PKG_ROOT / "sihc_hip" / "sihc_abi_selftest"

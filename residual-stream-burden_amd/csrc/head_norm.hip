@@ -1,0 +1,513 @@
+// Norms of query and key heads with the rotation by the token's positions, and their gradients.
+//
+//   hat = x r, r = 1 / sqrt(mean x^2 + eps);  n = w hat;  y = R n
+//   dn = R^T dy;  dw = sum dn hat;  dx = r (w dn - hat mean(w dn hat))
+//
+// R turns the pairs (2i, 2i + 1) of each axis' run of channels by position times
+// theta^(-2i / width); channels past the runs stay. Without weights there is no norm: y = R x.
+//
+// A wave owns a few tokens. Its lanes first take the sine and cosine of one pair each, once for
+// all heads, into the wave's own part of LDS. Then groups of LPH lanes take a head each, 8 channels
+// a lane, so that a head is read once and its statistics are a few moves between lanes.
+//
+// The angle is a product in 64 bits, in turns, whose whole turns are dropped before it is rounded to
+// fp32: a position of 2^31 still has its angle to 2^-24 of a turn.
+#include "cond_common.h"
+
+#include <cmath>
+
+namespace {
+using namespace sihc_cond;
+
+constexpr int V = 8;       // channels of a lane
+constexpr int UNROLL = 4;  // heads of a lane whose loads are in flight together
+constexpr int MAX_PAIRS = SIHC_MAX_ROTARY_DIM / 2;
+constexpr int MAX_GROUP = 8;  // tokens of a wave
+
+struct Args {
+  const void *x[2], *grad[2], *weight[2], *positions;
+  void* y[2];
+  float* part;         // [blocks][2][dim] sums of the weights' gradients
+  int64_t stride[2][3];
+  int64_t position_batch;  // positions between two sequences, 0 where all share them
+  int heads[2];
+  int dim, tokens, total, axes, turned, group;
+  bool float_positions, w_f32;
+  float eps, sign;
+  double rate[MAX_PAIRS];  // turns of a pair per position
+  uint8_t axis[MAX_PAIRS];
+};
+
+template <typename T>
+struct Chunk {  // a lane's 8 channels as they are in memory
+  static constexpr int N = V * int(sizeof(T)) / 16;
+  u32x4 raw[N];
+  __device__ __forceinline__ void get(const T* p, int left) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) raw[i] = u32x4{};
+    if (left >= V) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) raw[i] = load<T, V / N>(p + i * (V / N)).raw;
+    } else if (left > 0) {
+      T e[V] = {};
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i < left) e[i] = p[i];
+      __builtin_memcpy(raw, e, sizeof(e));
+    }
+  }
+  __device__ __forceinline__ void to(float* o) const {
+    T e[V];
+    __builtin_memcpy(e, raw, sizeof(e));
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = to_f32(e[i]);
+  }
+  __device__ __forceinline__ static void put(T* p, const float* v, int left) {
+    if (left >= V) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) store(p + i * (V / N), Vec<T, V / N>::of(v + i * (V / N)));
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i < left) p[i] = from_f32<T>(v[i]);
+    }
+  }
+};
+
+// Sum over the LPH lanes of a head, in each of them.
+template <int LPH>
+__device__ __forceinline__ float head_sum(float v) {
+  if constexpr (LPH >= 2) v += moved<0xb1>(v);
+  if constexpr (LPH >= 4) v += moved<0x4e>(v);
+  if constexpr (LPH >= 8) v += moved<0x141>(v);
+  if constexpr (LPH >= 16) v += moved<0x140>(v);
+  if constexpr (LPH >= 32) v += __shfl_xor(v, 16);
+  return v;
+}
+template <int LPH>
+__device__ __forceinline__ float head_max(float v) {
+#pragma unroll
+  for (int k = 1; k < LPH; k *= 2) v = fmaxf(v, __shfl_xor(v, k));
+  return v;
+}
+
+// 1 / sqrt(mean x^2 + eps) of a head. Where the squares leave the range of fp32, all lanes of the
+// wave take them again of values scaled by a power of two.
+template <int LPH>
+__device__ __forceinline__ float reciprocal_rms(const float* x, int dim, float eps) {
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) sum += x[i] * x[i];
+  sum = head_sum<LPH>(sum);
+  float r = rsqrtf(sum / float(dim) + eps);
+  const bool odd = !(sum < 0x1p125f) || (sum < 0x1p-90f && eps < 0x1p-90f);
+  if (__builtin_expect(__any(odd), 0)) {
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) most = fmaxf(most, fabsf(x[i]));
+    most = head_max<LPH>(most);
+    const float s = most >= 1.f ? 0x1p-66f : 0x1p80f;
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum += (x[i] * s) * (x[i] * s);
+    sum = head_sum<LPH>(sum);
+    if (odd) r = s * rsqrtf(sum / float(dim) + eps * s * s);
+  }
+  return r;
+}
+
+// The lane's pairs turned by their angles (sign -1: back).
+__device__ __forceinline__ void turn(float* v, const float2* angle, float sign) {
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) {
+    const float c = angle[i].x, s = angle[i].y * sign, a = v[2 * i], b = v[2 * i + 1];
+    v[2 * i] = a * c - b * s;
+    v[2 * i + 1] = a * s + b * c;
+  }
+}
+
+// Pair p of a token's angles: its cosine and sine, 1 and 0 where nothing turns.
+__device__ __forceinline__ float2 angle_of(const Args& a, int64_t at, double rate, int axis, bool turns) {
+  if (!turns) return make_float2(1.f, 0.f);
+  const double position = a.float_positions ? double(static_cast<const float*>(a.positions)[at + axis])
+                                            : double(static_cast<const int32_t*>(a.positions)[at + axis]);
+  const double turned = position * rate;
+  float s, c;
+  sincospif(float(2.0 * (turned - rint(turned))), &s, &c);
+  return make_float2(c, s);
+}
+
+// What a lane keeps over the tokens of its wave.
+struct Lane {
+  int first, left;      // its channels of a head: the first, how many there are from it on
+  int sub;              // its head among those of a pass
+  float2* angles;       // the wave's angles in LDS: [group][pairs]
+  int pairs;
+  double rate[2];
+  int axis[2];
+};
+template <int LPH>
+__device__ __forceinline__ Lane lane_of(const Args& a, float2* lds) {
+  Lane l;
+  const int lane = threadIdx.x & 63;
+  l.sub = lane / LPH;
+  l.first = (lane % LPH) * V;
+  l.left = a.dim - l.first;
+  l.pairs = LPH * V / 2;  // (whole chunks: those past dim have no turn)
+  l.angles = lds + (threadIdx.x >> 6) * a.group * l.pairs;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int p = min(lane + 64 * k, MAX_PAIRS - 1);
+    l.rate[k] = a.rate[p];
+    l.axis[k] = a.axis[p];
+  }
+  return l;
+}
+// Tokens first .. first + count - 1: their angles into LDS.
+__device__ __forceinline__ void take_angles(const Args& a, const Lane& l, int first, int count) {
+  const int lane = threadIdx.x & 63;
+  for (int t = 0; t < count; ++t) {
+    const int token = first + t, b = token / a.tokens, n = token - b * a.tokens;
+    const int64_t at = (int64_t(b) * a.position_batch + n) * a.axes;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int p = lane + 64 * k;
+      if (p < l.pairs) l.angles[t * l.pairs + p] = angle_of(a, at, l.rate[k], l.axis[k], p < a.turned);
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // a wave's own LDS traffic is in order
+}
+
+// Calls f(side's heads in turn): one pass a head of the group's tokens for each group of LPH lanes,
+// UNROLL passes at a time; load(u, token, head, valid), work(u, token of the group, token, head, valid).
+template <int LPH, bool ONE, typename Load, typename Work>
+__device__ __forceinline__ void each_head(const Args& a, const Lane& l, int side, int first, int count, Load load,
+                                          Work work) {
+  constexpr int SUB = 64 / LPH;
+  const int heads = a.heads[side], items = ONE ? heads : heads * count;
+  for (int base = 0; base < items; base += SUB * UNROLL) {
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int item = base + u * SUB + l.sub, t = ONE ? 0 : item / heads;
+      load(u, first + t, item - t * heads, item < items);
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      if (base + u * SUB >= items) break;
+      const int item = base + u * SUB + l.sub, t = ONE ? 0 : item / heads;
+      // (lanes without a head work on the last one, so that all take part in the sums)
+      work(u, ONE ? 0 : min(t, count - 1), first + t, item - t * heads, item < items);
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ const T* head_at(const Args& a, const void* x, int side, int token, int head) {
+  const int b = token / a.tokens, n = token - b * a.tokens;
+  return static_cast<const T*>(x) + int64_t(b) * a.stride[side][0] + int64_t(n) * a.stride[side][1] +
+         int64_t(head) * a.stride[side][2];
+}
+__device__ __forceinline__ int64_t packed_at(const Args& a, int side, int token, int head) {
+  return (int64_t(token) * a.heads[side] + head) * a.dim;
+}
+__device__ __forceinline__ void weights_of(const Args& a, int side, const Lane& l, bool f32, bool bf, float* w) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = l.first + i;
+    w[i] = c >= a.dim ? 0.f
+           : f32      ? static_cast<const float*>(a.weight[side])[c]
+                      : to_f32(static_cast<const bf16*>(a.weight[side])[c]);
+  }
+}
+
+template <typename T, int LPH, bool NORM, bool ONE>
+__global__ __launch_bounds__(256) void heads_kernel(const Args a) {
+  extern __shared__ float2 lds[];
+  const Lane l = lane_of<LPH>(a, lds);
+  const int waves = blockDim.x >> 6;
+  const int wave = xcd_block(blockIdx.x, gridDim.x) * waves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int first = wave * a.group;
+  if (first >= a.total) return;
+  const int count = min(a.group, a.total - first);
+  take_angles(a, l, first, count);
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    if (a.heads[side] == 0) continue;
+    float w[V];
+    if constexpr (NORM) weights_of(a, side, l, a.w_f32, !a.w_f32, w);
+    Chunk<T> in[UNROLL];
+    each_head<LPH, ONE>(
+        a, l, side, first, count,
+        [&](int u, int token, int head, bool valid) {
+          in[u].get(head_at<T>(a, a.x[side], side, token, head) + l.first, valid ? l.left : 0);
+        },
+        [&](int u, int t, int token, int head, bool valid) {
+          float v[V];
+          in[u].to(v);
+          if constexpr (NORM) {
+            const float r = reciprocal_rms<LPH>(v, a.dim, a.eps);
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] *= r * w[i];
+          }
+          turn(v, l.angles + t * l.pairs + l.first / 2, a.sign);
+          if (valid) Chunk<T>::put(static_cast<T*>(a.y[side]) + packed_at(a, side, token, head) + l.first, v, l.left);
+        });
+  }
+}
+
+template <typename T, int LPH, bool ONE>
+__global__ __launch_bounds__(256) void heads_backward_kernel(const Args a) {
+  extern __shared__ float2 lds[];
+  const Lane l = lane_of<LPH>(a, lds);
+  const int waves = blockDim.x >> 6, groups = (a.total + a.group - 1) / a.group;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  float dw[2][V] = {};
+  // every wave takes a run of groups of tokens
+  const int all = gridDim.x * waves, id = xcd_block(blockIdx.x, gridDim.x) * waves + wave;
+  const int64_t from = int64_t(groups) * id / all, to = int64_t(groups) * (id + 1) / all;
+  for (int group = int(from); group < int(to); ++group) {
+    const int first = group * a.group, count = min(a.group, a.total - first);
+    take_angles(a, l, first, count);
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      if (a.heads[side] == 0) continue;
+      float w[V];
+      weights_of(a, side, l, a.w_f32, !a.w_f32, w);
+      Chunk<T> in[UNROLL], grad[UNROLL];
+      each_head<LPH, ONE>(
+          a, l, side, first, count,
+          [&](int u, int token, int head, bool valid) {
+            const int left = valid ? l.left : 0;
+            in[u].get(head_at<T>(a, a.x[side], side, token, head) + l.first, left);
+            grad[u].get(static_cast<const T*>(a.grad[side]) + packed_at(a, side, token, head) + l.first, left);
+          },
+          [&](int u, int t, int token, int head, bool valid) {
+            float x[V], g[V];
+            in[u].to(x);
+            grad[u].to(g);
+            turn(g, l.angles + t * l.pairs + l.first / 2, -1.f);
+            const float r = reciprocal_rms<LPH>(x, a.dim, a.eps);
+            float dot = 0.f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              x[i] *= r;
+              if (valid) dw[side][i] += g[i] * x[i];
+              g[i] *= w[i];
+              dot += g[i] * x[i];
+            }
+            dot = head_sum<LPH>(dot) / float(a.dim);
+#pragma unroll
+            for (int i = 0; i < V; ++i) g[i] = r * (g[i] - x[i] * dot);
+            if (valid) Chunk<T>::put(static_cast<T*>(a.y[side]) + packed_at(a, side, token, head) + l.first, g, l.left);
+          });
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  // the block's sums: over a wave's heads by moves, over its waves in LDS
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(lds);  // [waves][2][LPH * V]
+#pragma unroll
+  for (int side = 0; side < 2; ++side)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float v = dw[side][i];
+#pragma unroll
+      for (int k = LPH; k < 64; k *= 2) v += __shfl_xor(v, k);
+      if (l.sub == 0) sums[(wave * 2 + side) * LPH * V + l.first + i] = v;
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * a.dim; i += blockDim.x) {
+    const int side = i / a.dim, c = i - side * a.dim;
+    float v = 0.f;
+    for (int k = 0; k < waves; ++k) v += sums[(k * 2 + side) * LPH * V + c];
+    a.part[int64_t(blockIdx.x) * 2 * a.dim + i] = v;
+  }
+}
+
+// The weights' gradients from the blocks' sums: 8 columns a block, 32 threads each.
+template <typename W>
+__global__ __launch_bounds__(256) void weights_kernel(const float* part, W* dq, W* dk, int dim, int parts) {
+  __shared__ float lds[32][9];
+  const int c = threadIdx.x & 7, row = threadIdx.x >> 3, column = blockIdx.x * 8 + c;
+  float v = 0.f;
+  if (column < 2 * dim)
+#pragma unroll 8
+    for (int i = row; i < parts; i += 32) v += part[int64_t(i) * 2 * dim + column];
+  lds[row][c] = v;
+  __syncthreads();
+  if (threadIdx.x >= 8 || column >= 2 * dim) return;
+  v = 0.f;
+  for (int i = 0; i < 32; ++i) v += lds[i][c];
+  W* to = column < dim ? dq : dk;
+  if (to) to[column < dim ? column : column - dim] = from_f32<W>(v);
+}
+
+// ---------------------------------------------------------------------------------- host
+constexpr int BACKWARD_BLOCKS = 1024;  // four of four waves on every CU
+
+int lanes_of(int dim) {
+  int lanes = 1;
+  while (lanes * V < dim) lanes *= 2;
+  return lanes;
+}
+int check(const sihc_heads* h, const void* k, const void* q_weight, const void* k_weight, const char* what) {
+  if (!h) return fail(SIHC_ERR_INVALID, "%s: null sizes", what);
+  if (!valid_dtype(h->dtype) || !valid_dtype(h->w_dtype)) return fail(SIHC_ERR_INVALID, "%s: bad dtype", what);
+  if (h->w_dtype != h->dtype && h->w_dtype != SIHC_DTYPE_F32)
+    return fail(SIHC_ERR_INVALID, "%s: weights of the heads' type or fp32", what);
+  if (h->position_dtype != SIHC_POSITION_I32 && h->position_dtype != SIHC_POSITION_F32)
+    return fail(SIHC_ERR_INVALID, "%s: positions are int32 or fp32", what);
+  if (h->batch < 0 || h->tokens < 0 || h->heads < 1 || h->kv_heads < 0)
+    return fail(SIHC_ERR_INVALID, "%s: bad sizes", what);
+  if (h->dim < 1 || h->dim > SIHC_MAX_ROTARY_DIM)
+    return fail(SIHC_ERR_INVALID, "%s: heads of 1..%d channels", what, SIHC_MAX_ROTARY_DIM);
+  if (h->heads > (1 << 20) || h->kv_heads > (1 << 20)) return fail(SIHC_ERR_INVALID, "%s: too many heads", what);
+  if (h->tokens > INT32_MAX - 64 || (h->tokens && h->batch > (INT32_MAX - 64) / h->tokens))
+    return fail(SIHC_ERR_INVALID, "%s: at most 2^31 - 64 tokens", what);
+  if (h->axes < 0 || h->axes > SIHC_MAX_AXES) return fail(SIHC_ERR_INVALID, "%s: 0..%d axes", what, SIHC_MAX_AXES);
+  int sum = 0;
+  for (int i = 0; i < h->axes; ++i) {
+    if (h->widths[i] < 0 || h->widths[i] > h->dim || h->widths[i] % 2)
+      return fail(SIHC_ERR_INVALID, "%s: axis %d turns %d channels of %d", what, i, h->widths[i], h->dim);
+    sum += h->widths[i];
+  }
+  if (sum > h->dim) return fail(SIHC_ERR_INVALID, "%s: the axes turn %d channels of %d", what, sum, h->dim);
+  if (!(h->theta > 0.0) || !std::isfinite(h->theta)) return fail(SIHC_ERR_INVALID, "%s: theta must be positive", what);
+  if (!(h->eps >= 0.f)) return fail(SIHC_ERR_INVALID, "%s: eps must not be negative", what);
+  if ((h->kv_heads != 0) != (k != nullptr)) return fail(SIHC_ERR_INVALID, "%s: keys go with kv_heads", what);
+  if (k ? (q_weight == nullptr) != (k_weight == nullptr) : k_weight != nullptr)
+    return fail(SIHC_ERR_INVALID, "%s: weights of both sides or of none", what);
+  return SIHC_OK;
+}
+Args args_of(const sihc_heads* h) {
+  Args a{};
+  const int64_t* strides[2] = {h->q_stride, h->k_stride};
+  for (int s = 0; s < 2; ++s)
+    for (int i = 0; i < 3; ++i) a.stride[s][i] = strides[s][i];
+  a.position_batch = h->position_batch_stride;
+  a.heads[0] = h->heads;
+  a.heads[1] = h->kv_heads;
+  a.dim = h->dim;
+  a.tokens = int(h->tokens);
+  a.total = int(h->batch * h->tokens);
+  a.axes = h->axes;
+  a.float_positions = h->position_dtype == SIHC_POSITION_F32;
+  a.w_f32 = h->w_dtype == SIHC_DTYPE_F32;
+  a.eps = h->eps;
+  a.sign = h->inverse ? -1.f : 1.f;
+  int pair = 0;
+  for (int i = 0; i < h->axes; ++i)
+    for (int c = 0; c < h->widths[i]; c += 2, ++pair) {
+      a.rate[pair] = std::pow(h->theta, -double(c) / double(h->widths[i])) / 6.283185307179586476925;
+      a.axis[pair] = uint8_t(i);
+    }
+  a.turned = pair;
+  // Tokens of a wave: one where a token's heads fill 4 passes, else as many as do.
+  const int sub = 64 / lanes_of(h->dim), heads = h->heads + h->kv_heads;
+  a.group = std::max(1, std::min(MAX_GROUP, 4 * sub / heads));
+  return a;
+}
+template <typename F>
+int by_lanes(int lanes, F&& f) {
+  switch (lanes) {
+    case 1: return f(IC<1>{});
+    case 2: return f(IC<2>{});
+    case 4: return f(IC<4>{});
+    case 8: return f(IC<8>{});
+    case 16: return f(IC<16>{});
+    default: return f(IC<32>{});
+  }
+}
+int64_t backward_blocks(const Args& a) {
+  return std::min<int64_t>(BACKWARD_BLOCKS, ceil_div(ceil_div(a.total, a.group), 4));
+}
+}  // namespace
+
+extern "C" int sihc_qk_norm_rotary(const sihc_heads* h, const void* q, const void* k, const void* q_weight,
+                                   const void* k_weight, const void* positions, void* q_out, void* k_out,
+                                   void* stream) {
+  if (const int rc = check(h, k, q_weight, k_weight, "qk_norm_rotary")) return rc;
+  Args a = args_of(h);
+  if (a.total == 0) return SIHC_OK;
+  if (!q || !q_out || (k && !k_out) || (a.turned && !positions))
+    return fail(SIHC_ERR_INVALID, "qk_norm_rotary: null pointer");
+  a.x[0] = q;
+  a.x[1] = k;
+  a.weight[0] = q_weight;
+  a.weight[1] = k_weight;
+  a.positions = positions;
+  a.y[0] = q_out;
+  a.y[1] = k_out;
+  const int64_t groups = ceil_div(a.total, a.group);
+  const int waves = groups >= 2048 ? 4 : 1;  // few tokens: a wave a block, over more CUs
+  return by_dtype(h->dtype, [&](auto t) {
+    using T = decltype(t);
+    return by_lanes(lanes_of(h->dim), [&](auto lanes) {
+      constexpr int LPH = decltype(lanes)::value;
+      const size_t lds = size_t(waves) * a.group * (LPH * V / 2) * sizeof(float2);
+      const dim3 grid{unsigned(ceil_div(groups, waves))}, block{unsigned(waves * 64)};
+      auto launch = [&](auto norm) {
+        constexpr bool NORM = decltype(norm)::value != 0;
+        if (a.group == 1)
+          heads_kernel<T, LPH, NORM, true><<<grid, block, lds, hipStream_t(stream)>>>(a);
+        else
+          heads_kernel<T, LPH, NORM, false><<<grid, block, lds, hipStream_t(stream)>>>(a);
+      };
+      q_weight ? launch(IC<1>{}) : launch(IC<0>{});
+      return check_launch("qk_norm_rotary");
+    });
+  });
+}
+
+extern "C" size_t sihc_qk_norm_rotary_backward_workspace_size(const sihc_heads* h) {
+  if (!h || check(h, h->kv_heads ? h : nullptr, nullptr, nullptr, "qk_norm_rotary_backward")) return 0;
+  const Args a = args_of(h);
+  return size_t(backward_blocks(a)) * 2 * size_t(a.dim) * sizeof(float);
+}
+
+extern "C" int sihc_qk_norm_rotary_backward(const sihc_heads* h, const void* grad_q, const void* grad_k,
+                                            const void* q, const void* k, const void* q_weight,
+                                            const void* k_weight, const void* positions, void* dq, void* dk,
+                                            void* dq_weight, void* dk_weight, void* workspace,
+                                            size_t workspace_bytes, void* stream) {
+  if (const int rc = check(h, k, q_weight, k_weight, "qk_norm_rotary_backward")) return rc;
+  Args a = args_of(h);
+  if (!q_weight || !dq_weight || (k && !dk_weight))
+    return fail(SIHC_ERR_INVALID, "qk_norm_rotary_backward: the weights and their gradients are needed");
+  if (a.total && (!q || !grad_q || !dq || (k && (!grad_k || !dk)) || (a.turned && !positions) || !workspace))
+    return fail(SIHC_ERR_INVALID, "qk_norm_rotary_backward: null pointer");
+  const int64_t blocks = backward_blocks(a);
+  if (workspace_bytes < size_t(blocks) * 2 * size_t(a.dim) * sizeof(float))
+    return fail(SIHC_ERR_INVALID, "qk_norm_rotary_backward: workspace of %zu bytes is too small", workspace_bytes);
+  a.x[0] = q;
+  a.x[1] = k;
+  a.grad[0] = grad_q;
+  a.grad[1] = grad_k;
+  a.weight[0] = q_weight;
+  a.weight[1] = k_weight;
+  a.positions = positions;
+  a.y[0] = dq;
+  a.y[1] = dk;
+  a.part = static_cast<float*>(workspace);
+  if (a.total) {
+    const int rc = by_dtype(h->dtype, [&](auto t) {
+      using T = decltype(t);
+      return by_lanes(lanes_of(h->dim), [&](auto lanes) {
+        constexpr int LPH = decltype(lanes)::value;
+        const size_t lds = 4 * std::max(size_t(a.group) * (LPH * V / 2) * sizeof(float2), size_t(2 * LPH * V) * 4);
+        const dim3 grid{unsigned(blocks)}, block{256};
+        if (a.group == 1)
+          heads_backward_kernel<T, LPH, true><<<grid, block, lds, hipStream_t(stream)>>>(a);
+        else
+          heads_backward_kernel<T, LPH, false><<<grid, block, lds, hipStream_t(stream)>>>(a);
+        return check_launch("qk_norm_rotary_backward");
+      });
+    });
+    if (rc) return rc;
+  }
+  return by_dtype(h->w_dtype, [&](auto w) {
+    using W = decltype(w);
+    weights_kernel<W><<<unsigned(ceil_div(2 * a.dim, 8)), 256, 0, hipStream_t(stream)>>>(
+        a.part, static_cast<W*>(dq_weight), static_cast<W*>(dk_weight), a.dim, a.total ? int(blocks) : 0);
+    return check_launch("qk_norm_rotary_backward (weights)");
+  });
+}

@@ -1,0 +1,728 @@
+// Projections with their epilogue, and their gradients.
+//
+//   h = x W^T + b;  u = h | silu(h) | silu(h_a) h_b (h = [h_a, h_b]);  y = residual + gate u
+//   du = gate dy;  dgate = sum over the image's rows of dy u;  dh = du act'(h);  db = sum over rows of dh
+//   dx = dh W;  dW = dh^T x
+//
+// Every product runs on the matrix cores in 32 x 32 tiles (bf16 32x32x16, fp32 32x32x2, fp32 sums).
+// A block owns a tile of the result; pieces of both operands, BK of the contraction at a time, pass
+// through two buffers in LDS: while one is worked on, the next piece is stored from registers to the
+// other one and the loads of the piece after it are under way, so that a piece costs one barrier and a
+// load has a whole piece's products to arrive. An operand whose contraction runs along its rows lies in
+// LDS as it is in memory, and is read by the transposing load. The result passes through LDS once more,
+// a wave's own 32 rows at a time, so that the epilogue has 8 adjacent channels of a row and reads and
+// writes whole vectors. With SwiGLU a block's columns alternate between 32 rows of W_a and their 32 of
+// W_b, so that both halves of a channel meet in one wave.
+#include "cond_common.h"
+
+namespace {
+using namespace sihc_cond;
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int V = 8;  // adjacent channels of a thread in every epilogue
+
+// ------------------------------------------------------------------------------- row vectors
+// n <= V channels of a row from p as fp32, zeros past them.
+template <typename T>
+__device__ __forceinline__ void get(const T* p, int left, float* o) {
+  if (left >= V) {
+    load_f32<T, V>(p, o);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = i < left ? to_f32(p[i]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void put(T* p, int left, const float* v) {
+  constexpr int PIECE = 16 / int(sizeof(T));
+  if (left >= V) {
+#pragma unroll
+    for (int i = 0; i < V; i += PIECE) store(p + i, Vec<T, PIECE>::of(v + i));
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < left) p[i] = from_f32<T>(v[i]);
+  }
+}
+// N elements of a row from p, as far as the row's `left` go, zeros past them.
+template <typename T, int N>
+__device__ __forceinline__ Vec<T, N> load_some(const T* p, int left) {
+  if (left >= N) return load<T, N>(p);
+  T e[N] = {};
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < left) e[i] = p[i];
+  Vec<T, N> v;
+  __builtin_memcpy(&v.raw, e, sizeof(e));
+  return v;
+}
+
+// ---------------------------------------------------------------------------------- epilogue
+struct Epilogue {
+  const void *bias, *gate, *residual;
+  void *y, *h;         // the result; h as the backward wants it (rounded), or null
+  float* part;         // [splits][rows][columns] sums instead of the result, or null
+  int64_t gate_stride;
+  int rows, outer, act, rows_per_gate;
+};
+__device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + __expf(-v)); }
+
+// Channels col .. col + V - 1 of row `row` from the products: a of W's first rows, b (SwiGLU) of its second.
+template <typename T, bool SWIGLU>
+__device__ __forceinline__ void finish(const Epilogue& e, int row, int col, float* a, float* b) {
+  const int left = e.outer - col;
+  float t[V];
+  if (e.bias) {
+    get(static_cast<const T*>(e.bias) + col, left, t);
+#pragma unroll
+    for (int i = 0; i < V; ++i) a[i] += t[i];
+    if constexpr (SWIGLU) {
+      get(static_cast<const T*>(e.bias) + e.outer + col, left, t);
+#pragma unroll
+      for (int i = 0; i < V; ++i) b[i] += t[i];
+    }
+  }
+  if (e.h) {
+    T* h = static_cast<T*>(e.h) + int64_t(row) * (SWIGLU ? 2 : 1) * e.outer + col;
+    put(h, left, a);
+    if constexpr (SWIGLU) put(h + e.outer, left, b);
+  }
+  if constexpr (SWIGLU) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) a[i] = a[i] * sigmoid(a[i]) * b[i];
+  } else if (e.act == SIHC_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) a[i] *= sigmoid(a[i]);
+  }
+  if (e.gate) {
+    get(static_cast<const T*>(e.gate) + int64_t(row / e.rows_per_gate) * e.gate_stride + col, left, t);
+#pragma unroll
+    for (int i = 0; i < V; ++i) a[i] *= t[i];
+  }
+  const int64_t at = int64_t(row) * e.outer + col;
+  if (e.residual) {
+    get(static_cast<const T*>(e.residual) + at, left, t);
+#pragma unroll
+    for (int i = 0; i < V; ++i) a[i] += t[i];
+  }
+  put(static_cast<T*>(e.y) + at, left, a);
+}
+
+// ---------------------------------------------------------------------------------- products
+// c[m, n] = sum over k of a[m, k] b[n, k]; an operand is [rows, contraction], or transposed.
+struct Gemm {
+  const void *a, *b;
+  int64_t lda, ldb;
+  int m, n, k;      // (SwiGLU: n is the result's channels, half of b's rows)
+  int splits;       // parts of the contraction
+  int steps;        // pieces of a part
+  int tiles_m, tiles_n;
+  Epilogue e;
+};
+
+template <typename T> struct Matrix;
+template <>
+struct Matrix<bf16> {
+  static constexpr int STEP = 16;  // contraction of one fragment
+  using Frag = bf16x8;
+  static __device__ __forceinline__ f32x16 multiply(const Frag& a, const Frag& b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Matrix<float> {
+  static constexpr int STEP = 8;
+  using Frag = f32x4;
+  static __device__ __forceinline__ f32x16 multiply(const Frag& a, const Frag& b, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+};
+__device__ __forceinline__ constexpr int row_of(int i, int half) { return (i / 4) * 8 + half * 4 + i % 4; }
+
+template <typename T, int BM_, int BN_, int BK_, int WAVES_M_, int WAVES_N_, int PER_SIMD_>
+struct Config {
+  static constexpr int BM = BM_, BN = BN_, BK = BK_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, PER_SIMD = PER_SIMD_;
+  static constexpr int THREADS = WAVES_M * WAVES_N * 64;
+  static constexpr int MT = BM / WAVES_M / 32, NT = BN / WAVES_N / 32;  // a wave's tiles
+};
+
+// ROWS rows of an operand, BK of the contraction: in registers on their way, and in LDS.
+template <typename T, int ROWS, int BK, int THREADS, bool TRANSPOSED, bool SWIGLU>
+struct Piece {
+  static constexpr int N = 16 / int(sizeof(T));
+  // padded: 16 rows of 16 bytes, or 4 rows of 64 (transposing loads), fall into different banks
+  static constexpr int STRIDE = TRANSPOSED ? ROWS + 64 / int(sizeof(T)) : BK + N;
+  static constexpr int SIZE = (TRANSPOSED ? BK : ROWS) * STRIDE;
+  static constexpr int VECS = (TRANSPOSED ? ROWS : BK) / N;  // vectors of a row in memory
+  static constexpr int STEP = THREADS / VECS, COUNT = ROWS * BK / N / THREADS;
+  static_assert(THREADS % VECS == 0 && COUNT * THREADS * N == ROWS * BK, "every thread has the same vectors");
+
+  const T* base;
+  int64_t offset[TRANSPOSED ? 1 : COUNT];
+  int64_t ld;
+  int line, at;  // the thread's first row in the piece and its place in the row
+  int left;      // (transposed) rows of the operand from its place on
+  Vec<T, N> v[COUNT];
+
+  __device__ __forceinline__ Piece(const void* p, int64_t ld_, int first, int rows, int outer) : ld(ld_) {
+    base = static_cast<const T*>(p);
+    line = int(threadIdx.x) / VECS;
+    at = (int(threadIdx.x) % VECS) * N;
+    if constexpr (TRANSPOSED) {
+      left = rows - first - at;
+      offset[0] = first + at;
+    } else {
+#pragma unroll
+      for (int i = 0; i < COUNT; ++i) {
+        const int r = line + i * STEP;
+        int64_t row;
+        if constexpr (SWIGLU)
+          row = min(first + r / 64 * 32 + r % 32, rows - 1) + int64_t(r / 32 % 2) * outer;
+        else
+          row = min(first + r, rows - 1);
+        offset[i] = row * ld + at;
+      }
+    }
+  }
+  // Whether piece k0 of a contraction that ends at k needs no care.
+  __device__ __forceinline__ static bool whole(int k0, int k, int first, int rows) {
+    return k0 + BK <= k && (!TRANSPOSED || first + ROWS <= rows);
+  }
+  template <bool WHOLE>
+  __device__ __forceinline__ void fetch(int k0, int k) {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+      if constexpr (TRANSPOSED) {
+        const int row = k0 + line + i * STEP;
+        if constexpr (WHOLE)
+          v[i] = load<T, N>(base + offset[0] + int64_t(row) * ld);
+        else
+          v[i] = row < k && left > 0 ? load_some<T, N>(base + offset[0] + int64_t(row) * ld, left) : Vec<T, N>::zero();
+      } else {
+        if constexpr (WHOLE)
+          v[i] = load<T, N>(base + offset[i] + k0);
+        else
+          v[i] = k0 + at < k ? load_some<T, N>(base + offset[i] + k0, k - k0 - at) : Vec<T, N>::zero();
+      }
+    }
+  }
+  __device__ __forceinline__ void commit(T* lds) const {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) *reinterpret_cast<u32x4*>(lds + (line + i * STEP) * STRIDE + at) = v[i].raw;
+  }
+  // The lane's part of rows `row` .. row + 31 at step s of the piece.
+  static __device__ __forceinline__ typename Matrix<T>::Frag fragment(const T* lds, int row, int s) {
+    const int lane = int(threadIdx.x) & 63, half = lane >> 5;
+    if constexpr (!TRANSPOSED) {
+      return *reinterpret_cast<const typename Matrix<T>::Frag*>(lds + (row + (lane & 31)) * STRIDE +
+                                                                s * Matrix<T>::STEP + half * (Matrix<T>::STEP / 2));
+    } else if constexpr (sizeof(T) == 2) {
+      typedef __attribute__((address_space(3))) s16x4* LdsPtr;
+      const int j = lane & 15;
+      const T* p = lds + (s * 16 + half * 8 + j / 4) * STRIDE + row + (lane & 16) + (j % 4) * 4;
+      const s16x4 low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)p);
+      const s16x4 high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p + 4 * STRIDE));
+      return __builtin_bit_cast(bf16x8, __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      f32x4 f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[j] = lds[(s * 8 + half * 4 + j) * STRIDE + row + (lane & 31)];
+      return f;
+    }
+  }
+};
+
+template <typename T, typename C, bool TA, bool TB, bool SWIGLU>
+struct Layout {
+  using A = Piece<T, C::BM, C::BK, C::THREADS, TA, false>;
+  using B = Piece<T, C::BN, C::BK, C::THREADS, TB, SWIGLU>;
+  static constexpr int BUFFER = A::SIZE + B::SIZE;  // elements
+  static constexpr int STRIP = C::NT * 32 + 8;      // a row of a wave's strip in the epilogue (fp32)
+  static constexpr size_t BYTES = std::max(size_t(2) * BUFFER * sizeof(T),
+                                           size_t(C::THREADS / 64) * 32 * STRIP * sizeof(float));
+};
+
+template <typename T, typename C, bool TA, bool TB, bool SWIGLU>
+__global__ __launch_bounds__(C::THREADS, C::PER_SIMD) void gemm_kernel(const Gemm g) {
+  using L = Layout<T, C, TA, TB, SWIGLU>;
+  using A = typename L::A;
+  using B = typename L::B;
+  extern __shared__ __align__(16) char lds_bytes[];
+  T* lds = reinterpret_cast<T*>(lds_bytes);
+  constexpr int COLUMNS = SWIGLU ? C::BN / 2 : C::BN;  // the result's
+
+  // Tiles of one part, 8 rows of tiles at a time: neighbours on an XCD share rows and columns.
+  const int tiles = g.tiles_m * g.tiles_n;
+  const int block = xcd_block(blockIdx.x, gridDim.x), part = block / tiles, tile = block - part * tiles;
+  const int band = tile / (8 * g.tiles_n), in = tile - band * 8 * g.tiles_n;
+  const int high = min(8, g.tiles_m - band * 8);
+  const int m0 = (band * 8 + in % high) * C::BM, n0 = in / high * COLUMNS;
+  const int from = part * g.steps * C::BK, k = min(g.k, from + g.steps * C::BK);
+
+  A a(g.a, g.lda, m0, g.m, 0);
+  B b(g.b, g.ldb, n0, g.n, g.n);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / C::WAVES_N * C::MT * 32, wn = wave % C::WAVES_N * C::NT * 32;
+  auto fetch = [&](int k0) {
+    if (A::whole(k0, k, m0, g.m)) a.template fetch<true>(k0, k);
+    else a.template fetch<false>(k0, k);
+    if (B::whole(k0, k, n0, g.n)) b.template fetch<true>(k0, k);
+    else b.template fetch<false>(k0, k);
+  };
+  f32x16 acc[C::MT][C::NT] = {};
+  fetch(from);
+  a.commit(lds);
+  b.commit(lds + A::SIZE);
+  if (from + C::BK < k) fetch(from + C::BK);
+  __syncthreads();
+  int buffer = 0;
+  for (int k0 = from; k0 < k; k0 += C::BK, buffer ^= 1) {
+    T* next = lds + (buffer ^ 1) * L::BUFFER;
+    if (k0 + C::BK < k) {
+      a.commit(next);
+      b.commit(next + A::SIZE);
+      if (k0 + 2 * C::BK < k) fetch(k0 + 2 * C::BK);
+    }
+    const T *pa = lds + buffer * L::BUFFER, *pb = pa + A::SIZE;
+#pragma unroll
+    for (int s = 0; s < C::BK / Matrix<T>::STEP; ++s) {
+      typename Matrix<T>::Frag fa[C::MT], fb[C::NT];
+#pragma unroll
+      for (int i = 0; i < C::MT; ++i) fa[i] = A::fragment(pa, wm + i * 32, s);
+#pragma unroll
+      for (int j = 0; j < C::NT; ++j) fb[j] = B::fragment(pb, wn + j * 32, s);
+#pragma unroll
+      for (int i = 0; i < C::MT; ++i)
+#pragma unroll
+        for (int j = 0; j < C::NT; ++j) acc[i][j] = Matrix<T>::multiply(fa[i], fb[j], acc[i][j]);
+    }
+    __syncthreads();
+  }
+
+  // a strip of 32 rows at a time through the wave's own LDS
+  const int lane = threadIdx.x & 63;
+  float* strip = reinterpret_cast<float*>(lds_bytes) + wave * 32 * L::STRIP;
+  constexpr int WIDE = SWIGLU ? C::NT * 16 : C::NT * 32;  // the result's channels of a wave
+  constexpr int GROUPS = WIDE / V, ROWS = 64 / GROUPS;
+  const int col = n0 + (SWIGLU ? wn / 2 : wn) + lane % GROUPS * V;
+#pragma unroll
+  for (int i = 0; i < C::MT; ++i) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int j = 0; j < C::NT; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) strip[row_of(r, lane >> 5) * L::STRIP + j * 32 + (lane & 31)] = acc[i][j][r];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
+    for (int r = lane / GROUPS; r < 32; r += ROWS) {
+      const int row = m0 + wm + i * 32 + r;
+      if (row >= g.m || col >= g.n) continue;
+      const int c = lane % GROUPS * V;
+      float p[V], q[V];
+      const float* from_strip = strip + r * L::STRIP + (SWIGLU ? c / 32 * 64 + c % 32 : c);
+#pragma unroll
+      for (int x = 0; x < V; ++x) p[x] = from_strip[x];
+      if constexpr (SWIGLU)
+#pragma unroll
+        for (int x = 0; x < V; ++x) q[x] = from_strip[32 + x];
+      if (g.e.part) {
+        float* to = g.e.part + (int64_t(part) * g.m + row) * (SWIGLU ? 2 : 1) * g.n + col;
+        put(to, g.n - col, p);
+        if constexpr (SWIGLU) put(to + g.n, g.n - col, q);
+      } else {
+        finish<T, SWIGLU>(g.e, row, col, p, q);
+      }
+    }
+  }
+}
+
+// The result from the parts' sums, in their order.
+template <typename T, bool SWIGLU>
+__global__ __launch_bounds__(256) void join_kernel(const Epilogue e, int splits) {
+  const int groups = (e.outer + V - 1) / V;
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t row = i / groups;
+  if (row >= e.rows) return;
+  const int col = int(i - row * groups) * V, left = e.outer - col;
+  const int64_t wide = (SWIGLU ? 2 : 1) * int64_t(e.outer), all = int64_t(e.rows) * wide;
+  const float* p = e.part + row * wide + col;
+  float a[V] = {}, b[V] = {};
+#pragma unroll 2
+  for (int s = 0; s < splits; ++s) {
+    float t[V];
+    get(p + s * all, left, t);
+#pragma unroll
+    for (int x = 0; x < V; ++x) a[x] += t[x];
+    if constexpr (SWIGLU) {
+      get(p + s * all + e.outer, left, t);
+#pragma unroll
+      for (int x = 0; x < V; ++x) b[x] += t[x];
+    }
+  }
+  finish<T, SWIGLU>(e, int(row), col, a, b);
+}
+
+// ------------------------------------------------------------------------------ dh and its sums
+struct Slopes {
+  const void *grad, *h, *gate;
+  void *dh;            // null where dh is the gradient itself
+  float *bias_part, *gate_part;
+  int64_t gate_stride;
+  int rows, outer, act, rows_per_gate, chunks;  // chunks of an image's rows
+};
+constexpr int CHUNK = 64;  // rows whose sums are one partial row
+
+// A block: 256 channels (32 threads of V) by 8 rows at a time, over one chunk of one image.
+template <typename T, bool SWIGLU>
+__global__ __launch_bounds__(256) void slopes_kernel(const Slopes s) {
+  __shared__ float lds[8][32 * V + 4];
+  const int across = threadIdx.x & 31, down = threadIdx.x >> 5;
+  const int blocks = (s.outer + 32 * V - 1) / (32 * V);
+  const int chunk = int(blockIdx.x / unsigned(blocks)), col = (int(blockIdx.x % unsigned(blocks)) * 32 + across) * V;
+  const int image = chunk / s.chunks, first = (chunk - image * s.chunks) * CHUNK;
+  const int count = min(CHUNK, s.rows_per_gate - first), left = s.outer - col;
+  const int64_t row0 = int64_t(image) * s.rows_per_gate + first;
+  const int wide = SWIGLU ? 2 : 1;
+  float sums[3][V] = {}, gate[V];
+  if (left > 0) {
+    if (s.gate) get(static_cast<const T*>(s.gate) + image * s.gate_stride + col, left, gate);
+#pragma unroll 2
+    for (int r = down; r < count; r += 8) {
+      float g[V], a[V], b[V];
+      const int64_t row = row0 + r;
+      get(static_cast<const T*>(s.grad) + row * s.outer + col, left, g);
+      if (s.h) {
+        const T* h = static_cast<const T*>(s.h) + row * wide * s.outer + col;
+        get(h, left, a);
+        if constexpr (SWIGLU) get(h + s.outer, left, b);
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float u = a[i], slope = 1.f;
+        if (SWIGLU || s.act == SIHC_ACT_SILU) {
+          const float sigma = sigmoid(a[i]);
+          u = a[i] * sigma;
+          slope = sigma * (1.f + a[i] * (1.f - sigma));
+        }
+        float du = g[i];
+        if (s.gate) {
+          sums[2][i] += g[i] * (SWIGLU ? u * b[i] : u);
+          du *= gate[i];
+        }
+        if constexpr (SWIGLU) {
+          a[i] = du * b[i] * slope;
+          b[i] = du * u;
+          sums[1][i] += b[i];
+        } else {
+          a[i] = du * slope;
+        }
+        sums[0][i] += a[i];
+      }
+      if (s.dh) {
+        T* dh = static_cast<T*>(s.dh) + row * wide * s.outer + col;
+        put(dh, left, a);
+        if constexpr (SWIGLU) put(dh + s.outer, left, b);
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    if (k == 1 && !SWIGLU) continue;
+    float* part = k == 2 ? s.gate_part : s.bias_part;
+    if (!part) continue;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < V; ++i) lds[down][across * V + i] = sums[k][i];
+    __syncthreads();
+    const int c = int(blockIdx.x % unsigned(blocks)) * 32 * V + int(threadIdx.x);
+    if (c < s.outer) {
+      float v = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v += lds[i][threadIdx.x];
+      part[k == 2 ? int64_t(chunk) * s.outer + c : (int64_t(chunk) * wide + k) * s.outer + c] = v;
+    }
+  }
+}
+// out[r, :] = sum over `parts` rows of part[r * parts + i, :]: 32 columns a block, 8 threads each.
+template <typename T>
+__global__ __launch_bounds__(256) void sums_kernel(const float* part, T* out, int rows, int columns, int parts) {
+  __shared__ float lds[8][33];
+  const int across = threadIdx.x & 31, down = threadIdx.x >> 5;
+  const int blocks = (columns + 31) / 32;
+  const int64_t r = blockIdx.x / unsigned(blocks);
+  const int c = int(blockIdx.x % unsigned(blocks)) * 32 + across;
+  float v = 0.f;
+  if (c < columns) {
+    const float* p = part + r * parts * columns + c;
+#pragma unroll 8
+    for (int i = down; i < parts; i += 8) v += p[int64_t(i) * columns];
+  }
+  lds[down][across] = v;
+  __syncthreads();
+  if (down || c >= columns) return;
+  v = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v += lds[i][across];
+  out[r * columns + c] = from_f32<T>(v);
+}
+
+// ---------------------------------------------------------------------------------- host
+template <typename T> struct Configs;
+template <>
+struct Configs<bf16> {
+  using Large = Config<bf16, 256, 256, 64, 2, 4, 2>;
+  using Middle = Config<bf16, 128, 128, 64, 2, 2, 2>;
+  using Small = Config<bf16, 64, 64, 64, 2, 1, 2>;
+};
+template <>
+struct Configs<float> {
+  using Large = Config<float, 128, 128, 32, 2, 2, 2>;
+  using Middle = Large;
+  using Small = Config<float, 64, 64, 32, 2, 1, 2>;
+};
+
+struct Plan {
+  int size;  // 0 large, 1 middle, 2 small
+  int splits, steps, tiles_m, tiles_n;
+  int64_t blocks;
+};
+constexpr int CUS = 256;
+
+// The tile and the parts of the contraction that promise the least time: rounds of blocks over the
+// CUs, each as long as its pieces and a fixed start and end, and the parts' sums through memory.
+template <typename T>
+Plan plan_of(int64_t m, int64_t n, int64_t k, bool swiglu) {
+  struct Shape { int bm, bn, bk, per_cu; double piece; };  // cycles of a piece where the CU is full
+  using C = Configs<T>;
+  auto shape = [](auto config, int per_cu, double rate) {  // rate: of the matrix cores' peak
+    using S = decltype(config);
+    const double flops = sizeof(T) == 2 ? 4096.0 : 256.0;
+    return Shape{S::BM, S::BN, S::BK, per_cu, 2.0 * S::BM * S::BN * S::BK / (flops * rate)};
+  };
+  const Shape shapes[3] = {shape(typename C::Large{}, sizeof(T) == 2 ? 1 : 2, sizeof(T) == 2 ? 0.5 : 0.8),
+                           shape(typename C::Middle{}, 2, sizeof(T) == 2 ? 0.35 : 0.8),
+                           shape(typename C::Small{}, 4, sizeof(T) == 2 ? 0.2 : 0.6)};
+  Plan best{};
+  double least = 1e30;
+  for (int s = 0; s < 3; ++s) {
+    const Shape& f = shapes[s];
+    const int64_t tm = ceil_div(m, f.bm), tn = ceil_div(n, swiglu ? f.bn / 2 : f.bn), pieces = ceil_div(k, f.bk);
+    for (int splits = 1; splits <= 64 && splits <= pieces; ++splits) {
+      const int64_t steps = ceil_div(pieces, splits);
+      if (ceil_div(pieces, steps) != splits) continue;
+      const int64_t blocks = tm * tn * splits;
+      // blocks that share a CU share its matrix cores
+      const double rounds = double(ceil_div(blocks, CUS));
+      const double alone = std::min<double>(rounds, f.per_cu);  // blocks of a CU at a time
+      double cycles = rounds * double(steps) * f.piece + ceil_div(int64_t(rounds), f.per_cu) * 3000.0;
+      // few blocks: a piece costs its loads' latency
+      cycles = std::max(cycles, double(steps) * 900.0 * rounds / alone);
+      if (splits > 1) cycles += 6000.0 + double(m) * double(n) * (swiglu ? 2 : 1) * 8.0 * splits / 1700.0;
+      if (cycles < least) {
+        least = cycles;
+        best = Plan{s, splits, int(steps), int(tm), int(tn), blocks};
+      }
+    }
+  }
+  return best;
+}
+Plan plan_for(int dtype, int64_t m, int64_t n, int64_t k, bool swiglu) {
+  return dtype == SIHC_DTYPE_BF16 ? plan_of<bf16>(m, n, k, swiglu) : plan_of<float>(m, n, k, swiglu);
+}
+size_t part_bytes(const Plan& p, int64_t m, int64_t n, bool swiglu) {
+  return p.splits > 1 ? size_t(p.splits) * size_t(m) * size_t(n) * (swiglu ? 2 : 1) * sizeof(float) : 0;
+}
+
+template <typename T, typename C, bool TA, bool TB, bool SWIGLU>
+int start(const Gemm& g, int64_t blocks, hipStream_t stream, const char* what) {
+  using L = Layout<T, C, TA, TB, SWIGLU>;
+  const void* kernel = reinterpret_cast<const void*>(&gemm_kernel<T, C, TA, TB, SWIGLU>);
+  if (L::BYTES > 65536) {
+    const hipError_t err = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, int(L::BYTES));
+    if (err != hipSuccess) return fail(SIHC_ERR_HIP, "%s: %s", what, hipGetErrorString(err));
+  }
+  gemm_kernel<T, C, TA, TB, SWIGLU><<<unsigned(blocks), C::THREADS, L::BYTES, stream>>>(g);
+  return check_launch(what);
+}
+// g.e, g.a, g.b and the sizes given; `part`: the parts' sums.
+template <typename T, bool TA, bool TB, bool SWIGLU>
+int product(Gemm g, float* part, hipStream_t stream, const char* what) {
+  const Plan p = plan_of<T>(g.m, g.n, g.k, SWIGLU);
+  if (p.blocks * 512 > MOST_LAUNCHED) return fail(SIHC_ERR_INVALID, "%s: too many rows for a launch", what);
+  g.splits = p.splits;
+  g.steps = p.steps;
+  g.tiles_m = p.tiles_m;
+  g.tiles_n = p.tiles_n;
+  g.e.part = p.splits > 1 ? part : nullptr;
+  g.e.rows = g.m;
+  g.e.outer = g.n;
+  int rc;
+  if (p.size == 0) rc = start<T, typename Configs<T>::Large, TA, TB, SWIGLU>(g, p.blocks, stream, what);
+  else if (p.size == 1) rc = start<T, typename Configs<T>::Middle, TA, TB, SWIGLU>(g, p.blocks, stream, what);
+  else rc = start<T, typename Configs<T>::Small, TA, TB, SWIGLU>(g, p.blocks, stream, what);
+  if (rc || p.splits == 1) return rc;
+  const int64_t threads = int64_t(g.m) * ceil_div(g.n, V);
+  if (threads > MOST_LAUNCHED) return fail(SIHC_ERR_INVALID, "%s: too many rows for a launch", what);
+  join_kernel<T, SWIGLU><<<unsigned(ceil_div(threads, 256)), 256, 0, stream>>>(g.e, p.splits);
+  return check_launch(what);
+}
+
+int check(const sihc_linear* l, const char* what) {
+  if (!l) return fail(SIHC_ERR_INVALID, "%s: null sizes", what);
+  if (!valid_dtype(l->dtype)) return fail(SIHC_ERR_INVALID, "%s: bad dtype %d", what, l->dtype);
+  if (l->act != SIHC_ACT_NONE && l->act != SIHC_ACT_SILU && l->act != SIHC_ACT_SWIGLU)
+    return fail(SIHC_ERR_INVALID, "%s: bad activation %d", what, l->act);
+  if (l->rows < 0 || l->rows > (int64_t(1) << 30) || l->inner < 1 || l->outer < 1 || l->inner > (1 << 24) ||
+      l->outer > (1 << 24))
+    return fail(SIHC_ERR_INVALID, "%s: at most 2^30 rows of 1..2^24 channels", what);
+  if (l->rows_per_gate < 1 || l->rows % l->rows_per_gate)
+    return fail(SIHC_ERR_INVALID, "%s: %lld rows of %lld a gate", what, (long long)l->rows, (long long)l->rows_per_gate);
+  return SIHC_OK;
+}
+int64_t align(int64_t bytes) { return ceil_div(bytes, 256) * 256; }
+
+// What the backward keeps in its workspace, in this order; sizes in bytes.
+struct Space {
+  int64_t dh, bias, gate, part;
+  int64_t chunks, images;
+  int64_t total() const { return dh + bias + gate + part; }
+};
+Space space_of(const sihc_linear* l, bool gated) {
+  Space s{};
+  const bool swiglu = l->act == SIHC_ACT_SWIGLU;
+  const int64_t wide = (swiglu ? 2 : 1) * int64_t(l->outer), size = l->dtype == SIHC_DTYPE_BF16 ? 2 : 4;
+  const int64_t each = gated ? l->rows_per_gate : std::max<int64_t>(l->rows, 1);
+  s.images = l->rows / each;
+  s.chunks = ceil_div(each, CHUNK);
+  if (l->act != SIHC_ACT_NONE || gated) s.dh = align(l->rows * wide * size);
+  s.bias = align(s.images * s.chunks * wide * 4);
+  if (gated) s.gate = align(s.images * s.chunks * l->outer * 4);
+  const Plan dx = plan_for(l->dtype, l->rows, l->inner, wide, false);
+  const Plan dw = plan_for(l->dtype, wide, l->inner, l->rows, false);
+  s.part = align(int64_t(std::max(part_bytes(dx, l->rows, l->inner, false), part_bytes(dw, wide, l->inner, false))));
+  return s;
+}
+}  // namespace
+
+extern "C" size_t sihc_linear_act_workspace_size(const sihc_linear* l) {
+  if (check(l, "linear_act") || l->rows == 0) return 0;
+  const bool swiglu = l->act == SIHC_ACT_SWIGLU;
+  return part_bytes(plan_for(l->dtype, l->rows, l->outer, l->inner, swiglu), l->rows, l->outer, swiglu);
+}
+
+extern "C" int sihc_linear_act(const sihc_linear* l, const void* x, const void* weight, const void* bias,
+                               const void* gate, const void* residual, void* y, void* h, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  if (const int rc = check(l, "linear_act")) return rc;
+  if (l->rows == 0) return SIHC_OK;
+  if (!x || !weight || !y) return fail(SIHC_ERR_INVALID, "linear_act: null pointer");
+  const size_t need = sihc_linear_act_workspace_size(l);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(SIHC_ERR_INVALID, "linear_act: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  Gemm g{};
+  g.a = x;
+  g.b = weight;
+  g.lda = g.ldb = l->inner;
+  g.m = int(l->rows);
+  g.n = l->outer;
+  g.k = l->inner;
+  g.e = Epilogue{bias, gate, residual, y, h, nullptr, l->gate_stride, 0, 0, l->act, int(l->rows_per_gate)};
+  return by_dtype(l->dtype, [&](auto t) {
+    using T = decltype(t);
+    float* part = static_cast<float*>(workspace);
+    return l->act == SIHC_ACT_SWIGLU ? product<T, false, false, true>(g, part, hipStream_t(stream), "linear_act")
+                                     : product<T, false, false, false>(g, part, hipStream_t(stream), "linear_act");
+  });
+}
+
+extern "C" size_t sihc_linear_act_backward_workspace_size(const sihc_linear* l, int gated) {
+  if (check(l, "linear_act_backward") || l->rows == 0) return 0;
+  return size_t(space_of(l, gated != 0).total());
+}
+
+extern "C" int sihc_linear_act_backward(const sihc_linear* l, const void* grad, const void* x, const void* weight,
+                                        const void* h, const void* gate, void* dx, void* dweight, void* dbias,
+                                        void* dgate, void* workspace, size_t workspace_bytes, void* stream) {
+  if (const int rc = check(l, "linear_act_backward")) return rc;
+  const bool swiglu = l->act == SIHC_ACT_SWIGLU, gated = gate != nullptr;
+  const int wide = (swiglu ? 2 : 1) * l->outer, images = int(l->rows / l->rows_per_gate);
+  const hipStream_t on = hipStream_t(stream);
+  if (dgate && !gated) return fail(SIHC_ERR_INVALID, "linear_act_backward: no gate, no gradient of it");
+  const char* what = "linear_act_backward";
+  if (l->rows == 0)  // sums over nothing
+    return by_dtype(l->dtype, [&](auto t) {
+      using T = decltype(t);
+      auto clear = [&](void* p, int64_t rows) {
+        if (!p) return int(SIHC_OK);
+        const int64_t blocks = rows * ceil_div(l->inner, 32);
+        if (blocks * 256 > MOST_LAUNCHED) return fail(SIHC_ERR_INVALID, "%s: too many rows for a launch", what);
+        sums_kernel<T><<<unsigned(blocks), 256, 0, on>>>(nullptr, static_cast<T*>(p), int(rows), l->inner, 0);
+        return check_launch(what);
+      };
+      if (const int rc = clear(dweight, wide)) return rc;
+      if (dbias) sums_kernel<T><<<unsigned(ceil_div(wide, 32)), 256, 0, on>>>(nullptr, static_cast<T*>(dbias), 1, wide, 0);
+      return check_launch(what);
+    });
+  if (!grad || !x || !weight || ((gated || l->act != SIHC_ACT_NONE) && !h))
+    return fail(SIHC_ERR_INVALID, "linear_act_backward: null pointer");
+  const Space s = space_of(l, gated);
+  if (!workspace || workspace_bytes < size_t(s.total()))
+    return fail(SIHC_ERR_INVALID, "linear_act_backward: workspace of %zu bytes, %lld needed", workspace_bytes,
+                (long long)s.total());
+  char* at = static_cast<char*>(workspace);
+  void* dh = s.dh ? at : nullptr;
+  float* bias_part = reinterpret_cast<float*>(at + s.dh);
+  float* gate_part = reinterpret_cast<float*>(at + s.dh + s.bias);
+  float* part = reinterpret_cast<float*>(at + s.dh + s.bias + s.gate);
+  return by_dtype(l->dtype, [&](auto t) {
+    using T = decltype(t);
+    if (dh || dbias) {
+      Slopes v{grad, dh ? h : nullptr, gate, dh, dbias ? bias_part : nullptr, dgate ? gate_part : nullptr,
+               l->gate_stride, int(l->rows), l->outer, l->act, gated ? int(l->rows_per_gate) : int(l->rows),
+               int(s.chunks)};
+      const int64_t blocks = s.images * s.chunks * ceil_div(l->outer, 32 * V);
+      if (blocks * 256 > MOST_LAUNCHED) return fail(SIHC_ERR_INVALID, "%s: too many rows for a launch", what);
+      if (swiglu) slopes_kernel<T, true><<<unsigned(blocks), 256, 0, on>>>(v);
+      else slopes_kernel<T, false><<<unsigned(blocks), 256, 0, on>>>(v);
+      if (const int rc = check_launch(what)) return rc;
+    }
+    auto sum = [&](const float* from, void* to, int64_t rows, int columns, int64_t parts) {
+      const int64_t blocks = rows * ceil_div(columns, 32);
+      if (blocks * 256 > MOST_LAUNCHED) return fail(SIHC_ERR_INVALID, "%s: too many rows for a launch", what);
+      sums_kernel<T><<<unsigned(blocks), 256, 0, on>>>(from, static_cast<T*>(to), int(rows), columns, int(parts));
+      return check_launch(what);
+    };
+    if (dbias)
+      if (const int rc = sum(bias_part, dbias, 1, wide, s.images * s.chunks)) return rc;
+    if (dgate)
+      if (const int rc = sum(gate_part, dgate, images, l->outer, s.chunks)) return rc;
+    const void* slopes = dh ? dh : grad;
+    Gemm g{};
+    g.a = slopes;
+    g.lda = wide;
+    g.ldb = l->inner;
+    if (dx) {
+      g.b = weight;
+      g.m = int(l->rows);
+      g.n = l->inner;
+      g.k = wide;
+      g.e = Epilogue{nullptr, nullptr, nullptr, dx, nullptr, nullptr, 0, 0, 0, SIHC_ACT_NONE, 1};
+      if (const int rc = product<T, false, true, false>(g, part, on, what)) return rc;
+    }
+    if (dweight) {
+      g.b = x;
+      g.m = wide;
+      g.n = l->inner;
+      g.k = int(l->rows);
+      g.e = Epilogue{nullptr, nullptr, nullptr, dweight, nullptr, nullptr, 0, 0, 0, SIHC_ACT_NONE, 1};
+      if (const int rc = product<T, true, true, false>(g, part, on, what)) return rc;
+    }
+    return int(SIHC_OK);
+  });
+}

@@ -8,6 +8,8 @@ Modules
   indexed            spatially indexed (int32 state index) gather/scatter and read/write
   conditioning       embedding lookup, cross attention and group norm with an activation: what
                      conditions a denoiser on an encoder's states
+  body               projections with an epilogue, head norms with rotation, dropout: what a block
+                     computes between its read and its write
   text_denoiser      a text-conditioned SiHC denoiser on them
   launch             tensor-level launchers over the C ABI (include/sihc_hip.h)
 """
@@ -15,6 +17,8 @@ from ._lib import LIB_PATH, lib  # noqa: F401
 from .sublayer_kernels import sublayer_read, sublayer_triangular, sublayer_write  # noqa: F401
 from .event_ops import event_write_read, literal_stage  # noqa: F401
 from .conditioning import cross_attention, embedding_lookup, group_norm_act  # noqa: F401
+from .body import axis_rotary, dropout, linear_act, qk_norm_rotary  # noqa: F401
 
 __all__ = ["LIB_PATH", "lib", "sublayer_read", "sublayer_write", "sublayer_triangular",
-           "event_write_read", "literal_stage", "embedding_lookup", "cross_attention", "group_norm_act"]
+           "event_write_read", "literal_stage", "embedding_lookup", "cross_attention", "group_norm_act",
+           "linear_act", "qk_norm_rotary", "axis_rotary", "dropout"]

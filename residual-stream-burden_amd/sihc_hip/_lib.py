@@ -10,13 +10,18 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().with_name("libsihc_hip.so")
-ABI_VERSION = 7
+ABI_VERSION = 8
 MAX_EVENTS = 32
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
 ACT_NONE = 0
 ACT_SILU = 1
+ACT_SWIGLU = 2
 MAX_HEAD_DIM = 128
+MAX_ROTARY_DIM = 256
+MAX_AXES = 4
+POSITION_I32 = 0
+POSITION_F32 = 1
 
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int
@@ -33,7 +38,24 @@ class Attention(ctypes.Structure):
                 ("v_stride", ctypes.c_int64 * 3), ("scale", ctypes.c_float), ("dtype", ctypes.c_int)]
 
 
+class Linear(ctypes.Structure):
+    """sihc_linear of include/sihc_hip.h."""
+    _fields_ = [("rows", ctypes.c_int64), ("inner", ctypes.c_int), ("outer", ctypes.c_int), ("act", ctypes.c_int),
+                ("dtype", ctypes.c_int), ("rows_per_gate", ctypes.c_int64), ("gate_stride", ctypes.c_int64)]
+
+
+class Heads(ctypes.Structure):
+    """sihc_heads of include/sihc_hip.h."""
+    _fields_ = [("batch", ctypes.c_int64), ("tokens", ctypes.c_int64), ("heads", ctypes.c_int),
+                ("kv_heads", ctypes.c_int), ("dim", ctypes.c_int), ("axes", ctypes.c_int),
+                ("widths", ctypes.c_int * MAX_AXES), ("q_stride", ctypes.c_int64 * 3),
+                ("k_stride", ctypes.c_int64 * 3), ("position_batch_stride", ctypes.c_int64),
+                ("theta", ctypes.c_double), ("eps", ctypes.c_float), ("dtype", ctypes.c_int),
+                ("w_dtype", ctypes.c_int), ("position_dtype", ctypes.c_int), ("inverse", ctypes.c_int)]
+
+
 _f32 = ctypes.c_float
+_linp, _headsp = ctypes.POINTER(Linear), ctypes.POINTER(Heads)
 _attp = ctypes.POINTER(Attention)
 
 # name -> (restype, argtypes); mirrors include/sihc_hip.h one for one.
@@ -88,6 +110,15 @@ PROTOTYPES: dict[str, tuple] = {
     "sihc_cross_attention_backward_workspace_size": (_sz, [_attp]),
     "sihc_cross_attention_backward": (_i32, [_attp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                              _sz, _vp]),
+    "sihc_linear_act_workspace_size": (_sz, [_linp]),
+    "sihc_linear_act": (_i32, [_linp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "sihc_linear_act_backward_workspace_size": (_sz, [_linp, _i32]),
+    "sihc_linear_act_backward": (_i32, [_linp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "sihc_qk_norm_rotary": (_i32, [_headsp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "sihc_qk_norm_rotary_backward_workspace_size": (_sz, [_headsp]),
+    "sihc_qk_norm_rotary_backward": (_i32, [_headsp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
+                                            _vp]),
+    "sihc_dropout": (_i32, [_vp, _vp, _vp, _i64, ctypes.c_double, _vp, _i64, _i32, _vp]),
     "sihc_fma_rate": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp]),
 }
 

@@ -16,10 +16,12 @@ from typing import Optional, Sequence
 import torch
 from torch import Tensor
 
-from ._lib import ACT_NONE, ACT_SILU, DTYPE_BF16, DTYPE_F32, MAX_EVENTS, Attention, check, lib, ptr_array
+from ._lib import (ACT_NONE, ACT_SILU, ACT_SWIGLU, DTYPE_BF16, DTYPE_F32, MAX_AXES, MAX_EVENTS, POSITION_F32, POSITION_I32,
+                   Attention, Heads, Linear, check, lib, ptr_array)
 
 _DTYPES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
 ACTIVATIONS = {"none": ACT_NONE, "silu": ACT_SILU}
+LINEAR_ACTIVATIONS = {**ACTIVATIONS, "swiglu": ACT_SWIGLU}
 
 
 def dtype_code(dtype: torch.dtype) -> int:
@@ -393,8 +395,119 @@ def cross_attention_backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, leng
     return dq, dk, dv
 
 
+def _linear(x: Tensor, weight: Tensor, act: str, gate: Optional[Tensor]) -> Linear:
+    rows = x.numel() // x.shape[-1]
+    outer = weight.shape[0] // 2 if act == "swiglu" else weight.shape[0]
+    each = max(rows, 1) if gate is None or not rows else rows // x.shape[0]
+    return Linear(rows, x.shape[-1], outer, LINEAR_ACTIVATIONS[act], dtype_code(x.dtype), each,
+                  0 if gate is None else gate.stride(0))
+
+
+@_on_tensor_device
+def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str, gate: Optional[Tensor],
+               residual: Optional[Tensor], train: bool) -> tuple[Tensor, Tensor]:
+    """(residual + gate * act(h) with h = x weight^T + bias, and for the backward h [..., weight rows]; empty
+    where the backward needs none or `train` is not set)."""
+    l = _linear(x, weight, act, gate)
+    keeps = train and (act != "none" or gate is not None)
+    out = torch.empty((*x.shape[:-1], l.outer), device=x.device, dtype=x.dtype)
+    h = torch.empty((*x.shape[:-1], weight.shape[0]) if keeps else (0,), device=x.device, dtype=x.dtype)
+    L = lib()
+    nbytes = L.sihc_linear_act_workspace_size(ctypes.byref(l))
+    ws = _workspace(nbytes, x.device) if nbytes else None
+    check(L.sihc_linear_act(ctypes.byref(l), x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(gate), _ptr(residual),
+                            out.data_ptr(), h.data_ptr() if keeps else None, _ptr(ws), nbytes, _stream(x.device)))
+    return out, h
+
+
+@_on_tensor_device
+def linear_act_backward(grad: Tensor, x: Tensor, weight: Tensor, h: Tensor, gate: Optional[Tensor], act: str,
+                        want_x: bool, want_weight: bool, want_bias: bool,
+                        want_gate: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """(input, weight, bias and gate gradients) of linear_act, those that are not wanted empty."""
+    l = _linear(x, weight, act, gate)
+
+    def output(wanted, shape):
+        return torch.empty(shape if wanted else (0,), device=x.device, dtype=x.dtype)
+
+    dx, dw = output(want_x, x.shape), output(want_weight, weight.shape)
+    db, dg = output(want_bias, weight.shape[:1]), output(want_gate, (x.shape[0], l.outer))
+    L = lib()
+    ws = _workspace(L.sihc_linear_act_backward_workspace_size(ctypes.byref(l), int(gate is not None)), x.device)
+    check(L.sihc_linear_act_backward(ctypes.byref(l), grad.data_ptr(), x.data_ptr(), weight.data_ptr(),
+                                     h.data_ptr() if h.numel() else None, _ptr(gate),
+                                     *(t.data_ptr() if wanted else None for t, wanted in
+                                       ((dx, want_x), (dw, want_weight), (db, want_bias), (dg, want_gate))),
+                                     ws.data_ptr(), ws.numel() * 4, _stream(x.device)))
+    if want_gate and not l.rows:
+        dg.zero_()  # a gate of no rows
+    return dx, dw, db, dg
+
+
+def _heads(q: Tensor, k: Optional[Tensor], weight: Optional[Tensor], positions: Tensor, axes: Sequence[int],
+           theta: float, eps: float, inverse: bool) -> Heads:
+    strides = [(ctypes.c_int64 * 3)(*(t.stride()[:3] if t is not None else ())) for t in (q, k)]
+    code = dtype_code(q.dtype)
+    return Heads(q.shape[0], q.shape[1], q.shape[2], 0 if k is None else k.shape[2], q.shape[3], len(axes),
+                 (ctypes.c_int * MAX_AXES)(*axes), *strides, q.shape[1] if positions.ndim == 3 else 0, theta, eps, code,
+                 code if weight is None else dtype_code(weight.dtype),
+                 POSITION_F32 if positions.dtype == torch.float32 else POSITION_I32, int(inverse))
+
+
+@_on_tensor_device
+def qk_norm_rotary(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, positions: Tensor, axes: Sequence[int],
+                   theta: float, eps: float) -> tuple[Tensor, Tensor]:
+    """q [B,N,H,D] and k [B,N,KH,D], normed by head and turned, packed."""
+    oq, ok = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k))
+    if not q.numel():
+        return oq, ok
+    h = _heads(q, k, q_weight, positions, axes, theta, eps, False)
+    check(lib().sihc_qk_norm_rotary(ctypes.byref(h), q.data_ptr(), k.data_ptr(), q_weight.data_ptr(),
+                                    k_weight.data_ptr(), positions.data_ptr(), oq.data_ptr(), ok.data_ptr(),
+                                    _stream(q.device)))
+    return oq, ok
+
+
+@_on_tensor_device
+def qk_norm_rotary_backward(grad_q: Tensor, grad_k: Tensor, q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor,
+                            positions: Tensor, axes: Sequence[int], theta: float,
+                            eps: float) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """(q, k, q_weight, k_weight gradients) of qk_norm_rotary, packed."""
+    dq, dk = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k))
+    if not q.numel():
+        return dq, dk, torch.zeros_like(q_weight), torch.zeros_like(k_weight)
+    dqw, dkw = torch.empty_like(q_weight), torch.empty_like(k_weight)
+    L, h = lib(), _heads(q, k, q_weight, positions, axes, theta, eps, False)
+    ws = _workspace(L.sihc_qk_norm_rotary_backward_workspace_size(ctypes.byref(h)), q.device)
+    check(L.sihc_qk_norm_rotary_backward(ctypes.byref(h), grad_q.data_ptr(), grad_k.data_ptr(), q.data_ptr(),
+                                         k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(),
+                                         positions.data_ptr(), dq.data_ptr(), dk.data_ptr(), dqw.data_ptr(), dkw.data_ptr(),
+                                         ws.data_ptr(), ws.numel() * 4, _stream(q.device)))
+    return dq, dk, dqw, dkw
+
+
+@_on_tensor_device
+def axis_rotary(x: Tensor, positions: Tensor, axes: Sequence[int], theta: float, inverse: bool) -> Tensor:
+    """x [B,N,H,D] turned by its positions, or back, packed."""
+    out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    h = _heads(x, None, None, positions, axes, theta, 0.0, inverse)
+    check(lib().sihc_qk_norm_rotary(ctypes.byref(h), x.data_ptr(), None, None, None, positions.data_ptr(),
+                                    out.data_ptr(), None, _stream(x.device)))
+    return out
+
+
+@_on_tensor_device
+def dropout(x: Tensor, p: float, seed: Tensor, stream: int, residual: Optional[Tensor]) -> Tensor:
+    """residual + x / (1 - p) where the mask of (seed, stream) keeps an element."""
+    out = torch.empty_like(x)
+    check(lib().sihc_dropout(x.data_ptr(), _ptr(residual), out.data_ptr(), x.numel(), p, seed.data_ptr(), stream,
+                             dtype_code(x.dtype), _stream(x.device)))
+    return out
+
+
 __all__ = [
-    "MAX_EVENTS", "ACTIVATIONS", "embedding", "embedding_backward", "group_norm", "group_norm_backward",
+    "MAX_EVENTS", "ACTIVATIONS", "LINEAR_ACTIVATIONS", "linear_act", "linear_act_backward", "qk_norm_rotary",
+    "qk_norm_rotary_backward", "axis_rotary", "dropout", "embedding", "embedding_backward", "group_norm", "group_norm_backward",
     "cross_attention", "cross_attention_backward", "dtype_code", "carrier_geometry", "read", "write", "weight_grad", "read_backward",
     "write_backward", "triangular",
     "triangular_gamma_grad", "triangular_backward", "event_forward", "event_backward", "gather_cells",
