@@ -394,17 +394,20 @@ Args args_of(const sihc_heads* h) {
   a.w_f32 = h->w_dtype == SIHC_DTYPE_F32;
   a.eps = h->eps;
   a.sign = h->inverse ? -1.f : 1.f;
-  int pair = 0;
-  for (int i = 0; i < h->axes; ++i)
-    for (int c = 0; c < h->widths[i]; c += 2, ++pair) {
-      a.rate[pair] = std::pow(h->theta, -double(c) / double(h->widths[i])) / 6.283185307179586476925;
-      a.axis[pair] = uint8_t(i);
-    }
-  a.turned = pair;
+  for (int i = 0; i < h->axes; ++i) a.turned += h->widths[i] / 2;
   // Tokens of a wave: one where a token's heads fill 4 passes, else as many as do.
   const int sub = 64 / lanes_of(h->dim), heads = h->heads + h->kv_heads;
   a.group = std::max(1, std::min(MAX_GROUP, 4 * sub / heads));
   return a;
+}
+void take_rates(const sihc_heads* h, Args& a) {
+  const double log = std::log2(h->theta);
+  int pair = 0;
+  for (int i = 0; i < h->axes; ++i)
+    for (int c = 0; c < h->widths[i]; c += 2, ++pair) {
+      a.rate[pair] = std::exp2(-double(c) / double(h->widths[i]) * log) / 6.283185307179586476925;
+      a.axis[pair] = uint8_t(i);
+    }
 }
 template <typename F>
 int by_lanes(int lanes, F&& f) {
@@ -428,6 +431,7 @@ extern "C" int sihc_qk_norm_rotary(const sihc_heads* h, const void* q, const voi
   if (const int rc = check(h, k, q_weight, k_weight, "qk_norm_rotary")) return rc;
   Args a = args_of(h);
   if (a.total == 0) return SIHC_OK;
+  take_rates(h, a);
   if (!q || !q_out || (k && !k_out) || (a.turned && !positions))
     return fail(SIHC_ERR_INVALID, "qk_norm_rotary: null pointer");
   a.x[0] = q;
@@ -471,6 +475,7 @@ extern "C" int sihc_qk_norm_rotary_backward(const sihc_heads* h, const void* gra
                                             size_t workspace_bytes, void* stream) {
   if (const int rc = check(h, k, q_weight, k_weight, "qk_norm_rotary_backward")) return rc;
   Args a = args_of(h);
+  take_rates(h, a);
   if (!q_weight || !dq_weight || (k && !dk_weight))
     return fail(SIHC_ERR_INVALID, "qk_norm_rotary_backward: the weights and their gradients are needed");
   if (a.total && (!q || !grad_q || !dq || (k && (!grad_k || !dk)) || (a.turned && !positions) || !workspace))

@@ -1,7 +1,7 @@
 // Native dispatch of the eager `sihc::` ops.
 //
 // The Python custom ops (sihc_hip/sublayer_kernels.py, event_ops.py, indexed.py, kernels.py,
-// conditioning.py) cost 50-150 us of interpreter and dispatcher time per forward and backward pair,
+// conditioning.py, body.py) cost 50-150 us of interpreter and dispatcher time per forward and backward pair,
 // more than the kernels of a small or ordinary call take. Each function here takes the arguments of one
 // of those ops and, where the call is plain, allocates the outputs, enqueues the C-ABI call on
 // the current stream and records one C++ autograd node whose backward does the same.
@@ -33,6 +33,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <optional>
 #include <string>
@@ -195,6 +196,65 @@ bool attention_fits(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
     return false;
   return !lengths.defined() || (plain(lengths) && lengths.scalar_type() == at::kInt && lengths.dim() == 1 &&
                                 lengths.size(0) == q.size(0) && lengths.device() == q.device());
+}
+// Absent operands are undefined tensors here.
+bool linear_fits(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& gate, const Tensor& residual,
+                 int act) {
+  if (!plain(x) || !plain(weight) || x.dim() < 2 || weight.dim() != 2 || x.numel() == 0 || weight.numel() == 0 ||
+      dtype_code(x) < 0 || x.size(-1) != weight.size(1) || weight.size(0) > (1 << 24) || weight.size(1) > (1 << 24) ||
+      x.numel() / x.size(-1) > (1 << 30) || (act == SIHC_ACT_SWIGLU && weight.size(0) % 2))
+    return false;
+  const int64_t outer = act == SIHC_ACT_SWIGLU ? weight.size(0) / 2 : weight.size(0);
+  for (const Tensor* t : {&weight, &bias, &gate, &residual})
+    if (t->defined() && (!plain_strided(*t) || t->scalar_type() != x.scalar_type() || t->device() != x.device()))
+      return false;
+  if (bias.defined() && (!bias.is_contiguous() || bias.dim() != 1 || bias.size(0) != weight.size(0))) return false;
+  if (gate.defined() && (gate.dim() != 2 || gate.size(0) != x.size(0) || gate.size(1) != outer ||
+                         (outer > 1 && gate.stride(1) != 1)))
+    return false;
+  return !residual.defined() ||
+         (residual.is_contiguous() && residual.dim() == x.dim() && residual.size(-1) == outer &&
+          residual.sizes().slice(0, size_t(x.dim()) - 1).equals(x.sizes().slice(0, size_t(x.dim()) - 1)));
+}
+// (k: undefined where x is turned alone)
+bool heads_fit(const Tensor& q, const Tensor& k, const Tensor& positions, const std::vector<int64_t>& axes,
+               double theta) {
+  for (const Tensor* t : {&q, &k}) {
+    if (t == &k && !k.defined()) continue;
+    if (!plain_strided(*t) || t->dim() != 4 || t->numel() == 0 || t->scalar_type() != q.scalar_type() ||
+        t->device() != q.device() || t->size(0) != q.size(0) || t->size(1) != q.size(1) || t->size(3) != q.size(3) ||
+        t->size(2) > (1 << 20) || (t->size(3) > 1 && t->stride(3) != 1))
+      return false;
+  }
+  int64_t sum = 0;
+  for (const int64_t w : axes) {
+    if (w < 0 || w % 2 || w > SIHC_MAX_ROTARY_DIM) return false;
+    sum += w;
+  }
+  if (dtype_code(q) < 0 || q.size(3) > SIHC_MAX_ROTARY_DIM || axes.size() > SIHC_MAX_AXES || sum > q.size(3) ||
+      q.size(0) * q.size(1) > (int64_t(1) << 31) - 64 || !(theta > 0.0) || !std::isfinite(theta))
+    return false;
+  if (!plain(positions) || positions.device() != q.device() ||
+      (positions.scalar_type() != at::kInt && positions.scalar_type() != at::kFloat))
+    return false;
+  const int64_t n = positions.dim(), count = int64_t(axes.size());
+  return (n == 2 && positions.size(0) == q.size(1) && positions.size(1) == count) ||
+         (n == 3 && positions.size(0) == q.size(0) && positions.size(1) == q.size(1) && positions.size(2) == count);
+}
+bool qk_fits(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw, const Tensor& positions,
+             const std::vector<int64_t>& axes, double theta, double eps) {
+  if (!k.defined() || !heads_fit(q, k, positions, axes, theta) || !(eps >= 0.0) || !std::isfinite(eps)) return false;
+  for (const Tensor* w : {&qw, &kw})
+    if (!plain(*w) || w->dim() != 1 || w->size(0) != q.size(3) || w->device() != q.device() ||
+        w->scalar_type() != qw.scalar_type())
+      return false;
+  return qw.scalar_type() == q.scalar_type() || qw.scalar_type() == at::kFloat;
+}
+bool dropout_fits(const Tensor& x, double p, const Tensor& seed, int64_t stream, const Tensor& residual) {
+  return plain(x) && x.numel() != 0 && dtype_code(x) >= 0 && p >= 0.0 && p < 1.0 && plain(seed) &&
+         seed.scalar_type() == at::kLong && seed.numel() == 1 && seed.device() == x.device() && stream >= 0 &&
+         (!residual.defined() || (plain(residual) && residual.sizes().equals(x.sizes()) &&
+                                  residual.scalar_type() == x.scalar_type() && residual.device() == x.device()));
 }
 // `t` is a packed tensor like `like` (an output gradient, a saved output).
 bool same(const Tensor& t, const Tensor& like) {
@@ -794,6 +854,276 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
   }
 };
 
+// ------------------------------------------------------------------------- body operators
+const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+const char* act_name(int act) {
+  return act == SIHC_ACT_SWIGLU ? "swiglu" : act == SIHC_ACT_SILU ? "silu" : "none";
+}
+sihc_linear linear_of(const Tensor& x, const Tensor& weight, const Tensor& gate, int act) {
+  sihc_linear l{};
+  l.rows = x.numel() / x.size(-1);
+  l.inner = int(x.size(-1));
+  l.outer = int(act == SIHC_ACT_SWIGLU ? weight.size(0) / 2 : weight.size(0));
+  l.act = act;
+  l.dtype = dtype_code(x);
+  l.rows_per_gate = gate.defined() ? l.rows / x.size(0) : l.rows;
+  l.gate_stride = gate.defined() ? gate.stride(0) : 0;
+  return l;
+}
+bool keeps(const Tensor& gate, int act) { return act != SIHC_ACT_NONE || gate.defined(); }
+bool keeps_low(const Tensor& x, int act) { return act != SIHC_ACT_NONE && x.scalar_type() == at::kBFloat16; }
+// (result, h and its next bits for the backward: empty unless `train`)
+variable_list run_linear(const Tensor& x, const Tensor& weight, const Tensor& bias, int act, const Tensor& gate,
+                         const Tensor& residual, bool train) {
+  const c10::DeviceGuard guard(x.device());
+  const sihc_linear l = linear_of(x, weight, gate, act);
+  std::vector<int64_t> sizes(x.sizes().begin(), x.sizes().end()), none{0};
+  sizes.back() = l.outer;
+  Tensor y = at::empty(sizes, x.options()), ws;
+  sizes.back() = weight.size(0);
+  const bool h_kept = train && keeps(gate, act), low_kept = train && keeps_low(x, act);
+  Tensor h = at::empty(h_kept ? sizes : none, x.options());
+  Tensor low = at::empty(low_kept ? sizes : none, x.options().dtype(at::kByte));
+  const size_t bytes = sihc_linear_act_workspace_size(&l);
+  if (bytes) ws = workspace(bytes, x);
+  check(sihc_linear_act(&l, x.const_data_ptr(), weight.const_data_ptr(), ptr(bias), ptr(gate), ptr(residual),
+                        y.data_ptr(), h_kept ? h.data_ptr() : nullptr, low_kept ? low.data_ptr<uint8_t>() : nullptr,
+                        bytes ? ws.data_ptr() : nullptr, bytes, stream_of(x)),
+        true);
+  return {y, h, low};
+}
+struct LinearFn : torch::autograd::Function<LinearFn> {
+  static constexpr bool is_traceable = true;
+  // rest: h and its next bits (NormFn's pointer)
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias,
+                        int64_t act, const std::optional<Tensor>& gate, const std::optional<Tensor>& residual,
+                        variable_list* rest) {
+    const Tensor g = gate.value_or(Tensor());
+    variable_list out = run_linear(x, weight, bias.value_or(Tensor()), int(act), g, residual.value_or(Tensor()), true);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, weight, g, out[1], out[2]});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["given"] = int64_t(bias.has_value()) + 2 * int64_t(residual.has_value());
+    *rest = {out[1], out[2]};
+    return out[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &weight = saved[1], &gate = saved[2], &h = saved[3], &low = saved[4];
+    if (!grads[0].defined()) return variable_list(7);
+    const int act = int(ctx->saved_data["act"].toInt());
+    const int64_t given = ctx->saved_data["given"].toInt();
+    size_t edge = 2;  // an edge for every tensor that was given
+    const bool has_bias = given & 1, has_gate = gate.defined(), has_residual = given & 2;
+    const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+    const bool want_b = has_bias && ctx->needs_input_grad(edge);
+    edge += has_bias;
+    const bool want_g = has_gate && ctx->needs_input_grad(edge);
+    edge += has_gate;
+    variable_list out(7);
+    if (has_residual && ctx->needs_input_grad(edge)) out[5] = grads[0];
+    if (!(want_x || want_w || want_b || want_g)) return out;
+    const Tensor grad = grads[0].contiguous();
+    Tensor dx, dw, db, dg;
+    bool fits = direct() && linear_fits(x, weight, Tensor(), gate, Tensor(), act) && plain(grad) &&
+                grad.scalar_type() == x.scalar_type() && grad.device() == x.device();
+    if (fits) {
+      std::vector<int64_t> sizes(x.sizes().begin(), x.sizes().end());
+      sizes.back() = weight.size(0);
+      fits = (!keeps(gate, act) || (plain(h) && h.sizes().equals(sizes) && h.scalar_type() == x.scalar_type() &&
+                                    h.device() == x.device())) &&
+             (!keeps_low(x, act) || (plain(low) && low.sizes().equals(sizes) && low.scalar_type() == at::kByte &&
+                                     low.device() == x.device()));
+      if (act == SIHC_ACT_SWIGLU) sizes.back() /= 2;
+      fits = fits && grad.sizes().equals(sizes);
+    }
+    if (fits) {
+      RECORD_FUNCTION("sihc::linear_act_backward", (Args{grad, x, weight, h, low, maybe(gate), act_name(act)}));
+      const c10::DeviceGuard device(x.device());
+      const sihc_linear l = linear_of(x, weight, gate, act);
+      if (want_x) dx = at::empty_like(x);
+      if (want_w) dw = at::empty_like(weight);
+      if (want_b) db = at::empty({weight.size(0)}, weight.options());
+      if (want_g) dg = at::empty({x.size(0), l.outer}, x.options());
+      const Tensor ws = workspace(sihc_linear_act_backward_workspace_size(&l, has_gate), x);
+      auto out_ptr = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+      check(sihc_linear_act_backward(&l, grad.const_data_ptr(), x.const_data_ptr(), weight.const_data_ptr(),
+                                     keeps(gate, act) ? h.const_data_ptr() : nullptr,
+                                     keeps_low(x, act) ? low.const_data_ptr<uint8_t>() : nullptr, ptr(gate),
+                                     out_ptr(dx), out_ptr(dw), out_ptr(db), out_ptr(dg), ws.data_ptr(),
+                                     size_t(ws.numel()) * 4, stream_of(x)),
+            false);
+    } else {
+      static auto op = registered<std::tuple<Tensor, Tensor, Tensor, Tensor>(
+          const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const std::optional<Tensor>&,
+          c10::string_view, bool, bool, bool, bool)>("sihc::linear_act_backward");
+      std::tie(dx, dw, db, dg) =
+          op.call(grad, x, weight, h, low, maybe(gate), act_name(act), want_x, want_w, want_b, want_g);
+    }
+    if (want_x) out[0] = dx;
+    if (want_w) out[1] = dw;
+    if (want_b) out[2] = db;
+    if (want_g) out[4] = dg;
+    return out;
+  }
+};
+
+using Axes = std::vector<int64_t>;
+sihc_heads heads_of(const Tensor& q, const Tensor& k, const Tensor& weight, const Tensor& positions, const Axes& axes,
+                    double theta, double eps, bool inverse) {
+  sihc_heads h{};
+  h.batch = q.size(0);
+  h.tokens = q.size(1);
+  h.heads = int(q.size(2));
+  h.kv_heads = k.defined() ? int(k.size(2)) : 0;
+  h.dim = int(q.size(3));
+  h.axes = int(axes.size());
+  for (size_t i = 0; i < axes.size(); ++i) h.widths[i] = int(axes[i]);
+  for (int i = 0; i < 3; ++i) {
+    h.q_stride[i] = q.stride(i);
+    h.k_stride[i] = k.defined() ? k.stride(i) : 0;
+  }
+  h.position_batch_stride = positions.dim() == 3 ? q.size(1) : 0;
+  h.theta = theta;
+  h.eps = float(eps);
+  h.dtype = dtype_code(q);
+  h.w_dtype = weight.defined() ? dtype_code(weight) : h.dtype;
+  h.position_dtype = positions.scalar_type() == at::kFloat ? SIHC_POSITION_F32 : SIHC_POSITION_I32;
+  h.inverse = inverse;
+  return h;
+}
+variable_list run_qk(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw, const Tensor& positions,
+                     const Axes& axes, double theta, double eps) {
+  const c10::DeviceGuard guard(q.device());
+  const sihc_heads h = heads_of(q, k, qw, positions, axes, theta, eps, false);
+  Tensor oq = at::empty(q.sizes(), q.options()), ok = at::empty(k.sizes(), k.options());
+  check(sihc_qk_norm_rotary(&h, q.const_data_ptr(), k.const_data_ptr(), qw.const_data_ptr(), kw.const_data_ptr(),
+                            positions.const_data_ptr(), oq.data_ptr(), ok.data_ptr(), stream_of(q)),
+        true);
+  return {oq, ok};
+}
+struct QkFn : torch::autograd::Function<QkFn> {
+  static constexpr bool is_traceable = true;
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& qw,
+                               const Tensor& kw, const Tensor& positions, const Axes& axes, double theta, double eps) {
+    ctx->save_for_backward({q, k, qw, kw, positions});
+    ctx->saved_data["axes"] = axes;
+    ctx->saved_data["theta"] = theta;
+    ctx->saved_data["eps"] = eps;
+    return run_qk(q, k, qw, kw, positions, axes, theta, eps);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &qw = saved[2], &kw = saved[3], &positions = saved[4];
+    const Axes axes = ctx->saved_data["axes"].toIntVector();
+    const double theta = ctx->saved_data["theta"].toDouble(), eps = ctx->saved_data["eps"].toDouble();
+    const Tensor gq = grads[0].contiguous(), gk = grads[1].contiguous();
+    auto fits = [](const Tensor& g, const Tensor& x) {
+      return plain(g) && g.sizes().equals(x.sizes()) && g.scalar_type() == x.scalar_type() && g.device() == x.device();
+    };
+    Tensor dq, dk, dqw, dkw;
+    if (direct() && qk_fits(q, k, qw, kw, positions, axes, theta, eps) && fits(gq, q) && fits(gk, k)) {
+      RECORD_FUNCTION("sihc::qk_norm_rotary_backward", (Args{gq, gk, q, k, qw, kw, positions, axes, theta, eps}));
+      const c10::DeviceGuard device(q.device());
+      const sihc_heads h = heads_of(q, k, qw, positions, axes, theta, eps, false);
+      dq = at::empty(q.sizes(), q.options());
+      dk = at::empty(k.sizes(), k.options());
+      dqw = at::empty_like(qw);
+      dkw = at::empty_like(kw);
+      const Tensor ws = workspace(sihc_qk_norm_rotary_backward_workspace_size(&h), q);
+      check(sihc_qk_norm_rotary_backward(&h, gq.const_data_ptr(), gk.const_data_ptr(), q.const_data_ptr(),
+                                         k.const_data_ptr(), qw.const_data_ptr(), kw.const_data_ptr(),
+                                         positions.const_data_ptr(), dq.data_ptr(), dk.data_ptr(), dqw.data_ptr(),
+                                         dkw.data_ptr(), ws.data_ptr(), size_t(ws.numel()) * 4, stream_of(q)),
+            false);
+    } else {
+      static auto op = registered<std::tuple<Tensor, Tensor, Tensor, Tensor>(
+          const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+          at::IntArrayRef, double, double)>("sihc::qk_norm_rotary_backward");
+      std::tie(dq, dk, dqw, dkw) = op.call(gq, gk, q, k, qw, kw, positions, axes, theta, eps);
+    }
+    return {dq, dk, dqw, dkw, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor run_rotary(const Tensor& x, const Tensor& positions, const Axes& axes, double theta, bool inverse,
+                  bool forward) {
+  const c10::DeviceGuard guard(x.device());
+  const sihc_heads h = heads_of(x, Tensor(), Tensor(), positions, axes, theta, 0.0, inverse);
+  Tensor y = at::empty(x.sizes(), x.options());
+  check(sihc_qk_norm_rotary(&h, x.const_data_ptr(), nullptr, nullptr, nullptr, positions.const_data_ptr(),
+                            y.data_ptr(), nullptr, stream_of(x)),
+        forward);
+  return y;
+}
+struct RotaryFn : torch::autograd::Function<RotaryFn> {
+  static constexpr bool is_traceable = true;
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& positions, const Axes& axes, double theta,
+                        bool inverse) {
+    ctx->save_for_backward({positions});
+    ctx->saved_data["axes"] = axes;
+    ctx->saved_data["theta"] = theta;
+    ctx->saved_data["inverse"] = inverse;
+    return run_rotary(x, positions, axes, theta, inverse, true);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor positions = ctx->get_saved_variables()[0], grad = grads[0].contiguous();
+    const Axes axes = ctx->saved_data["axes"].toIntVector();
+    const double theta = ctx->saved_data["theta"].toDouble();
+    const bool inverse = !ctx->saved_data["inverse"].toBool();
+    Tensor dx;
+    if (direct() && heads_fit(grad, Tensor(), positions, axes, theta)) {
+      RECORD_FUNCTION("sihc::axis_rotary", (Args{grad, positions, axes, theta, inverse}));
+      dx = run_rotary(grad, positions, axes, theta, inverse, false);
+    } else {
+      static auto op = registered<Tensor(const Tensor&, const Tensor&, at::IntArrayRef, double, bool)>(
+          "sihc::axis_rotary");
+      dx = op.call(grad, positions, axes, theta, inverse);
+    }
+    return {dx, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor run_dropout(const Tensor& x, double p, const Tensor& seed, int64_t stream, const Tensor& residual,
+                   bool forward) {
+  const c10::DeviceGuard guard(x.device());
+  Tensor y = at::empty_like(x);
+  check(sihc_dropout(x.const_data_ptr(), ptr(residual), y.data_ptr(), x.numel(), p, seed.const_data_ptr<int64_t>(),
+                     stream, dtype_code(x), stream_of(x)),
+        forward);
+  return y;
+}
+struct DropoutFn : torch::autograd::Function<DropoutFn> {
+  static constexpr bool is_traceable = true;
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, double p, const Tensor& seed, int64_t stream,
+                        const std::optional<Tensor>& residual) {
+    ctx->save_for_backward({seed});
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["stream"] = stream;
+    ctx->saved_data["added"] = residual.has_value();
+    return run_dropout(x, p, seed, stream, residual.value_or(Tensor()), true);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor seed = ctx->get_saved_variables()[0];
+    const double p = ctx->saved_data["p"].toDouble();
+    const int64_t stream = ctx->saved_data["stream"].toInt();
+    variable_list out(5);
+    // (edges: x, the seed, the residual)
+    if (ctx->saved_data["added"].toBool() && ctx->needs_input_grad(2)) out[4] = grads[0];
+    if (!ctx->needs_input_grad(0)) return out;
+    const Tensor grad = grads[0].contiguous();
+    if (direct() && dropout_fits(grad, p, seed, stream, Tensor())) {
+      RECORD_FUNCTION("sihc::dropout", (Args{grad, p, seed, stream}));
+      out[0] = run_dropout(grad, p, seed, stream, Tensor(), false);
+    } else {
+      static auto op = registered<Tensor(const Tensor&, double, const Tensor&, int64_t, const std::optional<Tensor>&)>(
+          "sihc::dropout");
+      out[0] = op.call(grad, p, seed, stream, std::nullopt);
+    }
+    return out;
+  }
+};
+
 // ------------------------------------------------------------------------ Python entries
 PyObject* to_list(const variable_list& ts) {
   PyObject* out = PyList_New(Py_ssize_t(ts.size()));
@@ -1040,6 +1370,89 @@ PyObject* py_attention(PyObject* self, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
+bool unwrap_maybe(PyObject* o, Tensor& t) { return o == Py_None || unwrap(o, t); }
+bool unwrap_axes(PyObject* o, Axes& axes) {
+  if (!PyList_CheckExact(o) && !PyTuple_CheckExact(o)) return false;
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(o);
+  axes.resize(size_t(n));
+  for (Py_ssize_t i = 0; i < n; ++i)
+    if (!unwrap_integer(PySequence_Fast_GET_ITEM(o, i), axes[size_t(i)])) return false;
+  return true;
+}
+PyObject* py_linear(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  if (n != 7 || !PyUnicode_CheckExact(args[3]) || !PyBool_Check(args[6])) return not_implemented();
+  int act = -1;
+  for (const int a : {int(SIHC_ACT_NONE), int(SIHC_ACT_SILU), int(SIHC_ACT_SWIGLU)})
+    if (PyUnicode_CompareWithASCIIString(args[3], act_name(a)) == 0) act = a;
+  if (act < 0) return not_implemented();
+  const bool train = args[6] == Py_True;
+  return guarded(self, [&]() -> PyObject* {
+    Tensor x, weight, bias, gate, residual;
+    if (!unwrap(args[0], x) || !unwrap(args[1], weight) || !unwrap_maybe(args[2], bias) ||
+        !unwrap_maybe(args[4], gate) || !unwrap_maybe(args[5], residual) ||
+        !linear_fits(x, weight, bias, gate, residual, act))
+      return not_implemented();
+    auto listing = [&] {
+      return Args{x, weight, maybe(bias), act_name(act), maybe(gate), maybe(residual), train};
+    };
+    return tuple_of(call(self, listing, [&] {
+      if (unrecorded() || !train) return run_linear(x, weight, bias, act, gate, residual, train);
+      variable_list rest;
+      const Tensor out =
+          LinearFn::apply(x, weight, maybe(bias), int64_t(act), maybe(gate), maybe(residual), &rest);
+      return variable_list{out, rest[0], rest[1]};
+    }));
+  });
+}
+PyObject* py_qk(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  if (n != 8) return not_implemented();
+  return guarded(self, [&]() -> PyObject* {
+    Tensor q, k, qw, kw, positions;
+    Axes axes;
+    double theta, eps;
+    if (!unwrap(args[0], q) || !unwrap(args[1], k) || !unwrap(args[2], qw) || !unwrap(args[3], kw) ||
+        !unwrap(args[4], positions) || !unwrap_axes(args[5], axes) || !unwrap_number(args[6], theta) ||
+        !unwrap_number(args[7], eps) || !qk_fits(q, k, qw, kw, positions, axes, theta, eps))
+      return not_implemented();
+    return tuple_of(call(self, [&] { return Args{q, k, qw, kw, positions, axes, theta, eps}; }, [&] {
+      return unrecorded() ? run_qk(q, k, qw, kw, positions, axes, theta, eps)
+                          : QkFn::apply(q, k, qw, kw, positions, axes, theta, eps);
+    }));
+  });
+}
+PyObject* py_rotary(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  if (n != 5 || !PyBool_Check(args[4])) return not_implemented();
+  const bool inverse = args[4] == Py_True;
+  return guarded(self, [&]() -> PyObject* {
+    Tensor x, positions;
+    Axes axes;
+    double theta;
+    if (!unwrap(args[0], x) || !unwrap(args[1], positions) || !unwrap_axes(args[2], axes) ||
+        !unwrap_number(args[3], theta) || !heads_fit(x, Tensor(), positions, axes, theta))
+      return not_implemented();
+    return THPVariable_Wrap(call(self, [&] { return Args{x, positions, axes, theta, inverse}; }, [&] {
+      return unrecorded() ? run_rotary(x, positions, axes, theta, inverse, true)
+                          : RotaryFn::apply(x, positions, axes, theta, inverse);
+    }));
+  });
+}
+PyObject* py_dropout(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  if (n != 5) return not_implemented();
+  return guarded(self, [&]() -> PyObject* {
+    Tensor x, seed, residual;
+    double p;
+    int64_t stream;
+    if (!unwrap(args[0], x) || !unwrap_number(args[1], p) || !unwrap(args[2], seed) ||
+        !unwrap_integer(args[3], stream) || !unwrap_maybe(args[4], residual) ||
+        !dropout_fits(x, p, seed, stream, residual))
+      return not_implemented();
+    return THPVariable_Wrap(call(self, [&] { return Args{x, p, seed, stream, maybe(residual)}; }, [&] {
+      return unrecorded() ? run_dropout(x, p, seed, stream, residual, true)
+                          : DropoutFn::apply(x, p, seed, stream, maybe(residual));
+    }));
+  });
+}
+
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyMethodDef define(const char* name) {
   return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F)), METH_FASTCALL, nullptr};
@@ -1051,6 +1464,8 @@ PyMethodDef entries[] = {
     define<py_block_write>("block_write"),   define<py_gather>("gather_cells"),
     define<py_scatter>("scatter_cells"),     define<py_embed>("embedding_lookup"),
     define<py_norm>("group_norm_act"),       define<py_attention>("cross_attention"),
+    define<py_linear>("linear_act"),         define<py_qk>("qk_norm_rotary"),
+    define<py_rotary>("axis_rotary"),        define<py_dropout>("dropout"),
 };
 // entry(name, op): the native entry `name` for the registered op `op` ("namespace::name")
 PyObject* py_entry(PyObject*, PyObject* args) {

@@ -111,9 +111,9 @@ PROTOTYPES: dict[str, tuple] = {
     "sihc_cross_attention_backward": (_i32, [_attp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                              _sz, _vp]),
     "sihc_linear_act_workspace_size": (_sz, [_linp]),
-    "sihc_linear_act": (_i32, [_linp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "sihc_linear_act": (_i32, [_linp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "sihc_linear_act_backward_workspace_size": (_sz, [_linp, _i32]),
-    "sihc_linear_act_backward": (_i32, [_linp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "sihc_linear_act_backward": (_i32, [_linp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "sihc_qk_norm_rotary": (_i32, [_headsp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "sihc_qk_norm_rotary_backward_workspace_size": (_sz, [_headsp]),
     "sihc_qk_norm_rotary_backward": (_i32, [_headsp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,

@@ -23,7 +23,8 @@ Specification (the reference's bodies are plain PyTorch, sihc/models/sihc/compon
 
 All sums and statistics are fp32, in a fixed order without atomics: identical inputs give identical
 bits. float32 and bfloat16; the norm's weights may be float32 beside bfloat16 heads. In bfloat16 the
-backward of an activation or a gate works on h and its gradient rounded to bfloat16. q, k and x of the
+backward of a gate works on h rounded to bfloat16, that of an activation on 24 bits of it, and the
+gradient of h enters the products rounded to bfloat16. q, k and x of the
 rotations are read through their strides (the channels of a head adjacent); the other tensors are packed.
 """
 from __future__ import annotations
@@ -37,6 +38,7 @@ from torch.library import custom_op, register_autograd
 
 from . import launch
 from ._lib import MAX_AXES, MAX_ROTARY_DIM
+from ._native import native
 from .conditioning import _TYPES, _require_gpu
 from .sublayer_kernels import _require_packed
 
@@ -87,7 +89,7 @@ def _check_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str, g
 
 @custom_op("sihc::linear_act", mutates_args=())
 def _linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str, gate: Optional[Tensor],
-                residual: Optional[Tensor], train: bool) -> tuple[Tensor, Tensor]:
+                residual: Optional[Tensor], train: bool) -> tuple[Tensor, Tensor, Tensor]:
     _check_linear(x, weight, bias, act, gate, residual)
     return launch.linear_act(x, weight, bias, act, gate, residual, train)
 
@@ -95,29 +97,32 @@ def _linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str, gat
 @_linear_act.register_fake
 def _linear_act_fake(x, weight, bias, act, gate, residual, train):
     keeps = train and (act != "none" or gate is not None)
-    return (x.new_empty((*x.shape[:-1], _linear_outer(weight, act))),
-            x.new_empty((*x.shape[:-1], weight.shape[0]) if keeps else (0,)))
+    wide = (*x.shape[:-1], weight.shape[0])
+    return (x.new_empty((*x.shape[:-1], _linear_outer(weight, act))), x.new_empty(wide if keeps else (0,)),
+            x.new_empty(wide if launch.keeps_low(x.dtype, act, train) else (0,), dtype=torch.uint8))
 
 
 @custom_op("sihc::linear_act_backward", mutates_args=())
-def _linear_act_backward(grad: Tensor, x: Tensor, weight: Tensor, h: Tensor, gate: Optional[Tensor], act: str,
-                         want_x: bool, want_weight: bool, want_bias: bool,
+def _linear_act_backward(grad: Tensor, x: Tensor, weight: Tensor, h: Tensor, low: Tensor, gate: Optional[Tensor],
+                         act: str, want_x: bool, want_weight: bool, want_bias: bool,
                          want_gate: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     _check_linear(x, weight, None, act, gate, None)  # saved tensors come back through the caller's hooks
-    _require_packed("linear_act backward", grad=grad, h=h)
+    _require_packed("linear_act backward", grad=grad, h=h, low=low)
     if grad.shape != (*x.shape[:-1], _linear_outer(weight, act)) or grad.dtype != x.dtype:
         raise ValueError("linear_act backward: the output gradient must match the output")
     if act != "none" or gate is not None:
         if h.shape != (*x.shape[:-1], weight.shape[0]) or h.dtype != x.dtype:
             raise ValueError("linear_act backward: h must be that of a call with train=True")
+    if launch.keeps_low(x.dtype, act, True) and (low.shape != h.shape or low.dtype != torch.uint8):
+        raise ValueError("linear_act backward: low must be that of a call with train=True")
     if want_gate and gate is None:
         raise ValueError("linear_act backward: no gate, no gradient of it")
-    _require_gpu("linear_act backward", x, grad=grad, h=h)
-    return launch.linear_act_backward(grad, x, weight, h, gate, act, want_x, want_weight, want_bias, want_gate)
+    _require_gpu("linear_act backward", x, grad=grad, h=h, low=low)
+    return launch.linear_act_backward(grad, x, weight, h, low, gate, act, want_x, want_weight, want_bias, want_gate)
 
 
 @_linear_act_backward.register_fake
-def _linear_act_backward_fake(grad, x, weight, h, gate, act, want_x, want_weight, want_bias, want_gate):
+def _linear_act_backward_fake(grad, x, weight, h, low, gate, act, want_x, want_weight, want_bias, want_gate):
     return (x.new_empty(x.shape if want_x else (0,)), x.new_empty(weight.shape if want_weight else (0,)),
             x.new_empty(weight.shape[:1] if want_bias else (0,)),
             x.new_empty((x.shape[0], _linear_outer(weight, act)) if want_gate else (0,)))
@@ -125,24 +130,25 @@ def _linear_act_backward_fake(grad, x, weight, h, gate, act, want_x, want_weight
 
 def _linear_setup(ctx, inputs, output):
     x, weight, bias, ctx.act, gate, residual, _ = inputs
-    ctx.mark_non_differentiable(output[1])
+    ctx.mark_non_differentiable(output[1], output[2])
     ctx.set_materialize_grads(False)
-    ctx.save_for_backward(x, weight, gate, output[1])
+    ctx.save_for_backward(x, weight, gate, output[1], output[2])
 
 
-def _linear_autograd(ctx, grad, _):
+def _linear_autograd(ctx, grad, _, __):
     if grad is None:
         return (None,) * 7
-    x, weight, gate, h = ctx.saved_tensors
+    x, weight, gate, h, low = ctx.saved_tensors
     want = [ctx.needs_input_grad[i] for i in (0, 1, 2, 4)]
     if not any(want):
         return None, None, None, None, None, grad, None
-    grads = _linear_act_backward(grad.contiguous(), x, weight, h, gate, ctx.act, *want)
+    grads = _linear_act_backward(grad.contiguous(), x, weight, h, low, gate, ctx.act, *want)
     dx, dweight, dbias, dgate = (g if w else None for g, w in zip(grads, want))
     return dx, dweight, dbias, None, dgate, grad if ctx.needs_input_grad[5] else None, None
 
 
 register_autograd(_linear_act, _linear_autograd, setup_context=_linear_setup)
+native(_linear_act, "linear_act")
 
 
 def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: str = "none",
@@ -237,6 +243,7 @@ def _qk_autograd(ctx, grad_q, grad_k):
 
 
 register_autograd(_qk_norm_rotary, _qk_autograd, setup_context=_qk_setup)
+native(_qk_norm_rotary, "qk_norm_rotary")
 
 
 def qk_norm_rotary(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, positions: Tensor,
@@ -268,6 +275,7 @@ def _rotary_autograd(ctx, grad):
 
 
 register_autograd(_axis_rotary, _rotary_autograd, setup_context=_rotary_setup)
+native(_axis_rotary, "axis_rotary")
 
 
 def axis_rotary(x: Tensor, positions: Tensor, axes: Sequence[int], theta: float = 10000.0) -> Tensor:
@@ -315,6 +323,7 @@ def _dropout_autograd(ctx, grad):
 
 
 register_autograd(_dropout, _dropout_autograd, setup_context=_dropout_setup)
+native(_dropout, "dropout")
 
 
 def dropout(x: Tensor, p: float, seed: Tensor, stream: int = 0, residual: Optional[Tensor] = None) -> Tensor:

@@ -403,26 +403,34 @@ def _linear(x: Tensor, weight: Tensor, act: str, gate: Optional[Tensor]) -> Line
                   0 if gate is None else gate.stride(0))
 
 
+def keeps_low(dtype: torch.dtype, act: str, train: bool) -> bool:
+    """Whether linear_act keeps more bits of h than its type has: bfloat16 before an activation's slope."""
+    return train and act != "none" and dtype == torch.bfloat16
+
+
 @_on_tensor_device
 def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str, gate: Optional[Tensor],
-               residual: Optional[Tensor], train: bool) -> tuple[Tensor, Tensor]:
-    """(residual + gate * act(h) with h = x weight^T + bias, and for the backward h [..., weight rows]; empty
-    where the backward needs none or `train` is not set)."""
+               residual: Optional[Tensor], train: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """(residual + gate * act(h) with h = x weight^T + bias, and for the backward h [..., weight rows] and its
+    next 8 bits; empty where the backward needs none or `train` is not set)."""
     l = _linear(x, weight, act, gate)
     keeps = train and (act != "none" or gate is not None)
     out = torch.empty((*x.shape[:-1], l.outer), device=x.device, dtype=x.dtype)
-    h = torch.empty((*x.shape[:-1], weight.shape[0]) if keeps else (0,), device=x.device, dtype=x.dtype)
+    wide = (*x.shape[:-1], weight.shape[0])
+    h = torch.empty(wide if keeps else (0,), device=x.device, dtype=x.dtype)
+    low = torch.empty(wide if keeps_low(x.dtype, act, train) else (0,), device=x.device, dtype=torch.uint8)
     L = lib()
     nbytes = L.sihc_linear_act_workspace_size(ctypes.byref(l))
     ws = _workspace(nbytes, x.device) if nbytes else None
     check(L.sihc_linear_act(ctypes.byref(l), x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(gate), _ptr(residual),
-                            out.data_ptr(), h.data_ptr() if keeps else None, _ptr(ws), nbytes, _stream(x.device)))
-    return out, h
+                            out.data_ptr(), h.data_ptr() or None, low.data_ptr() or None, _ptr(ws), nbytes,
+                            _stream(x.device)))
+    return out, h, low
 
 
 @_on_tensor_device
-def linear_act_backward(grad: Tensor, x: Tensor, weight: Tensor, h: Tensor, gate: Optional[Tensor], act: str,
-                        want_x: bool, want_weight: bool, want_bias: bool,
+def linear_act_backward(grad: Tensor, x: Tensor, weight: Tensor, h: Tensor, low: Tensor, gate: Optional[Tensor],
+                        act: str, want_x: bool, want_weight: bool, want_bias: bool,
                         want_gate: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     """(input, weight, bias and gate gradients) of linear_act, those that are not wanted empty."""
     l = _linear(x, weight, act, gate)
@@ -435,7 +443,7 @@ def linear_act_backward(grad: Tensor, x: Tensor, weight: Tensor, h: Tensor, gate
     L = lib()
     ws = _workspace(L.sihc_linear_act_backward_workspace_size(ctypes.byref(l), int(gate is not None)), x.device)
     check(L.sihc_linear_act_backward(ctypes.byref(l), grad.data_ptr(), x.data_ptr(), weight.data_ptr(),
-                                     h.data_ptr() if h.numel() else None, _ptr(gate),
+                                     h.data_ptr() or None, low.data_ptr() or None, _ptr(gate),
                                      *(t.data_ptr() if wanted else None for t, wanted in
                                        ((dx, want_x), (dw, want_weight), (db, want_bias), (dg, want_gate))),
                                      ws.data_ptr(), ws.numel() * 4, _stream(x.device)))
