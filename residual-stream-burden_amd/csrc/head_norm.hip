@@ -20,7 +20,8 @@ namespace {
 using namespace sihc_cond;
 
 constexpr int V = 8;       // channels of a lane
-constexpr int UNROLL = 4;  // heads of a lane whose loads are in flight together
+constexpr int UNROLL = 4;   // heads of a lane whose loads are in flight together
+constexpr int BACKWARD = 2;  // (in the backward: two inputs each, and four waves a SIMD)
 constexpr int MAX_PAIRS = SIHC_MAX_ROTARY_DIM / 2;
 constexpr int MAX_GROUP = 8;  // tokens of a wave
 
@@ -34,6 +35,7 @@ struct Args {
   int dim, tokens, total, axes, turned, group;
   bool float_positions, w_f32;
   float eps, sign;
+  float share, least;  // 1 / dim; the smallest sum of squares that is taken as it is
   double rate[MAX_PAIRS];  // turns of a pair per position
   uint8_t axis[MAX_PAIRS];
 };
@@ -62,10 +64,13 @@ struct Chunk {  // a lane's 8 channels as they are in memory
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = to_f32(e[i]);
   }
+  // (past the caches: 75.6 us instead of 81.5 for 168 MB each way)
   __device__ __forceinline__ static void put(T* p, const float* v, int left) {
+    typedef u32x4 words __attribute__((aligned(2)));
     if (left >= V) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) store(p + i * (V / N), Vec<T, V / N>::of(v + i * (V / N)));
+      for (int i = 0; i < N; ++i)
+        __builtin_nontemporal_store(Vec<T, V / N>::of(v + i * (V / N)).raw, reinterpret_cast<words*>(p + i * (V / N)));
     } else {
 #pragma unroll
       for (int i = 0; i < V; ++i)
@@ -94,13 +99,13 @@ __device__ __forceinline__ float head_max(float v) {
 // 1 / sqrt(mean x^2 + eps) of a head. Where the squares leave the range of fp32, all lanes of the
 // wave take them again of values scaled by a power of two.
 template <int LPH>
-__device__ __forceinline__ float reciprocal_rms(const float* x, int dim, float eps) {
+__device__ __forceinline__ float reciprocal_rms(const float* x, const Args& a) {
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < V; ++i) sum += x[i] * x[i];
   sum = head_sum<LPH>(sum);
-  float r = rsqrtf(sum / float(dim) + eps);
-  const bool odd = !(sum < 0x1p125f) || (sum < 0x1p-90f && eps < 0x1p-90f);
+  float r = rsqrtf(sum * a.share + a.eps);
+  const bool odd = !(sum < 0x1p125f && sum >= a.least);
   if (__builtin_expect(__any(odd), 0)) {
     float most = 0.f;
 #pragma unroll
@@ -111,16 +116,16 @@ __device__ __forceinline__ float reciprocal_rms(const float* x, int dim, float e
 #pragma unroll
     for (int i = 0; i < V; ++i) sum += (x[i] * s) * (x[i] * s);
     sum = head_sum<LPH>(sum);
-    if (odd) r = s * rsqrtf(sum / float(dim) + eps * s * s);
+    if (odd) r = s * rsqrtf(sum * a.share + a.eps * s * s);
   }
   return r;
 }
 
-// The lane's pairs turned by their angles (sign -1: back).
-__device__ __forceinline__ void turn(float* v, const float2* angle, float sign) {
+// A lane's pairs turned by their angles.
+__device__ __forceinline__ void turn(float* v, const float2* angle) {
 #pragma unroll
   for (int i = 0; i < V / 2; ++i) {
-    const float c = angle[i].x, s = angle[i].y * sign, a = v[2 * i], b = v[2 * i + 1];
+    const float c = angle[i].x, s = angle[i].y, a = v[2 * i], b = v[2 * i + 1];
     v[2 * i] = a * c - b * s;
     v[2 * i + 1] = a * s + b * c;
   }
@@ -134,7 +139,7 @@ __device__ __forceinline__ float2 angle_of(const Args& a, int64_t at, double rat
   const double turned = position * rate;
   float s, c;
   sincospif(float(2.0 * (turned - rint(turned))), &s, &c);
-  return make_float2(c, s);
+  return make_float2(c, s * a.sign);
 }
 
 // What a lane keeps over the tokens of its wave.
@@ -157,49 +162,31 @@ __device__ __forceinline__ Lane lane_of(const Args& a, float2* lds) {
   l.angles = lds + (threadIdx.x >> 6) * a.group * l.pairs;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const int p = min(lane + 64 * k, MAX_PAIRS - 1);
+    const int p = min(lane % (LPH * V / 2) + 64 * k, MAX_PAIRS - 1);
     l.rate[k] = a.rate[p];
     l.axis[k] = a.axis[p];
   }
   return l;
 }
-// Tokens first .. first + count - 1: their angles into LDS.
+// Tokens first .. first + count - 1: their angles into LDS, as many tokens at a time as fill the wave.
+template <int LPH>
 __device__ __forceinline__ void take_angles(const Args& a, const Lane& l, int first, int count) {
+  constexpr int PAIRS = LPH * V / 2, AT_ONCE = PAIRS < 64 ? 64 / PAIRS : 1;
   const int lane = threadIdx.x & 63;
-  for (int t = 0; t < count; ++t) {
+  for (int t0 = 0; t0 < count; t0 += AT_ONCE) {
+    const int t = t0 + lane / (PAIRS < 64 ? PAIRS : 64);
+    if (t >= count) break;
     const int token = first + t, b = token / a.tokens, n = token - b * a.tokens;
     const int64_t at = (int64_t(b) * a.position_batch + n) * a.axes;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int p = lane + 64 * k;
-      if (p < l.pairs) l.angles[t * l.pairs + p] = angle_of(a, at, l.rate[k], l.axis[k], p < a.turned);
+    for (int k = 0; k < (PAIRS + 63) / 64; ++k) {
+      const int p = lane % (PAIRS < 64 ? PAIRS : 64) + 64 * k;
+      l.angles[t * PAIRS + p] = angle_of(a, at, l.rate[k], l.axis[k], p < a.turned);
     }
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // a wave's own LDS traffic is in order
 }
 
-// Calls f(side's heads in turn): one pass a head of the group's tokens for each group of LPH lanes,
-// UNROLL passes at a time; load(u, token, head, valid), work(u, token of the group, token, head, valid).
-template <int LPH, bool ONE, typename Load, typename Work>
-__device__ __forceinline__ void each_head(const Args& a, const Lane& l, int side, int first, int count, Load load,
-                                          Work work) {
-  constexpr int SUB = 64 / LPH;
-  const int heads = a.heads[side], items = ONE ? heads : heads * count;
-  for (int base = 0; base < items; base += SUB * UNROLL) {
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int item = base + u * SUB + l.sub, t = ONE ? 0 : item / heads;
-      load(u, first + t, item - t * heads, item < items);
-    }
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      if (base + u * SUB >= items) break;
-      const int item = base + u * SUB + l.sub, t = ONE ? 0 : item / heads;
-      // (lanes without a head work on the last one, so that all take part in the sums)
-      work(u, ONE ? 0 : min(t, count - 1), first + t, item - t * heads, item < items);
-    }
-  }
-}
 template <typename T>
 __device__ __forceinline__ const T* head_at(const Args& a, const void* x, int side, int token, int head) {
   const int b = token / a.tokens, n = token - b * a.tokens;
@@ -218,9 +205,46 @@ __device__ __forceinline__ void weights_of(const Args& a, int side, const Lane& 
                       : to_f32(static_cast<const bf16*>(a.weight[side])[c]);
   }
 }
+// A wave's work is its tokens' heads, the queries' and then the keys', COUNT * 64 / LPH of them a batch: one
+// a pass for each group of LPH lanes. fetch(side, base) loads a batch, work(side, base) computes and
+// stores it; the next batch's loads leave before a batch is worked on.
+template <int LPH, bool ONE, int COUNT, typename Fetch, typename Keep, typename Work>
+__device__ __forceinline__ void each_batch(const Args& a, int count, Fetch fetch, Keep keep, Work work) {
+  constexpr int STEP = COUNT * (64 / LPH);
+  int side = 0, base = 0;
+  while (true) {
+    keep();
+    const int now = side, from = base, items = a.heads[side] * (ONE ? 1 : count);
+    base += STEP;
+    if (base >= items) {
+      ++side;
+      base = 0;
+    }
+    const bool more = side < 2 && a.heads[side] > 0;
+    if (more) fetch(side, base);
+    work(now, from);
+    if (!more) break;
+  }
+}
+// Item `item` of a side's heads: its token of the group and its head.
+struct Item {
+  int t, token, head;
+  bool valid;
+};
+template <bool ONE>
+__device__ __forceinline__ Item item_of(const Args& a, int side, int first, int count, int item) {
+  const int heads = a.heads[side];
+  Item i;
+  i.t = ONE ? 0 : min(item / heads, count - 1);  // (past the end: a lane that takes part in the sums alone)
+  i.token = first + i.t;
+  i.head = item - i.t * heads;
+  i.valid = item < heads * (ONE ? 1 : count);
+  return i;
+}
 
 template <typename T, int LPH, bool NORM, bool ONE>
 __global__ __launch_bounds__(256) void heads_kernel(const Args a) {
+  constexpr int SUB = 64 / LPH;
   extern __shared__ float2 lds[];
   const Lane l = lane_of<LPH>(a, lds);
   const int waves = blockDim.x >> 6;
@@ -228,34 +252,77 @@ __global__ __launch_bounds__(256) void heads_kernel(const Args a) {
   const int first = wave * a.group;
   if (first >= a.total) return;
   const int count = min(a.group, a.total - first);
-  take_angles(a, l, first, count);
+  Chunk<T> next[UNROLL], in[UNROLL];
+  auto fetch = [&](int side, int base) {
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    if (a.heads[side] == 0) continue;
-    float w[V];
+    for (int u = 0; u < UNROLL; ++u) {
+      const Item i = item_of<ONE>(a, side, first, count, base + u * SUB + l.sub);
+      next[u].get(head_at<T>(a, a.x[side], side, i.token, i.head) + l.first, i.valid ? l.left : 0);
+    }
+  };
+  fetch(0, 0);
+  take_angles<LPH>(a, l, first, count);
+  float w[V];
+  // One token: its angles stay in registers, and the weights in them: n_0 c - n_1 s = x_0 (w_0 c) - x_1 (w_1 s).
+  float2 angle[V / 2];
+  float first_of[V], second_of[V];
+  auto take_weights = [&](int side) {
     if constexpr (NORM) weights_of(a, side, l, a.w_f32, !a.w_f32, w);
-    Chunk<T> in[UNROLL];
-    each_head<LPH, ONE>(
-        a, l, side, first, count,
-        [&](int u, int token, int head, bool valid) {
-          in[u].get(head_at<T>(a, a.x[side], side, token, head) + l.first, valid ? l.left : 0);
-        },
-        [&](int u, int t, int token, int head, bool valid) {
-          float v[V];
-          in[u].to(v);
-          if constexpr (NORM) {
-            const float r = reciprocal_rms<LPH>(v, a.dim, a.eps);
+    if constexpr (ONE) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[i] *= r * w[i];
-          }
-          turn(v, l.angles + t * l.pairs + l.first / 2, a.sign);
-          if (valid) Chunk<T>::put(static_cast<T*>(a.y[side]) + packed_at(a, side, token, head) + l.first, v, l.left);
-        });
-  }
+      for (int i = 0; i < V / 2; ++i) {
+        angle[i] = l.angles[l.first / 2 + i];
+        if constexpr (NORM) {
+          first_of[2 * i] = w[2 * i] * angle[i].x;
+          first_of[2 * i + 1] = w[2 * i] * angle[i].y;
+          second_of[2 * i] = -w[2 * i + 1] * angle[i].y;
+          second_of[2 * i + 1] = w[2 * i + 1] * angle[i].x;
+        }
+      }
+    }
+  };
+  auto keep = [&] {
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) in[u] = next[u];
+  };
+  each_batch<LPH, ONE, UNROLL>(a, count, fetch, keep, [&](int side, int base) {
+    if (base == 0) take_weights(side);
+    const int items = a.heads[side] * (ONE ? 1 : count);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      if (base + u * SUB >= items) break;
+      const Item item = item_of<ONE>(a, side, first, count, base + u * SUB + l.sub);
+      float v[V];
+      in[u].to(v);
+      if constexpr (NORM && ONE) {
+        const float r = reciprocal_rms<LPH>(v, a);
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+          const float x = v[i] * r, y = v[i + 1] * r;
+          v[i] = x * first_of[i] + y * second_of[i];
+          v[i + 1] = x * first_of[i + 1] + y * second_of[i + 1];
+        }
+      } else {
+        if constexpr (NORM) {
+          const float r = reciprocal_rms<LPH>(v, a);
+#pragma unroll
+          for (int i = 0; i < V; ++i) v[i] *= r * w[i];
+        }
+        if constexpr (!ONE) {
+#pragma unroll
+          for (int i = 0; i < V / 2; ++i) angle[i] = l.angles[item.t * l.pairs + l.first / 2 + i];
+        }
+        turn(v, angle);
+      }
+      if (item.valid)
+        Chunk<T>::put(static_cast<T*>(a.y[side]) + packed_at(a, side, item.token, item.head) + l.first, v, l.left);
+    }
+  });
 }
 
 template <typename T, int LPH, bool ONE>
-__global__ __launch_bounds__(256) void heads_backward_kernel(const Args a) {
+__global__ __launch_bounds__(256, 4) void heads_backward_kernel(const Args a) {
+  constexpr int SUB = 64 / LPH;
   extern __shared__ float2 lds[];
   const Lane l = lane_of<LPH>(a, lds);
   const int waves = blockDim.x >> 6, groups = (a.total + a.group - 1) / a.group;
@@ -266,39 +333,55 @@ __global__ __launch_bounds__(256) void heads_backward_kernel(const Args a) {
   const int64_t from = int64_t(groups) * id / all, to = int64_t(groups) * (id + 1) / all;
   for (int group = int(from); group < int(to); ++group) {
     const int first = group * a.group, count = min(a.group, a.total - first);
-    take_angles(a, l, first, count);
+    take_angles<LPH>(a, l, first, count);
+    float2 angle[V / 2];
+    if constexpr (ONE) {
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) angle[i] = l.angles[l.first / 2 + i];
+    }
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
       if (a.heads[side] == 0) continue;
       float w[V];
       weights_of(a, side, l, a.w_f32, !a.w_f32, w);
-      Chunk<T> in[UNROLL], grad[UNROLL];
-      each_head<LPH, ONE>(
-          a, l, side, first, count,
-          [&](int u, int token, int head, bool valid) {
-            const int left = valid ? l.left : 0;
-            in[u].get(head_at<T>(a, a.x[side], side, token, head) + l.first, left);
-            grad[u].get(static_cast<const T*>(a.grad[side]) + packed_at(a, side, token, head) + l.first, left);
-          },
-          [&](int u, int t, int token, int head, bool valid) {
-            float x[V], g[V];
-            in[u].to(x);
-            grad[u].to(g);
-            turn(g, l.angles + t * l.pairs + l.first / 2, -1.f);
-            const float r = reciprocal_rms<LPH>(x, a.dim, a.eps);
-            float dot = 0.f;
+      const int items = a.heads[side] * (ONE ? 1 : count);
+      for (int base = 0; base < items; base += BACKWARD * SUB) {
+        Chunk<T> in[BACKWARD], grad[BACKWARD];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-              x[i] *= r;
-              if (valid) dw[side][i] += g[i] * x[i];
-              g[i] *= w[i];
-              dot += g[i] * x[i];
-            }
-            dot = head_sum<LPH>(dot) / float(a.dim);
+        for (int u = 0; u < BACKWARD; ++u) {
+          const Item i = item_of<ONE>(a, side, first, count, base + u * SUB + l.sub);
+          const int left = i.valid ? l.left : 0;
+          in[u].get(head_at<T>(a, a.x[side], side, i.token, i.head) + l.first, left);
+          grad[u].get(static_cast<const T*>(a.grad[side]) + packed_at(a, side, i.token, i.head) + l.first, left);
+        }
 #pragma unroll
-            for (int i = 0; i < V; ++i) g[i] = r * (g[i] - x[i] * dot);
-            if (valid) Chunk<T>::put(static_cast<T*>(a.y[side]) + packed_at(a, side, token, head) + l.first, g, l.left);
-          });
+        for (int u = 0; u < BACKWARD; ++u) {
+          if (base + u * SUB >= items) break;
+          const Item item = item_of<ONE>(a, side, first, count, base + u * SUB + l.sub);
+          float x[V], g[V];
+          in[u].to(x);
+          grad[u].to(g);
+          if constexpr (!ONE) {
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) angle[i] = l.angles[item.t * l.pairs + l.first / 2 + i];
+          }
+          turn(g, angle);  // (the angles are taken backwards)
+          const float r = reciprocal_rms<LPH>(x, a);
+          float dot = 0.f;
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            x[i] *= r;
+            const float t = g[i] * x[i];  // (zero for a lane without a head)
+            dw[side][i] += t;
+            dot += w[i] * t;
+          }
+          dot = head_sum<LPH>(dot) * a.share;
+#pragma unroll
+          for (int i = 0; i < V; ++i) g[i] = r * (w[i] * g[i] - x[i] * dot);
+          if (item.valid)
+            Chunk<T>::put(static_cast<T*>(a.y[side]) + packed_at(a, side, item.token, item.head) + l.first, g, l.left);
+        }
+      }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
@@ -394,6 +477,8 @@ Args args_of(const sihc_heads* h) {
   a.w_f32 = h->w_dtype == SIHC_DTYPE_F32;
   a.eps = h->eps;
   a.sign = h->inverse ? -1.f : 1.f;
+  a.share = 1.f / float(h->dim);
+  a.least = h->eps < 0x1p-90f ? 0x1p-90f : 0.f;  // (a larger eps hides what smaller squares lose)
   for (int i = 0; i < h->axes; ++i) a.turned += h->widths[i] / 2;
   // Tokens of a wave: one where a token's heads fill 4 passes, else as many as do.
   const int sub = 64 / lanes_of(h->dim), heads = h->heads + h->kv_heads;
@@ -476,6 +561,7 @@ extern "C" int sihc_qk_norm_rotary_backward(const sihc_heads* h, const void* gra
   if (const int rc = check(h, k, q_weight, k_weight, "qk_norm_rotary_backward")) return rc;
   Args a = args_of(h);
   take_rates(h, a);
+  a.sign = -a.sign;
   if (!q_weight || !dq_weight || (k && !dk_weight))
     return fail(SIHC_ERR_INVALID, "qk_norm_rotary_backward: the weights and their gradients are needed");
   if (a.total && (!q || !grad_q || !dq || (k && (!grad_k || !dk)) || (a.turned && !positions) || !workspace))

@@ -123,19 +123,64 @@ struct Epilogue {
   int64_t gate_stride;
   int rows, outer, act, rows_per_gate;
 };
-__device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + __expf(-v)); }
+__device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }  // (1 ulp)
+
+// V channels of a row as they are in memory, on their way while something else is done.
+template <typename T>
+struct Row {
+  static constexpr int N = V * int(sizeof(T)) / 16;
+  u32x4 raw[N];
+  __device__ __forceinline__ void fetch(const T* p, int left) {
+    if (left >= V) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) raw[i] = load<T, V / N>(p + i * (V / N)).raw;
+    } else {
+      T e[V] = {};
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i < left) e[i] = p[i];
+      __builtin_memcpy(raw, e, sizeof(e));
+    }
+  }
+  __device__ __forceinline__ void to(float* o) const {
+    T e[V];
+    __builtin_memcpy(e, raw, sizeof(e));
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = to_f32(e[i]);
+  }
+};
+// What the epilogue reads for channels col .. col + V - 1: the bias once, gate and residual for each row.
+template <typename T, bool SWIGLU>
+struct Bias {
+  Row<T> a, b;
+  __device__ __forceinline__ Bias(const Epilogue& e, int col) {
+    if (!e.bias || col >= e.outer) return;
+    a.fetch(static_cast<const T*>(e.bias) + col, e.outer - col);
+    if constexpr (SWIGLU) b.fetch(static_cast<const T*>(e.bias) + e.outer + col, e.outer - col);
+  }
+};
+template <typename T>
+struct Rest {
+  Row<T> gate, residual;
+  __device__ __forceinline__ void fetch(const Epilogue& e, int row, int col) {
+    if (e.gate)
+      gate.fetch(static_cast<const T*>(e.gate) + int64_t(row / e.rows_per_gate) * e.gate_stride + col, e.outer - col);
+    if (e.residual) residual.fetch(static_cast<const T*>(e.residual) + int64_t(row) * e.outer + col, e.outer - col);
+  }
+};
 
 // Channels col .. col + V - 1 of row `row` from the products: a of W's first rows, b (SwiGLU) of its second.
 template <typename T, bool SWIGLU>
-__device__ __forceinline__ void finish(const Epilogue& e, int row, int col, float* a, float* b) {
+__device__ __forceinline__ void finish(const Epilogue& e, const Bias<T, SWIGLU>& bias, const Rest<T>& rest, int row,
+                                       int col, float* a, float* b) {
   const int left = e.outer - col;
   float t[V];
   if (e.bias) {
-    get(static_cast<const T*>(e.bias) + col, left, t);
+    bias.a.to(t);
 #pragma unroll
     for (int i = 0; i < V; ++i) a[i] += t[i];
     if constexpr (SWIGLU) {
-      get(static_cast<const T*>(e.bias) + e.outer + col, left, t);
+      bias.b.to(t);
 #pragma unroll
       for (int i = 0; i < V; ++i) b[i] += t[i];
     }
@@ -153,17 +198,16 @@ __device__ __forceinline__ void finish(const Epilogue& e, int row, int col, floa
     for (int i = 0; i < V; ++i) a[i] *= sigmoid(a[i]);
   }
   if (e.gate) {
-    get(static_cast<const T*>(e.gate) + int64_t(row / e.rows_per_gate) * e.gate_stride + col, left, t);
+    rest.gate.to(t);
 #pragma unroll
     for (int i = 0; i < V; ++i) a[i] *= t[i];
   }
-  const int64_t at = int64_t(row) * e.outer + col;
   if (e.residual) {
-    get(static_cast<const T*>(e.residual) + at, left, t);
+    rest.residual.to(t);
 #pragma unroll
     for (int i = 0; i < V; ++i) a[i] += t[i];
   }
-  put(static_cast<T*>(e.y) + at, left, a);
+  put(static_cast<T*>(e.y) + int64_t(row) * e.outer + col, left, a);
 }
 
 // ---------------------------------------------------------------------------------- products
@@ -204,6 +248,7 @@ struct Config {
   static constexpr int BM = BM_, BN = BN_, BK = BK_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, PER_SIMD = PER_SIMD_;
   static constexpr int THREADS = WAVES_M * WAVES_N * 64;
   static constexpr int MT = BM / WAVES_M / 32, NT = BN / WAVES_N / 32;  // a wave's tiles
+  static constexpr int PER_CU = PER_SIMD * 256 / THREADS;               // blocks of a CU at a time
 };
 
 // ROWS rows of an operand, BK of the contraction: in registers on their way, and in LDS.
@@ -213,9 +258,11 @@ struct Piece {
   // padded: 16 rows of 16 bytes, or 4 rows of 64 (transposing loads), fall into different banks
   static constexpr int STRIDE = TRANSPOSED ? ROWS + 64 / int(sizeof(T)) : BK + N;
   static constexpr int SIZE = (TRANSPOSED ? BK : ROWS) * STRIDE;
-  static constexpr int VECS = (TRANSPOSED ? ROWS : BK) / N;  // vectors of a row in memory
-  static constexpr int STEP = THREADS / VECS, COUNT = ROWS * BK / N / THREADS;
-  static_assert(THREADS % VECS == 0 && COUNT * THREADS * N == ROWS * BK, "every thread has the same vectors");
+  // Vectors of a row that adjacent threads take: all of BK, or (transposed) a run of ROWS, one after another.
+  static constexpr int RUN = std::max(64, THREADS * N / BK);
+  static constexpr int VECS = (TRANSPOSED ? RUN : BK) / N, RUNS = TRANSPOSED ? ROWS / RUN : 1;
+  static constexpr int LINES = TRANSPOSED ? BK : ROWS, STEP = THREADS / VECS, COUNT = RUNS * LINES / STEP;
+  static_assert(THREADS % VECS == 0 && LINES % STEP == 0 && ROWS % (TRANSPOSED ? RUN : 1) == 0, "every thread has the same vectors");
 
   const T* base;
   int64_t offset[TRANSPOSED ? 1 : COUNT];
@@ -253,11 +300,12 @@ struct Piece {
 #pragma unroll
     for (int i = 0; i < COUNT; ++i) {
       if constexpr (TRANSPOSED) {
-        const int row = k0 + line + i * STEP;
+        const int row = k0 + line + i / RUNS * STEP, run = i % RUNS * RUN;
+        const T* p = base + offset[0] + int64_t(row) * ld + run;
         if constexpr (WHOLE)
-          v[i] = load<T, N>(base + offset[0] + int64_t(row) * ld);
+          v[i] = load<T, N>(p);
         else
-          v[i] = row < k && left > 0 ? load_some<T, N>(base + offset[0] + int64_t(row) * ld, left) : Vec<T, N>::zero();
+          v[i] = row < k && left > run ? load_some<T, N>(p, left - run) : Vec<T, N>::zero();
       } else {
         if constexpr (WHOLE)
           v[i] = load<T, N>(base + offset[i] + k0);
@@ -268,7 +316,8 @@ struct Piece {
   }
   __device__ __forceinline__ void commit(T* lds) const {
 #pragma unroll
-    for (int i = 0; i < COUNT; ++i) *reinterpret_cast<u32x4*>(lds + (line + i * STEP) * STRIDE + at) = v[i].raw;
+    for (int i = 0; i < COUNT; ++i)
+      *reinterpret_cast<u32x4*>(lds + (line + i / RUNS * STEP) * STRIDE + at + i % RUNS * RUN) = v[i].raw;
   }
   // The lane's part of rows `row` .. row + 31 at step s of the piece.
   static __device__ __forceinline__ typename Matrix<T>::Frag fragment(const T* lds, int row, int s) {
@@ -338,14 +387,14 @@ __global__ __launch_bounds__(C::THREADS, C::PER_SIMD) void gemm_kernel(const Gem
   int buffer = 0;
   for (int k0 = from; k0 < k; k0 += C::BK, buffer ^= 1) {
     T* next = lds + (buffer ^ 1) * L::BUFFER;
-    if (k0 + C::BK < k) {
-      a.commit(next);
-      b.commit(next + A::SIZE);
-      if (k0 + 2 * C::BK < k) fetch(k0 + 2 * C::BK);
-    }
     const T *pa = lds + buffer * L::BUFFER, *pb = pa + A::SIZE;
 #pragma unroll
     for (int s = 0; s < C::BK / Matrix<T>::STEP; ++s) {
+      if (s == 0 && k0 + C::BK < k) {
+        a.commit(next);
+        b.commit(next + A::SIZE);
+        if (k0 + 2 * C::BK < k) fetch(k0 + 2 * C::BK);
+      }
       typename Matrix<T>::Frag fa[C::MT], fb[C::NT];
 #pragma unroll
       for (int i = 0; i < C::MT; ++i) fa[i] = A::fragment(pa, wm + i * 32, s);
@@ -363,23 +412,30 @@ __global__ __launch_bounds__(C::THREADS, C::PER_SIMD) void gemm_kernel(const Gem
   const int lane = threadIdx.x & 63;
   float* strip = reinterpret_cast<float*>(lds_bytes) + wave * 32 * L::STRIP;
   constexpr int WIDE = SWIGLU ? C::NT * 16 : C::NT * 32;  // the result's channels of a wave
-  constexpr int GROUPS = WIDE / V, ROWS = 64 / GROUPS;
-  const int col = n0 + (SWIGLU ? wn / 2 : wn) + lane % GROUPS * V;
+  constexpr int GROUPS = WIDE / V, ROWS = 64 / GROUPS, PASSES = 32 / ROWS;
+  const int c = lane % GROUPS * V, col = n0 + (SWIGLU ? wn / 2 : wn) + c;
+  const Bias<T, SWIGLU> bias(g.e, col);
 #pragma unroll
   for (int i = 0; i < C::MT; ++i) {
+    const int row0 = m0 + wm + i * 32 + lane / GROUPS;
+    Rest<T> rest[PASSES];
+    if (!g.e.part && col < g.n)
+#pragma unroll
+      for (int r = 0; r < PASSES; ++r)
+        if (row0 + r * ROWS < g.m) rest[r].fetch(g.e, row0 + r * ROWS, col);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
     for (int j = 0; j < C::NT; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) strip[row_of(r, lane >> 5) * L::STRIP + j * 32 + (lane & 31)] = acc[i][j][r];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll 1
-    for (int r = lane / GROUPS; r < 32; r += ROWS) {
-      const int row = m0 + wm + i * 32 + r;
-      if (row >= g.m || col >= g.n) continue;
-      const int c = lane % GROUPS * V;
+    if (col >= g.n) continue;
+#pragma unroll
+    for (int r = 0; r < PASSES; ++r) {
+      const int row = row0 + r * ROWS;
+      if (row >= g.m) break;
       float p[V], q[V];
-      const float* from_strip = strip + r * L::STRIP + (SWIGLU ? c / 32 * 64 + c % 32 : c);
+      const float* from_strip = strip + (lane / GROUPS + r * ROWS) * L::STRIP + (SWIGLU ? c / 32 * 64 + c % 32 : c);
 #pragma unroll
       for (int x = 0; x < V; ++x) p[x] = from_strip[x];
       if constexpr (SWIGLU)
@@ -390,7 +446,7 @@ __global__ __launch_bounds__(C::THREADS, C::PER_SIMD) void gemm_kernel(const Gem
         put(to, g.n - col, p);
         if constexpr (SWIGLU) put(to + g.n, g.n - col, q);
       } else {
-        finish<T, SWIGLU>(g.e, row, col, p, q);
+        finish<T, SWIGLU>(g.e, bias, rest[r], row, col, p, q);
       }
     }
   }
@@ -407,6 +463,9 @@ __global__ __launch_bounds__(256) void join_kernel(const Epilogue e, int splits)
   const int64_t wide = (SWIGLU ? 2 : 1) * int64_t(e.outer), all = int64_t(e.rows) * wide;
   const float* p = e.part + row * wide + col;
   float a[V] = {}, b[V] = {};
+  const Bias<T, SWIGLU> bias(e, col);
+  Rest<T> rest;
+  rest.fetch(e, int(row), col);
 #pragma unroll 2
   for (int s = 0; s < splits; ++s) {
     float t[V];
@@ -419,7 +478,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Epilogue e, int splits)
       for (int x = 0; x < V; ++x) b[x] += t[x];
     }
   }
-  finish<T, SWIGLU>(e, int(row), col, a, b);
+  finish<T, SWIGLU>(e, bias, rest, int(row), col, a, b);
 }
 
 // ------------------------------------------------------------------------------ dh and its sums
@@ -528,67 +587,64 @@ __global__ __launch_bounds__(256) void sums_kernel(const float* part, T* out, in
 }
 
 // ---------------------------------------------------------------------------------- host
-template <typename T> struct Configs;
-template <>
-struct Configs<bf16> {
-  using Large = Config<bf16, 256, 256, 64, 2, 4, 2>;
-  using Middle = Config<bf16, 128, 128, 64, 2, 2, 2>;
-  using Small = Config<bf16, 64, 64, 64, 2, 1, 2>;
-};
-template <>
-struct Configs<float> {
-  using Large = Config<float, 128, 128, 32, 2, 2, 2>;
-  using Middle = Large;
-  using Small = Config<float, 64, 64, 32, 2, 1, 2>;
-};
-
-struct Plan {
-  int size;  // 0 large, 1 middle, 2 small
-  int splits, steps, tiles_m, tiles_n;
-  int64_t blocks;
-};
 constexpr int CUS = 256;
 
-// The tile and the parts of the contraction that promise the least time: rounds of blocks over the
-// CUs, each as long as its pieces and a fixed start and end, and the parts' sums through memory.
+// The tiles, the largest first, and what they take by measurement: the time of a piece (of a full CU's, for
+// each block in it; of a block alone on its CU) and of a tile's start and end, in microseconds.
+struct Cost {
+  double piece, alone, tile;
+};
+template <typename T, int SIZE> struct Tiles;
+template <> struct Tiles<bf16, 0> : Config<bf16, 256, 256, 64, 2, 4, 2> { static constexpr Cost COST{1.75, 1.75, 9.5}; };
+template <> struct Tiles<bf16, 1> : Config<bf16, 256, 192, 64, 4, 2, 2> { static constexpr Cost COST{1.33, 1.33, 10.0}; };
+template <> struct Tiles<bf16, 2> : Config<bf16, 256, 128, 64, 4, 2, 2> { static constexpr Cost COST{0.98, 0.98, 7.0}; };
+template <> struct Tiles<bf16, 3> : Config<bf16, 128, 128, 64, 2, 2, 2> { static constexpr Cost COST{0.63, 0.72, 3.0}; };
+template <> struct Tiles<bf16, 4> : Config<bf16, 64, 64, 64, 2, 1, 2> { static constexpr Cost COST{0.20, 0.50, 4.0}; };
+template <> struct Tiles<float, 0> : Config<float, 128, 128, 32, 2, 2, 2> { static constexpr Cost COST{2.1, 2.3, 4.0}; };
+template <> struct Tiles<float, 1> : Config<float, 64, 64, 32, 2, 1, 2> { static constexpr Cost COST{0.6, 1.6, 4.0}; };
 template <typename T>
-Plan plan_of(int64_t m, int64_t n, int64_t k, bool swiglu) {
-  struct Shape { int bm, bn, bk, per_cu; double piece; };  // cycles of a piece where the CU is full
-  using C = Configs<T>;
-  auto shape = [](auto config, int per_cu, double rate) {  // rate: of the matrix cores' peak
-    using S = decltype(config);
-    const double flops = sizeof(T) == 2 ? 4096.0 : 256.0;
-    return Shape{S::BM, S::BN, S::BK, per_cu, 2.0 * S::BM * S::BN * S::BK / (flops * rate)};
-  };
-  const Shape shapes[3] = {shape(typename C::Large{}, sizeof(T) == 2 ? 1 : 2, sizeof(T) == 2 ? 0.5 : 0.8),
-                           shape(typename C::Middle{}, 2, sizeof(T) == 2 ? 0.35 : 0.8),
-                           shape(typename C::Small{}, 4, sizeof(T) == 2 ? 0.2 : 0.6)};
+constexpr int SIZES = sizeof(T) == 2 ? 5 : 2;
+// Calls f(tile, its number) for every tile that the product can have: SwiGLU wants pairs of a wave's tiles.
+template <typename T, bool SWIGLU, int SIZE = 0, typename F>
+void each_tile(F&& f) {
+  if constexpr (SIZE < SIZES<T>) {
+    if constexpr (!SWIGLU || Tiles<T, SIZE>::NT % 2 == 0) f(Tiles<T, SIZE>{}, SIZE);
+    each_tile<T, SWIGLU, SIZE + 1>(f);
+  }
+}
+
+struct Plan {
+  int size, splits, steps, tiles_m, tiles_n;
+  int64_t blocks;
+};
+// The tile and the parts of the contraction that promise the least time: every CU's blocks one after
+// another, and the parts' sums through memory (at 8 TB/s, for they are still in a cache) and a launch.
+template <typename T, bool SWIGLU>
+Plan plan_of(int64_t m, int64_t n, int64_t k) {
   Plan best{};
   double least = 1e30;
-  for (int s = 0; s < 3; ++s) {
-    const Shape& f = shapes[s];
-    const int64_t tm = ceil_div(m, f.bm), tn = ceil_div(n, swiglu ? f.bn / 2 : f.bn), pieces = ceil_div(k, f.bk);
-    for (int splits = 1; splits <= 64 && splits <= pieces; ++splits) {
-      const int64_t steps = ceil_div(pieces, splits);
+  each_tile<T, SWIGLU>([&](auto tile, int size) {
+    using C = decltype(tile);
+    const int64_t tm = ceil_div(m, C::BM), tn = ceil_div(n, SWIGLU ? C::BN / 2 : C::BN), pieces = ceil_div(k, C::BK);
+    for (int splits = 1; splits <= 32 && splits <= pieces; ++splits) {
+      const int64_t steps = ceil_div(pieces, splits), blocks = tm * tn * splits;
       if (ceil_div(pieces, steps) != splits) continue;
-      const int64_t blocks = tm * tn * splits;
-      // blocks that share a CU share its matrix cores
-      const double rounds = double(ceil_div(blocks, CUS));
-      const double alone = std::min<double>(rounds, f.per_cu);  // blocks of a CU at a time
-      double cycles = rounds * double(steps) * f.piece + ceil_div(int64_t(rounds), f.per_cu) * 3000.0;
-      // few blocks: a piece costs its loads' latency
-      cycles = std::max(cycles, double(steps) * 900.0 * rounds / alone);
-      if (splits > 1) cycles += 6000.0 + double(m) * double(n) * (swiglu ? 2 : 1) * 8.0 * splits / 1700.0;
-      if (cycles < least) {
-        least = cycles;
-        best = Plan{s, splits, int(steps), int(tm), int(tn), blocks};
+      const int64_t each = ceil_div(blocks, CUS), rounds = ceil_div(each, C::PER_CU);
+      double us = std::max(double(each) * C::COST.piece, double(rounds) * C::COST.alone) * double(steps) +
+                  double(rounds) * C::COST.tile;
+      if (splits > 1) us += 4.0 + double(m) * double(n) * (SWIGLU ? 2 : 1) * 4.0 * (splits + 1) / 8e6;
+      if (us < least) {
+        least = us;
+        best = Plan{size, splits, int(steps), int(tm), int(tn), blocks};
       }
+      if (blocks > 8 * CUS) break;  // (more parts only add to the sums)
     }
-  }
+  });
   return best;
 }
 Plan plan_for(int dtype, int64_t m, int64_t n, int64_t k, bool swiglu) {
-  return dtype == SIHC_DTYPE_BF16 ? plan_of<bf16>(m, n, k, swiglu) : plan_of<float>(m, n, k, swiglu);
+  if (dtype == SIHC_DTYPE_BF16) return swiglu ? plan_of<bf16, true>(m, n, k) : plan_of<bf16, false>(m, n, k);
+  return swiglu ? plan_of<float, true>(m, n, k) : plan_of<float, false>(m, n, k);
 }
 size_t part_bytes(const Plan& p, int64_t m, int64_t n, bool swiglu) {
   return p.splits > 1 ? size_t(p.splits) * size_t(m) * size_t(n) * (swiglu ? 2 : 1) * sizeof(float) : 0;
@@ -608,7 +664,7 @@ int start(const Gemm& g, int64_t blocks, hipStream_t stream, const char* what) {
 // g.e, g.a, g.b and the sizes given; `part`: the parts' sums.
 template <typename T, bool TA, bool TB, bool SWIGLU>
 int product(Gemm g, float* part, hipStream_t stream, const char* what) {
-  const Plan p = plan_of<T>(g.m, g.n, g.k, SWIGLU);
+  const Plan p = plan_of<T, SWIGLU>(g.m, g.n, g.k);
   if (p.blocks * 512 > MOST_LAUNCHED) return fail(SIHC_ERR_INVALID, "%s: too many rows for a launch", what);
   g.splits = p.splits;
   g.steps = p.steps;
@@ -617,10 +673,10 @@ int product(Gemm g, float* part, hipStream_t stream, const char* what) {
   g.e.part = p.splits > 1 ? part : nullptr;
   g.e.rows = g.m;
   g.e.outer = g.n;
-  int rc;
-  if (p.size == 0) rc = start<T, typename Configs<T>::Large, TA, TB, SWIGLU>(g, p.blocks, stream, what);
-  else if (p.size == 1) rc = start<T, typename Configs<T>::Middle, TA, TB, SWIGLU>(g, p.blocks, stream, what);
-  else rc = start<T, typename Configs<T>::Small, TA, TB, SWIGLU>(g, p.blocks, stream, what);
+  int rc = SIHC_OK;
+  each_tile<T, SWIGLU>([&](auto tile, int size) {
+    if (size == p.size) rc = start<T, decltype(tile), TA, TB, SWIGLU>(g, p.blocks, stream, what);
+  });
   if (rc || p.splits == 1) return rc;
   const int64_t threads = int64_t(g.m) * ceil_div(g.n, V);
   if (threads > MOST_LAUNCHED) return fail(SIHC_ERR_INVALID, "%s: too many rows for a launch", what);
