@@ -405,11 +405,12 @@ typedef struct {
 size_t sihc_linear_act_workspace_size(const sihc_linear *l);
 /* h = x weight^T + bias; u = h, silu(h) or silu(h[:, :outer]) * h[:, outer:]; y = residual +
  * gate * u, in fp32 sums, rounded once. bias, gate and residual may be NULL. For the backward h,
- * if given, receives h [rows, weight rows] in dtype; low, if given as well (bf16 with an
- * activation), the next 8 bits of each value, and h the upper 16, cut and not rounded. The workspace
- * may be NULL where its size is 0. */
+ * if given, receives h [rows, weight rows] in dtype. low, if given as well (bf16 with an activation;
+ * [rows, parts, (outer + 7) / 8] words, 2 parts with SIHC_ACT_SWIGLU and else 1), receives 4 more
+ * bits of each value, those of 8 channels in a word, lowest channel first, and h the 16 above them.
+ * The workspace may be NULL where its size is 0. */
 int sihc_linear_act(const sihc_linear *l, const void *x, const void *weight, const void *bias,
-                    const void *gate, const void *residual, void *y, void *h, uint8_t *low,
+                    const void *gate, const void *residual, void *y, void *h, uint32_t *low,
                     void *workspace, size_t workspace_bytes, void *stream);
 
 size_t sihc_linear_act_backward_workspace_size(const sihc_linear *l, int gated);
@@ -418,7 +419,7 @@ size_t sihc_linear_act_backward_workspace_size(const sihc_linear *l, int gated);
  * [rows / rows_per_gate, outer] are packed; each may be NULL if it is not wanted. Sums in fp32 in
  * a fixed order, without atomics; the gradient of h is rounded to dtype as the products' operand. */
 int sihc_linear_act_backward(const sihc_linear *l, const void *grad, const void *x,
-                             const void *weight, const void *h, const uint8_t *low,
+                             const void *weight, const void *h, const uint32_t *low,
                              const void *gate, void *dx, void *dweight, void *dbias, void *dgate, void *workspace,
                              size_t workspace_bytes, void *stream);
 

@@ -61,64 +61,49 @@ __device__ __forceinline__ Vec<T, N> load_some(const T* p, int left) {
   return v;
 }
 
-// h as the backward has it. In bf16 with an activation it is cut after 24 bits, 16 of them where a bf16
-// would be and 8 beside it: rounded to 16 bits, it would put the gradients of a SwiGLU 1.75 times as far from
-// the exact ones as their own rounding does (with 24: 1.35, from the rounding of dh as an operand).
+// h as the backward has it. In bf16 with an activation that is 20 bits, the upper 16 where a bf16 would be and
+// 4 beside it, those of 8 channels in one word: rounded to 16 bits, h would put the gradients of a SwiGLU 1.75
+// times as far from the exact ones as their own rounding does (with 20: 1.35, from the rounding of dh as an
+// operand). `low` is [rows, parts of h, words_of(outer)].
+__host__ __device__ constexpr int words_of(int outer) { return (outer + V - 1) / V; }
 template <typename T>
-__device__ __forceinline__ void put_kept(void* h, uint8_t* low, int64_t at, int left, const float* v) {
+__device__ __forceinline__ void put_kept(void* h, uint32_t* low, int64_t at, int left, const float* v) {
   if (sizeof(T) == 4 || !low) {
     put(static_cast<T*>(h) + at, left, v);
     return;
   }
   uint16_t high[V];
-  uint8_t rest[V];
+  uint32_t rest = 0;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    uint32_t bits = __float_as_uint(v[i]);
-    if (v[i] != v[i]) bits |= 0x400000u;  // (what makes it a NaN may lie in the bits that are cut)
+  for (int i = 0; i < V; ++i) {  // (cut, not rounded: at most 2^-11 of the value; an arithmetic NaN has bit 22)
+    const uint32_t bits = __float_as_uint(v[i]);
     high[i] = uint16_t(bits >> 16);
-    rest[i] = uint8_t(bits >> 8);
+    rest |= (bits >> 12 & 0xfu) << (4 * i);
   }
   uint16_t* to = static_cast<uint16_t*>(h) + at;
   if (left >= V) {
     typedef u32x4 words __attribute__((aligned(2)));
-    typedef u32x2 bytes __attribute__((aligned(1)));
-    __builtin_memcpy(reinterpret_cast<words*>(to), high, 16);
-    bytes b;
-    __builtin_memcpy(&b, rest, 8);
-    *reinterpret_cast<bytes*>(low + at) = b;
+    words w;
+    __builtin_memcpy(&w, high, 16);
+    *reinterpret_cast<words*>(to) = w;
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (i < left) {
-        to[i] = high[i];
-        low[at + i] = rest[i];
-      }
+      if (i < left) to[i] = high[i];
   }
+  *low = rest;
 }
-template <typename T>
-__device__ __forceinline__ void get_kept(const void* h, const uint8_t* low, int64_t at, int left, float* v) {
-  get(static_cast<const T*>(h) + at, left, v);
-  if (sizeof(T) == 4 || !low) return;
-  uint8_t rest[V] = {};
-  if (left >= V) {
-    typedef u32x2 bytes __attribute__((aligned(1)));
-    const bytes b = *reinterpret_cast<const bytes*>(low + at);
-    __builtin_memcpy(rest, &b, 8);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (i < left) rest[i] = low[at + i];
-  }
-#pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = __uint_as_float(__float_as_uint(v[i]) | uint32_t(rest[i]) << 8);
+// A value of h from its upper 16 bits, as a float, and channel i's 4 of the word beside it.
+__device__ __forceinline__ float kept(float high, uint32_t rest, int i) {
+  const uint32_t nibble = i < 3 ? rest << (12 - 4 * i) : rest >> (4 * i - 12);
+  return __uint_as_float(__float_as_uint(high) | (nibble & 0xf000u));
 }
 
 // ---------------------------------------------------------------------------------- epilogue
 struct Epilogue {
   const void *bias, *gate, *residual;
   void *y, *h;         // the result; h as the backward wants it, or null
-  uint8_t* low;
+  uint32_t* low;       // (put_kept)
   float* part;         // [splits][rows][columns] sums instead of the result, or null
   int64_t gate_stride;
   int rows, outer, act, rows_per_gate;
@@ -186,9 +171,11 @@ __device__ __forceinline__ void finish(const Epilogue& e, const Bias<T, SWIGLU>&
     }
   }
   if (e.h) {
-    const int64_t at = int64_t(row) * (SWIGLU ? 2 : 1) * e.outer + col;
-    put_kept<T>(e.h, e.low, at, left, a);
-    if constexpr (SWIGLU) put_kept<T>(e.h, e.low, at + e.outer, left, b);
+    const int64_t first = int64_t(row) * (SWIGLU ? 2 : 1);
+    uint32_t* low = e.low ? e.low + first * words_of(e.outer) + col / V : nullptr;
+    put_kept<T>(e.h, low, first * e.outer + col, left, a);
+    if constexpr (SWIGLU)
+      put_kept<T>(e.h, low ? low + words_of(e.outer) : nullptr, (first + 1) * e.outer + col, left, b);
   }
   if constexpr (SWIGLU) {
 #pragma unroll
@@ -412,28 +399,28 @@ __global__ __launch_bounds__(C::THREADS, C::PER_SIMD) void gemm_kernel(const Gem
   const int lane = threadIdx.x & 63;
   float* strip = reinterpret_cast<float*>(lds_bytes) + wave * 32 * L::STRIP;
   constexpr int WIDE = SWIGLU ? C::NT * 16 : C::NT * 32;  // the result's channels of a wave
-  constexpr int GROUPS = WIDE / V, ROWS = 64 / GROUPS, PASSES = 32 / ROWS;
+  constexpr int GROUPS = WIDE / V, ROWS = 64 / GROUPS, PASSES = (32 + ROWS - 1) / ROWS;  // (three tiles: 60 lanes)
   const int c = lane % GROUPS * V, col = n0 + (SWIGLU ? wn / 2 : wn) + c;
   const Bias<T, SWIGLU> bias(g.e, col);
 #pragma unroll
   for (int i = 0; i < C::MT; ++i) {
-    const int row0 = m0 + wm + i * 32 + lane / GROUPS;
+    const int row0 = m0 + wm + i * 32;
+    const int end = lane < GROUPS * ROWS && col < g.n ? min(32, g.m - row0) : 0;  // the lane's rows of the strip
     Rest<T> rest[PASSES];
-    if (!g.e.part && col < g.n)
+    if (!g.e.part)
 #pragma unroll
       for (int r = 0; r < PASSES; ++r)
-        if (row0 + r * ROWS < g.m) rest[r].fetch(g.e, row0 + r * ROWS, col);
+        if (lane / GROUPS + r * ROWS < end) rest[r].fetch(g.e, row0 + lane / GROUPS + r * ROWS, col);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
     for (int j = 0; j < C::NT; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) strip[row_of(r, lane >> 5) * L::STRIP + j * 32 + (lane & 31)] = acc[i][j][r];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (col >= g.n) continue;
 #pragma unroll
     for (int r = 0; r < PASSES; ++r) {
-      const int row = row0 + r * ROWS;
-      if (row >= g.m) break;
+      if (lane / GROUPS + r * ROWS >= end) break;
+      const int row = row0 + lane / GROUPS + r * ROWS;
       float p[V], q[V];
       const float* from_strip = strip + (lane / GROUPS + r * ROWS) * L::STRIP + (SWIGLU ? c / 32 * 64 + c % 32 : c);
 #pragma unroll
@@ -450,6 +437,152 @@ __global__ __launch_bounds__(C::THREADS, C::PER_SIMD) void gemm_kernel(const Gem
       }
     }
   }
+}
+
+// Small products and few rows: a block owns 32 x 32 of the result (SwiGLU: of both halves; 16 x 32 where there
+// are no more rows), its waves a run of the contraction each, in 16 x 16 tiles (bf16 16x16x32, fp32 16x16x4).
+// Operands go from memory straight to the matrix cores' registers, 64 adjacent bytes of a row for four lanes;
+// (transposed) two adjacent elements a lane, one for each of its tiles. The waves' sums meet in LDS, in
+// the waves' order: one launch, and no wait but for the loads of the next piece.
+constexpr int SMALL = 32;       // columns of a block, and its rows
+constexpr int most_waves(bool swiglu, bool transposed) { return swiglu || transposed ? 8 : 16; }  // (their registers)
+template <typename T>
+constexpr int SMALL_PIECE = 128 / int(sizeof(T));  // of the contraction, in two steps
+
+// TILES tiles of 16 rows of an operand, a piece of the contraction. Row `lane` of tile t is 16 t + lane,
+// or (transposed) 2 lane + t.
+template <typename T, bool TRANSPOSED, int TILES>
+struct Direct {
+  using Frag = typename Matrix<T>::Frag;
+  static constexpr int N = 16 / int(sizeof(T)), STEP = 4 * N;
+  const T* base;
+  int64_t ld;
+  int64_t offset[TILES];
+  int first;   // the lane's place in a step
+  bool whole;  // (transposed) the tiles' rows all exist
+  Frag f[2][TILES];
+  // rows `row` .. of `rows`, which start at row `shift` of the operand
+  __device__ __forceinline__ Direct(const void* p, int64_t ld_, int row, int rows, int64_t shift)
+      : base(static_cast<const T*>(p)), ld(ld_) {
+    const int lane = int(threadIdx.x) & 15;
+    first = (int(threadIdx.x) >> 4 & 3) * N;
+    whole = row + 16 * TILES <= rows;
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+      offset[t] = TRANSPOSED ? shift + min(row + TILES * lane + t, rows - 1)
+                             : (shift + min(row + 16 * t + lane, rows - 1)) * ld + first;
+  }
+  __device__ __forceinline__ void fetch(int k0, int k) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int from = k0 + s * STEP, left = k - from - first;
+      T e[TILES][N];
+      if constexpr (!TRANSPOSED) {
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+          Vec<T, N> v;
+          if (k0 + 2 * STEP <= k) v = load<T, N>(base + offset[t] + from);
+          else v = left > 0 ? load_some<T, N>(base + offset[t] + from, left) : Vec<T, N>::zero();
+          __builtin_memcpy(e[t], &v.raw, 16);
+        }
+      } else if (k0 + 2 * STEP <= k && whole) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const Vec<T, TILES> v = load<T, TILES>(base + int64_t(from + first + i) * ld + offset[0]);
+          T pair[TILES];
+          __builtin_memcpy(pair, &v.raw, sizeof(pair));
+#pragma unroll
+          for (int t = 0; t < TILES; ++t) e[t][i] = pair[t];
+        }
+      } else {
+        __builtin_memset(e, 0, sizeof(e));
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (i < left)
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) e[t][i] = base[int64_t(from + first + i) * ld + offset[t]];
+      }
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) __builtin_memcpy(&f[s][t], e[t], 16);
+    }
+  }
+};
+__device__ __forceinline__ f32x4 multiply16(const bf16x8& a, const bf16x8& b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 multiply16(const f32x4& a, const f32x4& b, f32x4 c) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+  return c;
+}
+
+template <typename T, bool TA, bool TB, bool SWIGLU, int TILES_M>
+__global__ __launch_bounds__(64 * most_waves(SWIGLU, TA || TB)) void small_kernel(const Gemm g) {
+  extern __shared__ __align__(16) char lds_bytes[];
+  float* lds = reinterpret_cast<float*>(lds_bytes);
+  constexpr int HALVES = SWIGLU ? 2 : 1, ROWS = 16 * TILES_M, STRIDE = SMALL + 4, TILE = ROWS * STRIDE;
+  constexpr int PIECE = SMALL_PIECE<T>;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int tile = xcd_block(blockIdx.x, gridDim.x), m0 = tile / g.tiles_n * ROWS, n0 = tile % g.tiles_n * SMALL;
+  const int from = min(g.k, wave * g.steps * PIECE), k = min(g.k, from + g.steps * PIECE);
+  using A = Direct<T, TA, TILES_M>;
+  using B = Direct<T, TB, 2>;
+  A a(g.a, g.lda, m0, g.m, 0);
+  B b(g.b, g.ldb, n0, g.n, 0), c(g.b, g.ldb, n0, g.n, SWIGLU ? g.n : 0);
+  f32x4 acc[HALVES][TILES_M][2] = {};
+  if (from < k) {
+    a.fetch(from, k);
+    b.fetch(from, k);
+    if constexpr (SWIGLU) c.fetch(from, k);
+    for (int k0 = from; k0 < k; k0 += PIECE) {
+      const A now_a = a;
+      const B now_b = b, now_c = c;
+      if (k0 + PIECE < k) {
+        a.fetch(k0 + PIECE, k);
+        b.fetch(k0 + PIECE, k);
+        if constexpr (SWIGLU) c.fetch(k0 + PIECE, k);
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < TILES_M; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            acc[0][i][j] = multiply16(now_a.f[s][i], now_b.f[s][j], acc[0][i][j]);
+            if constexpr (SWIGLU) acc[1][i][j] = multiply16(now_a.f[s][i], now_c.f[s][j], acc[1][i][j]);
+          }
+    }
+  }
+  // a thread's V channels of a row
+  const int r = int(threadIdx.x) / (SMALL / V), cc = int(threadIdx.x) % (SMALL / V) * V, row = m0 + r, col = n0 + cc;
+  const bool owns = int(threadIdx.x) < ROWS * SMALL / V && row < g.m && col < g.n;
+  Rest<T> rest;
+  if (owns) rest.fetch(g.e, row, col);
+  const Bias<T, SWIGLU> bias(g.e, owns ? col : g.n);
+#pragma unroll
+  for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+    for (int i = 0; i < TILES_M; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int at = (lane >> 4) * 4 + x;  // of tile i's rows
+          lds[(wave * HALVES + h) * TILE + (TA ? TILES_M * at + i : 16 * i + at) * STRIDE +
+              (TB ? 2 * (lane & 15) + j : 16 * j + (lane & 15))] = acc[h][i][j][x];
+        }
+  __syncthreads();
+  if (!owns) return;
+  float p[V] = {}, q[V] = {};
+  for (int w = 0; w < waves; ++w) {
+    const float* t = lds + w * HALVES * TILE + r * STRIDE + cc;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      p[i] += t[i];
+      if constexpr (SWIGLU) q[i] += t[TILE + i];
+    }
+  }
+  finish<T, SWIGLU>(g.e, bias, rest, row, col, p, q);
 }
 
 // The result from the parts' sums, in their order.
@@ -484,7 +617,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Epilogue e, int splits)
 // ------------------------------------------------------------------------------ dh and its sums
 struct Slopes {
   const void *grad, *h, *gate;
-  const uint8_t* low;
+  const uint32_t* low;
   void *dh;            // null where dh is the gradient itself
   float *bias_part, *gate_part;
   int64_t gate_stride;
@@ -498,7 +631,8 @@ __global__ __launch_bounds__(256) void slopes_kernel(const Slopes s) {
   __shared__ float lds[8][32 * V + 4];
   const int across = threadIdx.x & 31, down = threadIdx.x >> 5;
   const int blocks = (s.outer + 32 * V - 1) / (32 * V);
-  const int chunk = int(blockIdx.x / unsigned(blocks)), col = (int(blockIdx.x % unsigned(blocks)) * 32 + across) * V;
+  const unsigned at = unsigned(xcd_block(int(blockIdx.x), int(gridDim.x)));  // a row's blocks on one XCD
+  const int chunk = int(at / unsigned(blocks)), col0 = int(at % unsigned(blocks)) * 32 * V, col = col0 + across * V;
   const int image = chunk / s.chunks, first = (chunk - image * s.chunks) * CHUNK;
   const int count = min(CHUNK, s.rows_per_gate - first), left = s.outer - col;
   const int64_t row0 = int64_t(image) * s.rows_per_gate + first;
@@ -512,9 +646,18 @@ __global__ __launch_bounds__(256) void slopes_kernel(const Slopes s) {
       const int64_t row = row0 + r;
       get(static_cast<const T*>(s.grad) + row * s.outer + col, left, g);
       if (s.h) {
-        const int64_t at = row * wide * s.outer + col;
-        get_kept<T>(s.h, s.low, at, left, a);
-        if constexpr (SWIGLU) get_kept<T>(s.h, s.low, at + s.outer, left, b);
+        const T* h = static_cast<const T*>(s.h) + row * wide * s.outer + col;
+        get(h, left, a);
+        if constexpr (SWIGLU) get(h + s.outer, left, b);
+        if (sizeof(T) == 2 && s.low) {
+          const uint32_t* low = s.low + row * wide * words_of(s.outer) + col / V;
+          const uint32_t rest_a = low[0], rest_b = SWIGLU ? low[words_of(s.outer)] : 0;
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            a[i] = kept(a[i], rest_a, i);
+            if constexpr (SWIGLU) b[i] = kept(b[i], rest_b, i);
+          }
+        }
       }
 #pragma unroll
       for (int i = 0; i < V; ++i) {
@@ -554,7 +697,7 @@ __global__ __launch_bounds__(256) void slopes_kernel(const Slopes s) {
 #pragma unroll
     for (int i = 0; i < V; ++i) lds[down][across * V + i] = sums[k][i];
     __syncthreads();
-    const int c = int(blockIdx.x % unsigned(blocks)) * 32 * V + int(threadIdx.x);
+    const int c = col0 + int(threadIdx.x);
     if (c < s.outer) {
       float v = 0.f;
 #pragma unroll
@@ -564,26 +707,36 @@ __global__ __launch_bounds__(256) void slopes_kernel(const Slopes s) {
   }
 }
 // out[r, :] = sum over `parts` rows of part[r * parts + i, :]: 32 columns a block, 8 threads each.
+struct Sums {
+  const float* part;
+  void* out;
+  int columns, parts;
+  int64_t blocks;
+};
+// Two such sums in one launch, the second's blocks after the first's.
 template <typename T>
-__global__ __launch_bounds__(256) void sums_kernel(const float* part, T* out, int rows, int columns, int parts) {
+__global__ __launch_bounds__(256) void sums_kernel(const Sums first, const Sums second) {
   __shared__ float lds[8][33];
+  const bool other = blockIdx.x >= first.blocks;
+  const Sums& s = other ? second : first;
+  const unsigned block = other ? blockIdx.x - unsigned(first.blocks) : blockIdx.x;
   const int across = threadIdx.x & 31, down = threadIdx.x >> 5;
-  const int blocks = (columns + 31) / 32;
-  const int64_t r = blockIdx.x / unsigned(blocks);
-  const int c = int(blockIdx.x % unsigned(blocks)) * 32 + across;
+  const int blocks = (s.columns + 31) / 32;
+  const int64_t r = block / unsigned(blocks);
+  const int c = int(block % unsigned(blocks)) * 32 + across;
   float v = 0.f;
-  if (c < columns) {
-    const float* p = part + r * parts * columns + c;
+  if (c < s.columns) {
+    const float* p = s.part + r * s.parts * s.columns + c;
 #pragma unroll 8
-    for (int i = down; i < parts; i += 8) v += p[int64_t(i) * columns];
+    for (int i = down; i < s.parts; i += 8) v += p[int64_t(i) * s.columns];
   }
   lds[down][across] = v;
   __syncthreads();
-  if (down || c >= columns) return;
+  if (down || c >= s.columns) return;
   v = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) v += lds[i][across];
-  out[r * columns + c] = from_f32<T>(v);
+  static_cast<T*>(s.out)[r * s.columns + c] = from_f32<T>(v);
 }
 
 // ---------------------------------------------------------------------------------- host
@@ -614,13 +767,15 @@ void each_tile(F&& f) {
 }
 
 struct Plan {
-  int size, splits, steps, tiles_m, tiles_n;
+  int size, splits, steps, tiles_m, tiles_n;  // size -1: small_kernel, whose waves are the splits
   int64_t blocks;
 };
+// small_kernel's: a piece where the CU is full, one that a wave waits for, start and end.
+constexpr Cost SMALL_COST{0.22, 2.0, 3.2};
 // The tile and the parts of the contraction that promise the least time: every CU's blocks one after
 // another, and the parts' sums through memory (at 8 TB/s, for they are still in a cache) and a launch.
 template <typename T, bool SWIGLU>
-Plan plan_of(int64_t m, int64_t n, int64_t k) {
+Plan plan_of(int64_t m, int64_t n, int64_t k, bool transposed) {
   Plan best{};
   double least = 1e30;
   each_tile<T, SWIGLU>([&](auto tile, int size) {
@@ -632,7 +787,7 @@ Plan plan_of(int64_t m, int64_t n, int64_t k) {
       const int64_t each = ceil_div(blocks, CUS), rounds = ceil_div(each, C::PER_CU);
       double us = std::max(double(each) * C::COST.piece, double(rounds) * C::COST.alone) * double(steps) +
                   double(rounds) * C::COST.tile;
-      if (splits > 1) us += 4.0 + double(m) * double(n) * (SWIGLU ? 2 : 1) * 4.0 * (splits + 1) / 8e6;
+      if (splits > 1) us += 5.0 + double(m) * double(n) * (SWIGLU ? 2 : 1) * 4.0 * (splits + 1) / 8e6;
       if (us < least) {
         least = us;
         best = Plan{size, splits, int(steps), int(tm), int(tn), blocks};
@@ -640,39 +795,66 @@ Plan plan_of(int64_t m, int64_t n, int64_t k) {
       if (blocks > 8 * CUS) break;  // (more parts only add to the sums)
     }
   });
+  const int64_t tm = ceil_div(m, SMALL), tn = ceil_div(n, SMALL), pieces = ceil_div(k, SMALL_PIECE<T>);
+  const int64_t each = ceil_div(tm * tn, CUS);
+  for (int waves = 4; waves <= most_waves(SWIGLU, transposed); waves *= 2) {
+    if (waves > 4 && pieces <= waves / 2) break;
+    const int64_t steps = ceil_div(pieces, waves), rounds = ceil_div(each * waves, 16);
+    const double us = std::max(double(each * pieces) * SMALL_COST.piece * (SWIGLU ? 1.5 : 1.0),
+                               double(rounds * steps) * SMALL_COST.alone) + SMALL_COST.tile;
+    if (us < least) {
+      least = us;
+      best = Plan{-1, waves, int(steps), int(tm), int(tn), tm * tn};
+    }
+  }
   return best;
 }
-Plan plan_for(int dtype, int64_t m, int64_t n, int64_t k, bool swiglu) {
-  if (dtype == SIHC_DTYPE_BF16) return swiglu ? plan_of<bf16, true>(m, n, k) : plan_of<bf16, false>(m, n, k);
-  return swiglu ? plan_of<float, true>(m, n, k) : plan_of<float, false>(m, n, k);
+Plan plan_for(int dtype, int64_t m, int64_t n, int64_t k, bool swiglu, bool transposed) {
+  if (dtype == SIHC_DTYPE_BF16)
+    return swiglu ? plan_of<bf16, true>(m, n, k, transposed) : plan_of<bf16, false>(m, n, k, transposed);
+  return swiglu ? plan_of<float, true>(m, n, k, transposed) : plan_of<float, false>(m, n, k, transposed);
 }
 size_t part_bytes(const Plan& p, int64_t m, int64_t n, bool swiglu) {
-  return p.splits > 1 ? size_t(p.splits) * size_t(m) * size_t(n) * (swiglu ? 2 : 1) * sizeof(float) : 0;
+  return p.size >= 0 && p.splits > 1 ? size_t(p.splits) * size_t(m) * size_t(n) * (swiglu ? 2 : 1) * sizeof(float) : 0;
 }
 
+// More dynamic LDS than a launch may have by itself.
+int allow(const void* kernel, size_t bytes, const char* what) {
+  if (bytes <= 65536) return SIHC_OK;
+  const hipError_t err = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+  return err == hipSuccess ? int(SIHC_OK) : fail(SIHC_ERR_HIP, "%s: %s", what, hipGetErrorString(err));
+}
 template <typename T, typename C, bool TA, bool TB, bool SWIGLU>
 int start(const Gemm& g, int64_t blocks, hipStream_t stream, const char* what) {
   using L = Layout<T, C, TA, TB, SWIGLU>;
-  const void* kernel = reinterpret_cast<const void*>(&gemm_kernel<T, C, TA, TB, SWIGLU>);
-  if (L::BYTES > 65536) {
-    const hipError_t err = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, int(L::BYTES));
-    if (err != hipSuccess) return fail(SIHC_ERR_HIP, "%s: %s", what, hipGetErrorString(err));
-  }
-  gemm_kernel<T, C, TA, TB, SWIGLU><<<unsigned(blocks), C::THREADS, L::BYTES, stream>>>(g);
+  const auto kernel = &gemm_kernel<T, C, TA, TB, SWIGLU>;
+  if (const int rc = allow(reinterpret_cast<const void*>(kernel), L::BYTES, what)) return rc;
+  kernel<<<unsigned(blocks), C::THREADS, L::BYTES, stream>>>(g);
   return check_launch(what);
 }
 // g.e, g.a, g.b and the sizes given; `part`: the parts' sums.
 template <typename T, bool TA, bool TB, bool SWIGLU>
 int product(Gemm g, float* part, hipStream_t stream, const char* what) {
-  const Plan p = plan_of<T, SWIGLU>(g.m, g.n, g.k);
-  if (p.blocks * 512 > MOST_LAUNCHED) return fail(SIHC_ERR_INVALID, "%s: too many rows for a launch", what);
+  const Plan p = plan_of<T, SWIGLU>(g.m, g.n, g.k, TA || TB);
+  if (p.blocks * 1024 > MOST_LAUNCHED) return fail(SIHC_ERR_INVALID, "%s: too many rows for a launch", what);
   g.splits = p.splits;
   g.steps = p.steps;
   g.tiles_m = p.tiles_m;
   g.tiles_n = p.tiles_n;
-  g.e.part = p.splits > 1 ? part : nullptr;
+  g.e.part = p.size >= 0 && p.splits > 1 ? part : nullptr;
   g.e.rows = g.m;
   g.e.outer = g.n;
+  if (p.size < 0) {
+    auto launch = [&](auto tiles) {
+      constexpr int TILES_M = decltype(tiles)::value;
+      const size_t lds = size_t(p.splits) * (SWIGLU ? 2 : 1) * 16 * TILES_M * (SMALL + 4) * sizeof(float);
+      const auto kernel = &small_kernel<T, TA, TB, SWIGLU, TILES_M>;
+      if (const int rc = allow(reinterpret_cast<const void*>(kernel), lds, what)) return rc;
+      kernel<<<unsigned(p.blocks), unsigned(64 * p.splits), lds, stream>>>(g);
+      return check_launch(what);
+    };
+    return g.m <= 16 ? launch(IC<1>{}) : launch(IC<2>{});
+  }
   int rc = SIHC_OK;
   each_tile<T, SWIGLU>([&](auto tile, int size) {
     if (size == p.size) rc = start<T, decltype(tile), TA, TB, SWIGLU>(g, p.blocks, stream, what);
@@ -714,8 +896,8 @@ Space space_of(const sihc_linear* l, bool gated) {
   if (l->act != SIHC_ACT_NONE || gated) s.dh = align(l->rows * wide * size);
   s.bias = align(s.images * s.chunks * wide * 4);
   if (gated) s.gate = align(s.images * s.chunks * l->outer * 4);
-  const Plan dx = plan_for(l->dtype, l->rows, l->inner, wide, false);
-  const Plan dw = plan_for(l->dtype, wide, l->inner, l->rows, false);
+  const Plan dx = plan_for(l->dtype, l->rows, l->inner, wide, false, true);
+  const Plan dw = plan_for(l->dtype, wide, l->inner, l->rows, false, true);
   s.part = align(int64_t(std::max(part_bytes(dx, l->rows, l->inner, false), part_bytes(dw, wide, l->inner, false))));
   return s;
 }
@@ -724,11 +906,11 @@ Space space_of(const sihc_linear* l, bool gated) {
 extern "C" size_t sihc_linear_act_workspace_size(const sihc_linear* l) {
   if (check(l, "linear_act") || l->rows == 0) return 0;
   const bool swiglu = l->act == SIHC_ACT_SWIGLU;
-  return part_bytes(plan_for(l->dtype, l->rows, l->outer, l->inner, swiglu), l->rows, l->outer, swiglu);
+  return part_bytes(plan_for(l->dtype, l->rows, l->outer, l->inner, swiglu, false), l->rows, l->outer, swiglu);
 }
 
 extern "C" int sihc_linear_act(const sihc_linear* l, const void* x, const void* weight, const void* bias,
-                               const void* gate, const void* residual, void* y, void* h, uint8_t* low,
+                               const void* gate, const void* residual, void* y, void* h, uint32_t* low,
                                void* workspace, size_t workspace_bytes, void* stream) {
   if (const int rc = check(l, "linear_act")) return rc;
   if (l->rows == 0) return SIHC_OK;
@@ -760,7 +942,7 @@ extern "C" size_t sihc_linear_act_backward_workspace_size(const sihc_linear* l, 
 }
 
 extern "C" int sihc_linear_act_backward(const sihc_linear* l, const void* grad, const void* x, const void* weight,
-                                        const void* h, const uint8_t* low, const void* gate, void* dx, void* dweight,
+                                        const void* h, const uint32_t* low, const void* gate, void* dx, void* dweight,
                                         void* dbias, void* dgate, void* workspace, size_t workspace_bytes, void* stream) {
   if (const int rc = check(l, "linear_act_backward")) return rc;
   const bool swiglu = l->act == SIHC_ACT_SWIGLU, gated = gate != nullptr;
@@ -768,20 +950,20 @@ extern "C" int sihc_linear_act_backward(const sihc_linear* l, const void* grad, 
   const hipStream_t on = hipStream_t(stream);
   if (dgate && !gated) return fail(SIHC_ERR_INVALID, "linear_act_backward: no gate, no gradient of it");
   const char* what = "linear_act_backward";
-  if (l->rows == 0)  // sums over nothing
+  auto sums_of = [](const float* part, void* out, int64_t rows, int columns, int64_t parts) {
+    return Sums{part, out, columns, int(parts), out ? rows * ceil_div(columns, 32) : 0};
+  };
+  auto sum = [&](const Sums& first, const Sums& second) {
+    const int64_t blocks = first.blocks + second.blocks;
+    if (blocks * 256 > MOST_LAUNCHED) return fail(SIHC_ERR_INVALID, "%s: too many rows for a launch", what);
+    if (blocks == 0) return int(SIHC_OK);
     return by_dtype(l->dtype, [&](auto t) {
-      using T = decltype(t);
-      auto clear = [&](void* p, int64_t rows) {
-        if (!p) return int(SIHC_OK);
-        const int64_t blocks = rows * ceil_div(l->inner, 32);
-        if (blocks * 256 > MOST_LAUNCHED) return fail(SIHC_ERR_INVALID, "%s: too many rows for a launch", what);
-        sums_kernel<T><<<unsigned(blocks), 256, 0, on>>>(nullptr, static_cast<T*>(p), int(rows), l->inner, 0);
-        return check_launch(what);
-      };
-      if (const int rc = clear(dweight, wide)) return rc;
-      if (dbias) sums_kernel<T><<<unsigned(ceil_div(wide, 32)), 256, 0, on>>>(nullptr, static_cast<T*>(dbias), 1, wide, 0);
+      sums_kernel<decltype(t)><<<unsigned(blocks), 256, 0, on>>>(first, second);
       return check_launch(what);
     });
+  };
+  if (l->rows == 0)  // sums over nothing
+    return sum(sums_of(nullptr, dweight, wide, l->inner, 0), sums_of(nullptr, dbias, 1, wide, 0));
   if (!grad || !x || !weight || ((gated || l->act != SIHC_ACT_NONE) && !h) ||
       (l->dtype == SIHC_DTYPE_BF16 && l->act != SIHC_ACT_NONE && !low))
     return fail(SIHC_ERR_INVALID, "linear_act_backward: null pointer");
@@ -806,16 +988,9 @@ extern "C" int sihc_linear_act_backward(const sihc_linear* l, const void* grad, 
       else slopes_kernel<T, false><<<unsigned(blocks), 256, 0, on>>>(v);
       if (const int rc = check_launch(what)) return rc;
     }
-    auto sum = [&](const float* from, void* to, int64_t rows, int columns, int64_t parts) {
-      const int64_t blocks = rows * ceil_div(columns, 32);
-      if (blocks * 256 > MOST_LAUNCHED) return fail(SIHC_ERR_INVALID, "%s: too many rows for a launch", what);
-      sums_kernel<T><<<unsigned(blocks), 256, 0, on>>>(from, static_cast<T*>(to), int(rows), columns, int(parts));
-      return check_launch(what);
-    };
-    if (dbias)
-      if (const int rc = sum(bias_part, dbias, 1, wide, s.images * s.chunks)) return rc;
-    if (dgate)
-      if (const int rc = sum(gate_part, dgate, images, l->outer, s.chunks)) return rc;
+    if (const int rc = sum(sums_of(bias_part, dbias, 1, wide, s.images * s.chunks),
+                           sums_of(gate_part, dgate, images, l->outer, s.chunks)))
+      return rc;
     const void* slopes = dh ? dh : grad;
     Gemm g{};
     g.a = slopes;

@@ -872,7 +872,14 @@ sihc_linear linear_of(const Tensor& x, const Tensor& weight, const Tensor& gate,
 }
 bool keeps(const Tensor& gate, int act) { return act != SIHC_ACT_NONE || gate.defined(); }
 bool keeps_low(const Tensor& x, int act) { return act != SIHC_ACT_NONE && x.scalar_type() == at::kBFloat16; }
-// (result, h and its next bits for the backward: empty unless `train`)
+std::vector<int64_t> low_sizes(const Tensor& x, int64_t outer, int act) {
+  std::vector<int64_t> sizes(x.sizes().begin(), x.sizes().end() - 1);
+  sizes.push_back(act == SIHC_ACT_SWIGLU ? 2 : 1);
+  sizes.push_back((outer + 7) / 8);
+  return sizes;
+}
+uint32_t* words(const Tensor& t) { return static_cast<uint32_t*>(t.data_ptr()); }
+// (result, h and more bits of it for the backward: empty unless `train`)
 variable_list run_linear(const Tensor& x, const Tensor& weight, const Tensor& bias, int act, const Tensor& gate,
                          const Tensor& residual, bool train) {
   const c10::DeviceGuard guard(x.device());
@@ -883,18 +890,18 @@ variable_list run_linear(const Tensor& x, const Tensor& weight, const Tensor& bi
   sizes.back() = weight.size(0);
   const bool h_kept = train && keeps(gate, act), low_kept = train && keeps_low(x, act);
   Tensor h = at::empty(h_kept ? sizes : none, x.options());
-  Tensor low = at::empty(low_kept ? sizes : none, x.options().dtype(at::kByte));
+  Tensor low = at::empty(low_kept ? low_sizes(x, l.outer, act) : none, x.options().dtype(at::kInt));
   const size_t bytes = sihc_linear_act_workspace_size(&l);
   if (bytes) ws = workspace(bytes, x);
   check(sihc_linear_act(&l, x.const_data_ptr(), weight.const_data_ptr(), ptr(bias), ptr(gate), ptr(residual),
-                        y.data_ptr(), h_kept ? h.data_ptr() : nullptr, low_kept ? low.data_ptr<uint8_t>() : nullptr,
+                        y.data_ptr(), h_kept ? h.data_ptr() : nullptr, low_kept ? words(low) : nullptr,
                         bytes ? ws.data_ptr() : nullptr, bytes, stream_of(x)),
         true);
   return {y, h, low};
 }
 struct LinearFn : torch::autograd::Function<LinearFn> {
   static constexpr bool is_traceable = true;
-  // rest: h and its next bits (NormFn's pointer)
+  // rest: h and more bits of it (NormFn's pointer)
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias,
                         int64_t act, const std::optional<Tensor>& gate, const std::optional<Tensor>& residual,
                         variable_list* rest) {
@@ -932,8 +939,8 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
       sizes.back() = weight.size(0);
       fits = (!keeps(gate, act) || (plain(h) && h.sizes().equals(sizes) && h.scalar_type() == x.scalar_type() &&
                                     h.device() == x.device())) &&
-             (!keeps_low(x, act) || (plain(low) && low.sizes().equals(sizes) && low.scalar_type() == at::kByte &&
-                                     low.device() == x.device()));
+             (!keeps_low(x, act) || (plain(low) && low.scalar_type() == at::kInt && low.device() == x.device() &&
+                                     low.sizes().equals(low_sizes(x, linear_of(x, weight, gate, act).outer, act))));
       if (act == SIHC_ACT_SWIGLU) sizes.back() /= 2;
       fits = fits && grad.sizes().equals(sizes);
     }
@@ -949,7 +956,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
       auto out_ptr = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
       check(sihc_linear_act_backward(&l, grad.const_data_ptr(), x.const_data_ptr(), weight.const_data_ptr(),
                                      keeps(gate, act) ? h.const_data_ptr() : nullptr,
-                                     keeps_low(x, act) ? low.const_data_ptr<uint8_t>() : nullptr, ptr(gate),
+                                     keeps_low(x, act) ? words(low) : nullptr, ptr(gate),
                                      out_ptr(dx), out_ptr(dw), out_ptr(db), out_ptr(dg), ws.data_ptr(),
                                      size_t(ws.numel()) * 4, stream_of(x)),
             false);

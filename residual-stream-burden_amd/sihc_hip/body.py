@@ -23,7 +23,7 @@ Specification (the reference's bodies are plain PyTorch, sihc/models/sihc/compon
 
 All sums and statistics are fp32, in a fixed order without atomics: identical inputs give identical
 bits. float32 and bfloat16; the norm's weights may be float32 beside bfloat16 heads. In bfloat16 the
-backward of a gate works on h rounded to bfloat16, that of an activation on 24 bits of it, and the
+backward of a gate works on h rounded to bfloat16, that of an activation on 20 bits of it, and the
 gradient of h enters the products rounded to bfloat16. q, k and x of the
 rotations are read through their strides (the channels of a head adjacent); the other tensors are packed.
 """
@@ -98,8 +98,9 @@ def _linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str, gat
 def _linear_act_fake(x, weight, bias, act, gate, residual, train):
     keeps = train and (act != "none" or gate is not None)
     wide = (*x.shape[:-1], weight.shape[0])
-    return (x.new_empty((*x.shape[:-1], _linear_outer(weight, act))), x.new_empty(wide if keeps else (0,)),
-            x.new_empty(wide if launch.keeps_low(x.dtype, act, train) else (0,), dtype=torch.uint8))
+    outer = _linear_outer(weight, act)
+    return (x.new_empty((*x.shape[:-1], outer)), x.new_empty(wide if keeps else (0,)),
+            x.new_empty(launch.low_shape(x, outer, act, train), dtype=torch.int32))
 
 
 @custom_op("sihc::linear_act_backward", mutates_args=())
@@ -113,7 +114,8 @@ def _linear_act_backward(grad: Tensor, x: Tensor, weight: Tensor, h: Tensor, low
     if act != "none" or gate is not None:
         if h.shape != (*x.shape[:-1], weight.shape[0]) or h.dtype != x.dtype:
             raise ValueError("linear_act backward: h must be that of a call with train=True")
-    if launch.keeps_low(x.dtype, act, True) and (low.shape != h.shape or low.dtype != torch.uint8):
+    bits = launch.low_shape(x, _linear_outer(weight, act), act, True)
+    if bits != (0,) and (low.shape != bits or low.dtype != torch.int32):
         raise ValueError("linear_act backward: low must be that of a call with train=True")
     if want_gate and gate is None:
         raise ValueError("linear_act backward: no gate, no gradient of it")

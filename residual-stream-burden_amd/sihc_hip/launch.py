@@ -403,22 +403,25 @@ def _linear(x: Tensor, weight: Tensor, act: str, gate: Optional[Tensor]) -> Line
                   0 if gate is None else gate.stride(0))
 
 
-def keeps_low(dtype: torch.dtype, act: str, train: bool) -> bool:
-    """Whether linear_act keeps more bits of h than its type has: bfloat16 before an activation's slope."""
-    return train and act != "none" and dtype == torch.bfloat16
+def low_shape(x: Tensor, outer: int, act: str, train: bool) -> tuple[int, ...]:
+    """Of the words in which linear_act keeps more bits of h than its type has: bfloat16 before an
+    activation's slope; (0,) elsewhere."""
+    if not train or act == "none" or x.dtype != torch.bfloat16:
+        return (0,)
+    return (*x.shape[:-1], 2 if act == "swiglu" else 1, (outer + 7) // 8)
 
 
 @_on_tensor_device
 def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str, gate: Optional[Tensor],
                residual: Optional[Tensor], train: bool) -> tuple[Tensor, Tensor, Tensor]:
-    """(residual + gate * act(h) with h = x weight^T + bias, and for the backward h [..., weight rows] and its
-    next 8 bits; empty where the backward needs none or `train` is not set)."""
+    """(residual + gate * act(h) with h = x weight^T + bias, and for the backward h [..., weight rows] and 4 more
+    bits of each of its values; empty where the backward needs none or `train` is not set)."""
     l = _linear(x, weight, act, gate)
     keeps = train and (act != "none" or gate is not None)
     out = torch.empty((*x.shape[:-1], l.outer), device=x.device, dtype=x.dtype)
     wide = (*x.shape[:-1], weight.shape[0])
     h = torch.empty(wide if keeps else (0,), device=x.device, dtype=x.dtype)
-    low = torch.empty(wide if keeps_low(x.dtype, act, train) else (0,), device=x.device, dtype=torch.uint8)
+    low = torch.empty(low_shape(x, l.outer, act, train), device=x.device, dtype=torch.int32)
     L = lib()
     nbytes = L.sihc_linear_act_workspace_size(ctypes.byref(l))
     ws = _workspace(nbytes, x.device) if nbytes else None

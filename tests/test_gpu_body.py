@@ -76,6 +76,23 @@ def test_linear_of_many_tiles(size, act, dtype):
     check_linear(linear_case(*size, act, True, True, True, dtype), f"{size} {act} {dtype}")
 
 
+# Sizes for which the forward and the two gradients' products take the larger tiles, one and several parts of
+# the contraction, and tiles that end inside the result.
+@pytest.mark.parametrize("size,act", [((64, 256, 768, 2048), "swiglu"), ((64, 256, 1152, 1152), "none"),
+                                      ((32, 256, 2730, 1024), "none"), ((64, 256, 768, 768), "silu"),
+                                      ((61, 259, 2050, 700), "none"), ((16, 256, 4096, 4096), "none"),
+                                      ((2, None, 1152, 6912), "none"), ((8, 250, 520, 1030), "swiglu")], ids=str)
+def test_linear_of_large_tiles(size, act):
+    announce(f"linear_act {size} {act}")
+    check_linear(linear_case(*size, act, True, True, True, BF16), f"{size} {act}")
+
+
+@pytest.mark.parametrize("size,act", [((16, 256, 1024, 1100), "swiglu"), ((3, 1500, 640, 1000), "silu")], ids=str)
+def test_linear_of_large_tiles_fp32(size, act):
+    announce(f"linear_act {size} {act} fp32")
+    check_linear(linear_case(*size, act, True, True, True, F32), f"{size} {act} fp32")
+
+
 # ------------------------------------------------------------------------- heads and rotation
 GRIDS = {"1": (1,), "grid": (5, 7), "clip": (2, 3, 5), "line": (67,)}
 
