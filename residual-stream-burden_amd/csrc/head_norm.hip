@@ -15,6 +15,7 @@
 #include "cond_common.h"
 
 #include <cmath>
+#include <cstring>
 
 namespace {
 using namespace sihc_cond;
@@ -486,13 +487,28 @@ Args args_of(const sihc_heads* h) {
   return a;
 }
 void take_rates(const sihc_heads* h, Args& a) {
-  const double log = std::log2(h->theta);
-  int pair = 0;
-  for (int i = 0; i < h->axes; ++i)
-    for (int c = 0; c < h->widths[i]; c += 2, ++pair) {
-      a.rate[pair] = std::exp2(-double(c) / double(h->widths[i]) * log) / 6.283185307179586476925;
-      a.axis[pair] = uint8_t(i);
-    }
+  // (a program has few of them: a thread keeps the last)
+  struct Kept {
+    double theta = 0.0;
+    int axes = -1, widths[SIHC_MAX_AXES] = {};
+    double rate[MAX_PAIRS] = {};
+    uint8_t axis[MAX_PAIRS] = {};
+  };
+  thread_local Kept kept;
+  if (kept.theta != h->theta || kept.axes != h->axes || std::memcmp(kept.widths, h->widths, sizeof(kept.widths))) {
+    const double log = std::log2(h->theta);
+    int pair = 0;
+    for (int i = 0; i < h->axes; ++i)
+      for (int c = 0; c < h->widths[i]; c += 2, ++pair) {
+        kept.rate[pair] = std::exp2(-double(c) / double(h->widths[i]) * log) / 6.283185307179586476925;
+        kept.axis[pair] = uint8_t(i);
+      }
+    kept.theta = h->theta;
+    kept.axes = h->axes;
+    std::memcpy(kept.widths, h->widths, sizeof(kept.widths));
+  }
+  std::memcpy(a.rate, kept.rate, sizeof(a.rate));
+  std::memcpy(a.axis, kept.axis, sizeof(a.axis));
 }
 template <typename F>
 int by_lanes(int lanes, F&& f) {

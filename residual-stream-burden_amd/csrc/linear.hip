@@ -15,6 +15,8 @@
 // W_b, so that both halves of a channel meet in one wave.
 #include "cond_common.h"
 
+#include <atomic>
+
 namespace {
 using namespace sihc_cond;
 
@@ -740,7 +742,7 @@ __global__ __launch_bounds__(256) void sums_kernel(const Sums first, const Sums 
 }
 
 // ---------------------------------------------------------------------------------- host
-constexpr int CUS = 256;
+constexpr int CUS = 256, MOST_LDS = 160 * 1024;
 
 // The tiles, the largest first, and what they take by measurement: the time of a piece (of a full CU's, for
 // each block in it; of a block alone on its CU) and of a tile's start and end, in microseconds.
@@ -775,7 +777,7 @@ constexpr Cost SMALL_COST{0.22, 2.0, 3.2};
 // The tile and the parts of the contraction that promise the least time: every CU's blocks one after
 // another, and the parts' sums through memory (at 8 TB/s, for they are still in a cache) and a launch.
 template <typename T, bool SWIGLU>
-Plan plan_of(int64_t m, int64_t n, int64_t k, bool transposed) {
+Plan make_plan(int64_t m, int64_t n, int64_t k, bool transposed) {
   Plan best{};
   double least = 1e30;
   each_tile<T, SWIGLU>([&](auto tile, int size) {
@@ -809,6 +811,20 @@ Plan plan_of(int64_t m, int64_t n, int64_t k, bool transposed) {
   }
   return best;
 }
+// A call asks for the same plan several times, and a program for few of them: a thread keeps the last ones.
+template <typename T, bool SWIGLU>
+Plan plan_of(int64_t m, int64_t n, int64_t k, bool transposed) {
+  struct Kept {
+    int64_t m = -1, n = 0, k = 0;
+    bool transposed = false;
+    Plan plan{};
+  };
+  thread_local Kept kept[64];
+  Kept& e = kept[uint64_t((m * 31 + n) * 31 + k * 2 + transposed) * 0x9E3779B97F4A7C15u >> 58];
+  if (e.m != m || e.n != n || e.k != k || e.transposed != transposed)
+    e = Kept{m, n, k, transposed, make_plan<T, SWIGLU>(m, n, k, transposed)};
+  return e.plan;
+}
 Plan plan_for(int dtype, int64_t m, int64_t n, int64_t k, bool swiglu, bool transposed) {
   if (dtype == SIHC_DTYPE_BF16)
     return swiglu ? plan_of<bf16, true>(m, n, k, transposed) : plan_of<bf16, false>(m, n, k, transposed);
@@ -818,17 +834,27 @@ size_t part_bytes(const Plan& p, int64_t m, int64_t n, bool swiglu) {
   return p.size >= 0 && p.splits > 1 ? size_t(p.splits) * size_t(m) * size_t(n) * (swiglu ? 2 : 1) * sizeof(float) : 0;
 }
 
-// More dynamic LDS than a launch may have by itself.
-int allow(const void* kernel, size_t bytes, const char* what) {
+// More dynamic LDS than a launch may have by itself, once for a kernel on every device.
+template <typename K>
+int allow(K kernel, size_t bytes, std::atomic<uint64_t>& allowed, const char* what) {
   if (bytes <= 65536) return SIHC_OK;
-  const hipError_t err = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
-  return err == hipSuccess ? int(SIHC_OK) : fail(SIHC_ERR_HIP, "%s: %s", what, hipGetErrorString(err));
+  int device = 0;
+  if (hipGetDevice(&device) != hipSuccess) device = 64;
+  const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+  if (allowed.load(std::memory_order_relaxed) & bit) return SIHC_OK;
+  const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, MOST_LDS);
+  if (err != hipSuccess) return fail(SIHC_ERR_HIP, "%s: %s", what, hipGetErrorString(err));
+  allowed.fetch_or(bit, std::memory_order_relaxed);
+  return SIHC_OK;
 }
 template <typename T, typename C, bool TA, bool TB, bool SWIGLU>
 int start(const Gemm& g, int64_t blocks, hipStream_t stream, const char* what) {
   using L = Layout<T, C, TA, TB, SWIGLU>;
   const auto kernel = &gemm_kernel<T, C, TA, TB, SWIGLU>;
-  if (const int rc = allow(reinterpret_cast<const void*>(kernel), L::BYTES, what)) return rc;
+  static_assert(L::BYTES <= MOST_LDS, "a CU's LDS");
+  static std::atomic<uint64_t> allowed{0};
+  if (const int rc = allow(kernel, L::BYTES, allowed, what)) return rc;
   kernel<<<unsigned(blocks), C::THREADS, L::BYTES, stream>>>(g);
   return check_launch(what);
 }
@@ -849,7 +875,8 @@ int product(Gemm g, float* part, hipStream_t stream, const char* what) {
       constexpr int TILES_M = decltype(tiles)::value;
       const size_t lds = size_t(p.splits) * (SWIGLU ? 2 : 1) * 16 * TILES_M * (SMALL + 4) * sizeof(float);
       const auto kernel = &small_kernel<T, TA, TB, SWIGLU, TILES_M>;
-      if (const int rc = allow(reinterpret_cast<const void*>(kernel), lds, what)) return rc;
+      static std::atomic<uint64_t> allowed{0};
+      if (const int rc = allow(kernel, lds, allowed, what)) return rc;
       kernel<<<unsigned(p.blocks), unsigned(64 * p.splits), lds, stream>>>(g);
       return check_launch(what);
     };

@@ -879,18 +879,19 @@ std::vector<int64_t> low_sizes(const Tensor& x, int64_t outer, int act) {
   return sizes;
 }
 uint32_t* words(const Tensor& t) { return static_cast<uint32_t*>(t.data_ptr()); }
-// (result, h and more bits of it for the backward: empty unless `train`)
+// (result, h and more bits of it for the backward: undefined where the backward needs none)
 variable_list run_linear(const Tensor& x, const Tensor& weight, const Tensor& bias, int act, const Tensor& gate,
                          const Tensor& residual, bool train) {
   const c10::DeviceGuard guard(x.device());
   const sihc_linear l = linear_of(x, weight, gate, act);
-  std::vector<int64_t> sizes(x.sizes().begin(), x.sizes().end()), none{0};
+  std::vector<int64_t> sizes(x.sizes().begin(), x.sizes().end());
   sizes.back() = l.outer;
   Tensor y = at::empty(sizes, x.options()), ws;
   sizes.back() = weight.size(0);
   const bool h_kept = train && keeps(gate, act), low_kept = train && keeps_low(x, act);
-  Tensor h = at::empty(h_kept ? sizes : none, x.options());
-  Tensor low = at::empty(low_kept ? low_sizes(x, l.outer, act) : none, x.options().dtype(at::kInt));
+  Tensor h, low;
+  if (h_kept) h = at::empty(sizes, x.options());
+  if (low_kept) low = at::empty(low_sizes(x, l.outer, act), x.options().dtype(at::kInt));
   const size_t bytes = sihc_linear_act_workspace_size(&l);
   if (bytes) ws = workspace(bytes, x);
   check(sihc_linear_act(&l, x.const_data_ptr(), weight.const_data_ptr(), ptr(bias), ptr(gate), ptr(residual),
@@ -945,7 +946,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
       fits = fits && grad.sizes().equals(sizes);
     }
     if (fits) {
-      RECORD_FUNCTION("sihc::linear_act_backward", (Args{grad, x, weight, h, low, maybe(gate), act_name(act)}));
+      RECORD_FUNCTION("sihc::linear_act_backward", (Args{grad, x, weight, maybe(h), maybe(low), maybe(gate), act_name(act)}));
       const c10::DeviceGuard device(x.device());
       const sihc_linear l = linear_of(x, weight, gate, act);
       if (want_x) dx = at::empty_like(x);
@@ -964,8 +965,12 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
       static auto op = registered<std::tuple<Tensor, Tensor, Tensor, Tensor>(
           const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const std::optional<Tensor>&,
           c10::string_view, bool, bool, bool, bool)>("sihc::linear_act_backward");
-      std::tie(dx, dw, db, dg) =
-          op.call(grad, x, weight, h, low, maybe(gate), act_name(act), want_x, want_w, want_b, want_g);
+      auto given_or_empty = [&](const Tensor& t, at::ScalarType type) {
+        return t.defined() ? t : at::empty({0}, x.options().dtype(type));
+      };
+      std::tie(dx, dw, db, dg) = op.call(grad, x, weight, given_or_empty(h, x.scalar_type()),
+                                         given_or_empty(low, at::kInt), maybe(gate), act_name(act), want_x, want_w,
+                                         want_b, want_g);
     }
     if (want_x) out[0] = dx;
     if (want_w) out[1] = dw;
@@ -1402,12 +1407,13 @@ PyObject* py_linear(PyObject* self, PyObject* const* args, Py_ssize_t n) {
     auto listing = [&] {
       return Args{x, weight, maybe(bias), act_name(act), maybe(gate), maybe(residual), train};
     };
+    // (None in the place of what is not kept: the caller reads the result alone, and two empty tensors cost
+    // as much as the launch)
     return tuple_of(call(self, listing, [&] {
       if (unrecorded() || !train) return run_linear(x, weight, bias, act, gate, residual, train);
       variable_list rest;
-      const Tensor out =
-          LinearFn::apply(x, weight, maybe(bias), int64_t(act), maybe(gate), maybe(residual), &rest);
-      return variable_list{out, rest[0], rest[1]};
+      const Tensor y = LinearFn::apply(x, weight, maybe(bias), int64_t(act), maybe(gate), maybe(residual), &rest);
+      return variable_list{y, rest[0], rest[1]};
     }));
   });
 }

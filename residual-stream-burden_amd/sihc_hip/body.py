@@ -157,8 +157,9 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: st
                gate: Optional[Tensor] = None, residual: Optional[Tensor] = None) -> Tensor:
     """residual + gate * act(x weight^T + bias) of x [batch, ..., inner]; act is "none", "silu" or
     "swiglu"; gate [batch, outer], residual like the result [batch, ..., outer]."""
-    train = torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad for t in (x, weight, bias, gate, residual))
+    train = torch.is_grad_enabled() and (
+        x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
+        (gate is not None and gate.requires_grad) or (residual is not None and residual.requires_grad))
     return _linear_act(x, weight, bias, act, gate, residual, train)[0]
 
 
