@@ -367,12 +367,12 @@ __global__ __launch_bounds__(256, 4) void heads_backward_kernel(const Args a) {
             for (int i = 0; i < V / 2; ++i) angle[i] = l.angles[item.t * l.pairs + l.first / 2 + i];
           }
           turn(g, angle);  // (the angles are taken backwards)
-          const float r = reciprocal_rms<LPH>(x, a);
+          const float rms = reciprocal_rms<LPH>(x, a), r = item.valid ? rms : 0.f;  // (0 / 0 without eps)
           float dot = 0.f;
 #pragma unroll
           for (int i = 0; i < V; ++i) {
             x[i] *= r;
-            const float t = g[i] * x[i];  // (zero for a lane without a head)
+            const float t = g[i] * x[i];
             dw[side][i] += t;
             dot += w[i] * t;
           }
@@ -535,6 +535,9 @@ extern "C" int sihc_qk_norm_rotary(const sihc_heads* h, const void* q, const voi
   take_rates(h, a);
   if (!q || !q_out || (k && !k_out) || (a.turned && !positions))
     return fail(SIHC_ERR_INVALID, "qk_norm_rotary: null pointer");
+  for (const void* in : {q, k, q_weight, k_weight, positions})
+    if (in && (in == q_out || in == k_out))
+      return fail(SIHC_ERR_INVALID, "qk_norm_rotary: an output is one of the inputs");
   a.x[0] = q;
   a.x[1] = k;
   a.weight[0] = q_weight;
@@ -582,6 +585,9 @@ extern "C" int sihc_qk_norm_rotary_backward(const sihc_heads* h, const void* gra
     return fail(SIHC_ERR_INVALID, "qk_norm_rotary_backward: the weights and their gradients are needed");
   if (a.total && (!q || !grad_q || !dq || (k && (!grad_k || !dk)) || (a.turned && !positions) || !workspace))
     return fail(SIHC_ERR_INVALID, "qk_norm_rotary_backward: null pointer");
+  for (const void* in : {grad_q, grad_k, q, k, q_weight, k_weight, positions})
+    if (in && (in == dq || in == dk || in == dq_weight || in == dk_weight))
+      return fail(SIHC_ERR_INVALID, "qk_norm_rotary_backward: an output is one of the inputs");
   const int64_t blocks = backward_blocks(a);
   if (workspace_bytes < size_t(blocks) * 2 * size_t(a.dim) * sizeof(float))
     return fail(SIHC_ERR_INVALID, "qk_norm_rotary_backward: workspace of %zu bytes is too small", workspace_bytes);

@@ -944,6 +944,8 @@ extern "C" int sihc_linear_act(const sihc_linear* l, const void* x, const void* 
   if (!x || !weight || !y || (low && !h)) return fail(SIHC_ERR_INVALID, "linear_act: null pointer");
   if (low && (l->dtype != SIHC_DTYPE_BF16 || l->act == SIHC_ACT_NONE))
     return fail(SIHC_ERR_INVALID, "linear_act: more bits of h are for bf16 with an activation");
+  for (const void* in : {x, weight, bias, gate})
+    if (in && (in == y || in == h)) return fail(SIHC_ERR_INVALID, "linear_act: an output is one of the inputs");
   const size_t need = sihc_linear_act_workspace_size(l);
   if (need && (!workspace || workspace_bytes < need))
     return fail(SIHC_ERR_INVALID, "linear_act: workspace of %zu bytes, %zu needed", workspace_bytes, need);
@@ -994,6 +996,10 @@ extern "C" int sihc_linear_act_backward(const sihc_linear* l, const void* grad, 
   if (!grad || !x || !weight || ((gated || l->act != SIHC_ACT_NONE) && !h) ||
       (l->dtype == SIHC_DTYPE_BF16 && l->act != SIHC_ACT_NONE && !low))
     return fail(SIHC_ERR_INVALID, "linear_act_backward: null pointer");
+  for (const void* out : {static_cast<const void*>(dx), static_cast<const void*>(dweight),
+                          static_cast<const void*>(dbias), static_cast<const void*>(dgate)})
+    for (const void* in : {grad, x, weight, h, gate})
+      if (out && out == in) return fail(SIHC_ERR_INVALID, "linear_act_backward: an output is one of the inputs");
   const Space s = space_of(l, gated);
   if (!workspace || workspace_bytes < size_t(s.total()))
     return fail(SIHC_ERR_INVALID, "linear_act_backward: workspace of %zu bytes, %lld needed", workspace_bytes,

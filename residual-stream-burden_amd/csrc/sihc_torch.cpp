@@ -879,7 +879,7 @@ std::vector<int64_t> low_sizes(const Tensor& x, int64_t outer, int act) {
   return sizes;
 }
 uint32_t* words(const Tensor& t) { return static_cast<uint32_t*>(t.data_ptr()); }
-// (result, h and more bits of it for the backward: undefined where the backward needs none)
+// (result, h and more bits of it for the backward: undefined unless `train`, empty where it needs none)
 variable_list run_linear(const Tensor& x, const Tensor& weight, const Tensor& bias, int act, const Tensor& gate,
                          const Tensor& residual, bool train) {
   const c10::DeviceGuard guard(x.device());
@@ -890,8 +890,11 @@ variable_list run_linear(const Tensor& x, const Tensor& weight, const Tensor& bi
   sizes.back() = weight.size(0);
   const bool h_kept = train && keeps(gate, act), low_kept = train && keeps_low(x, act);
   Tensor h, low;
-  if (h_kept) h = at::empty(sizes, x.options());
-  if (low_kept) low = at::empty(low_sizes(x, l.outer, act), x.options().dtype(at::kInt));
+  if (train) {
+    const std::vector<int64_t> none{0};
+    h = at::empty(h_kept ? sizes : none, x.options());
+    low = at::empty(low_kept ? low_sizes(x, l.outer, act) : none, x.options().dtype(at::kInt));
+  }
   const size_t bytes = sihc_linear_act_workspace_size(&l);
   if (bytes) ws = workspace(bytes, x);
   check(sihc_linear_act(&l, x.const_data_ptr(), weight.const_data_ptr(), ptr(bias), ptr(gate), ptr(residual),
@@ -946,7 +949,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
       fits = fits && grad.sizes().equals(sizes);
     }
     if (fits) {
-      RECORD_FUNCTION("sihc::linear_act_backward", (Args{grad, x, weight, maybe(h), maybe(low), maybe(gate), act_name(act)}));
+      RECORD_FUNCTION("sihc::linear_act_backward", (Args{grad, x, weight, h, low, maybe(gate), act_name(act)}));
       const c10::DeviceGuard device(x.device());
       const sihc_linear l = linear_of(x, weight, gate, act);
       if (want_x) dx = at::empty_like(x);
@@ -965,12 +968,8 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
       static auto op = registered<std::tuple<Tensor, Tensor, Tensor, Tensor>(
           const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const std::optional<Tensor>&,
           c10::string_view, bool, bool, bool, bool)>("sihc::linear_act_backward");
-      auto given_or_empty = [&](const Tensor& t, at::ScalarType type) {
-        return t.defined() ? t : at::empty({0}, x.options().dtype(type));
-      };
-      std::tie(dx, dw, db, dg) = op.call(grad, x, weight, given_or_empty(h, x.scalar_type()),
-                                         given_or_empty(low, at::kInt), maybe(gate), act_name(act), want_x, want_w,
-                                         want_b, want_g);
+      std::tie(dx, dw, db, dg) =
+          op.call(grad, x, weight, h, low, maybe(gate), act_name(act), want_x, want_w, want_b, want_g);
     }
     if (want_x) out[0] = dx;
     if (want_w) out[1] = dw;
@@ -1391,30 +1390,30 @@ bool unwrap_axes(PyObject* o, Axes& axes) {
     if (!unwrap_integer(PySequence_Fast_GET_ITEM(o, i), axes[size_t(i)])) return false;
   return true;
 }
+template <bool KEEPS>  // what the backward needs, with an autograd node; else the result alone
 PyObject* py_linear(PyObject* self, PyObject* const* args, Py_ssize_t n) {
-  if (n != 7 || !PyUnicode_CheckExact(args[3]) || !PyBool_Check(args[6])) return not_implemented();
+  if (n != 6 || !PyUnicode_CheckExact(args[3])) return not_implemented();
   int act = -1;
   for (const int a : {int(SIHC_ACT_NONE), int(SIHC_ACT_SILU), int(SIHC_ACT_SWIGLU)})
     if (PyUnicode_CompareWithASCIIString(args[3], act_name(a)) == 0) act = a;
   if (act < 0) return not_implemented();
-  const bool train = args[6] == Py_True;
   return guarded(self, [&]() -> PyObject* {
     Tensor x, weight, bias, gate, residual;
     if (!unwrap(args[0], x) || !unwrap(args[1], weight) || !unwrap_maybe(args[2], bias) ||
         !unwrap_maybe(args[4], gate) || !unwrap_maybe(args[5], residual) ||
         !linear_fits(x, weight, bias, gate, residual, act))
       return not_implemented();
-    auto listing = [&] {
-      return Args{x, weight, maybe(bias), act_name(act), maybe(gate), maybe(residual), train};
-    };
-    // (None in the place of what is not kept: the caller reads the result alone, and two empty tensors cost
-    // as much as the launch)
-    return tuple_of(call(self, listing, [&] {
-      if (unrecorded() || !train) return run_linear(x, weight, bias, act, gate, residual, train);
+    if (!KEEPS && !unrecorded())  // (an op without a rule: autograd says so)
+      for (const Tensor* t : {&x, &weight, &bias, &gate, &residual})
+        if (t->defined() && t->requires_grad()) return not_implemented();
+    auto listing = [&] { return Args{x, weight, maybe(bias), act_name(act), maybe(gate), maybe(residual)}; };
+    const variable_list out = call(self, listing, [&] {
+      if (!KEEPS || unrecorded()) return run_linear(x, weight, bias, act, gate, residual, KEEPS);
       variable_list rest;
       const Tensor y = LinearFn::apply(x, weight, maybe(bias), int64_t(act), maybe(gate), maybe(residual), &rest);
       return variable_list{y, rest[0], rest[1]};
-    }));
+    });
+    return KEEPS ? tuple_of(out) : THPVariable_Wrap(out[0]);
   });
 }
 PyObject* py_qk(PyObject* self, PyObject* const* args, Py_ssize_t n) {
@@ -1477,7 +1476,8 @@ PyMethodDef entries[] = {
     define<py_block_write>("block_write"),   define<py_gather>("gather_cells"),
     define<py_scatter>("scatter_cells"),     define<py_embed>("embedding_lookup"),
     define<py_norm>("group_norm_act"),       define<py_attention>("cross_attention"),
-    define<py_linear>("linear_act"),         define<py_qk>("qk_norm_rotary"),
+    define<py_linear<true>>("linear_act"),   define<py_linear<false>>("linear_act_result"),
+    define<py_qk>("qk_norm_rotary"),
     define<py_rotary>("axis_rotary"),        define<py_dropout>("dropout"),
 };
 // entry(name, op): the native entry `name` for the registered op `op` ("namespace::name")

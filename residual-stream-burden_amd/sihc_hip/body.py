@@ -87,20 +87,36 @@ def _check_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str, g
     _require_gpu("linear_act", x, **others)
 
 
+# The result alone, for a call that nothing differentiates.
+@custom_op("sihc::linear_act_result", mutates_args=())
+def _linear_act_result(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str, gate: Optional[Tensor],
+                       residual: Optional[Tensor]) -> Tensor:
+    _check_linear(x, weight, bias, act, gate, residual)
+    return launch.linear_act(x, weight, bias, act, gate, residual, False)[0]
+
+
+@_linear_act_result.register_fake
+def _linear_act_result_fake(x, weight, bias, act, gate, residual):
+    return x.new_empty((*x.shape[:-1], _linear_outer(weight, act)))
+
+
+native(_linear_act_result, "linear_act_result")
+
+
+# The result and what the backward needs of h (empty where it needs nothing).
 @custom_op("sihc::linear_act", mutates_args=())
 def _linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str, gate: Optional[Tensor],
-                residual: Optional[Tensor], train: bool) -> tuple[Tensor, Tensor, Tensor]:
+                residual: Optional[Tensor]) -> tuple[Tensor, Tensor, Tensor]:
     _check_linear(x, weight, bias, act, gate, residual)
-    return launch.linear_act(x, weight, bias, act, gate, residual, train)
+    return launch.linear_act(x, weight, bias, act, gate, residual, True)
 
 
 @_linear_act.register_fake
-def _linear_act_fake(x, weight, bias, act, gate, residual, train):
-    keeps = train and (act != "none" or gate is not None)
-    wide = (*x.shape[:-1], weight.shape[0])
+def _linear_act_fake(x, weight, bias, act, gate, residual):
     outer = _linear_outer(weight, act)
-    return (x.new_empty((*x.shape[:-1], outer)), x.new_empty(wide if keeps else (0,)),
-            x.new_empty(launch.low_shape(x, outer, act, train), dtype=torch.int32))
+    kept = (*x.shape[:-1], weight.shape[0]) if act != "none" or gate is not None else (0,)
+    return (x.new_empty((*x.shape[:-1], outer)), x.new_empty(kept),
+            x.new_empty(launch.low_shape(x, outer, act), dtype=torch.int32))
 
 
 @custom_op("sihc::linear_act_backward", mutates_args=())
@@ -113,10 +129,10 @@ def _linear_act_backward(grad: Tensor, x: Tensor, weight: Tensor, h: Tensor, low
         raise ValueError("linear_act backward: the output gradient must match the output")
     if act != "none" or gate is not None:
         if h.shape != (*x.shape[:-1], weight.shape[0]) or h.dtype != x.dtype:
-            raise ValueError("linear_act backward: h must be that of a call with train=True")
-    bits = launch.low_shape(x, _linear_outer(weight, act), act, True)
+            raise ValueError("linear_act backward: h must be that of the forward")
+    bits = launch.low_shape(x, _linear_outer(weight, act), act)
     if bits != (0,) and (low.shape != bits or low.dtype != torch.int32):
-        raise ValueError("linear_act backward: low must be that of a call with train=True")
+        raise ValueError("linear_act backward: low must be that of the forward")
     if want_gate and gate is None:
         raise ValueError("linear_act backward: no gate, no gradient of it")
     _require_gpu("linear_act backward", x, grad=grad, h=h, low=low)
@@ -131,7 +147,7 @@ def _linear_act_backward_fake(grad, x, weight, h, low, gate, act, want_x, want_w
 
 
 def _linear_setup(ctx, inputs, output):
-    x, weight, bias, ctx.act, gate, residual, _ = inputs
+    x, weight, bias, ctx.act, gate, residual = inputs
     ctx.mark_non_differentiable(output[1], output[2])
     ctx.set_materialize_grads(False)
     ctx.save_for_backward(x, weight, gate, output[1], output[2])
@@ -139,14 +155,14 @@ def _linear_setup(ctx, inputs, output):
 
 def _linear_autograd(ctx, grad, _, __):
     if grad is None:
-        return (None,) * 7
+        return (None,) * 6
     x, weight, gate, h, low = ctx.saved_tensors
     want = [ctx.needs_input_grad[i] for i in (0, 1, 2, 4)]
     if not any(want):
-        return None, None, None, None, None, grad, None
+        return None, None, None, None, None, grad
     grads = _linear_act_backward(grad.contiguous(), x, weight, h, low, gate, ctx.act, *want)
     dx, dweight, dbias, dgate = (g if w else None for g, w in zip(grads, want))
-    return dx, dweight, dbias, None, dgate, grad if ctx.needs_input_grad[5] else None, None
+    return dx, dweight, dbias, None, dgate, grad if ctx.needs_input_grad[5] else None
 
 
 register_autograd(_linear_act, _linear_autograd, setup_context=_linear_setup)
@@ -157,10 +173,11 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: st
                gate: Optional[Tensor] = None, residual: Optional[Tensor] = None) -> Tensor:
     """residual + gate * act(x weight^T + bias) of x [batch, ..., inner]; act is "none", "silu" or
     "swiglu"; gate [batch, outer], residual like the result [batch, ..., outer]."""
-    train = torch.is_grad_enabled() and (
-        x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
-        (gate is not None and gate.requires_grad) or (residual is not None and residual.requires_grad))
-    return _linear_act(x, weight, bias, act, gate, residual, train)[0]
+    if torch.is_grad_enabled() and (
+            x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
+            (gate is not None and gate.requires_grad) or (residual is not None and residual.requires_grad)):
+        return _linear_act(x, weight, bias, act, gate, residual)[0]
+    return _linear_act_result(x, weight, bias, act, gate, residual)
 
 
 # --------------------------------------------------------------------- head norms and rotation
@@ -189,7 +206,6 @@ def _check_heads(op: str, positions: Tensor, axes: Sequence[int], theta: float, 
                          f"{tuple(positions.shape)}")
     if positions.dtype not in (torch.int32, torch.float32):
         raise ValueError(f"{op}: positions must be int32 or float32, got {positions.dtype}")
-    _require_gpu(op, first, positions=positions, **heads)
 
 
 def _check_qk(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, positions: Tensor, axes: Sequence[int],
@@ -203,7 +219,7 @@ def _check_qk(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, position
         raise ValueError(f"{op}: weights of the heads' type or float32")
     if not 0.0 <= eps < math.inf:
         raise ValueError(f"{op}: eps must not be negative, got {eps}")
-    _require_gpu(op, q, q_weight=q_weight, k_weight=k_weight)
+    _require_gpu(op, q, k=k, q_weight=q_weight, k_weight=k_weight, positions=positions)
 
 
 @custom_op("sihc::qk_norm_rotary", mutates_args=())
@@ -259,6 +275,7 @@ def qk_norm_rotary(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, pos
 @custom_op("sihc::axis_rotary", mutates_args=())
 def _axis_rotary(x: Tensor, positions: Tensor, axes: Sequence[int], theta: float, inverse: bool) -> Tensor:
     _check_heads("axis_rotary", positions, axes, theta, x=x)
+    _require_gpu("axis_rotary", x, positions=positions)
     return launch.axis_rotary(x, positions, axes, theta, inverse)
 
 

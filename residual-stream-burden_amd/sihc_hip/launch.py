@@ -403,10 +403,10 @@ def _linear(x: Tensor, weight: Tensor, act: str, gate: Optional[Tensor]) -> Line
                   0 if gate is None else gate.stride(0))
 
 
-def low_shape(x: Tensor, outer: int, act: str, train: bool) -> tuple[int, ...]:
+def low_shape(x: Tensor, outer: int, act: str) -> tuple[int, ...]:
     """Of the words in which linear_act keeps more bits of h than its type has: bfloat16 before an
     activation's slope; (0,) elsewhere."""
-    if not train or act == "none" or x.dtype != torch.bfloat16:
+    if act == "none" or x.dtype != torch.bfloat16:
         return (0,)
     return (*x.shape[:-1], 2 if act == "swiglu" else 1, (outer + 7) // 8)
 
@@ -421,7 +421,7 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str, gate
     out = torch.empty((*x.shape[:-1], l.outer), device=x.device, dtype=x.dtype)
     wide = (*x.shape[:-1], weight.shape[0])
     h = torch.empty(wide if keeps else (0,), device=x.device, dtype=x.dtype)
-    low = torch.empty(low_shape(x, l.outer, act, train), device=x.device, dtype=torch.int32)
+    low = torch.empty(low_shape(x, l.outer, act) if train else (0,), device=x.device, dtype=torch.int32)
     L = lib()
     nbytes = L.sihc_linear_act_workspace_size(ctypes.byref(l))
     ws = _workspace(nbytes, x.device) if nbytes else None

@@ -6,7 +6,8 @@ sihc/models/sihc/sublayer.py:30-128) with what a prompt needs: its token ids are
 every block's attention update also attends them (`cross_attention`, each image with its prompt's
 own length, 0 for the unconditional half of classifier-free guidance), and the carrier passes a
 group norm with SiLU (`group_norm_act`) before the head. Routing and the other bodies are those
-of `e2e`. The reference has no text conditioning.
+of `e2e`, and so are `body="fused"` and `dropout`, which take the cross attention's projections and
+update too. The reference has no text conditioning.
 
     model = TextSiHCDenoiser(hidden=1152, heads=16, vocab=32768).to("cuda", torch.bfloat16)
     out = model(images, t, labels, tokens, lengths)     # tokens [B, L] int32, lengths [B] int32
@@ -20,6 +21,7 @@ import torch
 import torch.nn as nn
 from torch import Tensor
 
+from .body import linear_act
 from .conditioning import cross_attention, embedding_lookup, group_norm_act
 from .e2e import RMSNorm, SiHCDenoiser
 
@@ -42,6 +44,16 @@ class CrossAttention(nn.Module):
         q = self.q_norm(self.q(self.norm(z)).reshape(b, n, self.heads, self.head_dim))
         k, v = self.kv(states).reshape(b, -1, 2, self.kv_heads, self.head_dim).unbind(2)
         return self.proj(attend(q, self.k_norm(k), v, lengths).reshape(b, n, c))
+
+    def fused(self, z: Tensor, states: Tensor, lengths: Tensor, attend, gate: Tensor,
+              residual: Optional[Tensor]) -> Tensor:
+        """residual + gate * forward(z, ...), the projections on the HIP operators."""
+        b, n, c = z.shape
+        q = self.q_norm(linear_act(self.norm(z), self.q.weight, self.q.bias).reshape(b, n, self.heads, self.head_dim))
+        kv = linear_act(states, self.kv.weight, self.kv.bias)
+        k, v = kv.reshape(b, -1, 2, self.kv_heads, self.head_dim).unbind(2)
+        out = attend(q, self.k_norm(k), v, lengths).reshape(b, n, c)
+        return linear_act(out, self.proj.weight, self.proj.bias, gate=gate, residual=residual)
 
 
 class GroupNormAct(nn.Module):
@@ -78,7 +90,15 @@ class TextSiHCDenoiser(SiHCDenoiser):
         prefix, text = context
         dz, prefix = super()._update(block, part, z, mod, prefix, index)
         if part == 0 and text is not None:
-            dz = dz + mod[2].unsqueeze(1) * self.cross[index](z, *text, self.attend)
+            seed = prefix[1]
+            if self.body == "torch":
+                update = mod[2].unsqueeze(1) * self.cross[index](z, *text, self.attend)
+                dz = self._dropped(update, seed, 4 * index + 2, dz)
+            elif seed is None:
+                dz = self.cross[index].fused(z, *text, self.attend, mod[2], dz)
+            else:
+                update = self.cross[index].fused(z, *text, self.attend, mod[2], None)
+                dz = self._dropped(update, seed, 4 * index + 2, dz)
         return dz, (prefix, text)
 
     def forward(self, x: Tensor, t: Tensor, y: Tensor, tokens: Optional[Tensor] = None,
