@@ -28,20 +28,20 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 constexpr int V = 8;  // adjacent channels of a thread in every epilogue
 
 // ------------------------------------------------------------------------------- row vectors
-// n <= V channels of a row from p as fp32, zeros past them.
-template <typename T>
+// n <= V channels of a row from p as fp32, zeros past them (WHOLE: there are V).
+template <bool WHOLE = false, typename T>
 __device__ __forceinline__ void get(const T* p, int left, float* o) {
-  if (left >= V) {
+  if (WHOLE || left >= V) {
     load_f32<T, V>(p, o);
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = i < left ? to_f32(p[i]) : 0.f;
   }
 }
-template <typename T>
+template <bool WHOLE = false, typename T>
 __device__ __forceinline__ void put(T* p, int left, const float* v) {
   constexpr int PIECE = 16 / int(sizeof(T));
-  if (left >= V) {
+  if (WHOLE || left >= V) {
 #pragma unroll
     for (int i = 0; i < V; i += PIECE) store(p + i, Vec<T, PIECE>::of(v + i));
   } else {
@@ -68,10 +68,10 @@ __device__ __forceinline__ Vec<T, N> load_some(const T* p, int left) {
 // times as far from the exact ones as their own rounding does (with 20: 1.35, from the rounding of dh as an
 // operand). `low` is [rows, parts of h, words_of(outer)].
 __host__ __device__ constexpr int words_of(int outer) { return (outer + V - 1) / V; }
-template <typename T>
+template <typename T, bool WHOLE>
 __device__ __forceinline__ void put_kept(void* h, uint32_t* low, int64_t at, int left, const float* v) {
   if (sizeof(T) == 4 || !low) {
-    put(static_cast<T*>(h) + at, left, v);
+    put<WHOLE>(static_cast<T*>(h) + at, left, v);
     return;
   }
   uint16_t high[V];
@@ -83,7 +83,7 @@ __device__ __forceinline__ void put_kept(void* h, uint32_t* low, int64_t at, int
     rest |= (bits >> 12 & 0xfu) << (4 * i);
   }
   uint16_t* to = static_cast<uint16_t*>(h) + at;
-  if (left >= V) {
+  if (WHOLE || left >= V) {
     typedef u32x4 words __attribute__((aligned(2)));
     words w;
     __builtin_memcpy(&w, high, 16);
@@ -109,7 +109,12 @@ struct Epilogue {
   float* part;         // [splits][rows][columns] sums instead of the result, or null
   int64_t gate_stride;
   int rows, outer, act, rows_per_gate;
+  uint32_t magic;  // row / rows_per_gate is the high word of row * magic, shifted (magic 0: the row itself)
+  int shift;
 };
+__device__ __forceinline__ int image_of(const Epilogue& e, int row) {
+  return e.magic ? int(__umulhi(uint32_t(row), e.magic) >> e.shift) : row;
+}
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }  // (1 ulp)
 
 // V channels of a row as they are in memory, on their way while something else is done.
@@ -117,8 +122,9 @@ template <typename T>
 struct Row {
   static constexpr int N = V * int(sizeof(T)) / 16;
   u32x4 raw[N];
+  template <bool WHOLE>
   __device__ __forceinline__ void fetch(const T* p, int left) {
-    if (left >= V) {
+    if (WHOLE || left >= V) {
 #pragma unroll
       for (int i = 0; i < N; ++i) raw[i] = load<T, V / N>(p + i * (V / N)).raw;
     } else {
@@ -142,22 +148,25 @@ struct Bias {
   Row<T> a, b;
   __device__ __forceinline__ Bias(const Epilogue& e, int col) {
     if (!e.bias || col >= e.outer) return;
-    a.fetch(static_cast<const T*>(e.bias) + col, e.outer - col);
-    if constexpr (SWIGLU) b.fetch(static_cast<const T*>(e.bias) + e.outer + col, e.outer - col);
+    a.template fetch<false>(static_cast<const T*>(e.bias) + col, e.outer - col);
+    if constexpr (SWIGLU) b.template fetch<false>(static_cast<const T*>(e.bias) + e.outer + col, e.outer - col);
   }
 };
 template <typename T>
 struct Rest {
   Row<T> gate, residual;
+  template <bool WHOLE>
   __device__ __forceinline__ void fetch(const Epilogue& e, int row, int col) {
+    const int left = e.outer - col;
     if (e.gate)
-      gate.fetch(static_cast<const T*>(e.gate) + int64_t(row / e.rows_per_gate) * e.gate_stride + col, e.outer - col);
-    if (e.residual) residual.fetch(static_cast<const T*>(e.residual) + int64_t(row) * e.outer + col, e.outer - col);
+      gate.template fetch<WHOLE>(static_cast<const T*>(e.gate) + image_of(e, row) * e.gate_stride + col, left);
+    if (e.residual)
+      residual.template fetch<WHOLE>(static_cast<const T*>(e.residual) + int64_t(row) * e.outer + col, left);
   }
 };
 
 // Channels col .. col + V - 1 of row `row` from the products: a of W's first rows, b (SwiGLU) of its second.
-template <typename T, bool SWIGLU>
+template <typename T, bool SWIGLU, bool WHOLE>
 __device__ __forceinline__ void finish(const Epilogue& e, const Bias<T, SWIGLU>& bias, const Rest<T>& rest, int row,
                                        int col, float* a, float* b) {
   const int left = e.outer - col;
@@ -175,9 +184,9 @@ __device__ __forceinline__ void finish(const Epilogue& e, const Bias<T, SWIGLU>&
   if (e.h) {
     const int64_t first = int64_t(row) * (SWIGLU ? 2 : 1);
     uint32_t* low = e.low ? e.low + first * words_of(e.outer) + col / V : nullptr;
-    put_kept<T>(e.h, low, first * e.outer + col, left, a);
+    put_kept<T, WHOLE>(e.h, low, first * e.outer + col, left, a);
     if constexpr (SWIGLU)
-      put_kept<T>(e.h, low ? low + words_of(e.outer) : nullptr, (first + 1) * e.outer + col, left, b);
+      put_kept<T, WHOLE>(e.h, low ? low + words_of(e.outer) : nullptr, (first + 1) * e.outer + col, left, b);
   }
   if constexpr (SWIGLU) {
 #pragma unroll
@@ -196,7 +205,7 @@ __device__ __forceinline__ void finish(const Epilogue& e, const Bias<T, SWIGLU>&
 #pragma unroll
     for (int i = 0; i < V; ++i) a[i] += t[i];
   }
-  put(static_cast<T*>(e.y) + int64_t(row) * e.outer + col, left, a);
+  put<WHOLE>(static_cast<T*>(e.y) + int64_t(row) * e.outer + col, left, a);
 }
 
 // ---------------------------------------------------------------------------------- products
@@ -377,13 +386,13 @@ __global__ __launch_bounds__(C::THREADS, C::PER_SIMD) void gemm_kernel(const Gem
   for (int k0 = from; k0 < k; k0 += C::BK, buffer ^= 1) {
     T* next = lds + (buffer ^ 1) * L::BUFFER;
     const T *pa = lds + buffer * L::BUFFER, *pb = pa + A::SIZE;
+    if (k0 + C::BK < k) {
+      a.commit(next);
+      b.commit(next + A::SIZE);
+      if (k0 + 2 * C::BK < k) fetch(k0 + 2 * C::BK);
+    }
 #pragma unroll
     for (int s = 0; s < C::BK / Matrix<T>::STEP; ++s) {
-      if (s == 0 && k0 + C::BK < k) {
-        a.commit(next);
-        b.commit(next + A::SIZE);
-        if (k0 + 2 * C::BK < k) fetch(k0 + 2 * C::BK);
-      }
       typename Matrix<T>::Frag fa[C::MT], fb[C::NT];
 #pragma unroll
       for (int i = 0; i < C::MT; ++i) fa[i] = A::fragment(pa, wm + i * 32, s);
@@ -404,38 +413,54 @@ __global__ __launch_bounds__(C::THREADS, C::PER_SIMD) void gemm_kernel(const Gem
   constexpr int GROUPS = WIDE / V, ROWS = 64 / GROUPS, PASSES = (32 + ROWS - 1) / ROWS;  // (three tiles: 60 lanes)
   const int c = lane % GROUPS * V, col = n0 + (SWIGLU ? wn / 2 : wn) + c;
   const Bias<T, SWIGLU> bias(g.e, col);
+  auto leave = [&](auto whole, const Rest<T>& rest, int r, int row) {
+    constexpr bool WHOLE = decltype(whole)::value != 0;
+    float p[V], q[V];
+    const float* from_strip = strip + r * L::STRIP + (SWIGLU ? c / 32 * 64 + c % 32 : c);
 #pragma unroll
+    for (int x = 0; x < V; ++x) p[x] = from_strip[x];
+    if constexpr (SWIGLU)
+#pragma unroll
+      for (int x = 0; x < V; ++x) q[x] = from_strip[32 + x];
+    if (g.e.part) {
+      float* to = g.e.part + (int64_t(part) * g.m + row) * (SWIGLU ? 2 : 1) * g.n + col;
+      put<WHOLE>(to, g.n - col, p);
+      if constexpr (SWIGLU) put<WHOLE>(to + g.n, g.n - col, q);
+    } else {
+      finish<T, SWIGLU, WHOLE>(g.e, bias, rest, row, col, p, q);
+    }
+  };
+  const bool inside = m0 + C::BM <= g.m && n0 + COLUMNS <= g.n;  // (the block's tile: no test for a row or a channel)
+  const int r0 = lane / GROUPS;
+  // two strips side by side, so that both have their loads under way; four would be too much code
+  constexpr int STRIPS = C::MT <= 2 ? 2 : 1;
+#pragma unroll STRIPS
   for (int i = 0; i < C::MT; ++i) {
     const int row0 = m0 + wm + i * 32;
-    const int end = lane < GROUPS * ROWS && col < g.n ? min(32, g.m - row0) : 0;  // the lane's rows of the strip
     Rest<T> rest[PASSES];
-    if (!g.e.part)
+    if (inside && !g.e.part)
+#pragma unroll
+      for (int r = 0; r < PASSES; ++r) rest[r].template fetch<true>(g.e, min(row0 + r0 + r * ROWS, g.m - 1), col);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int x = 0; x < C::MT; ++x)
+      if (x == i)
+#pragma unroll
+        for (int j = 0; j < C::NT; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) strip[row_of(r, lane >> 5) * L::STRIP + j * 32 + (lane & 31)] = acc[x][j][r];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (inside) {
 #pragma unroll
       for (int r = 0; r < PASSES; ++r)
-        if (lane / GROUPS + r * ROWS < end) rest[r].fetch(g.e, row0 + lane / GROUPS + r * ROWS, col);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-    for (int j = 0; j < C::NT; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) strip[row_of(r, lane >> 5) * L::STRIP + j * 32 + (lane & 31)] = acc[i][j][r];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-    for (int r = 0; r < PASSES; ++r) {
-      if (lane / GROUPS + r * ROWS >= end) break;
-      const int row = row0 + lane / GROUPS + r * ROWS;
-      float p[V], q[V];
-      const float* from_strip = strip + (lane / GROUPS + r * ROWS) * L::STRIP + (SWIGLU ? c / 32 * 64 + c % 32 : c);
-#pragma unroll
-      for (int x = 0; x < V; ++x) p[x] = from_strip[x];
-      if constexpr (SWIGLU)
-#pragma unroll
-        for (int x = 0; x < V; ++x) q[x] = from_strip[32 + x];
-      if (g.e.part) {
-        float* to = g.e.part + (int64_t(part) * g.m + row) * (SWIGLU ? 2 : 1) * g.n + col;
-        put(to, g.n - col, p);
-        if constexpr (SWIGLU) put(to + g.n, g.n - col, q);
-      } else {
-        finish<T, SWIGLU>(g.e, bias, rest[r], row, col, p, q);
+        if ((32 % ROWS == 0 || r0 + r * ROWS < 32) && (64 % GROUPS == 0 || lane < GROUPS * ROWS))
+          leave(IC<1>{}, rest[r], r0 + r * ROWS, row0 + r0 + r * ROWS);
+    } else {
+#pragma unroll 1
+      for (int r = r0; r < 32; r += ROWS) {
+        if (row0 + r >= g.m || col >= g.n || lane >= GROUPS * ROWS) break;
+        if (!g.e.part) rest[0].template fetch<false>(g.e, row0 + r, col);
+        leave(IC<0>{}, rest[0], r, row0 + r);
       }
     }
   }
@@ -519,13 +544,11 @@ __device__ __forceinline__ f32x4 multiply16(const f32x4& a, const f32x4& b, f32x
 }
 
 template <typename T, bool TA, bool TB, bool SWIGLU, int TILES_M>
-__global__ __launch_bounds__(64 * most_waves(SWIGLU, TA || TB)) void small_kernel(const Gemm g) {
-  extern __shared__ __align__(16) char lds_bytes[];
-  float* lds = reinterpret_cast<float*>(lds_bytes);
+__device__ __forceinline__ void small_product(const Gemm& g, int block, int blocks, float* lds) {
   constexpr int HALVES = SWIGLU ? 2 : 1, ROWS = 16 * TILES_M, STRIDE = SMALL + 4, TILE = ROWS * STRIDE;
   constexpr int PIECE = SMALL_PIECE<T>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const int tile = xcd_block(blockIdx.x, gridDim.x), m0 = tile / g.tiles_n * ROWS, n0 = tile % g.tiles_n * SMALL;
+  const int tile = xcd_block(block, blocks), m0 = tile / g.tiles_n * ROWS, n0 = tile % g.tiles_n * SMALL;
   const int from = min(g.k, wave * g.steps * PIECE), k = min(g.k, from + g.steps * PIECE);
   using A = Direct<T, TA, TILES_M>;
   using B = Direct<T, TB, 2>;
@@ -559,7 +582,7 @@ __global__ __launch_bounds__(64 * most_waves(SWIGLU, TA || TB)) void small_kerne
   const int r = int(threadIdx.x) / (SMALL / V), cc = int(threadIdx.x) % (SMALL / V) * V, row = m0 + r, col = n0 + cc;
   const bool owns = int(threadIdx.x) < ROWS * SMALL / V && row < g.m && col < g.n;
   Rest<T> rest;
-  if (owns) rest.fetch(g.e, row, col);
+  if (owns) rest.template fetch<false>(g.e, row, col);
   const Bias<T, SWIGLU> bias(g.e, owns ? col : g.n);
 #pragma unroll
   for (int h = 0; h < HALVES; ++h)
@@ -584,7 +607,12 @@ __global__ __launch_bounds__(64 * most_waves(SWIGLU, TA || TB)) void small_kerne
       if constexpr (SWIGLU) q[i] += t[TILE + i];
     }
   }
-  finish<T, SWIGLU>(g.e, bias, rest, row, col, p, q);
+  finish<T, SWIGLU, false>(g.e, bias, rest, row, col, p, q);
+}
+template <typename T, bool TA, bool TB, bool SWIGLU, int TILES_M>
+__global__ __launch_bounds__(64 * most_waves(SWIGLU, TA || TB)) void small_kernel(const Gemm g) {
+  extern __shared__ __align__(16) char lds_bytes[];
+  small_product<T, TA, TB, SWIGLU, TILES_M>(g, blockIdx.x, gridDim.x, reinterpret_cast<float*>(lds_bytes));
 }
 
 // The result from the parts' sums, in their order.
@@ -600,7 +628,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Epilogue e, int splits)
   float a[V] = {}, b[V] = {};
   const Bias<T, SWIGLU> bias(e, col);
   Rest<T> rest;
-  rest.fetch(e, int(row), col);
+  rest.template fetch<false>(e, int(row), col);
 #pragma unroll 2
   for (int s = 0; s < splits; ++s) {
     float t[V];
@@ -613,7 +641,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Epilogue e, int splits)
       for (int x = 0; x < V; ++x) b[x] += t[x];
     }
   }
-  finish<T, SWIGLU>(e, bias, rest, int(row), col, a, b);
+  finish<T, SWIGLU, false>(e, bias, rest, int(row), col, a, b);
 }
 
 // ------------------------------------------------------------------------------ dh and its sums
@@ -715,24 +743,20 @@ struct Sums {
   int columns, parts;
   int64_t blocks;
 };
-// Two such sums in one launch, the second's blocks after the first's.
+// (threads past 256 take no part)
 template <typename T>
-__global__ __launch_bounds__(256) void sums_kernel(const Sums first, const Sums second) {
-  __shared__ float lds[8][33];
-  const bool other = blockIdx.x >= first.blocks;
-  const Sums& s = other ? second : first;
-  const unsigned block = other ? blockIdx.x - unsigned(first.blocks) : blockIdx.x;
+__device__ __forceinline__ void add_up(const Sums& s, unsigned block, float (*lds)[33]) {
   const int across = threadIdx.x & 31, down = threadIdx.x >> 5;
   const int blocks = (s.columns + 31) / 32;
   const int64_t r = block / unsigned(blocks);
   const int c = int(block % unsigned(blocks)) * 32 + across;
   float v = 0.f;
-  if (c < s.columns) {
+  if (c < s.columns && down < 8) {
     const float* p = s.part + r * s.parts * s.columns + c;
 #pragma unroll 8
     for (int i = down; i < s.parts; i += 8) v += p[int64_t(i) * s.columns];
   }
-  lds[down][across] = v;
+  if (down < 8) lds[down][across] = v;
   __syncthreads();
   if (down || c >= s.columns) return;
   v = 0.f;
@@ -740,23 +764,62 @@ __global__ __launch_bounds__(256) void sums_kernel(const Sums first, const Sums 
   for (int i = 0; i < 8; ++i) v += lds[i][across];
   static_cast<T*>(s.out)[r * s.columns + c] = from_f32<T>(v);
 }
+// Two such sums in one launch, the second's blocks after the first's.
+template <typename T>
+__global__ __launch_bounds__(256) void sums_kernel(const Sums first, const Sums second) {
+  __shared__ float lds[8][33];
+  const bool other = blockIdx.x >= first.blocks;
+  add_up<T>(other ? second : first, other ? blockIdx.x - unsigned(first.blocks) : blockIdx.x, lds);
+}
+// What follows the slopes of a small backward, in one launch: dx and dW as small products, and both sums.
+template <typename T>
+__global__ __launch_bounds__(64 * most_waves(false, true)) void small_backward_kernel(const Gemm dx, const Gemm dw,
+                                                                                      int dx_blocks, int dw_blocks,
+                                                                                      const Sums first,
+                                                                                      const Sums second) {
+  extern __shared__ __align__(16) char lds_bytes[];
+  float* lds = reinterpret_cast<float*>(lds_bytes);
+  int block = blockIdx.x;
+  if (block < dx_blocks) return small_product<T, false, true, false, 2>(dx, block, dx_blocks, lds);
+  block -= dx_blocks;
+  if (block < dw_blocks) return small_product<T, true, true, false, 2>(dw, block, dw_blocks, lds);
+  block -= dw_blocks;
+  const bool other = block >= first.blocks;
+  add_up<T>(other ? second : first, unsigned(other ? block - int(first.blocks) : block),
+            reinterpret_cast<float(*)[33]>(lds));
+}
 
 // ---------------------------------------------------------------------------------- host
 constexpr int CUS = 256, MOST_LDS = 160 * 1024;
 
-// The tiles, the largest first, and what they take by measurement: the time of a piece (of a full CU's, for
-// each block in it; of a block alone on its CU) and of a tile's start and end, in microseconds.
+// The tiles, the largest first, and what they take by measurement, with rows and with transposed operands: the
+// time of a piece (of a full CU's, for each block in it; of a block alone on its CU) and of a tile's start and
+// end, in microseconds.
 struct Cost {
   double piece, alone, tile;
 };
 template <typename T, int SIZE> struct Tiles;
-template <> struct Tiles<bf16, 0> : Config<bf16, 256, 256, 64, 2, 4, 2> { static constexpr Cost COST{1.75, 1.75, 9.5}; };
-template <> struct Tiles<bf16, 1> : Config<bf16, 256, 192, 64, 4, 2, 2> { static constexpr Cost COST{1.33, 1.33, 10.0}; };
-template <> struct Tiles<bf16, 2> : Config<bf16, 256, 128, 64, 4, 2, 2> { static constexpr Cost COST{0.98, 0.98, 7.0}; };
-template <> struct Tiles<bf16, 3> : Config<bf16, 128, 128, 64, 2, 2, 2> { static constexpr Cost COST{0.63, 0.72, 3.0}; };
-template <> struct Tiles<bf16, 4> : Config<bf16, 64, 64, 64, 2, 1, 2> { static constexpr Cost COST{0.20, 0.50, 4.0}; };
-template <> struct Tiles<float, 0> : Config<float, 128, 128, 32, 2, 2, 2> { static constexpr Cost COST{2.1, 2.3, 4.0}; };
-template <> struct Tiles<float, 1> : Config<float, 64, 64, 32, 2, 1, 2> { static constexpr Cost COST{0.6, 1.6, 4.0}; };
+template <> struct Tiles<bf16, 0> : Config<bf16, 256, 256, 64, 2, 4, 2> {
+  static constexpr Cost COST[2]{{1.75, 1.75, 9.0}, {1.75, 1.75, 8.7}};
+};
+template <> struct Tiles<bf16, 1> : Config<bf16, 256, 192, 64, 4, 2, 2> {
+  static constexpr Cost COST[2]{{1.33, 1.33, 10.0}, {1.3, 1.3, 7.5}};
+};
+template <> struct Tiles<bf16, 2> : Config<bf16, 256, 128, 64, 4, 2, 2> {
+  static constexpr Cost COST[2]{{1.1, 1.1, 4.5}, {1.05, 1.05, 5.2}};
+};
+template <> struct Tiles<bf16, 3> : Config<bf16, 128, 128, 64, 2, 2, 2> {
+  static constexpr Cost COST[2]{{0.62, 0.72, 2.6}, {0.7, 0.8, 3.0}};
+};
+template <> struct Tiles<bf16, 4> : Config<bf16, 64, 64, 64, 2, 1, 2> {
+  static constexpr Cost COST[2]{{0.21, 0.5, 3.5}, {0.28, 0.55, 3.5}};
+};
+template <> struct Tiles<float, 0> : Config<float, 128, 128, 32, 2, 2, 2> {
+  static constexpr Cost COST[2]{{2.1, 2.3, 4.0}, {2.1, 2.3, 4.0}};
+};
+template <> struct Tiles<float, 1> : Config<float, 64, 64, 32, 2, 1, 2> {
+  static constexpr Cost COST[2]{{0.6, 1.6, 4.0}, {0.6, 1.6, 4.0}};
+};
 template <typename T>
 constexpr int SIZES = sizeof(T) == 2 ? 5 : 2;
 // Calls f(tile, its number) for every tile that the product can have: SwiGLU wants pairs of a wave's tiles.
@@ -787,8 +850,9 @@ Plan make_plan(int64_t m, int64_t n, int64_t k, bool transposed) {
       const int64_t steps = ceil_div(pieces, splits), blocks = tm * tn * splits;
       if (ceil_div(pieces, steps) != splits) continue;
       const int64_t each = ceil_div(blocks, CUS), rounds = ceil_div(each, C::PER_CU);
-      double us = std::max(double(each) * C::COST.piece, double(rounds) * C::COST.alone) * double(steps) +
-                  double(rounds) * C::COST.tile;
+      const Cost cost = C::COST[transposed];
+      double us = std::max(double(each) * cost.piece, double(rounds) * cost.alone) * double(steps) +
+                  double(rounds) * cost.tile;
       if (splits > 1) us += 5.0 + double(m) * double(n) * (SWIGLU ? 2 : 1) * 4.0 * (splits + 1) / 8e6;
       if (us < least) {
         least = us;
@@ -870,6 +934,12 @@ int product(Gemm g, float* part, hipStream_t stream, const char* what) {
   g.e.part = p.size >= 0 && p.splits > 1 ? part : nullptr;
   g.e.rows = g.m;
   g.e.outer = g.n;
+  if (const uint32_t d = uint32_t(g.e.rows_per_gate); d > 1) {  // exact below 2^31
+    int log = 0;
+    while ((uint64_t(1) << log) < d) ++log;
+    g.e.magic = uint32_t((uint64_t(1) << (31 + log)) / d + 1);
+    g.e.shift = log - 1;
+  }
   if (p.size < 0) {
     auto launch = [&](auto tiles) {
       constexpr int TILES_M = decltype(tiles)::value;
@@ -956,7 +1026,7 @@ extern "C" int sihc_linear_act(const sihc_linear* l, const void* x, const void* 
   g.m = int(l->rows);
   g.n = l->outer;
   g.k = l->inner;
-  g.e = Epilogue{bias, gate, residual, y, h, low, nullptr, l->gate_stride, 0, 0, l->act, int(l->rows_per_gate)};
+  g.e = Epilogue{bias, gate, residual, y, h, low, nullptr, l->gate_stride, 0, 0, l->act, int(l->rows_per_gate), 0, 0};
   return by_dtype(l->dtype, [&](auto t) {
     using T = decltype(t);
     float* part = static_cast<float*>(workspace);
@@ -1021,30 +1091,49 @@ extern "C" int sihc_linear_act_backward(const sihc_linear* l, const void* grad, 
       else slopes_kernel<T, false><<<unsigned(blocks), 256, 0, on>>>(v);
       if (const int rc = check_launch(what)) return rc;
     }
-    if (const int rc = sum(sums_of(bias_part, dbias, 1, wide, s.images * s.chunks),
-                           sums_of(gate_part, dgate, images, l->outer, s.chunks)))
-      return rc;
     const void* slopes = dh ? dh : grad;
-    Gemm g{};
-    g.a = slopes;
-    g.lda = wide;
-    g.ldb = l->inner;
-    if (dx) {
-      g.b = weight;
-      g.m = int(l->rows);
+    const Sums bias_sums = sums_of(bias_part, dbias, 1, wide, s.images * s.chunks);
+    const Sums gate_sums = sums_of(gate_part, dgate, images, l->outer, s.chunks);
+    auto gradient = [&](const void* b, void* out, int m, int k) {
+      Gemm g{};
+      g.a = slopes;
+      g.b = b;
+      g.lda = wide;
+      g.ldb = l->inner;
+      g.m = m;
       g.n = l->inner;
-      g.k = wide;
-      g.e = Epilogue{nullptr, nullptr, nullptr, dx, nullptr, nullptr, nullptr, 0, 0, 0, SIHC_ACT_NONE, 1};
-      if (const int rc = product<T, false, true, false>(g, part, on, what)) return rc;
+      g.k = k;
+      g.e = Epilogue{nullptr, nullptr, nullptr, out, nullptr, nullptr, nullptr, 0, 0, 0, SIHC_ACT_NONE, 1, 0, 0};
+      return g;
+    };
+    Gemm gx = gradient(weight, dx, int(l->rows), wide), gw = gradient(x, dweight, wide, int(l->rows));
+    if (dx && dweight) {
+      const Plan px = plan_of<T, false>(gx.m, gx.n, gx.k, true), pw = plan_of<T, false>(gw.m, gw.n, gw.k, true);
+      if (px.size < 0 && pw.size < 0) {
+        // one launch has one number of waves: a product that wants fewer has more of them, each with less
+        const int waves = std::max(px.splits, pw.splits);
+        auto place = [&](Gemm& g, const Plan& p) {
+          g.steps = int(ceil_div(ceil_div(g.k, SMALL_PIECE<T>), waves));
+          g.tiles_m = p.tiles_m;
+          g.tiles_n = p.tiles_n;
+          g.e.rows = g.m;
+          g.e.outer = g.n;
+        };
+        place(gx, px);
+        place(gw, pw);
+        const int64_t blocks = px.blocks + pw.blocks + bias_sums.blocks + gate_sums.blocks;
+        if (blocks * 64 * waves > MOST_LAUNCHED) return fail(SIHC_ERR_INVALID, "%s: too many rows for a launch", what);
+        const size_t lds = size_t(waves) * SMALL * (SMALL + 4) * sizeof(float);
+        small_backward_kernel<T><<<unsigned(blocks), unsigned(64 * waves), lds, on>>>(
+            gx, gw, int(px.blocks), int(pw.blocks), bias_sums, gate_sums);
+        return check_launch(what);
+      }
     }
-    if (dweight) {
-      g.b = x;
-      g.m = wide;
-      g.n = l->inner;
-      g.k = int(l->rows);
-      g.e = Epilogue{nullptr, nullptr, nullptr, dweight, nullptr, nullptr, nullptr, 0, 0, 0, SIHC_ACT_NONE, 1};
-      if (const int rc = product<T, true, true, false>(g, part, on, what)) return rc;
-    }
+    if (const int rc = sum(bias_sums, gate_sums)) return rc;
+    if (dx)
+      if (const int rc = product<T, false, true, false>(gx, part, on, what)) return rc;
+    if (dweight)
+      if (const int rc = product<T, true, true, false>(gw, part, on, what)) return rc;
     return int(SIHC_OK);
   });
 }
