@@ -8,11 +8,20 @@
 // A block owns a tile of the result; pieces of both operands, BK of the contraction at a time, pass
 // through two buffers in LDS: while one is worked on, the next piece is stored from registers to the
 // other one and the loads of the piece after it are under way, so that a piece costs one barrier and a
-// load has a whole piece's products to arrive. An operand whose contraction runs along its rows lies in
+// load has a whole piece's products to arrive. An operand whose contraction runs across its rows lies in
 // LDS as it is in memory, and is read by the transposing load. The result passes through LDS once more,
 // a wave's own 32 rows at a time, so that the epilogue has 8 adjacent channels of a row and reads and
 // writes whole vectors. With SwiGLU a block's columns alternate between 32 rows of W_a and their 32 of
-// W_b, so that both halves of a channel meet in one wave.
+// W_b, so that both halves of a channel meet in one wave. Which tile, and in how many parts the
+// contraction is cut, is what the measured costs of the tiles promise the least time for (make_plan).
+// Small products and few rows have a kernel without LDS buffers or parts (small_product).
+//
+// What bounds it (bf16, one MI355X). At 8,192 cubed 1,150 to 1,240 TFLOP/s, as the library's product: the
+// card's power. At 16,384 x 768 to a SwiGLU of 2,048: 112 us without and 134 with what the backward
+// needs of h (168 MB more), 920 TFLOP/s, where every tile of 256 x 256 starts and ends within 12 pieces; dx 96
+// (1,070 TFLOP/s), dW 105 (in 4 parts), the slopes between them 80 for 369 MB. At 16,384 x 1,152 to 1,152 with gate
+// and residual 68 us (640 TFLOP/s; the library's product alone 61): 4.5 tiles of 128 x 128 a CU. Two rows
+// of 1,152 to 6,912: 6 us of 16 MB, a launch and two loads' latency.
 #include "cond_common.h"
 
 #include <atomic>
@@ -656,8 +665,10 @@ struct Slopes {
 constexpr int CHUNK = 64;  // rows whose sums are one partial row
 
 // A block: 256 channels (32 threads of V) by 8 rows at a time, over one chunk of one image.
+// (A row at a time: two a thread, and three waves a SIMD for them, took 98 us instead of 80 for 16,384 rows of
+// a SwiGLU of 2,048, 369 MB.)
 template <typename T, bool SWIGLU>
-__global__ __launch_bounds__(256) void slopes_kernel(const Slopes s) {
+__global__ __launch_bounds__(256, 4) void slopes_kernel(const Slopes s) {
   __shared__ float lds[8][32 * V + 4];
   const int across = threadIdx.x & 31, down = threadIdx.x >> 5;
   const int blocks = (s.outer + 32 * V - 1) / (32 * V);
@@ -670,7 +681,7 @@ __global__ __launch_bounds__(256) void slopes_kernel(const Slopes s) {
   float sums[3][V] = {}, gate[V];
   if (left > 0) {
     if (s.gate) get(static_cast<const T*>(s.gate) + image * s.gate_stride + col, left, gate);
-#pragma unroll 2
+#pragma unroll 1
     for (int r = down; r < count; r += 8) {
       float g[V], a[V], b[V];
       const int64_t row = row0 + r;
