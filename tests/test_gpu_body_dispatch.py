@@ -376,3 +376,73 @@ def test_offsets_past_32_bits():
     at[-3:] = 1000
     y = body.axis_rotary(q, at, (40,))
     assert torch.equal(y[:, -3:], body.axis_rotary(q[:, -3:].contiguous(), at[-3:].contiguous(), (40,)))
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+def test_tensors_that_start_anywhere(dtype):
+    """Packed views one element into their storage: no access is aligned to more than an element."""
+    def moved(t):
+        whole = torch.empty(t.numel() + 1, device="cuda", dtype=t.dtype)
+        whole[1:] = t.reshape(-1)
+        return whole[1:].view(t.shape)
+
+    for size, act in (((2, 40, 64, 72), "swiglu"), ((3, 1, 200, 40), "silu"), ((4, 300, 512, 600), "none")):
+        batch, tokens, inner, outer = size
+        wide = 2 * outer if act == "swiglu" else outer
+        t = [normal(batch, tokens, inner, dtype=dtype), normal(wide, inner, dtype=dtype) * inner ** -0.5,
+             normal(wide, dtype=dtype), normal(batch, outer, dtype=dtype), normal(batch, tokens, outer, dtype=dtype)]
+        results = []
+        for values in (t, [moved(v) for v in t]):
+            leaves = [v.detach().requires_grad_() for v in values]
+            y = body.linear_act(*leaves[:3], act, *leaves[3:])
+            results.append([y.detach(), *torch.autograd.grad(y, leaves, torch.ones_like(y))])
+        assert equal(*results)
+    x, seed = normal(5, 1003, dtype=dtype), torch.tensor([4], device="cuda")
+    assert torch.equal(body.dropout(moved(x), 0.3, seed, 1, moved(x)), body.dropout(x, 0.3, seed, 1, x))
+
+
+@pytest.mark.parametrize("name", PUBLIC)
+def test_vmap(name):
+    call, values = public(name)
+    with torch.no_grad():
+        want = [call(factor * values[0], *values[1:]) for factor in (1, 2)]
+        got = torch.func.vmap(lambda t: call(t, *values[1:]))(torch.stack([values[0], 2 * values[0]]))
+    assert equal(list(got), want)
+
+
+@pytest.mark.parametrize("name", PUBLIC)
+def test_subclasses_and_modes_in_the_backward(name):
+    call, values = public(name)
+    want, seen = grads_of(call, values), []
+
+    class Log(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    leaves = [v.clone().requires_grad_() for v in values]
+    out = call(*leaves)
+    with Log():
+        got = torch.autograd.grad(out, leaves, torch.ones_like(out))
+    assert any("sihc" in s for s in seen) and equal(list(got), want[1:])
+
+    class Sub(torch.Tensor):
+        pass
+
+    with torch.no_grad():
+        out = call(values[0].as_subclass(Sub), *values[1:])
+        assert isinstance(out, Sub) and torch.equal(out.as_subclass(torch.Tensor), want[0])
+        assert torch.equal(call(torch.nn.Parameter(values[0]), *values[1:]), want[0])
+
+
+def test_a_large_product_is_captured_at_its_first_call():
+    """Kernels with more than 64 KB of LDS have it allowed at their first launch, which a capture may hold."""
+    x, w = normal(4096, 520, dtype=BF16), normal(2064, 520, dtype=BF16) * 0.05
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = body.linear_act(x, w, None, "swiglu")
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, body.linear_act(x, w, None, "swiglu"))
