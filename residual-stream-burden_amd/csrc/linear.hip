@@ -658,9 +658,11 @@ struct Slopes {
   const void *grad, *h, *gate;
   const uint32_t* low;
   void *dh;            // null where dh is the gradient itself
+  void* dgate;         // the gate's gradient, where a chunk's sum is all of it
   float *bias_part, *gate_part;
   int64_t gate_stride;
   int rows, outer, act, rows_per_gate, chunks;  // chunks of an image's rows
+  bool gate_of_row;    // every row has a gate of its own: no sums of it, and images matter no more
 };
 constexpr int CHUNK = 64;  // rows whose sums are one partial row
 
@@ -680,11 +682,12 @@ __global__ __launch_bounds__(256, 4) void slopes_kernel(const Slopes s) {
   const int wide = SWIGLU ? 2 : 1;
   float sums[3][V] = {}, gate[V];
   if (left > 0) {
-    if (s.gate) get(static_cast<const T*>(s.gate) + image * s.gate_stride + col, left, gate);
+    if (s.gate && !s.gate_of_row) get(static_cast<const T*>(s.gate) + image * s.gate_stride + col, left, gate);
 #pragma unroll 1
     for (int r = down; r < count; r += 8) {
-      float g[V], a[V], b[V];
+      float g[V], a[V], b[V], gate_grad[V];
       const int64_t row = row0 + r;
+      if (s.gate_of_row) get(static_cast<const T*>(s.gate) + row * s.gate_stride + col, left, gate);
       get(static_cast<const T*>(s.grad) + row * s.outer + col, left, g);
       if (s.h) {
         const T* h = static_cast<const T*>(s.h) + row * wide * s.outer + col;
@@ -710,7 +713,8 @@ __global__ __launch_bounds__(256, 4) void slopes_kernel(const Slopes s) {
         }
         float du = g[i];
         if (s.gate) {
-          sums[2][i] += g[i] * (SWIGLU ? u * b[i] : u);
+          gate_grad[i] = g[i] * (SWIGLU ? u * b[i] : u);
+          sums[2][i] += gate_grad[i];
           du *= gate[i];
         }
         if constexpr (SWIGLU) {
@@ -722,6 +726,7 @@ __global__ __launch_bounds__(256, 4) void slopes_kernel(const Slopes s) {
         }
         sums[0][i] += a[i];
       }
+      if (s.gate_of_row && s.dgate) put(static_cast<T*>(s.dgate) + row * s.outer + col, left, gate_grad);
       if (s.dh) {
         T* dh = static_cast<T*>(s.dh) + row * wide * s.outer + col;
         put(dh, left, a);
@@ -733,7 +738,8 @@ __global__ __launch_bounds__(256, 4) void slopes_kernel(const Slopes s) {
   for (int k = 0; k < 3; ++k) {
     if (k == 1 && !SWIGLU) continue;
     float* part = k == 2 ? s.gate_part : s.bias_part;
-    if (!part) continue;
+    const bool whole = k == 2 && s.dgate && !s.gate_of_row;
+    if (!part && !whole) continue;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < V; ++i) lds[down][across * V + i] = sums[k][i];
@@ -743,7 +749,8 @@ __global__ __launch_bounds__(256, 4) void slopes_kernel(const Slopes s) {
       float v = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) v += lds[i][threadIdx.x];
-      part[k == 2 ? int64_t(chunk) * s.outer + c : (int64_t(chunk) * wide + k) * s.outer + c] = v;
+      if (whole) static_cast<T*>(s.dgate)[int64_t(chunk) * s.outer + c] = from_f32<T>(v);
+      else part[k == 2 ? int64_t(chunk) * s.outer + c : (int64_t(chunk) * wide + k) * s.outer + c] = v;
     }
   }
 }
@@ -929,6 +936,7 @@ int start(const Gemm& g, int64_t blocks, hipStream_t stream, const char* what) {
   const auto kernel = &gemm_kernel<T, C, TA, TB, SWIGLU>;
   static_assert(L::BYTES <= MOST_LDS, "a CU's LDS");
   static std::atomic<uint64_t> allowed{0};
+  if (blocks * C::THREADS > MOST_LAUNCHED) return fail(SIHC_ERR_INVALID, "%s: too many rows for a launch", what);
   if (const int rc = allow(kernel, L::BYTES, allowed, what)) return rc;
   kernel<<<unsigned(blocks), C::THREADS, L::BYTES, stream>>>(g);
   return check_launch(what);
@@ -937,7 +945,6 @@ int start(const Gemm& g, int64_t blocks, hipStream_t stream, const char* what) {
 template <typename T, bool TA, bool TB, bool SWIGLU>
 int product(Gemm g, float* part, hipStream_t stream, const char* what) {
   const Plan p = plan_of<T, SWIGLU>(g.m, g.n, g.k, TA || TB);
-  if (p.blocks * 1024 > MOST_LAUNCHED) return fail(SIHC_ERR_INVALID, "%s: too many rows for a launch", what);
   g.splits = p.splits;
   g.steps = p.steps;
   g.tiles_m = p.tiles_m;
@@ -952,6 +959,8 @@ int product(Gemm g, float* part, hipStream_t stream, const char* what) {
     g.e.shift = log - 1;
   }
   if (p.size < 0) {
+    if (p.blocks * 64 * p.splits > MOST_LAUNCHED)
+      return fail(SIHC_ERR_INVALID, "%s: too many rows for a launch", what);
     auto launch = [&](auto tiles) {
       constexpr int TILES_M = decltype(tiles)::value;
       const size_t lds = size_t(p.splits) * (SWIGLU ? 2 : 1) * 16 * TILES_M * (SMALL + 4) * sizeof(float);
@@ -998,12 +1007,12 @@ Space space_of(const sihc_linear* l, bool gated) {
   Space s{};
   const bool swiglu = l->act == SIHC_ACT_SWIGLU;
   const int64_t wide = (swiglu ? 2 : 1) * int64_t(l->outer), size = l->dtype == SIHC_DTYPE_BF16 ? 2 : 4;
-  const int64_t each = gated ? l->rows_per_gate : std::max<int64_t>(l->rows, 1);
+  const int64_t each = gated && l->rows_per_gate > 1 ? l->rows_per_gate : l->rows;
   s.images = l->rows / each;
   s.chunks = ceil_div(each, CHUNK);
   if (l->act != SIHC_ACT_NONE || gated) s.dh = align(l->rows * wide * size);
   s.bias = align(s.images * s.chunks * wide * 4);
-  if (gated) s.gate = align(s.images * s.chunks * l->outer * 4);
+  if (gated && l->rows_per_gate > CHUNK) s.gate = align(s.images * s.chunks * l->outer * 4);
   const Plan dx = plan_for(l->dtype, l->rows, l->inner, wide, false, true);
   const Plan dw = plan_for(l->dtype, wide, l->inner, l->rows, false, true);
   s.part = align(int64_t(std::max(part_bytes(dx, l->rows, l->inner, false), part_bytes(dw, wide, l->inner, false))));
@@ -1087,15 +1096,29 @@ extern "C" int sihc_linear_act_backward(const sihc_linear* l, const void* grad, 
                 (long long)s.total());
   char* at = static_cast<char*>(workspace);
   void* dh = s.dh ? at : nullptr;
+  const bool gate_summed = dgate && s.gate;  // (else a chunk has all of an image)
   float* bias_part = reinterpret_cast<float*>(at + s.dh);
   float* gate_part = reinterpret_cast<float*>(at + s.dh + s.bias);
   float* part = reinterpret_cast<float*>(at + s.dh + s.bias + s.gate);
   return by_dtype(l->dtype, [&](auto t) {
     using T = decltype(t);
     if (dh || dbias) {
-      Slopes v{grad, dh ? h : nullptr, gate, l->act == SIHC_ACT_NONE ? nullptr : low, dh, dbias ? bias_part : nullptr, dgate ? gate_part : nullptr,
-               l->gate_stride, int(l->rows), l->outer, l->act, gated ? int(l->rows_per_gate) : int(l->rows),
-               int(s.chunks)};
+      Slopes v{};
+      v.grad = grad;
+      v.h = dh ? h : nullptr;
+      v.gate = gate;
+      v.low = l->act == SIHC_ACT_NONE ? nullptr : low;
+      v.dh = dh;
+      v.dgate = gate_summed ? nullptr : dgate;
+      v.bias_part = dbias ? bias_part : nullptr;
+      v.gate_part = gate_summed ? gate_part : nullptr;
+      v.gate_stride = l->gate_stride;
+      v.rows = int(l->rows);
+      v.outer = l->outer;
+      v.act = l->act;
+      v.gate_of_row = gated && l->rows_per_gate == 1;
+      v.rows_per_gate = int(gated && !v.gate_of_row ? l->rows_per_gate : l->rows);
+      v.chunks = int(s.chunks);
       const int64_t blocks = s.images * s.chunks * ceil_div(l->outer, 32 * V);
       if (blocks * 256 > MOST_LAUNCHED) return fail(SIHC_ERR_INVALID, "%s: too many rows for a launch", what);
       if (swiglu) slopes_kernel<T, true><<<unsigned(blocks), 256, 0, on>>>(v);
@@ -1104,7 +1127,7 @@ extern "C" int sihc_linear_act_backward(const sihc_linear* l, const void* grad, 
     }
     const void* slopes = dh ? dh : grad;
     const Sums bias_sums = sums_of(bias_part, dbias, 1, wide, s.images * s.chunks);
-    const Sums gate_sums = sums_of(gate_part, dgate, images, l->outer, s.chunks);
+    const Sums gate_sums = sums_of(gate_part, gate_summed ? dgate : nullptr, images, l->outer, s.chunks);
     auto gradient = [&](const void* b, void* out, int m, int k) {
       Gemm g{};
       g.a = slopes;

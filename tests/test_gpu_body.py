@@ -76,6 +76,15 @@ def test_linear_of_many_tiles(size, act, dtype):
     check_linear(linear_case(*size, act, True, True, True, dtype), f"{size} {act} {dtype}")
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("act", ["none", "swiglu"])
+@pytest.mark.parametrize("batch,tokens", [(300, None), (1, 1), (70, 2), (33, 63), (9, 64), (5, 65), (2, 130)])
+def test_gates_of_few_and_many_rows(batch, tokens, act, dtype):
+    """A gate for every row, images that one partial sum holds, and larger ones."""
+    announce(f"linear_act gates of {tokens} rows {act} {dtype}")
+    check_linear(linear_case(batch, tokens, 48, 264, act, True, True, True, dtype), f"{batch} x {tokens} {act} {dtype}")
+
+
 # Sizes for which the forward and the two gradients' products take the larger tiles, one and several parts of
 # the contraction, and tiles that end inside the result.
 @pytest.mark.parametrize("size,act", [((64, 256, 768, 2048), "swiglu"), ((64, 256, 1152, 1152), "none"),
