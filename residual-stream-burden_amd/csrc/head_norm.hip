@@ -553,6 +553,8 @@ extern "C" int sihc_qk_norm_rotary(const sihc_heads* h, const void* q, const voi
   a.y[1] = k_out;
   const int64_t groups = ceil_div(a.total, a.group);
   const int waves = groups >= 2048 ? 4 : 1;  // few tokens: a wave a block, over more CUs
+  if (ceil_div(groups, waves) * waves * 64 > MOST_LAUNCHED)
+    return fail(SIHC_ERR_INVALID, "qk_norm_rotary: too many tokens for a launch");
   return by_dtype(h->dtype, [&](auto t) {
     using T = decltype(t);
     return by_lanes(lanes_of(h->dim), [&](auto lanes) {

@@ -81,6 +81,7 @@ def test_heads_arguments():
     refused(call(heads_sizes(dim=257)), b"1..256 channels")
     refused(call(heads_sizes(heads=(1 << 20) + 1)), b"too many heads")
     refused(call(heads_sizes(batch=1 << 40, tokens=1 << 20)), b"at most 2^31 - 64 tokens")
+    refused(call(heads_sizes(batch=1, tokens=1 << 30, heads=64, dim=64)), b"too many tokens for a launch")
     refused(call(heads_sizes(axes=5)), b"0..4 axes")
     refused(call(heads_sizes(widths=(ctypes.c_int * 4)(3, 4))), b"turns 3 channels")
     refused(call(heads_sizes(widths=(ctypes.c_int * 4)(10, 8))), b"turn 18 channels of 16")
