@@ -1,4 +1,5 @@
-// What the conditioning kernels (embedding.hip, group_norm.hip, cross_attention.hip) share:
+// What the conditioning kernels (embedding.hip, group_norm.hip, cross_attention.hip) and the body kernels
+// (linear.hip, head_norm.hip, dropout.hip) share:
 // element types, unaligned row vectors, block order and the host's error reporting.
 #ifndef SIHC_COND_COMMON_H
 #define SIHC_COND_COMMON_H
