@@ -70,6 +70,12 @@ bool plain_strided(const Tensor& t) {
          !t.key_set().has_any(special) && !t._fw_grad(0).defined();
 }
 bool plain(const Tensor& t) { return plain_strided(t) && t.is_contiguous(); }
+// The registered ops of a backward would drop a forward-mode tangent (a transform's tensor may hide one).
+void refuse_tangents(const char* op, std::initializer_list<Tensor> grads) {
+  for (const Tensor& t : grads)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined() && !t.key_set().has(c10::DispatchKey::FuncTorchGradWrapper), op,
+                                ": no forward-mode derivative");
+}
 bool below_autograd() {
   const auto tls = c10::impl::tls_local_dispatch_key_set();
   return tls.excluded_.has(c10::DispatchKey::AutogradCUDA);
@@ -965,6 +971,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
                                      size_t(ws.numel()) * 4, stream_of(x)),
             false);
     } else {
+      refuse_tangents("linear_act backward", {grad});
       static auto op = registered<std::tuple<Tensor, Tensor, Tensor, Tensor>(
           const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const std::optional<Tensor>&,
           c10::string_view, bool, bool, bool, bool)>("sihc::linear_act_backward");
@@ -1048,6 +1055,7 @@ struct QkFn : torch::autograd::Function<QkFn> {
                                          dkw.data_ptr(), ws.data_ptr(), size_t(ws.numel()) * 4, stream_of(q)),
             false);
     } else {
+      refuse_tangents("qk_norm_rotary backward", {gq, gk});
       static auto op = registered<std::tuple<Tensor, Tensor, Tensor, Tensor>(
           const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
           at::IntArrayRef, double, double)>("sihc::qk_norm_rotary_backward");
@@ -1087,6 +1095,7 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
       RECORD_FUNCTION("sihc::axis_rotary", (Args{grad, positions, axes, theta, inverse}));
       dx = run_rotary(grad, positions, axes, theta, inverse, false);
     } else {
+      refuse_tangents("axis_rotary backward", {grad});
       static auto op = registered<Tensor(const Tensor&, const Tensor&, at::IntArrayRef, double, bool)>(
           "sihc::axis_rotary");
       dx = op.call(grad, positions, axes, theta, inverse);
@@ -1127,6 +1136,7 @@ struct DropoutFn : torch::autograd::Function<DropoutFn> {
       RECORD_FUNCTION("sihc::dropout", (Args{grad, p, seed, stream}));
       out[0] = run_dropout(grad, p, seed, stream, Tensor(), false);
     } else {
+      refuse_tangents("dropout backward", {grad});
       static auto op = registered<Tensor(const Tensor&, double, const Tensor&, int64_t, const std::optional<Tensor>&)>(
           "sihc::dropout");
       out[0] = op.call(grad, p, seed, stream, std::nullopt);
@@ -1498,7 +1508,14 @@ PyObject* py_entry(PyObject*, PyObject* args) {
   }
   return PyErr_Format(PyExc_AttributeError, "no native entry %s", name);
 }
-PyMethodDef methods[] = {{"entry", py_entry, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
+// has_tangent(t): whether a tensor is a dual one, read without a dispatch, so that transforms do not answer for it
+PyObject* py_has_tangent(PyObject*, PyObject* o) {
+  if (THPVariable_Check(o) && THPVariable_Unpack(o)._fw_grad(0).defined()) Py_RETURN_TRUE;
+  Py_RETURN_FALSE;
+}
+PyMethodDef methods[] = {{"entry", py_entry, METH_VARARGS, nullptr},
+                         {"has_tangent", py_has_tangent, METH_O, nullptr},
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_sihc_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -26,6 +26,7 @@ bits. float32 and bfloat16; the norm's weights may be float32 beside bfloat16 he
 backward of a gate works on h rounded to bfloat16, that of an activation on 20 bits of it, and the
 gradient of h enters the products rounded to bfloat16. q, k and x of the
 rotations are read through their strides (the channels of a head adjacent); the other tensors are packed.
+Derivatives are reverse-mode ones: a forward-mode tangent is refused.
 """
 from __future__ import annotations
 
@@ -38,7 +39,7 @@ from torch.library import custom_op, register_autograd
 
 from . import launch
 from ._lib import MAX_AXES, MAX_ROTARY_DIM
-from ._native import native
+from ._native import native, refuse_tangents
 from .conditioning import _TYPES, _require_gpu
 from .sublayer_kernels import _require_packed
 
@@ -100,7 +101,7 @@ def _linear_act_result_fake(x, weight, bias, act, gate, residual):
     return x.new_empty((*x.shape[:-1], _linear_outer(weight, act)))
 
 
-native(_linear_act_result, "linear_act_result")
+native(_linear_act_result, "linear_act_result", tangents=False)
 
 
 # The result and what the backward needs of h (empty where it needs nothing).
@@ -160,13 +161,14 @@ def _linear_autograd(ctx, grad, _, __):
     want = [ctx.needs_input_grad[i] for i in (0, 1, 2, 4)]
     if not any(want):
         return None, None, None, None, None, grad
+    refuse_tangents("linear_act backward", (grad,))
     grads = _linear_act_backward(grad.contiguous(), x, weight, h, low, gate, ctx.act, *want)
     dx, dweight, dbias, dgate = (g if w else None for g, w in zip(grads, want))
     return dx, dweight, dbias, None, dgate, grad if ctx.needs_input_grad[5] else None
 
 
 register_autograd(_linear_act, _linear_autograd, setup_context=_linear_setup)
-native(_linear_act, "linear_act")
+native(_linear_act, "linear_act", tangents=False)
 
 
 def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: str = "none",
@@ -257,12 +259,13 @@ def _qk_setup(ctx, inputs, output):
 
 
 def _qk_autograd(ctx, grad_q, grad_k):
+    refuse_tangents("qk_norm_rotary backward", (grad_q, grad_k))
     return (*_qk_norm_rotary_backward(grad_q.contiguous(), grad_k.contiguous(), *ctx.saved_tensors, ctx.axes,
                                       ctx.theta, ctx.eps), None, None, None, None)
 
 
 register_autograd(_qk_norm_rotary, _qk_autograd, setup_context=_qk_setup)
-native(_qk_norm_rotary, "qk_norm_rotary")
+native(_qk_norm_rotary, "qk_norm_rotary", tangents=False)
 
 
 def qk_norm_rotary(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, positions: Tensor,
@@ -295,7 +298,7 @@ def _rotary_autograd(ctx, grad):
 
 
 register_autograd(_axis_rotary, _rotary_autograd, setup_context=_rotary_setup)
-native(_axis_rotary, "axis_rotary")
+native(_axis_rotary, "axis_rotary", tangents=False)
 
 
 def axis_rotary(x: Tensor, positions: Tensor, axes: Sequence[int], theta: float = 10000.0) -> Tensor:
@@ -343,7 +346,7 @@ def _dropout_autograd(ctx, grad):
 
 
 register_autograd(_dropout, _dropout_autograd, setup_context=_dropout_setup)
-native(_dropout, "dropout")
+native(_dropout, "dropout", tangents=False)
 
 
 def dropout(x: Tensor, p: float, seed: Tensor, stream: int = 0, residual: Optional[Tensor] = None) -> Tensor:
