@@ -103,27 +103,39 @@ __device__ __forceinline__ float head_max(float v) {
   return v;
 }
 
-// 1 / sqrt(mean x^2 + eps) of a head. Where the squares leave the range of fp32, all lanes of the
-// wave take them again of values scaled by a power of two.
+// What a head's values are multiplied by before their squares are summed: 1 where fp32 has the squares.
+struct Scale {
+  bool any, large, small;  // of the wave's heads; of the lane's
+  __device__ __forceinline__ float of() const { return large ? 0x1p-70f : small ? 0x1p100f : 1.f; }
+};
+// 1 / sqrt(mean x^2 + eps) of a head's scaled values. Where squares leave the range of fp32, all lanes of the wave scale
+// their heads by a power of two: 256 values of 2^128 2^-70 have a sum of 2^124, and the least value of all, 2^-149, a
+// square of 2^-98. The root and the scale stay two factors, for their product may be too large for fp32 or subnormal.
 template <int LPH>
-__device__ __forceinline__ float reciprocal_rms(const float* x, const Args& a) {
+__device__ __forceinline__ float reciprocal_rms(float* x, const Args& a, Scale& scale) {
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < V; ++i) sum += x[i] * x[i];
   sum = head_sum<LPH>(sum);
   float r = rsqrtf(sum * a.share + a.eps);
   const bool odd = !(sum < 0x1p125f && sum >= a.least);
-  if (__builtin_expect(__any(odd), 0)) {
+  scale = Scale{__any(odd) != 0, false, false};
+  if (__builtin_expect(scale.any, 0)) {
     float most = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) most = fmaxf(most, fabsf(x[i]));
     most = head_max<LPH>(most);
-    const float s = most >= 1.f ? 0x1p-66f : 0x1p80f;
+    scale.large = odd && most >= 1.f;
+    scale.small = odd && !(most >= 1.f);
+    const float s = scale.of();
     sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) sum += (x[i] * s) * (x[i] * s);
+    for (int i = 0; i < V; ++i) {
+      x[i] *= s;
+      sum += x[i] * x[i];
+    }
     sum = head_sum<LPH>(sum);
-    if (odd) r = s * rsqrtf(sum * a.share + a.eps * s * s);
+    if (odd) r = rsqrtf(sum * a.share + a.eps * s * s);
   }
   return r;
 }
@@ -302,7 +314,8 @@ __global__ __launch_bounds__(256) void heads_kernel(const Args a) {
       float v[V];
       in[u].to(v);
       if constexpr (NORM && ONE) {
-        const float r = reciprocal_rms<LPH>(v, a);
+        Scale scale;
+        const float r = reciprocal_rms<LPH>(v, a, scale);
 #pragma unroll
         for (int i = 0; i < V; i += 2) {
           const float x = v[i] * r, y = v[i + 1] * r;
@@ -311,7 +324,8 @@ __global__ __launch_bounds__(256) void heads_kernel(const Args a) {
         }
       } else {
         if constexpr (NORM) {
-          const float r = reciprocal_rms<LPH>(v, a);
+          Scale scale;
+          const float r = reciprocal_rms<LPH>(v, a, scale);
 #pragma unroll
           for (int i = 0; i < V; ++i) v[i] *= r * w[i];
         }
@@ -373,7 +387,8 @@ __global__ __launch_bounds__(256, 4) void heads_backward_kernel(const Args a) {
             for (int i = 0; i < V / 2; ++i) angle[i] = l.angles[item.t * l.pairs + l.first / 2 + i];
           }
           turn(g, angle);  // (the angles are taken backwards)
-          const float rms = reciprocal_rms<LPH>(x, a), r = item.valid ? rms : 0.f;  // (0 / 0 without eps)
+          Scale scale;
+          const float rms = reciprocal_rms<LPH>(x, a, scale), r = item.valid ? rms : 0.f;  // (0 / 0 without eps)
           float dot = 0.f;
 #pragma unroll
           for (int i = 0; i < V; ++i) {
@@ -385,6 +400,11 @@ __global__ __launch_bounds__(256, 4) void heads_backward_kernel(const Args a) {
           dot = head_sum<LPH>(dot) * a.share;
 #pragma unroll
           for (int i = 0; i < V; ++i) g[i] = r * (w[i] * g[i] - x[i] * dot);
+          if (__builtin_expect(scale.any, 0)) {
+            const float s = scale.of();
+#pragma unroll
+            for (int i = 0; i < V; ++i) g[i] *= s;
+          }
           if (item.valid)
             Chunk<T>::put(static_cast<T*>(a.y[side]) + packed_at(a, side, item.token, item.head) + l.first, g, l.left);
         }
