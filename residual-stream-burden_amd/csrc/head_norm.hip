@@ -140,17 +140,22 @@ __device__ __forceinline__ float reciprocal_rms(float* x, const Args& a, Scale& 
   return r;
 }
 
-// A lane's pairs turned by their angles.
-__device__ __forceinline__ void turn(float* v, const float2* angle) {
+// A lane's pairs turned by their angles, if not WHOLE (every channel turns) then those of its `turns` first pairs: the
+// others stay as they are, for an infinite value times a sine of 0 would be its neighbour's NaN. (WHOLE is the kernels'
+// parameter: choosing pair by pair takes 117 us for the training pass of 16,384 tokens of 32 heads of 72 in place of
+// 115, a branch on it in the kernels 125.)
+template <bool WHOLE>
+__device__ __forceinline__ void turn(float* v, const float2* angle, int turns) {
 #pragma unroll
   for (int i = 0; i < V / 2; ++i) {
     const float c = angle[i].x, s = angle[i].y, a = v[2 * i], b = v[2 * i + 1];
-    v[2 * i] = a * c - b * s;
-    v[2 * i + 1] = a * s + b * c;
+    const bool turned = WHOLE || i < turns;
+    v[2 * i] = turned ? a * c - b * s : a;
+    v[2 * i + 1] = turned ? a * s + b * c : b;
   }
 }
 
-// Pair p of a token's angles: its cosine and sine, 1 and 0 where nothing turns.
+// Pair p of a token's angles: its cosine and sine, 1 and 0 where nothing turns (a norm's weights are multiplied by them).
 __device__ __forceinline__ float2 angle_of(const Args& a, int64_t at, double rate, int axis, bool turns) {
   if (!turns) return make_float2(1.f, 0.f);
   const double position = a.float_positions ? double(static_cast<const float*>(a.positions)[at + axis])
@@ -164,6 +169,7 @@ __device__ __forceinline__ float2 angle_of(const Args& a, int64_t at, double rat
 // What a lane keeps over the tokens of its wave.
 struct Lane {
   int first, left;      // its channels of a head: the first, how many there are from it on
+  int turns;            // how many pairs turn from its first on (fewer than one: none)
   int sub;              // its head among those of a pass
   float2* angles;       // the wave's angles in LDS: [group][pairs]
   int pairs;
@@ -177,6 +183,7 @@ __device__ __forceinline__ Lane lane_of(const Args& a, float2* lds) {
   l.sub = lane / LPH;
   l.first = (lane % LPH) * V;
   l.left = a.dim - l.first;
+  l.turns = a.turned - l.first / 2;
   l.pairs = LPH * V / 2;  // (whole chunks: those past dim have no turn)
   l.angles = lds + (threadIdx.x >> 6) * a.group * l.pairs;
 #pragma unroll
@@ -261,7 +268,7 @@ __device__ __forceinline__ Item item_of(const Args& a, int side, int first, int 
   return i;
 }
 
-template <typename T, int LPH, bool NORM, bool ONE>
+template <typename T, int LPH, bool NORM, bool ONE, bool WHOLE>
 __global__ __launch_bounds__(256) void heads_kernel(const Args a) {
   constexpr int SUB = 64 / LPH;
   extern __shared__ float2 lds[];
@@ -319,8 +326,9 @@ __global__ __launch_bounds__(256) void heads_kernel(const Args a) {
 #pragma unroll
         for (int i = 0; i < V; i += 2) {
           const float x = v[i] * r, y = v[i + 1] * r;
-          v[i] = x * first_of[i] + y * second_of[i];
-          v[i + 1] = x * first_of[i + 1] + y * second_of[i + 1];
+          const bool turned = WHOLE || i / 2 < l.turns;
+          v[i] = turned ? x * first_of[i] + y * second_of[i] : x * first_of[i];
+          v[i + 1] = turned ? x * first_of[i + 1] + y * second_of[i + 1] : y * second_of[i + 1];
         }
       } else {
         if constexpr (NORM) {
@@ -333,7 +341,7 @@ __global__ __launch_bounds__(256) void heads_kernel(const Args a) {
 #pragma unroll
           for (int i = 0; i < V / 2; ++i) angle[i] = l.angles[item.t * l.pairs + l.first / 2 + i];
         }
-        turn(v, angle);
+        turn<WHOLE>(v, angle, l.turns);
       }
       if (item.valid)
         Chunk<T>::put(static_cast<T*>(a.y[side]) + packed_at(a, side, item.token, item.head) + l.first, v, l.left);
@@ -341,7 +349,7 @@ __global__ __launch_bounds__(256) void heads_kernel(const Args a) {
   });
 }
 
-template <typename T, int LPH, bool ONE>
+template <typename T, int LPH, bool ONE, bool WHOLE>
 __global__ __launch_bounds__(256, 4) void heads_backward_kernel(const Args a) {
   constexpr int SUB = 64 / LPH;
   extern __shared__ float2 lds[];
@@ -386,7 +394,7 @@ __global__ __launch_bounds__(256, 4) void heads_backward_kernel(const Args a) {
 #pragma unroll
             for (int i = 0; i < V / 2; ++i) angle[i] = l.angles[item.t * l.pairs + l.first / 2 + i];
           }
-          turn(g, angle);  // (the angles are taken backwards)
+          turn<WHOLE>(g, angle, l.turns);  // (the angles are taken backwards)
           Scale scale;
           const float rms = reciprocal_rms<LPH>(x, a, scale), r = item.valid ? rms : 0.f;  // (0 / 0 without eps)
           float dot = 0.f;
@@ -547,6 +555,14 @@ int by_lanes(int lanes, F&& f) {
     default: return f(IC<32>{});
   }
 }
+// Calls f with a constant for every truth value.
+template <typename F>
+void choose(F&& f) { f(); }
+template <typename F, typename... Rest>
+void choose(F&& f, bool first, Rest... rest) {
+  if (first) choose([&](auto... others) { f(std::true_type{}, others...); }, rest...);
+  else choose([&](auto... others) { f(std::false_type{}, others...); }, rest...);
+}
 int64_t backward_blocks(const Args& a) {
   return std::min<int64_t>(BACKWARD_BLOCKS, ceil_div(ceil_div(a.total, a.group), 4));
 }
@@ -581,14 +597,10 @@ extern "C" int sihc_qk_norm_rotary(const sihc_heads* h, const void* q, const voi
       constexpr int LPH = decltype(lanes)::value;
       const size_t lds = size_t(waves) * a.group * (LPH * V / 2) * sizeof(float2);
       const dim3 grid{unsigned(ceil_div(groups, waves))}, block{unsigned(waves * 64)};
-      auto launch = [&](auto norm) {
-        constexpr bool NORM = decltype(norm)::value != 0;
-        if (a.group == 1)
-          heads_kernel<T, LPH, NORM, true><<<grid, block, lds, hipStream_t(stream)>>>(a);
-        else
-          heads_kernel<T, LPH, NORM, false><<<grid, block, lds, hipStream_t(stream)>>>(a);
-      };
-      q_weight ? launch(IC<1>{}) : launch(IC<0>{});
+      choose([&](auto norm, auto one, auto whole) {
+        heads_kernel<T, LPH, decltype(norm)::value, decltype(one)::value, decltype(whole)::value>
+            <<<grid, block, lds, hipStream_t(stream)>>>(a);
+      }, q_weight != nullptr, a.group == 1, 2 * a.turned == a.dim);
       return check_launch("qk_norm_rotary");
     });
   });
@@ -636,10 +648,10 @@ extern "C" int sihc_qk_norm_rotary_backward(const sihc_heads* h, const void* gra
         constexpr int LPH = decltype(lanes)::value;
         const size_t lds = 4 * std::max(size_t(a.group) * (LPH * V / 2) * sizeof(float2), size_t(2 * LPH * V) * 4);
         const dim3 grid{unsigned(blocks)}, block{256};
-        if (a.group == 1)
-          heads_backward_kernel<T, LPH, true><<<grid, block, lds, hipStream_t(stream)>>>(a);
-        else
-          heads_backward_kernel<T, LPH, false><<<grid, block, lds, hipStream_t(stream)>>>(a);
+        choose([&](auto one, auto whole) {
+          heads_backward_kernel<T, LPH, decltype(one)::value, decltype(whole)::value>
+              <<<grid, block, lds, hipStream_t(stream)>>>(a);
+        }, a.group == 1, 2 * a.turned == a.dim);
         return check_launch("qk_norm_rotary_backward");
       });
     });
