@@ -431,7 +431,10 @@ enum { SIHC_POSITION_I32 = 0, SIHC_POSITION_F32 = 1 };
  * heads, the channels of a head adjacent; dim is 1..SIHC_MAX_ROTARY_DIM. positions are [tokens,
  * axes], position_batch_stride 0, or [batch, tokens, axes], position_batch_stride tokens (in
  * positions). Axis i turns the pairs of the next widths[i] (even) channels of a head by position *
- * theta^(-2 j / widths[i]), pair j; channels past the axes stay. inverse turns back. */
+ * theta^(-2 j / widths[i]), pair j; channels past the axes stay. inverse turns back. At most
+ * 2^31 - 64 tokens, and in the forward what one launch of fewer than 2^26 waves takes: a wave has
+ * 4 * (64 / lanes) / (heads + kv_heads) tokens, at least 1 and at most 8, where lanes is the least
+ * power of two with 8 * lanes >= dim. */
 typedef struct {
   int64_t batch, tokens;
   int heads, kv_heads, dim, axes;

@@ -238,8 +238,8 @@ bool heads_fit(const Tensor& q, const Tensor& k, const Tensor& positions, const 
     sum += w;
   }
   if (dtype_code(q) < 0 || q.size(3) > SIHC_MAX_ROTARY_DIM || axes.size() > SIHC_MAX_AXES || sum > q.size(3) ||
-      q.size(0) * q.size(1) > (int64_t(1) << 31) - 64 || !(theta > 0.0) || !std::isfinite(theta))
-    return false;
+      q.size(0) * q.size(1) > (int64_t(1) << 26) - 4 || !(theta > 0.0) || !std::isfinite(theta))
+    return false;  // (of more tokens, the registered op knows whether a launch takes them)
   if (!plain(positions) || positions.device() != q.device() ||
       (positions.scalar_type() != at::kInt && positions.scalar_type() != at::kFloat))
     return false;

@@ -183,6 +183,13 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: st
 
 
 # --------------------------------------------------------------------- head norms and rotation
+def _most_tokens(heads: int, dim: int) -> int:
+    """What the forward's launch takes: fewer than 2^26 waves, each of one token if its heads fill four passes of the
+    wave (8 channels a lane, a power of two of lanes a head), else of as many as do, up to 8."""
+    lanes = 1 << ((dim - 1) // 8).bit_length()
+    return min(_MOST_TOKENS, ((1 << 26) - 4) * max(1, min(8, 4 * (64 // lanes) // heads)))
+
+
 def _check_heads(op: str, positions: Tensor, axes: Sequence[int], theta: float, **heads: Tensor) -> None:
     first = next(iter(heads.values()))
     for name, x in heads.items():
@@ -196,8 +203,9 @@ def _check_heads(op: str, positions: Tensor, axes: Sequence[int], theta: float, 
         if x.dtype not in _TYPES or x.dtype != first.dtype:
             raise ValueError(f"{op}: heads must share float32 or bfloat16")
     batch, tokens, _, dim = first.shape
-    if batch * tokens > _MOST_TOKENS:
-        raise ValueError(f"{op}: at most {_MOST_TOKENS} tokens, got {batch * tokens}")
+    most = _most_tokens(sum(x.shape[2] for x in heads.values()), dim)
+    if batch * tokens > most:
+        raise ValueError(f"{op}: at most {most} tokens of these heads, got {batch * tokens}")
     if len(axes) > MAX_AXES or any(w < 0 or w % 2 for w in axes) or sum(axes) > dim:
         raise ValueError(f"{op}: up to {MAX_AXES} axes of even widths within {dim} channels, got {list(axes)}")
     if not 0.0 < theta < math.inf:
