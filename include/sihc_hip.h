@@ -417,7 +417,8 @@ size_t sihc_linear_act_backward_workspace_size(const sihc_linear *l, int gated);
 /* Adjoint of sihc_linear_act (the residual's gradient is grad). h is needed where there is an
  * activation or a gate, low too in bf16 with an activation. dx [rows, inner], dweight like weight, dbias [its rows] and dgate
  * [rows / rows_per_gate, outer] are packed; each may be NULL if it is not wanted. Sums in fp32 in
- * a fixed order, without atomics; the gradient of h is rounded to dtype as the products' operand. */
+ * a fixed order, without atomics; the gradient of h is rounded to dtype as the products' operand.
+ * Refused from 2^24 pieces on, of up to 64 rows of one gate by 256 channels: a launch's blocks. */
 int sihc_linear_act_backward(const sihc_linear *l, const void *grad, const void *x,
                              const void *weight, const void *h, const uint32_t *low,
                              const void *gate, void *dx, void *dweight, void *dbias, void *dgate, void *workspace,

@@ -853,6 +853,7 @@ struct Plan {
   int size, splits, steps, tiles_m, tiles_n;  // size -1: small_kernel, whose waves are the splits
   int64_t blocks;
 };
+constexpr double NOT_LAUNCHED = 1e15;  // of more threads than a launch has: the plan only where there is no other, to be refused
 // small_kernel's: a piece where the CU is full, one that a wave waits for, start and end.
 constexpr Cost SMALL_COST{0.22, 2.0, 3.2};
 // The tile and the parts of the contraction that promise the least time: every CU's blocks one after
@@ -872,6 +873,7 @@ Plan make_plan(int64_t m, int64_t n, int64_t k, bool transposed) {
       double us = std::max(double(each) * cost.piece, double(rounds) * cost.alone) * double(steps) +
                   double(rounds) * cost.tile;
       if (splits > 1) us += 5.0 + double(m) * double(n) * (SWIGLU ? 2 : 1) * 4.0 * (splits + 1) / 8e6;
+      if (blocks * C::THREADS > MOST_LAUNCHED) us += NOT_LAUNCHED;
       if (us < least) {
         least = us;
         best = Plan{size, splits, int(steps), int(tm), int(tn), blocks};
@@ -885,7 +887,8 @@ Plan make_plan(int64_t m, int64_t n, int64_t k, bool transposed) {
     if (waves > 4 && pieces <= waves / 2) break;
     const int64_t steps = ceil_div(pieces, waves), rounds = ceil_div(each * waves, 16);
     const double us = std::max(double(each * pieces) * SMALL_COST.piece * (SWIGLU ? 1.5 : 1.0),
-                               double(rounds * steps) * SMALL_COST.alone) + SMALL_COST.tile;
+                               double(rounds * steps) * SMALL_COST.alone) + SMALL_COST.tile +
+                      (tm * tn * 64 * waves > MOST_LAUNCHED ? NOT_LAUNCHED : 0.0);
     if (us < least) {
       least = us;
       best = Plan{-1, waves, int(steps), int(tm), int(tn), tm * tn};

@@ -8,7 +8,28 @@ from helpers import announce
 from sihc_hip import body
 
 pytestmark = pytest.mark.gpu
-BF16 = torch.bfloat16
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.mark.parametrize("rows,inner,outer,act", [(2 ** 30, 1, 1, "none"), (2 ** 29 + 5, 3, 2, "swiglu"), (2 ** 26 + 1, 8, 300, "swiglu")],
+                         ids=str)
+def test_as_many_rows_as_fit(rows, inner, outer, act):
+    """A product whose cheapest tiles are more than a launch takes has others."""
+    wide = 2 * outer if act == "swiglu" else outer
+    if torch.cuda.mem_get_info()[0] < rows * (inner + outer) * 4 + (8 << 30):
+        pytest.skip("needs more memory")
+    announce(f"linear_act of {rows} rows of {inner} to {outer} {act} fp32")
+    x = torch.zeros(rows, inner, device="cuda", dtype=F32)
+    g = torch.Generator().manual_seed(0)
+    w, b, tail = (torch.randn(*s, generator=g).cuda() for s in ((wide, inner), (wide,), (500, inner)))
+    x[-500:] = tail
+    y = body.linear_act(x, w, b, act)
+    few = x[:70].contiguous(), x[-500:].contiguous()
+    h = [(v.double() @ w.double().t() + b.double()) for v in few]
+    want = [v if act == "none" else torch.nn.functional.silu(v[:, :outer]) * v[:, outer:] for v in h]
+    for got, exact in ((y[:70], want[0]), (y[-500:], want[1])):
+        assert float((got.double() - exact).abs().max()) <= 2.0 ** -16 * float(exact.abs().max())
+    del y
 
 
 def test_as_many_tokens_as_a_launch_takes():
