@@ -407,7 +407,8 @@ size_t sihc_linear_act_workspace_size(const sihc_linear *l);
  * gate * u, in fp32 sums, rounded once. bias, gate and residual may be NULL. For the backward h,
  * if given, receives h [rows, weight rows] in dtype. low, if given as well (bf16 with an activation;
  * [rows, parts, (outer + 7) / 8] words, 2 parts with SIHC_ACT_SWIGLU and else 1), receives 4 more
- * bits of each value, those of 8 channels in a word, lowest channel first, and h the 16 above them.
+ * bits of each value, rounded to nearest at 20, those of 8 channels in a word, lowest channel first,
+ * and h the 16 above them.
  * y may be the residual and no other input. The workspace may be NULL where its size is 0. */
 int sihc_linear_act(const sihc_linear *l, const void *x, const void *weight, const void *bias,
                     const void *gate, const void *residual, void *y, void *h, uint32_t *low,
