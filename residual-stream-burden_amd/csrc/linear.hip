@@ -127,7 +127,9 @@ struct Epilogue {
 __device__ __forceinline__ int image_of(const Epilogue& e, int row) {
   return e.magic ? int(__umulhi(uint32_t(row), e.magic) >> e.shift) : row;
 }
-__device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }  // (1 ulp)
+// Off by at most (2 |v| + 8) 2^-24 of its value, nearly all of it for negative v, where the exponential's argument is
+// rounded as a multiple of log2(e); 0 below -88.7, where the exponential passes fp32.
+__device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
 
 // V channels of a row as they are in memory, on their way while something else is done.
 template <typename T>
@@ -226,8 +228,7 @@ struct Gemm {
   const void *a, *b;
   int64_t lda, ldb;
   int m, n, k;      // (SwiGLU: n is the result's channels, half of b's rows)
-  int splits;       // parts of the contraction
-  int steps;        // pieces of a part
+  int steps;        // pieces of a part of the contraction
   int tiles_m, tiles_n;
   Epilogue e;
 };
@@ -664,7 +665,7 @@ struct Slopes {
   void* dgate;         // the gate's gradient, where a chunk's sum is all of it
   float *bias_part, *gate_part;
   int64_t gate_stride;
-  int rows, outer, act, rows_per_gate, chunks;  // chunks of an image's rows
+  int outer, act, rows_per_gate, chunks;  // chunks of an image's rows
   bool gate_of_row;    // every row has a gate of its own: no sums of it, and images matter no more
 };
 constexpr int CHUNK = 64;  // rows whose sums are one partial row
@@ -951,7 +952,6 @@ int start(const Gemm& g, int64_t blocks, hipStream_t stream, const char* what) {
 template <typename T, bool TA, bool TB, bool SWIGLU>
 int product(Gemm g, float* part, hipStream_t stream, const char* what) {
   const Plan p = plan_of<T, SWIGLU>(g.m, g.n, g.k, TA || TB);
-  g.splits = p.splits;
   g.steps = p.steps;
   g.tiles_m = p.tiles_m;
   g.tiles_n = p.tiles_n;
@@ -1119,7 +1119,6 @@ extern "C" int sihc_linear_act_backward(const sihc_linear* l, const void* grad, 
       v.bias_part = dbias ? bias_part : nullptr;
       v.gate_part = gate_summed ? gate_part : nullptr;
       v.gate_stride = l->gate_stride;
-      v.rows = int(l->rows);
       v.outer = l->outer;
       v.act = l->act;
       v.gate_of_row = gated && l->rows_per_gate == 1;
