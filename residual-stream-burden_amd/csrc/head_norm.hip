@@ -11,9 +11,10 @@
 // a lane, so that a head is read once and its statistics are a few moves between lanes.
 //
 // What bounds it (bf16, one MI355X): memory, with the vector instructions close behind. 16,384 tokens of 32 heads of 72
-// take 40 us (151 MB, 3.8 TB/s) forward and 72 backward (226 MB, 3.1 TB/s, two loads of two heads ahead: more
-// of them leave three waves on a SIMD, which took 83 to 109); 32,768 of 20 heads of 128 take 76 (336 MB, 4.4
-// TB/s) and 125 (503 MB, 4.0). A head of 72 fills 9 of its 16 lanes. Two images of 256 tokens: 8 us, four loads' latency
+// take 41 us (151 MB, 3.7 TB/s) forward and 71 backward (226 MB, 3.2 TB/s, two loads of two heads ahead, at the 128
+// registers of four waves a SIMD: more loads leave three waves, which took 83 to 109); 32,768 of 20 heads of 128 take 76 (336 MB, 4.4
+// TB/s) and 123 (503 MB, 4.1). In fp32 69 and 103, 143 and 231. A head of 72 fills 9 of its 16 lanes. Heads past 128
+// channels, 32 lanes each, spill 6 registers (fp32 10) in the backward. Two images of 256 tokens: 8 us, four loads' latency
 // in a row.
 //
 // The angle is a product in 64 bits, in turns, whose whole turns are dropped before it is rounded to

@@ -16,11 +16,12 @@
 // contraction is cut, is what the measured costs of the tiles promise the least time for (make_plan).
 // Small products and few rows have a kernel without LDS buffers or parts (small_product).
 //
-// What bounds it (bf16, one MI355X). At 8,192 cubed 1,150 to 1,240 TFLOP/s, as the library's product: the
-// card's power. At 16,384 x 768 to a SwiGLU of 2,048: 112 us without and 134 with what the backward
-// needs of h (168 MB more), 920 TFLOP/s, where every tile of 256 x 256 starts and ends within 12 pieces; dx 96
-// (1,070 TFLOP/s), dW 105 (in 4 parts), the slopes between them 80 for 369 MB. At 16,384 x 1,152 to 1,152 with gate
-// and residual 68 us (640 TFLOP/s; the library's product alone 61): 4.5 tiles of 128 x 128 a CU. Two rows
+// What bounds it (bf16, one MI355X, long runs). At 8,192 cubed 1,150 to 1,240 TFLOP/s; the library's products take 0.72
+// (both operands in rows), 0.82 (dx) and 1.01 (dW) of these times, so that the card's power is not the bound: the tiles' waves are
+// not fed without a pause. At 16,384 x 768 to a SwiGLU of 2,048: 120 us without and 135 with what the backward
+// needs of h (168 MB more), 760 TFLOP/s, where every tile of 256 x 256 starts and ends within 12 pieces; dx 106
+// (970 TFLOP/s), dW 99 and 11 to join its 4 parts, the slopes between them 83 for 369 MB. At 16,384 x 1,152 to 1,152 with gate
+// and residual 67 us (650 TFLOP/s; the library's product alone 60): 4.5 tiles of 128 x 128 a CU. Two rows
 // of 1,152 to 6,912: 6 us of 16 MB, a launch and two loads' latency.
 #include "cond_common.h"
 
@@ -672,7 +673,8 @@ constexpr int CHUNK = 64;  // rows whose sums are one partial row
 
 // A block: 256 channels (32 threads of V) by 8 rows at a time, over one chunk of one image.
 // (A row at a time: two a thread, and three waves a SIMD for them, took 98 us instead of 80 for 16,384 rows of
-// a SwiGLU of 2,048, 369 MB.)
+// a SwiGLU of 2,048, 369 MB. An image of few rows leaves row lanes idle and a partial row of every sum: a SwiGLU of 768
+// over 16,384 rows takes 29 us with its sums at 64 rows a gate, 46 at 8, 77 at 4, 155 at 2, and 35 at one, which has no sums.)
 template <typename T, bool SWIGLU>
 __global__ __launch_bounds__(256, 4) void slopes_kernel(const Slopes s) {
   __shared__ float lds[8][32 * V + 4];
@@ -816,7 +818,7 @@ constexpr int CUS = 256, MOST_LDS = 160 * 1024;
 
 // The tiles, the largest first, and what they take by measurement, with rows and with transposed operands: the
 // time of a piece (of a full CU's, for each block in it; of a block alone on its CU) and of a tile's start and
-// end, in microseconds.
+// end, in microseconds. (fp32 takes the same either way: 4,096 cubed 1.02 ms with rows, dx 1.03, dW 1.05.)
 struct Cost {
   double piece, alone, tile;
 };
